@@ -1,0 +1,27 @@
+/*
+ * attn_common.h - what the attention kernels take beside the cache and the
+ * batch, and their launchers (internal).
+ */
+#ifndef SERA_ATTN_COMMON_H
+#define SERA_ATTN_COMMON_H
+
+#include "kv_common.h"
+
+struct attn_args {
+    const void *q;
+    void *out;
+    int64_t q_stride, out_stride;   /* elements */
+    int heads, group;               /* query heads, query heads per kv head */
+    float scale_log2;               /* scale * log2(e) */
+    int window, sinks;              /* window 0: none */
+    float *workspace;
+    int cus;                        /* compute units of the device */
+};
+
+hipError_t sera_launch_kv_move(bool write, uint32_t cache_type, uint32_t type, int dim, const kv_args &a, void *k,
+                               int64_t k_stride, void *v, int64_t v_stride, hipStream_t s);
+size_t sera_attn_workspace(const kv_args &a, int dim, int heads, int cus);
+hipError_t sera_launch_attn(uint32_t cache_type, uint32_t type, int dim, const kv_args &a, const attn_args &t,
+                            hipStream_t s);
+
+#endif

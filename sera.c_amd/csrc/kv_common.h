@@ -1,0 +1,97 @@
+/*
+ * kv_common.h - the paged cache on the device: layout, batch lookup and
+ * element conversions shared by the cache and the attention kernels
+ * (internal; the layout itself is stated in include/sera_attn.h).
+ */
+#ifndef SERA_KV_COMMON_H
+#define SERA_KV_COMMON_H
+
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "../../include/sera_attn.h"
+
+/* What the kernels take of a sera_kv_cache and a sera_kv_batch. */
+struct kv_args {
+    uint8_t *data;
+    size_t page_bytes;       /* one page, all kv heads */
+    uint32_t head_bytes;     /* one kv head's run of a page */
+    int page_shift;          /* log2(page_tokens) */
+    int pages;
+    int kv_heads;
+    int sequences, rows, max_new, max_kv;
+    int64_t table_stride;
+    const int32_t *row_start, *kv_len, *table;
+};
+
+/* Bytes of one element; the head's run of a page. */
+static inline uint32_t kv_head_bytes(uint32_t type, int page_tokens, int head_dim) {
+    const uint32_t n = (uint32_t)page_tokens * (uint32_t)head_dim;
+    return type == SERA_KV_F16 ? 4u * n : 2u * n + 8u * (uint32_t)page_tokens;
+}
+
+/* One sequence of a batch, checked against the host's bounds. */
+struct kv_seq {
+    int b;          /* sequence, or -1: none */
+    int row0, n;    /* its packed rows */
+    int len;        /* its positions */
+    bool bad;       /* rows or length outside the bounds */
+};
+
+__device__ __forceinline__ kv_seq kv_sequence(const kv_args &a, int b) {
+    kv_seq s;
+    s.b = b;
+    const int r0 = a.row_start[b], r1 = a.row_start[b + 1], len = a.kv_len[b];
+    s.bad = r0 < 0 || r1 < r0 || r1 > a.rows || r1 - r0 > a.max_new || len < 0 || len > a.max_kv;
+    const int lo = min(max(r0, 0), a.rows), hi = min(max(r1, lo), a.rows);
+    s.row0 = lo;
+    s.n = hi - lo;
+    s.len = len;
+    return s;
+}
+
+/* Grids over (sequence, unit of `per` rows) when only the packed rows' count
+ * is known on the host: sequence b has the slots from row_start[b] / per +
+ * extra * b on. That leaves it floor(n / per) + extra slots or more, in
+ * floor(rows / per) + extra * sequences in all. Returns the sequence and the
+ * unit in it of slot `slot` (wave-uniform): a 64-way search, one load of
+ * row_start per level, a single one up to 64 sequences. */
+__device__ __forceinline__ int kv_find(const kv_args &a, int slot, int per, int extra, int *unit) {
+    const int lane = (int)(threadIdx.x & 63);
+    int lo = 0, span = a.sequences;          /* the answer is in [lo, lo + span) */
+    int base = 0;
+    while (span > 0) {
+        const int step = (span + 63) / 64;
+        const int b = lo + lane * step;
+        int key = 0x7fffffff;
+        if (lane * step < span) {
+            const int r = min(max(a.row_start[b], 0), a.rows);
+            key = r / per + extra * b;
+        }
+        const int hits = __popcll(__ballot(key <= slot));
+        if (!hits) return -1;                /* unordered row_start */
+        base = __shfl(key, hits - 1, 64);
+        lo += (hits - 1) * step;
+        if (step == 1) break;
+        span = min(step, a.sequences - lo);
+    }
+    *unit = slot - base;
+    if (slot < base) return -1;
+    return __builtin_amdgcn_readfirstlane(lo);
+}
+
+static inline int64_t kv_slots(int rows, int sequences, int per, int extra) {
+    return (int64_t)rows / per + (int64_t)extra * sequences;
+}
+
+/* Row elements. */
+__device__ __forceinline__ float kv_to_f32(float x) { return x; }
+__device__ __forceinline__ float kv_to_f32(_Float16 x) { return (float)x; }
+__device__ __forceinline__ float kv_to_f32(__bf16 x) { return (float)x; }
+template <typename T>
+__device__ __forceinline__ T kv_from_f32(float x) { return (T)x; }
+
+#endif

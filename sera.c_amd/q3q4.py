@@ -16,7 +16,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libsera_q4k.so")
 ROOT = os.path.dirname(HERE)
 HEADERS = [os.path.join(ROOT, "include", "q3_q4_linear.h"),
-           os.path.join(ROOT, "include", "sera_q4k.h")]
+           os.path.join(ROOT, "include", "sera_q4k.h"),
+           os.path.join(ROOT, "include", "sera_attn.h")]
 
 QTYPE_Q4_K = 12
 QTYPE_Q6_K = 14
@@ -42,6 +43,19 @@ class Geometry(ctypes.Structure):
     """q3_q4_linear_geometry (src/q3_q4_linear.h:49-55)."""
     _fields_ = [("M", ctypes.c_int32), ("N", ctypes.c_int32), ("K", ctypes.c_int32),
                 ("qtype", ctypes.c_uint32), ("weight_bytes", ctypes.c_uint64)]
+
+
+class KVCacheArgs(ctypes.Structure):
+    """sera_kv_cache (include/sera_attn.h)."""
+    _fields_ = [("type", ctypes.c_uint32), ("page_tokens", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("pages", ctypes.c_int64), ("data", ctypes.c_void_p)]
+
+
+class KVBatchArgs(ctypes.Structure):
+    """sera_kv_batch (include/sera_attn.h)."""
+    _fields_ = [("sequences", ctypes.c_int32), ("rows", ctypes.c_int32), ("max_new", ctypes.c_int32),
+                ("max_kv", ctypes.c_int32), ("table_stride", ctypes.c_int64), ("row_start", ctypes.c_void_p),
+                ("kv_len", ctypes.c_void_p), ("page_table", ctypes.c_void_p)]
 
 
 class Q3Q4Error(RuntimeError):
@@ -161,6 +175,12 @@ def load():
         "sera_q4k_bench_stream": ([P, P, P, P, P, I, P, I, I, I, ctypes.POINTER(ctypes.c_double)], I),
         "sera_q4k_bench_kernel": ([I, P, I, P, P, P, SZ, I, I, I, I, P, I, I,
                                    ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double)], I),
+        # sera_attn.h
+        "sera_kv_page_bytes": ([U32, I, I, I], SZ),
+        "sera_kv_write": ([P, P, U32, P, I64, P, I64, P], I),
+        "sera_kv_read": ([P, P, U32, P, I64, P, I64, P], I),
+        "sera_attention_workspace_bytes": ([P, P, I], SZ),
+        "sera_attention": ([P, P, U32, P, I64, P, I64, I, ctypes.c_float, I, I, P, SZ, P], I),
     }
     for name, (args, res) in sigs.items():
         fn = getattr(L, name)
@@ -527,3 +547,116 @@ def linear_group(geometries, weights, outputs, x, x2=None, gamma=None, eps=0.0, 
     Yp = (ctypes.c_void_p * n)(*[y.data_ptr() for y in outputs])
     _check(load().sera_linear_group(n, G, Wp, Yp, _ptr(x), _ptr(x2), _ptr(gamma), float(eps), x.shape[0], flags,
                                     _stream(stream)), "sera_linear_group")
+
+
+# ---------------------------------------------------------------------------
+# Paged key/value cache and its attention (include/sera_attn.h)
+# ---------------------------------------------------------------------------
+
+KV_F16 = 1      # SERA_KV_F16
+KV_Q8 = 264     # SERA_KV_Q8: int8 codes, one float scale per token and kv head
+_ROW_TYPES = None
+
+
+def _row_type(t):
+    """(type id, data pointer, row stride) of rows [n, width]."""
+    global _ROW_TYPES
+    if _ROW_TYPES is None:
+        import torch
+        _ROW_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
+    if t.dtype not in _ROW_TYPES or t.dim() != 2 or t.stride(1) != 1 or not t.is_cuda:
+        raise Q3Q4Error("rows must be a 2-d float32, float16 or bfloat16 device tensor with contiguous rows, "
+                        f"got {tuple(t.shape)} {t.dtype} strides {t.stride()}")
+    return _ROW_TYPES[t.dtype], t.data_ptr(), t.stride(0)
+
+
+def kv_page_bytes(type, page_tokens, kv_heads, head_dim):
+    return load().sera_kv_page_bytes(type, page_tokens, kv_heads, head_dim)
+
+
+class KVCache:
+    """A paged cache: `data` is a contiguous uint8 device tensor of
+    pages * kv_page_bytes(...) bytes, made here when none is given."""
+
+    def __init__(self, type, pages, page_tokens, kv_heads, head_dim, data=None, device=0):
+        import torch
+        self.page_bytes = kv_page_bytes(type, page_tokens, kv_heads, head_dim)
+        if not self.page_bytes:
+            raise Q3Q4Error(f"no cache of type {type} with pages of {page_tokens} tokens, {kv_heads} kv heads of "
+                            f"{head_dim}")
+        if data is None:
+            data = torch.empty(pages * self.page_bytes, dtype=torch.uint8, device=f"cuda:{device}")
+        if data.dtype != torch.uint8 or not data.is_contiguous() or data.numel() < pages * self.page_bytes:
+            raise Q3Q4Error(f"the cache's data must be {pages * self.page_bytes} contiguous uint8")
+        self.type, self.pages, self.page_tokens = type, pages, page_tokens
+        self.kv_heads, self.head_dim, self.data = kv_heads, head_dim, data
+        self.args = KVCacheArgs(type, page_tokens, kv_heads, head_dim, pages, data.data_ptr())
+        self.ref = ctypes.addressof(self.args)
+
+
+class KVBatch:
+    """The sequences of a call (sera_kv_batch): int32 device tensors
+    row_start [sequences + 1], kv_len [sequences] and page_table
+    [sequences, entries], which are read when the work runs, and the host's
+    bounds for them."""
+
+    def __init__(self, row_start, kv_len, page_table, rows, max_new, max_kv):
+        import torch
+        n = kv_len.numel()
+        for t, shape in ((row_start, (n + 1,)), (kv_len, (n,)), (page_table, (n, page_table.shape[-1]))):
+            if t.dtype != torch.int32 or tuple(t.shape) != shape or (t.numel() > 1 and t.stride(-1) != 1):
+                raise Q3Q4Error(f"batch tensors are int32 with contiguous rows, got {t.dtype} {tuple(t.shape)}")
+        self.row_start, self.kv_len, self.page_table = row_start, kv_len, page_table
+        self.rows, self.max_new, self.max_kv = rows, max_new, max_kv
+        # one sequence's table may have any stride: it is never used
+        stride = max(page_table.stride(0), page_table.shape[1]) if n == 1 else page_table.stride(0) if n else 0
+        if n > 1 and stride < page_table.shape[1]:
+            raise Q3Q4Error("page_table rows overlap")
+        if max_kv > page_table.shape[1] * 1024:
+            raise Q3Q4Error(f"max_kv={max_kv} is more than {page_table.shape[1]} pages hold")
+        self.entries = page_table.shape[1]
+        self.args = KVBatchArgs(n, rows, max_new, max_kv, stride, row_start.data_ptr(), kv_len.data_ptr(),
+                                page_table.data_ptr())
+        self.ref = ctypes.addressof(self.args)
+
+
+def _kv_rows(cache, batch, width, *tensors):
+    """(type, pointers and strides) of row operands, checked against the batch."""
+    if batch.max_kv > batch.entries * cache.page_tokens:
+        raise Q3Q4Error(f"max_kv={batch.max_kv} is more than {batch.entries} pages of {cache.page_tokens} hold")
+    got = [_row_type(t) for t in tensors]
+    for t, g in zip(tensors, got):
+        if t.shape[0] < batch.rows or t.shape[1] != width or g[0] != got[0][0]:
+            raise Q3Q4Error(f"rows must be [{batch.rows}, {width}] of one type, got {tuple(t.shape)} {t.dtype}")
+    return got
+
+
+def kv_write(cache, batch, k, v, stream=None):
+    """k, v [rows, kv_heads * head_dim] into the cache."""
+    (ty, kp, ks), (_, vp, vs) = _kv_rows(cache, batch, cache.kv_heads * cache.head_dim, k, v)
+    _check(load().sera_kv_write(cache.ref, batch.ref, ty, kp, ks, vp, vs, _stream(stream)), "sera_kv_write")
+
+
+def kv_read(cache, batch, k, v, stream=None):
+    """The cached values of the batch's rows into k, v [rows, kv_heads * head_dim]."""
+    (ty, kp, ks), (_, vp, vs) = _kv_rows(cache, batch, cache.kv_heads * cache.head_dim, k, v)
+    _check(load().sera_kv_read(cache.ref, batch.ref, ty, kp, ks, vp, vs, _stream(stream)), "sera_kv_read")
+
+
+def attention_workspace(cache, batch, heads):
+    """Scratch for attention() with this batch's bounds (None: none needed)."""
+    import torch
+    n = load().sera_attention_workspace_bytes(cache.ref, batch.ref, heads)
+    return torch.empty(n, dtype=torch.uint8, device=cache.data.device) if n else None
+
+
+def attention(cache, batch, q, out, scale, window=0, sinks=0, workspace=None, stream=None):
+    """out[row] = attention of q[row] over its sequence's cache; q, out
+    [rows, heads * head_dim] of one type. window 0: the whole context."""
+    width = q.shape[1]
+    (ty, qp, qs), (_, op, os_) = _kv_rows(cache, batch, width, q, out)
+    if width % cache.head_dim:
+        raise Q3Q4Error(f"rows of {width} are no heads of {cache.head_dim}")
+    wp, wb = (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if workspace is not None else (0, 0)
+    _check(load().sera_attention(cache.ref, batch.ref, ty, qp, qs, op, os_, width // cache.head_dim, scale, window,
+                                 sinks, wp, wb, _stream(stream)), "sera_attention")
