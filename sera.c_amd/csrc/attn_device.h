@@ -1,0 +1,157 @@
+/*
+ * attn_device.h - what the attention kernels share on the device: the
+ * visible range of a sequence's rows, query fragments, the mask, and the
+ * treatment of what the cache holds in places that a row does not see.
+ */
+#ifndef SERA_ATTN_DEVICE_H
+#define SERA_ATTN_DEVICE_H
+
+#include "attn_common.h"
+
+typedef _Float16 attn_h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 attn_h8 __attribute__((ext_vector_type(8)));
+typedef float attn_f2 __attribute__((ext_vector_type(2)));
+typedef float attn_f4 __attribute__((ext_vector_type(4)));
+typedef float attn_f16 __attribute__((ext_vector_type(16)));
+typedef uint32_t attn_u2 __attribute__((ext_vector_type(2)));
+typedef uint32_t attn_u4 __attribute__((ext_vector_type(4)));
+
+constexpr float kAttnLowest = -3.402823466e38f;
+/* Weights are held as 2^(s - m + kAttnBias), m the running maximum. m may lag
+ * behind the true maximum by kAttnLag, so they reach 2^15, inside fp16, and a
+ * weight keeps its 11 (two terms: 22) bits down to 2^-21 (2^-10) of the
+ * largest; below that its error is 2^-31 of the largest. The factor 2^kAttnBias
+ * is in the sum of the weights as well and leaves with the division. */
+constexpr float kAttnBias = 7.0f, kAttnLag = 8.0f;
+
+/* Tiles of 2^shift positions that the rows from position p0 (>= 0) to len-1 see:
+ * the sinks' tiles, then those from the first row's window to the end. */
+struct attn_range {
+    int sink_tiles, low, count;
+    __device__ __forceinline__ int tile(int v) const { return v < sink_tiles ? v : low + v - sink_tiles; }
+};
+
+__device__ __forceinline__ attn_range attn_range_of(const attn_args &t, int p0, int end, int shift) {
+    attn_range r;
+    const int first = t.window > 0 ? max(p0 - t.window + 1, 0) : 0;
+    r.low = first >> shift;
+    /* sinks can be as large as an int: no sum before the minimum */
+    r.sink_tiles = t.window > 0 ? min((min(t.sinks, first) + (1 << shift) - 1) >> shift, r.low) : 0;
+    r.count = end > 0 ? r.sink_tiles + ((end + (1 << shift) - 1) >> shift) - r.low : 0;
+    return r;
+}
+
+/* Whether every row with positions p0 .. p1 sees all positions j .. j+n-1. */
+__device__ __forceinline__ bool attn_all_seen(const attn_args &t, int j, int n, int p0, int p1) {
+    return j + n - 1 <= p0 && (t.window == 0 || j > p1 - t.window || j + n <= t.sinks);
+}
+
+__device__ __forceinline__ bool attn_sees(const attn_args &t, int p, int j) {
+    return j <= p && (t.window == 0 || j > p - t.window || j < t.sinks);
+}
+
+/* The page of positions pos .. pos+15 of sequence b, or -1 if its id is
+ * outside the pool. Past the end: page 0, which is in the pool (its content
+ * is masked). */
+__device__ __forceinline__ int attn_page(const kv_args &a, int b, int pos, int len) {
+    if (pos >= len) return 0;
+    const int page = a.table[(size_t)b * a.table_stride + (pos >> a.page_shift)];
+    return page < 0 || page >= a.pages ? -1 : page;
+}
+
+__device__ __forceinline__ float attn_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+/* The power of two that brings the largest |q| of a row near 2^10 (products
+ * and sums then stay clear of fp16's and fp32's borders whatever the rows' size),
+ * as its exponent. */
+__device__ __forceinline__ int attn_q_exponent(float amax) {
+    const int e = (int)((__float_as_uint(amax) >> 23) & 255u);
+    return e == 0 || e == 255 ? (amax > 0.0f && e == 0 ? 126 : 0) : min(max(137 - e, -126), 126);
+}
+
+__device__ __forceinline__ attn_h2 attn_pack(float a, float b) {
+    const attn_f2 f = {a, b};
+    return __builtin_convertvector(f, attn_h2);
+}
+
+/* x as one fp16 or the sum of two: hi = x rounded, lo = the rest (exact in fp32) rounded. */
+template <bool TWO>
+__device__ __forceinline__ void attn_split(const float *x, attn_h8 &hi, attn_h8 &lo) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const attn_h2 h = attn_pack(x[i], x[i + 1]);
+        hi[i] = h[0];
+        hi[i + 1] = h[1];
+        if (TWO) {
+            const attn_h2 l = attn_pack(x[i] - (float)h[0], x[i + 1] - (float)h[1]);
+            lo[i] = l[0];
+            lo[i + 1] = l[1];
+        }
+    }
+}
+
+/* Eight int8 codes as fp16, exact: 1024 + (code + 128) is the fp16 number
+ * with the byte in its low bits. */
+__device__ __forceinline__ attn_h8 attn_codes(uint32_t a, uint32_t b) {
+    const uint32_t x = a ^ 0x80808080u, y = b ^ 0x80808080u, c = 0x64646464u;
+    attn_u4 w;
+    w[0] = __builtin_amdgcn_perm(c, x, 0x04010400u);
+    w[1] = __builtin_amdgcn_perm(c, x, 0x04030402u);
+    w[2] = __builtin_amdgcn_perm(c, y, 0x04010400u);
+    w[3] = __builtin_amdgcn_perm(c, y, 0x04030402u);
+    attn_h8 h = __builtin_bit_cast(attn_h8, w);
+    const _Float16 k = (_Float16)1152.0f;
+    return h - attn_h8{k, k, k, k, k, k, k, k};
+}
+
+/* Non-finite values of v: 1 in `odd` there (0 elsewhere) and 0 in v. Returns
+ * whether there is one. */
+__device__ __forceinline__ bool attn_take_odd(attn_h8 &v, attn_h8 &odd) {
+    attn_u4 w = __builtin_bit_cast(attn_u4, v), f;
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const bool lo = (w[i] & 0x7c00u) == 0x7c00u, hi = (w[i] & 0x7c000000u) == 0x7c000000u;
+        any |= lo | hi;
+        f[i] = (lo ? 0x3c00u : 0u) | (hi ? 0x3c000000u : 0u);
+        w[i] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+    }
+    v = __builtin_bit_cast(attn_h8, w);
+    odd = __builtin_bit_cast(attn_h8, f);
+    return any;
+}
+
+/* log2 of a V scale, held inside the range where weights and their sum stay
+ * normal fp32 numbers: 8-bit caches take the running maximum over s +
+ * log2(V scale), so that weight * scale fits fp16 however far the scales are
+ * apart. A NaN stays out of the maximum (fmaxf takes the other). */
+__device__ __forceinline__ float attn_log_scale(float vs) {
+    const float l = __builtin_amdgcn_logf(fabsf(vs));
+    return l < -100.0f ? -100.0f : l > 121.0f ? 121.0f : l;
+}
+
+template <typename T>
+__device__ __forceinline__ void attn_load8(const T *p, float *x) {
+    struct __attribute__((aligned(16))) vec { T v[8]; };
+    const vec w = *(const vec *)p;
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = kv_to_f32(w.v[i]);
+}
+
+template <typename T, int N>
+struct __attribute__((aligned(sizeof(T) * N))) attn_vec {
+    T v[N];
+};
+
+template <typename T>
+__device__ __forceinline__ void attn_store4(T *p, const float *x) {
+    attn_vec<T, 4> o;
+#pragma unroll
+    for (int i = 0; i < 4; i++) o.v[i] = kv_from_f32<T>(x[i]);
+    *(attn_vec<T, 4> *)p = o;
+}
+
+/* A partial result: rows of D sums, then (m, l) of every row. */
+__device__ __forceinline__ size_t attn_partial_floats(int rows, int dim) { return (size_t)rows * (dim + 2); }
+
+#endif
