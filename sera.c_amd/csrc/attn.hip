@@ -1,5 +1,7 @@
 /*
- * attn.hip - attention of packed rows over the paged cache.
+ * attn.hip - attention of packed rows over the paged cache: which kernel takes
+ * a call and how it is cut up, and the kernel that joins contexts split over
+ * workgroups.
  *
  *   s_j = scale * q . k_j,  o = sum_j 2^(s_j' - m) v_j / sum_j 2^(s_j' - m)
  *
@@ -11,115 +13,6 @@
 
 namespace {
 
-/* One wave: the sums of one row over the visible positions in
- * [j0, j1), with plain FMAs. Lane l has the channels E*l .. E*l+E-1. */
-template <int TYPE, int D>
-struct attn_row {
-    static constexpr int E = D / 64;
-    float m, l, o[E];
-
-    __device__ void run(const kv_args &a, const kv_seq &s, int head, const float *q, float c, int p, int window,
-                        int sinks, int j0, int j1) {
-        const int lane = threadIdx.x & 63;
-        m = -3.402823466e38f;
-        l = 0.0f;
-#pragma unroll
-        for (int e = 0; e < E; e++) o[e] = 0.0f;
-        const int mask = (1 << a.page_shift) - 1;
-        const size_t kv_elems = (size_t)D << a.page_shift;
-        const int low = window > 0 ? max(p - window + 1, 0) : 0;
-        for (int j = j0; j < min(j1, p + 1); j++) {
-            if (j < low && j >= sinks) {
-                j = min(low, j1) - 1;
-                continue;
-            }
-            const int page = a.table[(size_t)s.b * a.table_stride + (j >> a.page_shift)];
-            const bool lost = page < 0 || page >= a.pages;
-            const uint8_t *run = a.data + (lost ? 0 : (size_t)page * a.page_bytes) + (size_t)head * a.head_bytes;
-            const int slot = j & mask;
-            const size_t ke = (size_t)slot * D + E * lane;
-            const size_t ve = kv_elems + (size_t)(slot >> 4) * (16 * D) + (size_t)E * lane * 16 + (slot & 15);
-            float acc = 0.0f, vx[E], ks = 1.0f, vs = 1.0f;
-            if (TYPE == (int)SERA_KV_Q8) {
-                const float *sc = (const float *)(run + 2 * kv_elems) + slot;
-                ks = sc[0];
-                vs = sc[(size_t)1 << a.page_shift];
-            }
-#pragma unroll
-            for (int e = 0; e < E; e++) {
-                float kx;
-                if (TYPE == (int)SERA_KV_F16) {
-                    kx = (float)((const _Float16 *)run)[ke + e];
-                    vx[e] = (float)((const _Float16 *)run)[ve + 16 * e];
-                } else {
-                    kx = (float)((const int8_t *)run)[ke + e];
-                    vx[e] = (float)((const int8_t *)run)[ve + 16 * e] * vs;
-                }
-                acc = fmaf(kx, q[e], acc);
-            }
-#pragma unroll
-            for (int x = 32; x >= 1; x >>= 1) acc += __shfl_xor(acc, x, 64);
-            const float t = lost ? __builtin_nanf("") : acc * ks * c;
-            const float mn = fmaxf(m, t), f = exp2f(m - mn), w = exp2f(t - mn);
-            l = fmaf(l, f, w);
-#pragma unroll
-            for (int e = 0; e < E; e++) o[e] = fmaf(o[e], f, w * vx[e]);
-            m = mn;
-        }
-    }
-};
-
-}  // namespace
-
-template <int TYPE, typename T, int D>
-__global__ __launch_bounds__(256) void sera_attn_row_kernel(kv_args a, attn_args t) {
-    constexpr int E = D / 64;
-    const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (unit >= (int64_t)a.rows * t.heads) return;
-    const int row = (int)(unit / t.heads), h = (int)(unit % t.heads), lane = threadIdx.x & 63;
-    int i;
-    const int b = kv_find(a, row, 1, 0, &i);
-    const T *q = (const T *)t.q + row * t.q_stride + (int64_t)h * D + E * lane;
-    T *out = (T *)t.out + row * t.out_stride + (int64_t)h * D + E * lane;
-    if (b < 0) return;
-    const kv_seq s = kv_sequence(a, b);
-    if (i >= s.n) return;
-    attn_row<TYPE, D> r;
-    const int p = s.len - s.n + i;
-    float qx[E];
-#pragma unroll
-    for (int e = 0; e < E; e++) qx[e] = kv_to_f32(q[e]);
-    if (!s.bad) r.run(a, s, h / t.group, qx, t.scale_log2, p, t.window, t.sinks, 0, s.len);
-#pragma unroll
-    for (int e = 0; e < E; e++)
-        out[e] = kv_from_f32<T>(s.bad ? __builtin_nanf("") : p < 0 ? 0.0f : r.o[e] / r.l);
-}
-
-namespace {
-
-template <int TYPE, typename T, int D>
-hipError_t attn_go(const kv_args &a, const attn_args &t, hipStream_t s) {
-    hipLaunchKernelGGL((sera_attn_row_kernel<TYPE, T, D>), dim3((unsigned)(((int64_t)a.rows * t.heads + 3) / 4)),
-                       dim3(256), 0, s, a, t);
-    return hipGetLastError();
-}
-
-template <int TYPE, typename T>
-hipError_t attn_d(int dim, const kv_args &a, const attn_args &t, hipStream_t s) {
-    return dim == 64 ? attn_go<TYPE, T, 64>(a, t, s) : attn_go<TYPE, T, 128>(a, t, s);
-}
-
-template <int TYPE>
-hipError_t attn_t(uint32_t type, int dim, const kv_args &a, const attn_args &t, hipStream_t s) {
-    if (type == SERA_TYPE_F32) return attn_d<TYPE, float>(dim, a, t, s);
-    if (type == SERA_TYPE_F16) return attn_d<TYPE, _Float16>(dim, a, t, s);
-    return attn_d<TYPE, __bf16>(dim, a, t, s);
-}
-
-}  // namespace
-
-namespace {
-
 constexpr int kMaxSplits = 64;
 
 /* The workspace has no window in its size (it is asked for before the call
@@ -127,17 +20,31 @@ constexpr int kMaxSplits = 64;
  * shortens the chunks. */
 attn_plan plan_of(uint32_t cache_type, const kv_args &a, int heads, int cus) {
     attn_plan p = {};
-    const int columns = a.max_new * (heads / a.kv_heads);
-    if ((int64_t)a.max_new * (heads / a.kv_heads) > 32) return p;
-    p.columns = columns <= 16 ? 16 : 32;
-    p.waves = 4;
-    const int tile = sera_attn_few_tile(cache_type);
-    const int tiles = (a.max_kv + tile - 1) / tile;
-    const int64_t units = (int64_t)a.sequences * a.kv_heads;
-    /* Two workgroups per CU are resident at once: more of them only repeat the start. */
-    int64_t want = 2 * (int64_t)cus / units;
-    const int most = (tiles + p.waves - 1) / p.waves;       /* a tile for every wave */
-    if (want > most) want = most;
+    const int group = heads / a.kv_heads;
+    const int64_t columns = (int64_t)a.max_new * group;
+    int64_t want;
+    int least;           /* tiles of a chunk, at least */
+    if (columns <= 32) {
+        p.columns = columns <= 16 ? 16 : 32;
+        p.waves = 4;
+        p.slots = a.sequences;
+        p.shift = cache_type == SERA_KV_Q8 ? 6 : 5;
+        /* Two workgroups per CU are resident at once: more of them only repeat the start. */
+        want = 2 * (int64_t)cus / ((int64_t)a.sequences * a.kv_heads);
+        least = p.waves;                      /* a tile for every wave */
+    } else {
+        p.waves = 8;
+        p.shift = 5;
+        const int64_t all = (int64_t)a.rows * group;
+        p.columns = 256;
+        while (p.columns > 64 && columns <= p.columns / 2) p.columns /= 2;
+        p.slots = (int)(all / p.columns + a.sequences);
+        const int64_t units = (all + p.columns - 1) / p.columns * a.kv_heads;
+        want = cus / units;
+        least = 8;
+    }
+    const int tiles = (a.max_kv + (1 << p.shift) - 1) >> p.shift;
+    if (want > tiles / least) want = tiles / least;
     if (want > kMaxSplits) want = kMaxSplits;
     p.splits = want < 1 ? 1 : (int)want;
     p.chunk = (tiles + p.splits - 1) / p.splits;
@@ -146,9 +53,11 @@ attn_plan plan_of(uint32_t cache_type, const kv_args &a, int heads, int cus) {
 
 }  // namespace
 
-/* Joins the partial sums of a row: a wave for each (row, query head). */
+/* Joins the partial sums of a row: a wave for each (row, query head).
+ * per 0: a unit of partial sums has a sequence's rows (all max_new); otherwise `per` rows of the tile kernel. */
 template <typename T, int D>
-__global__ __launch_bounds__(256) void sera_attn_join_kernel(kv_args a, attn_args t, int splits, int chunk, int shift) {
+__global__ __launch_bounds__(256) void sera_attn_join_kernel(kv_args a, attn_args t, int per, int splits, int chunk,
+                                                             int shift) {
     constexpr int E = D / 64;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int i;
@@ -156,16 +65,19 @@ __global__ __launch_bounds__(256) void sera_attn_join_kernel(kv_args a, attn_arg
     if (b < 0) return;
     const kv_seq s = kv_sequence(a, b);
     if (s.bad || i >= s.n) return;
-    const int part_rows = a.max_new * t.group, p = s.len - s.n + i;
-    const attn_range range = attn_range_of(t, max(s.len - s.n, 0), s.len, shift);
-    const int used = max((range.count + chunk - 1) / chunk, 1);
+    const int first = s.len - s.n, rows = s.n * t.group, unit_rows = per ? per : a.max_new * t.group;
     for (int h = (int)blockIdx.y * 4 + wave; h < t.heads; h += (int)gridDim.y * 4) {
-        const int head = h / t.group, r = i * t.group + h % t.group;
-        const size_t step = attn_partial_floats(part_rows, D);
-        const float *part = t.workspace + ((size_t)b * a.kv_heads + head) * splits * step;
+        const int head = h / t.group, row = i * t.group + h % t.group, unit = row / unit_rows;
+        const int r = row - unit * unit_rows, last = min((unit + 1) * unit_rows, rows) - 1;
+        const attn_range range = attn_range_of(t, max(first + unit * unit_rows / t.group, 0),
+                                               first + last / t.group + 1, shift);
+        const int used = max((range.count + chunk - 1) / chunk, 1);
+        const size_t step = attn_partial_floats(unit_rows, D);
+        const int slot = per ? s.row0 * t.group / per + b + unit : b;
+        const float *part = t.workspace + ((size_t)slot * a.kv_heads + head) * splits * step;
         float m = kAttnLowest, l = 0.0f;
         if (lane < used) {
-            const attn_f2 x = *(const attn_f2 *)(part + lane * step + (size_t)part_rows * D + 2 * r);
+            const attn_f2 x = *(const attn_f2 *)(part + lane * step + (size_t)unit_rows * D + 2 * r);
             m = x[0];
             l = x[1];
         }
@@ -185,7 +97,7 @@ __global__ __launch_bounds__(256) void sera_attn_join_kernel(kv_args a, attn_arg
         }
         attn_vec<T, E> o;
 #pragma unroll
-        for (int e = 0; e < E; e++) o.v[e] = kv_from_f32<T>(p < 0 ? 0.0f : y[e] / l);
+        for (int e = 0; e < E; e++) o.v[e] = kv_from_f32<T>(first + i < 0 ? 0.0f : y[e] / l);
         *(attn_vec<T, E> *)((T *)t.out + (s.row0 + i) * t.out_stride + (int64_t)h * D + E * lane) = o;
     }
 }
@@ -193,12 +105,13 @@ __global__ __launch_bounds__(256) void sera_attn_join_kernel(kv_args a, attn_arg
 namespace {
 
 template <typename T>
-void join_t(int dim, const kv_args &a, const attn_args &t, const attn_plan &p, int shift, hipStream_t s) {
+void join_t(int dim, const kv_args &a, const attn_args &t, const attn_plan &p, hipStream_t s) {
     const dim3 grid((unsigned)a.rows, (unsigned)((t.heads + 3) / 4));
+    const int per = p.columns > 32 ? p.columns : 0;
     if (dim == 64)
-        hipLaunchKernelGGL((sera_attn_join_kernel<T, 64>), grid, dim3(256), 0, s, a, t, p.splits, p.chunk, shift);
+        hipLaunchKernelGGL((sera_attn_join_kernel<T, 64>), grid, dim3(256), 0, s, a, t, per, p.splits, p.chunk, p.shift);
     else
-        hipLaunchKernelGGL((sera_attn_join_kernel<T, 128>), grid, dim3(256), 0, s, a, t, p.splits, p.chunk, shift);
+        hipLaunchKernelGGL((sera_attn_join_kernel<T, 128>), grid, dim3(256), 0, s, a, t, per, p.splits, p.chunk, p.shift);
 }
 
 }  // namespace
@@ -206,29 +119,25 @@ void join_t(int dim, const kv_args &a, const attn_args &t, const attn_plan &p, i
 size_t sera_attn_workspace(uint32_t cache_type, const kv_args &a, int dim, int heads, int cus) {
     const attn_plan p = plan_of(cache_type, a, heads, cus);
     if (p.splits < 2) return 0;
-    return (size_t)a.sequences * a.kv_heads * p.splits * (size_t)a.max_new * (heads / a.kv_heads) * (dim + 2) *
-           sizeof(float);
+    const size_t rows = p.columns > 32 ? (size_t)p.columns : (size_t)a.max_new * (heads / a.kv_heads);
+    return (size_t)p.slots * a.kv_heads * p.splits * rows * (dim + 2) * sizeof(float);
 }
 
 /* Arguments are checked by the caller (sera_attn_runtime.hip). */
 hipError_t sera_launch_attn(uint32_t cache_type, uint32_t type, int dim, const kv_args &a, const attn_args &t,
                             hipStream_t s) {
     attn_plan p = plan_of(cache_type, a, t.heads, t.cus);
-    if (!p.columns)
-        return cache_type == SERA_KV_F16 ? attn_t<(int)SERA_KV_F16>(type, dim, a, t, s)
-                                         : attn_t<(int)SERA_KV_Q8>(type, dim, a, t, s);
-    const int tile = sera_attn_few_tile(cache_type);
     if (t.window > 0) {
-        const int64_t sinks = t.sinks < a.max_kv ? t.sinks : a.max_kv;
+        const int64_t tile = 1 << p.shift, sinks = t.sinks < a.max_kv ? t.sinks : a.max_kv;
         const int64_t tiles = (sinks + tile - 1) / tile + ((int64_t)t.window + a.max_new + tile - 2) / tile + 1;
         const int64_t chunk = (tiles + p.splits - 1) / p.splits;
         if (chunk < p.chunk) p.chunk = (int)chunk;
     }
-    hipError_t e = sera_launch_attn_few(cache_type, type, dim, a, t, p, s);
+    hipError_t e = p.columns > 32 ? sera_launch_attn_tile(cache_type, type, dim, a, t, p, s)
+                                  : sera_launch_attn_few(cache_type, type, dim, a, t, p, s);
     if (e != hipSuccess || p.splits < 2) return e;
-    const int shift = __builtin_ctz((unsigned)tile);
-    if (type == SERA_TYPE_F32) join_t<float>(dim, a, t, p, shift, s);
-    else if (type == SERA_TYPE_F16) join_t<_Float16>(dim, a, t, p, shift, s);
-    else join_t<__bf16>(dim, a, t, p, shift, s);
+    if (type == SERA_TYPE_F32) join_t<float>(dim, a, t, p, s);
+    else if (type == SERA_TYPE_F16) join_t<_Float16>(dim, a, t, p, s);
+    else join_t<__bf16>(dim, a, t, p, s);
     return hipGetLastError();
 }

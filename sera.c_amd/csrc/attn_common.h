@@ -22,16 +22,19 @@ struct attn_args {
 struct attn_plan {
     int columns;         /* rows of q (tokens x heads of a group) that a workgroup has */
     int waves;           /* of a workgroup */
+    int slots;           /* row tiles, of `columns` rows each */
     int splits, chunk;   /* workgroups over a context, tiles of each */
+    int shift;           /* log2 of a tile's tokens */
 };
 
 hipError_t sera_launch_kv_move(bool write, uint32_t cache_type, uint32_t type, int dim, const kv_args &a, void *k,
                                int64_t k_stride, void *v, int64_t v_stride, hipStream_t s);
 size_t sera_attn_workspace(uint32_t cache_type, const kv_args &a, int dim, int heads, int cus);
-int sera_attn_few_tile(uint32_t cache_type);
 hipError_t sera_launch_attn_few(uint32_t cache_type, uint32_t type, int dim, const kv_args &a, const attn_args &t,
                                 const attn_plan &p, hipStream_t s);
 hipError_t sera_launch_attn(uint32_t cache_type, uint32_t type, int dim, const kv_args &a, const attn_args &t,
                             hipStream_t s);
+hipError_t sera_launch_attn_tile(uint32_t cache_type, uint32_t type, int dim, const kv_args &a, const attn_args &t,
+                                 const attn_plan &p, hipStream_t s);
 
 #endif

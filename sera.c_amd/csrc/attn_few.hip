@@ -379,7 +379,6 @@ void few_t(uint32_t type, int dim, const kv_args &a, const attn_args &t, const a
 
 }  // namespace
 
-int sera_attn_few_tile(uint32_t cache_type) { return cache_type == SERA_KV_Q8 ? 64 : 32; }
 
 hipError_t sera_launch_attn_few(uint32_t cache_type, uint32_t type, int dim, const kv_args &a, const attn_args &t,
                                 const attn_plan &p, hipStream_t s) {

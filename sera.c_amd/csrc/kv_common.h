@@ -58,8 +58,10 @@ __device__ __forceinline__ kv_seq kv_sequence(const kv_args &a, int b) {
  * extra * b on. That leaves it floor(n / per) + extra slots or more, in
  * floor(rows / per) + extra * sequences in all. Returns the sequence and the
  * unit in it of slot `slot` (wave-uniform): a 64-way search, one load of
- * row_start per level, a single one up to 64 sequences. */
-__device__ __forceinline__ int kv_find(const kv_args &a, int slot, int per, int extra, int *unit) {
+ * row_start per level, a single one up to 64 sequences. With a scale, a unit
+ * is `per` of rows * scale (which stays below 2^31). */
+__device__ __forceinline__ int kv_find(const kv_args &a, int slot, int per, int extra, int *unit,
+                                       int scale = 1) {
     const int lane = (int)(threadIdx.x & 63);
     int lo = 0, span = a.sequences;          /* the answer is in [lo, lo + span) */
     int base = 0;
@@ -69,7 +71,7 @@ __device__ __forceinline__ int kv_find(const kv_args &a, int slot, int per, int 
         int key = 0x7fffffff;
         if (lane * step < span) {
             const int r = min(max(a.row_start[b], 0), a.rows);
-            key = r / per + extra * b;
+            key = r * scale / per + extra * b;
         }
         const int hits = __popcll(__ballot(key <= slot));
         if (!hits) return -1;                /* unordered row_start */
