@@ -36,8 +36,13 @@ attn_plan plan_of(uint32_t cache_type, const kv_args &a, int heads, int cus) {
         p.waves = 8;
         p.shift = 5;
         const int64_t all = (int64_t)a.rows * group;
+        /* 256 rows a workgroup load each key and value for the most rows, if that leaves every CU one. If not, 128
+         * rows (two groups of waves over the tokens) for contexts up to 8192 tokens, where partial sums cost more
+         * than they give: 16 branches of 256 rows over 1568 tokens take 74 us so and 93 us as 256 rows split in two;
+         * 512 rows x 8 over 32768 tokens 1175 us so and 1031 us split. */
         p.columns = 256;
         while (p.columns > 64 && columns <= p.columns / 2) p.columns /= 2;
+        if (p.columns == 256 && (all + 255) / 256 * a.kv_heads < cus && a.max_kv <= 8192) p.columns = 128;
         p.slots = (int)(all / p.columns + a.sequences);
         const int64_t units = (all + p.columns - 1) / p.columns * a.kv_heads;
         want = cus / units;
@@ -66,6 +71,7 @@ __global__ __launch_bounds__(256) void sera_attn_join_kernel(kv_args a, attn_arg
     const kv_seq s = kv_sequence(a, b);
     if (s.bad || i >= s.n) return;
     const int first = s.len - s.n, rows = s.n * t.group, unit_rows = per ? per : a.max_new * t.group;
+    const int tile0 = per ? attn_first_tile(a, t.group, per, b, s.row0) : 0;
     for (int h = (int)blockIdx.y * 4 + wave; h < t.heads; h += (int)gridDim.y * 4) {
         const int head = h / t.group, row = i * t.group + h % t.group, unit = row / unit_rows;
         const int r = row - unit * unit_rows, last = min((unit + 1) * unit_rows, rows) - 1;
@@ -73,7 +79,7 @@ __global__ __launch_bounds__(256) void sera_attn_join_kernel(kv_args a, attn_arg
                                                first + last / t.group + 1, shift);
         const int used = max((range.count + chunk - 1) / chunk, 1);
         const size_t step = attn_partial_floats(unit_rows, D);
-        const int slot = per ? s.row0 * t.group / per + b + unit : b;
+        const int slot = per ? tile0 + unit : b;
         const float *part = t.workspace + ((size_t)slot * a.kv_heads + head) * splits * step;
         float m = kAttnLowest, l = 0.0f;
         if (lane < used) {

@@ -7,6 +7,7 @@
 #define SERA_ATTN_DEVICE_H
 
 #include "attn_common.h"
+#include "sera_dpp.h"
 
 typedef _Float16 attn_h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 attn_h8 __attribute__((ext_vector_type(8)));
@@ -39,6 +40,21 @@ __device__ __forceinline__ attn_range attn_range_of(const attn_args &t, int p0, 
     r.sink_tiles = t.window > 0 ? min((min(t.sinks, first) + (1 << shift) - 1) >> shift, r.low) : 0;
     r.count = end > 0 ? r.sink_tiles + ((end + (1 << shift) - 1) >> shift) - r.low : 0;
     return r;
+}
+
+/* The tiles v0 <= v < v1 of a range that rows with positions p0 .. p1 (those with p0 < 0 see no tile whole) all see
+ * whole, but for tiles of sinks. */
+struct attn_whole {
+    int v0, v1;
+};
+
+__device__ __forceinline__ attn_whole attn_whole_of(const attn_args &t, const attn_range &r, int p0, int p1, int shift) {
+    attn_whole w;
+    const int past = r.sink_tiles - r.low;       /* v - tile */
+    const int from = t.window > 0 ? max(p1 - t.window + 1, 0) : 0;
+    w.v0 = max(((from + (1 << shift) - 1) >> shift) + past, r.sink_tiles);
+    w.v1 = p0 < 0 ? 0 : ((p0 + 1) >> shift) + past;
+    return w;
 }
 
 /* Whether every row with positions p0 .. p1 sees all positions j .. j+n-1. */
@@ -74,18 +90,21 @@ __device__ __forceinline__ attn_h2 attn_pack(float a, float b) {
     return __builtin_convertvector(f, attn_h2);
 }
 
-/* x as one fp16 or the sum of two: hi = x rounded, lo = the rest (exact in fp32) rounded. */
+/* x as one fp16 or the sum of two: hi = x rounded, lo = the rest (exact in fp32) rounded. The rest is
+ * written as an FMA with a -1 that the compiler does not see through, so it and its rounding become one mixed
+ * instruction (v_fma_mixlo/hi_f16). */
 template <bool TWO>
 __device__ __forceinline__ void attn_split(const float *x, attn_h8 &hi, attn_h8 &lo) {
+    float minus = -1.0f;
+    asm("" : "+s"(minus));
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
         const attn_h2 h = attn_pack(x[i], x[i + 1]);
         hi[i] = h[0];
         hi[i + 1] = h[1];
         if (TWO) {
-            const attn_h2 l = attn_pack(x[i] - (float)h[0], x[i + 1] - (float)h[1]);
-            lo[i] = l[0];
-            lo[i + 1] = l[1];
+            lo[i] = (_Float16)fmaf((float)h[0], minus, x[i]);
+            lo[i + 1] = (_Float16)fmaf((float)h[1], minus, x[i + 1]);
         }
     }
 }
@@ -149,6 +168,64 @@ __device__ __forceinline__ void attn_store4(T *p, const float *x) {
 #pragma unroll
     for (int i = 0; i < 4; i++) o.v[i] = kv_from_f32<T>(x[i]);
     *(attn_vec<T, 4> *)p = o;
+}
+
+/* Row tiles of `per` rows (tokens x heads of a group), numbered through the sequences without gaps: a workgroup
+ * that finds no rows still takes a turn on a compute unit, and where every second one does (sequences of one tile
+ * each, with slots for two), half of the units get nothing but those: 16 sequences of 256 rows took as long as 32. Up to
+ * kAttnCounted sequences are counted, one load of a wave for 64 of them; beyond, kv_find's gaps are few against the rest. */
+constexpr int kAttnCounted = 256;
+
+__device__ __forceinline__ int attn_tiles_of(const kv_args &a, int b, int group, int per) {
+    if (b >= a.sequences) return 0;
+    const int r0 = min(max(a.row_start[b], 0), a.rows), r1 = min(max(a.row_start[b + 1], r0), a.rows);
+    return ((r1 - r0) * group + per - 1) / per;
+}
+
+/* Sequence and tile of it in place `slot`, counted from the last: late rows see most and start first. -1: none.
+ * *place: the tile's number. */
+__device__ __forceinline__ int attn_find_tile(const kv_args &a, int group, int per, int slots, int slot, int *tile,
+                                              int *place) {
+    const int lane = (int)(threadIdx.x & 63);
+    if (a.sequences > kAttnCounted) {
+        *place = slots - 1 - slot;
+        return kv_find(a, *place, per, 1, tile, group);
+    }
+    int n[kAttnCounted / 64], upto[kAttnCounted / 64], total = 0;
+#pragma unroll
+    for (int i = 0; i < kAttnCounted / 64; i++) {
+        n[i] = 64 * i < a.sequences ? attn_tiles_of(a, 64 * i + lane, group, per) : 0;
+        upto[i] = n[i];
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int x = __shfl_up(upto[i], o, 64);
+            upto[i] += lane >= o ? x : 0;
+        }
+        upto[i] += total;
+        total = __builtin_amdgcn_readfirstlane(__shfl(upto[i], 63, 64));
+    }
+    *place = total - 1 - slot;
+    if (*place < 0) return -1;
+    for (int i = 0; i < kAttnCounted / 64; i++) {
+        const unsigned long long past = __ballot(upto[i] > *place);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            *tile = __builtin_amdgcn_readfirstlane(*place - (__shfl(upto[i], l, 64) - __shfl(n[i], l, 64)));
+            return 64 * i + l;
+        }
+    }
+    return -1;
+}
+
+/* The number of sequence b's first tile, row0 its first row. */
+__device__ __forceinline__ int attn_first_tile(const kv_args &a, int group, int per, int b, int row0) {
+    if (a.sequences > kAttnCounted) return row0 * group / per + b;
+    const int lane = (int)(threadIdx.x & 63);
+    int sum = 0;
+    for (int i = lane; i < b; i += 64) sum += attn_tiles_of(a, i, group, per);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    return sum;
 }
 
 /* A partial result: rows of D sums, then (m, l) of every row. */

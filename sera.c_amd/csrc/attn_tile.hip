@@ -22,48 +22,79 @@ namespace {
 
 constexpr int kListed = 512;    /* tiles whose page ids are in LDS at a time */
 
-template <int D, int RG, int KG>
+template <int TYPE, int D, int RG, int KG>
 struct tile_shape {
+    static constexpr bool Q8 = TYPE == (int)SERA_KV_Q8;
     static constexpr int NW = RG * KG, NT = 64 * NW;
-    static constexpr int NSUB = KG > 2 ? KG : 2;     /* 32-token tiles of a step */
+    static constexpr int NSUB = 2;                   /* 32-token tiles of a step */
     static constexpr int UNITS = 32 * D / 8;         /* 16-byte fp16 units of K (and V) in a tile */
     static constexpr int KC = D / 16, NC = D / 32;
     static constexpr int XOR = D / 8 < 16 ? D / 8 - 1 : 15;
+    static constexpr int PER = UNITS * 2 / (Q8 ? 2 : 1);    /* 16-byte loads of a tile, K's then V's */
+    static constexpr int PIECES = NSUB * PER / NT;          /* of a thread and step */
+    /* Buffers of the step whose V is read, of the next one, whose K is read already, and, fp16, of those on
+     * their way; 8-bit codes land in a ring of their own and are converted. */
+    static constexpr int RING = Q8 ? 2 : NW == 8 ? 4 : 3;
+    static constexpr int BUFS = Q8 ? 3 : RING;
+    static constexpr int AHEAD = Q8 ? 2 : RING - 1;         /* steps on their way at first */
+    static constexpr int LOADS = PIECES + (Q8 ? 1 : 0);     /* of a wave and step */
 };
 
 __device__ __forceinline__ int swap_token(int r) { return (r & ~12) | ((r & 4) << 1) | ((r & 8) >> 1); }
 
-template <int D, int RG, int KG>
+template <int TYPE, int D, int RG, int KG>
 struct tile_lds {
-    using S = tile_shape<D, RG, KG>;
-    attn_u4 k[2][S::NSUB][S::UNITS], v[2][S::NSUB][S::UNITS];
-    float scale[2][S::NSUB][3][32];          /* K scale, V scale, log2 of the V scale */
-    int ids[2 * kListed];
+    using S = tile_shape<TYPE, D, RG, KG>;
+    attn_u4 buf[S::BUFS][S::NSUB][2][S::UNITS];                /* K, V */
+    attn_u4 raw[S::Q8 ? S::RING : 1][S::Q8 ? S::PIECES * S::NT : 1];
+    float raw_scale[S::Q8 ? S::RING : 1][S::Q8 ? S::NT : 1];
+    float scale[S::Q8 ? 3 : 1][S::NSUB][3][32];                /* K scale, V scale, log2 of the V scale */
+    alignas(16) int ids[2 * kListed + 4];
+    int lost;                                                  /* a page of those is lost */
+    int any;                                                    /* tiles with values taken out, and which */
+    uint8_t odd[S::Q8 ? 4 : kListed];
 };
+
+typedef const __attribute__((address_space(1))) void attn_global;
+typedef __attribute__((address_space(3))) void attn_local;
+typedef __attribute__((address_space(3))) attn_u4 attn_local_u4;
+
+/* All but the last LEFT of this wave's loads have landed. */
+template <int LEFT>
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory"); }
+
+/* The loads of a step have landed when at most `after` later steps (of LOADS each) are on their way. */
+template <int LOADS>
+__device__ __forceinline__ void wait_step(int after) {
+    if (after >= 2) wait_loads<2 * LOADS>();
+    else if (after == 1) wait_loads<LOADS>();
+    else wait_loads<0>();
+}
+
+__device__ __forceinline__ void barrier_lds() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 }  // namespace
 
 template <int TYPE, typename T, int D, int RG, int KG>
-__global__ __launch_bounds__(64 * RG * KG, 2) void sera_attn_tile_kernel(kv_args a, attn_args t, int slots, int splits,
+__global__ __launch_bounds__(64 * RG * KG, RG * KG / 4) void sera_attn_tile_kernel(kv_args a, attn_args t, int slots, int splits,
                                                                          int chunk) {
-    using S = tile_shape<D, RG, KG>;
-    constexpr bool Q8 = TYPE == (int)SERA_KV_Q8, TWO = sizeof(T) == 4;
+    using S = tile_shape<TYPE, D, RG, KG>;
+    constexpr bool Q8 = S::Q8, TWO = sizeof(T) == 4;
     constexpr int NT = S::NT, NSUB = S::NSUB, UNITS = S::UNITS, KC = S::KC, NC = S::NC, BR = 32 * RG;
-    constexpr int PIECES = NSUB * UNITS * 2 / (Q8 ? 2 : 1) / NT;     /* 16-byte loads of a thread and step */
-    constexpr int ES = Q8 ? 1 : 2;
-    __shared__ tile_lds<D, RG, KG> lds;
+    constexpr int PER = S::PER, PIECES = S::PIECES, ES = Q8 ? 1 : 2;
+    __shared__ tile_lds<TYPE, D, RG, KG> lds;
 
     int slot = (int)(blockIdx.z * gridDim.y + blockIdx.y);
     if (slot >= slots) return;
-    slot = slots - 1 - slot;                          /* the last rows see most: they start first */
     const int head = (int)blockIdx.x % a.kv_heads, split = (int)blockIdx.x / a.kv_heads;
     int unit;
-    const int b = kv_find(a, slot, BR, 1, &unit, t.group);
+    const int b = attn_find_tile(a, t.group, BR, slots, slot, &unit, &slot);
     if (b < 0) return;
     const kv_seq s = kv_sequence(a, b);
     const int rows = s.n * t.group, r0 = unit * BR;
     if (r0 >= rows) return;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 31, half = lane >> 5;
     const int64_t q0 = (int64_t)head * t.group * D;
     if (s.bad) {
         if (split == 0)
@@ -85,7 +116,11 @@ __global__ __launch_bounds__(64 * RG * KG, 2) void sera_attn_tile_kernel(kv_args
     const int w0 = r0 + 32 * rg, row = min(w0 + col, rows - 1), at = row / t.group;
     const int pos = first + at;
     const int pw0 = first + min(w0, rows - 1) / t.group, pw1 = first + min(w0 + 31, rows - 1) / t.group;
-    const bool idle = w0 >= rows;
+    const attn_whole whole = attn_whole_of(t, range, first < 0 ? -1 : pw0, pw1, 5);                /* of this wave */
+    const attn_whole all = attn_whole_of(t, range, max(first + r0 / t.group, 0), end - 1, 5);      /* of all waves */
+    /* Tiles that a row of this wave sees: of those before `last`, sinks and those from `from` on. */
+    const int last = w0 >= rows ? 0 : (pw1 >= 0 ? pw1 >> 5 : -1) + 1 + range.sink_tiles - range.low;
+    const int from = t.window > 0 ? (max(pw0 - t.window + 1, 0) >> 5) + range.sink_tiles - range.low : 0;
 
     attn_h8 qh[KC], ql[TWO ? KC : 1];
     float c;
@@ -100,10 +135,10 @@ __global__ __launch_bounds__(64 * RG * KG, 2) void sera_attn_tile_kernel(kv_args
 #pragma unroll
             for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(x[j]));
         }
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        top = fmaxf(top, xor_partner<32>(top));
         const int e = attn_q_exponent(top);
         const float up = ldexpf(t.scale_log2 < 0.0f ? -1.0f : 1.0f, e);
-        c = ldexpf(fabsf(t.scale_log2), -e);
+        c = fmaxf(ldexpf(fabsf(t.scale_log2), -e), 1.17549435e-38f);   /* not 0: a masked score is -inf * c */
 #pragma unroll
         for (int k = 0; k < KC; k++) {
             float x[8];
@@ -116,7 +151,7 @@ __global__ __launch_bounds__(64 * RG * KG, 2) void sera_attn_tile_kernel(kv_args
         }
     }
 
-    float m = kAttnLowest, l = 0.0f;
+    float m = kAttnLowest, l = 0.0f, l1 = 0.0f;
     attn_f16 o[NC];
 #pragma unroll
     for (int n = 0; n < NC; n++)
@@ -126,205 +161,324 @@ __global__ __launch_bounds__(64 * RG * KG, 2) void sera_attn_tile_kernel(kv_args
     const int mask = (1 << a.page_shift) - 1;
     const size_t kv_bytes = ((size_t)D << a.page_shift) * ES;
     const uint8_t *base = a.data + (size_t)head * a.head_bytes;
-    attn_u4 raw[PIECES];
-    float raw_scale = 0.0f;
-    int g = v0;
+    int g = v0, stop = v0;
+    bool lost = false;
 
-    /* Piece e of this thread of the step at tile v: which tile, K or V, and its place. */
-    auto stage_load = [&](int v, int stop) {
-        constexpr int PER = UNITS * 2 / (Q8 ? 2 : 1);       /* pieces of a tile, K then V */
+    /* The loads of a step are 16-token blocks of UB pieces, tile by tile: K's two, V's two. A wave's 64 pieces of
+     * round e are of block e * (NT / UB) + wave * 64 / UB; a thread has the same place in all its blocks, so one offset
+     * for K's and one for V's. */
+    constexpr int UB = D * ES, STEP_UNITS = NSUB * PER;
+    int off_k, off_v;
+    {
+        constexpr int ROW = D * ES / 16;
+        const int z = tid % UB, row = z / ROW, u = z % ROW;
+        off_k = swap_token(row) * (D * ES) + (Q8 ? u : u ^ (row & S::XOR)) * 16;
+        off_v = Q8 ? z * 16 : (z / 64 * 32 + z % 32) * 32 + z / 32 % 2 * 16;
+    }
+    /* Starts the loads of the step at tile v into ring place r. Past the last tile they read page 0. */
+    auto stage_load = [&](int v, int r) {
+        int id[4];
+        const attn_u4 four = *(const attn_u4 *)&lds.ids[2 * (v - g)];
+#pragma unroll
+        for (int i = 0; i < 4; i++) id[i] = max(__builtin_amdgcn_readfirstlane((int)four[i]), 0);
+        const int wb = wave * 64 / UB;
 #pragma unroll
         for (int e = 0; e < PIECES; e++) {
-            const int x = e * NT + tid, sub = x / PER, y = x % PER;
-            if (v + sub >= stop) continue;
-            const int j = range.tile(v + sub) * 32;
-            const bool is_k = y < PER / 2;
-            const int z = is_k ? y : y - PER / 2;
-            int token, off;
-            if (is_k) {
-                constexpr int ROW = D * ES / 16;
-                const int r = z / ROW;
-                token = swap_token(r);
-                off = (Q8 ? z % ROW : (z % ROW) ^ (r & S::XOR)) * 16;
-            } else if (Q8) {
-                token = z / D * 16;
-                off = z % D * 16;
-            } else {
-                token = z / (2 * D) * 16;
-                off = (z % (2 * D) / 64 * 32 + z % 32) * 32 + z / 32 % 2 * 16;
-            }
-            const int id = max(lds.ids[2 * (v - g + sub) + (token >> 4)], 0);
-            raw[e] = *(const attn_u4 *)(base + (size_t)id * a.page_bytes + (is_k ? 0 : kv_bytes) +
-                                        (size_t)((j + token) & mask) * (D * ES) + off);
+            const int block = e * (NT / UB) + wb, sub = block >> 2, odd = block & 1;
+            const bool is_v = block & 2;
+            const int page = sub ? odd ? id[3] : id[2] : odd ? id[1] : id[0];
+            const uint8_t *p = base + (size_t)page * a.page_bytes + (is_v ? kv_bytes : 0) +
+                               (size_t)((range.tile(v + sub) * 32 + 16 * odd) & mask) * (D * ES);
+            asm("" : "+s"(p));     /* a scalar address and the thread's 32-bit offset, kept apart */
+            attn_u4 *to = (Q8 ? lds.raw[0] : lds.buf[0][0][0]) + r * STEP_UNITS + e * NT + wave * 64;
+            __builtin_amdgcn_global_load_lds((attn_global *)(p + (uint32_t)(is_v ? off_v : off_k)), (attn_local *)to, 16, 0, 0);
         }
-        if (Q8 && tid < NSUB * 64 && v + (tid >> 6) < stop) {
-            const int j = range.tile(v + (tid >> 6)) * 32, token = tid & 31;
-            const int id = max(lds.ids[2 * (v - g + (tid >> 6)) + (token >> 4)], 0);
-            raw_scale = ((const float *)(base + (size_t)id * a.page_bytes + 2 * kv_bytes))
-                [((size_t)(tid >> 5 & 1) << a.page_shift) + ((j + token) & mask)];
+        if (Q8) {      /* both scales of a tile; every wave loads some, those of the first NSUB are used */
+            const int token = lane & 31, sub = wave % NSUB;
+            const int page = token & 16 ? sub ? id[3] : id[1] : sub ? id[2] : id[0];
+            const float *p = (const float *)(base + (size_t)page * a.page_bytes + 2 * kv_bytes) +
+                             ((size_t)half << a.page_shift) + ((range.tile(v + sub) * 32 + token) & mask);
+            __builtin_amdgcn_global_load_lds((attn_global *)p, (attn_local *)&lds.raw_scale[r][wave * 64], 4, 0, 0);
         }
     };
-    auto stage_store = [&](int v, int stop, int buf) {
-        constexpr int PER = UNITS * 2 / (Q8 ? 2 : 1);
+    /* Converts this thread's codes of ring place r into buffer `to`. */
+    auto convert = [&](int r, int to) {
 #pragma unroll
         for (int e = 0; e < PIECES; e++) {
-            const int x = e * NT + tid, sub = x / PER, y = x % PER;
-            if (v + sub >= stop) continue;
-            const bool is_k = y < PER / 2;
-            const int z = is_k ? y : y - PER / 2;
-            attn_u4 *to = is_k ? lds.k[buf][sub] : lds.v[buf][sub];
-            if (!Q8) {
-                to[z] = raw[e];
+            const int x = e * NT + tid, y = x % PER, z = y % (PER / 2);
+            const attn_u4 w = lds.raw[r][x];
+            const attn_u4 x0 = __builtin_bit_cast(attn_u4, attn_codes(w[0], w[1]));
+            const attn_u4 x1 = __builtin_bit_cast(attn_u4, attn_codes(w[2], w[3]));
+            attn_u4 *p = lds.buf[to][x / PER][y >= PER / 2];
+            if (y < PER / 2) {
+                constexpr int ROW = D / 16;
+                const int row = z / ROW, u = 2 * (z % ROW);
+                p[row * (D / 8) + (u ^ (row & S::XOR))] = x0;
+                p[row * (D / 8) + ((u + 1) ^ (row & S::XOR))] = x1;
             } else {
-                const attn_u4 x0 = __builtin_bit_cast(attn_u4, attn_codes(raw[e][0], raw[e][1]));
-                const attn_u4 x1 = __builtin_bit_cast(attn_u4, attn_codes(raw[e][2], raw[e][3]));
-                int u0, u1;
-                if (is_k) {
-                    constexpr int ROW = D / 16;
-                    const int r = z / ROW, u = 2 * (z % ROW);
-                    u0 = r * (D / 8) + (u ^ (r & S::XOR));
-                    u1 = r * (D / 8) + ((u + 1) ^ (r & S::XOR));
-                } else {
-                    u0 = z / D * (2 * D) + z % D / 32 * 64 + z % 32;
-                    u1 = u0 + 32;
-                }
-                to[u0] = x0;
-                to[u1] = x1;
+                const int u = z / D * (2 * D) + z % D / 32 * 64 + z % 32;
+                p[u] = x0;
+                p[u + 32] = x1;
             }
         }
-        if (Q8 && tid < NSUB * 64 && v + (tid >> 6) < stop) {
-            float (*to)[32] = lds.scale[buf][tid >> 6];
-            to[tid >> 5 & 1][tid & 31] = raw_scale;
-            if (tid & 32) to[2][tid & 31] = attn_log_scale(raw_scale);
+        if (wave < NSUB) {
+            const float x = lds.raw_scale[r][tid];
+            float (*p)[32] = lds.scale[to][wave];
+            p[half][col] = x;
+            if (half) p[2][col] = attn_log_scale(x);
         }
     };
 
-    auto compute = [&](int v, int buf, int sub) {
-        const int j = range.tile(v) * 32;
-        if (idle || j > pw1 || (t.window > 0 && j + 31 <= pw0 - t.window && j >= t.sinks)) return;
-        const bool seen = first >= 0 && attn_all_seen(t, j, 32, pw0, pw1);
-        const int id0 = lds.ids[2 * (v - g)], id1 = lds.ids[2 * (v - g) + 1];
-        attn_f16 x;
+    attn_f16 x;                        /* scores: score i is of token 16 * (i / 8) + 8 * half + i % 8 */
+    attn_f4 vs[Q8 ? 4 : 1];            /* and the scales of those tokens' values */
+    float top = kAttnLowest;           /* their largest, as an exponent */
+    const int half8 = 8 * half;
+
+    /* Fragment i of the products: V's of this tile (i < 2 NC), then K's of the next one. K's units are xored in
+     * address bits that the fragment's number has to itself, so one address serves all. */
+    constexpr uint32_t TILE_BYTES = UNITS * 16;
+    const uint32_t lds_at = (uint32_t)(uintptr_t)(attn_local *)lds.buf;
+    const uint32_t k_at = lds_at + col * (D * 2) + ((half ^ (col & S::XOR)) << 4), v_at = lds_at + TILE_BYTES + lane * 16;
+    auto fragment = [&](int i, uint32_t k_tile, uint32_t v_tile) {
+        const uint32_t at = i < 2 * NC ? v_at + v_tile + (uint32_t)i * 1024u
+                                       : (k_at + k_tile) ^ (uint32_t)((i - 2 * NC) << 5);
+        return __builtin_bit_cast(attn_h8, *(const attn_local_u4 *)(uintptr_t)at);
+    };
+    /* The scores x are complete: 8-bit keys' scales, and the largest. */
+    auto finish = [&](int buf, int sub) {
+        top = kAttnLowest;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int at = 16 * (i / 2) + half8 + 4 * (i % 2);
+            attn_f4 ks, lv;
+            if (Q8) {
+                ks = *(const attn_f4 *)&lds.scale[buf][sub][0][at];
+                lv = *(const attn_f4 *)&lds.scale[buf][sub][2][at];
+            }
+#pragma unroll
+            for (int z = 0; z < 4; z++) {
+                if (Q8) x[4 * i + z] *= ks[z];
+                top = fmaxf(top, Q8 ? fmaf(x[4 * i + z], c, lv[z]) : x[4 * i + z]);
+            }
+            if (Q8 && i == 1) __builtin_amdgcn_sched_barrier(0);      /* registers: half of the scales at a time */
+        }
+        if (!Q8) top *= c;
+    };
+    auto scores = [&](int buf, int sub) {
 #pragma unroll
         for (int i = 0; i < 16; i++) x[i] = 0.0f;
 #pragma unroll
         for (int k = 0; k < KC; k++) {
-            const attn_h8 kf = __builtin_bit_cast(attn_h8,
-                lds.k[buf][sub][col * (D / 8) + ((2 * k + half) ^ (col & S::XOR))]);
-            x = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh[k], x, 0, 0, 0);
-            if (TWO) x = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[TWO ? k : 0], x, 0, 0, 0);
+            const attn_h8 f = fragment(2 * NC + k, (buf * NSUB + sub) * 2 * TILE_BYTES, 0);
+            x = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, qh[k], x, 0, 0, 0);
+            if (TWO) x = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, ql[TWO ? k : 0], x, 0, 0, 0);
         }
-        /* Score i belongs to token 16 * (i / 8) + 8 * half + i % 8. */
-        attn_f4 vs[Q8 ? 4 : 1];
-        float top = kAttnLowest;
-        if (Q8) {
-            const float (*sc)[32] = lds.scale[buf][sub];
+        finish(buf, sub);
+    };
+    /* Mask of tile v, and the running maximum with it. False: no row of this wave sees any of it. */
+    auto look = [&](int v, int buf, int sub) {
+        if (v >= last || (v < from && range.tile(v) * 32 >= t.sinks)) return false;
+        if (Q8)
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const attn_f4 ks = *(const attn_f4 *)&sc[0][16 * (i / 8) + 8 * half + i % 8];
-                vs[i / 4] = *(const attn_f4 *)&sc[1][16 * (i / 8) + 8 * half + i % 8];
+            for (int i = 0; i < 4; i++) vs[i] = *(const attn_f4 *)&lds.scale[buf][sub][1][16 * (i / 2) + half8 + 4 * (i % 2)];
+        if (lost || v < whole.v0 || v >= whole.v1) {
+            const int j = range.tile(v) * 32;
+            const int id0 = lds.ids[2 * (v - g)], id1 = lds.ids[2 * (v - g) + 1];
+            top = kAttnLowest;
 #pragma unroll
-                for (int y = 0; y < 4; y++) x[i + y] *= ks[y] * c;
+            for (int i = 0; i < 16; i++) {
+                const int at = 16 * (i / 8) + half8 + i % 8;
+                const bool sees = attn_sees(t, pos, j + at);
+                x[i] = !sees ? -INFINITY : (i < 8 ? id0 : id1) < 0 ? __builtin_nanf("") : x[i];
+                top = fmaxf(top, Q8 ? fmaf(x[i], c, lds.scale[Q8 ? buf : 0][sub][2][at]) : x[i] * c);
+                if (Q8) vs[i / 4][i % 4] = sees ? vs[i / 4][i % 4] : 0.0f;
+                if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; i++) x[i] *= c;
         }
-        if ((id0 | id1) < 0)
-#pragma unroll
-            for (int i = 0; i < 16; i++) x[i] = (i < 8 ? id0 : id1) < 0 ? __builtin_nanf("") : x[i];
-        if (!seen)
-#pragma unroll
-            for (int i = 0; i < 16; i++)
-                x[i] = attn_sees(t, pos, j + 16 * (i / 8) + 8 * half + i % 8) ? x[i] : -INFINITY;
-        if (Q8) {
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const attn_f4 lv = *(const attn_f4 *)&lds.scale[buf][sub][2][16 * (i / 8) + 8 * half + i % 8];
-#pragma unroll
-                for (int y = 0; y < 4; y++) top = fmaxf(top, x[i + y] + lv[y]);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; i++) top = fmaxf(top, x[i]);
-        }
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        top = fmaxf(top, xor_partner<32>(top));
         if (__ballot(top > m + kAttnLag)) {
             const float f = attn_exp2(m - fmaxf(top, m));
             m = fmaxf(top, m);
             l *= f;
+            l1 *= f;
 #pragma unroll
             for (int n = 0; n < NC; n++) o[n] *= f;
         }
-        const float shift = m - kAttnBias;
-        attn_h8 ph[2], pl[2];
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-            float w[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                w[i] = attn_exp2(x[8 * k + i] - shift);
-                l += w[i];
-                if (Q8) {
-                    w[i] *= vs[Q8 ? 2 * k + i / 4 : 0][i % 4];
-                    if (!seen) w[i] = attn_sees(t, pos, j + 16 * k + 8 * half + i) ? w[i] : 0.0f;
-                }
+        return true;
+    };
+    /* The weights of tile (buf, sub) from its scores x, its sums, and the scores of the next tile (nb, ns) into x: in
+     * stages of one fragment's MFMAs each, in a fixed order, with the fragments read DEPTH stages ahead. The second
+     * half of the weights is made under the MFMAs of the first. */
+    auto tile = [&](int buf, int sub, int nb, int ns) {
+        constexpr int DEPTH = 2, STAGES = KC + 2 * NC;
+        const float shift = kAttnBias - m;
+        float minus = -1.0f;
+        asm("" : "+s"(minus));
+        const uint32_t kt = (nb * NSUB + ns) * 2 * TILE_BYTES, vt = (buf * NSUB + sub) * 2 * TILE_BYTES;
+        attn_h8 f[DEPTH + 1], ph[2], pl[2];
+        auto weigh = [&](int e) {
+            float a0 = attn_exp2(fmaf(x[e], c, shift)), a1 = attn_exp2(fmaf(x[e + 1], c, shift));
+            l += a0;
+            l1 += a1;
+            if (Q8) {
+                a0 *= vs[Q8 ? e / 4 : 0][e % 4];
+                a1 *= vs[Q8 ? e / 4 : 0][e % 4 + 1];
             }
-            attn_split<TWO>(w, ph[k], pl[k]);
+            const attn_h2 h = attn_pack(a0, a1);
+            ph[e / 8][e % 8] = h[0];
+            ph[e / 8][e % 8 + 1] = h[1];
+            if (TWO) {
+                pl[e / 8][e % 8] = (_Float16)fmaf((float)h[0], minus, a0);
+                pl[e / 8][e % 8 + 1] = (_Float16)fmaf((float)h[1], minus, a1);
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < DEPTH; i++) f[i] = fragment(i, kt, vt);
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) weigh(e);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int st = 0; st < STAGES; st++) {
+            const attn_h8 w = f[st % (DEPTH + 1)];
+            if (st + DEPTH < STAGES) f[(st + DEPTH) % (DEPTH + 1)] = fragment(st + DEPTH, kt, vt);
+            const int n = st % NC, k = st < 2 * NC ? st / NC : st - 2 * NC;
+            if (st < 2 * NC) {
+                o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, ph[k], o[n], 0, 0, 0);
+                if (TWO) o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, pl[k], o[n], 0, 0, 0);
+            } else {
+                if (k == 0)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) x[i] = 0.0f;
+                x = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, qh[k], x, 0, 0, 0);
+                if (TWO) x = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, ql[TWO ? k : 0], x, 0, 0, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (st < NC) {
+#pragma unroll
+                for (int e = 8 + st * (8 / NC); e < 8 + (st + 1) * (8 / NC); e += 2) weigh(e);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
+        finish(nb, ns);
+    };
+
+    /* fp16 values that are not finite, in tiles that some rows of the workgroup see and others do not: a product
+     * would carry them into rows that do not see them (0 * inf). They are taken out of the step's buffer, each
+     * thread looking at what it loaded, and their tiles marked... */
+    auto take_out = [&](int v, int buf) {
+        if (Q8 || (v >= all.v0 && v + NSUB <= all.v1)) return;
 #pragma unroll
-        for (int n = 0; n < NC; n++)
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                attn_h8 vf = __builtin_bit_cast(attn_h8, lds.v[buf][sub][k * 2 * D + n * 64 + lane]);
-                if (!Q8 && !seen) {
-                    /* fp16 values that are not finite: rows that see them get NaN in their channels, others nothing */
-                    attn_h8 odd;
-                    if (__ballot(attn_take_odd(vf, odd))) {
-                        attn_h8 sees;
-#pragma unroll
-                        for (int i = 0; i < 8; i++)
-                            sees[i] = attn_sees(t, pos, j + 16 * k + 8 * half + i) ? (_Float16)1.0f : (_Float16)0.0f;
-                        attn_f16 hit;
-#pragma unroll
-                        for (int i = 0; i < 16; i++) hit[i] = 0.0f;
-                        hit = __builtin_amdgcn_mfma_f32_32x32x16_f16(odd, sees, hit, 0, 0, 0);
-#pragma unroll
-                        for (int i = 0; i < 16; i++) o[n][i] = hit[i] > 0.0f ? __builtin_nanf("") : o[n][i];
-                    }
-                }
-                o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, ph[k], o[n], 0, 0, 0);
-                if (TWO) o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl[k], o[n], 0, 0, 0);
+        for (int e = 0; e < PIECES; e++) {
+            const int x = e * NT + wave * 64, y = x % PER, tile = v + x / PER;
+            if (y < PER / 2 || tile >= stop || (tile >= all.v0 && tile < all.v1)) continue;
+            int here = lane;
+            asm volatile("" : "+v"(here));
+            attn_u4 *p = &lds.buf[buf][x / PER][1][y % (PER / 2) + here];
+            attn_h8 w = __builtin_bit_cast(attn_h8, *p), bad;
+            if (attn_take_odd(w, bad)) {
+                *p = __builtin_bit_cast(attn_u4, w);
+                lds.odd[tile - g] = 1;
+                lds.any = 1;
             }
+        }
+    };
+    /* ... and in the end the rows that see one get NaN in its channel. */
+    auto put_back = [&](int v) {
+        int col = lane & 31, half = lane >> 5;
+        asm volatile("" : "+v"(col), "+v"(half));       /* nothing of this is kept through the loop */
+        const int j = range.tile(v) * 32;
+#pragma unroll 1
+        for (int k = 0; k < 2; k++) {
+            const int id = max(__builtin_amdgcn_readfirstlane(lds.ids[2 * (v - g) + k]), 0);
+            const uint8_t *p = base + (size_t)id * a.page_bytes + kv_bytes +
+                               (size_t)((j + 16 * k) & mask) * (D * ES) + col * 32 + half * 16;
+            attn_h8 sees;
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                sees[i] = attn_sees(t, pos, j + 16 * k + 8 * half + i) ? (_Float16)1.0f : (_Float16)0.0f;
+#pragma unroll
+            for (int n = 0; n < NC; n++) {
+                attn_h8 w = *(const attn_h8 *)(p + n * 1024), bad;
+                attn_take_odd(w, bad);
+                attn_f16 hit;
+#pragma unroll
+                for (int i = 0; i < 16; i++) hit[i] = 0.0f;
+                hit = __builtin_amdgcn_mfma_f32_32x32x16_f16(bad, sees, hit, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[n][i] = hit[i] > 0.0f ? __builtin_nanf("") : o[n][i];
+                __builtin_amdgcn_sched_barrier(0);         /* few registers: this must not spill what the loop holds */
+            }
+        }
     };
 
     for (; g < v1; g += kListed) {
-        const int stop = min(v1, g + kListed);
-        __syncthreads();
-        for (int e = tid; e < 2 * (stop - g); e += NT)
-            lds.ids[e] = attn_page(a, b, range.tile(g + (e >> 1)) * 32 + 16 * (e & 1), s.len);
-        __syncthreads();
-        stage_load(g, stop);
-        stage_store(g, stop, 0);
-        int buf = 0;
-        for (int v = g; v < stop; v += NSUB) {
-            __syncthreads();
-            if (v + NSUB < stop) stage_load(v + NSUB, stop);
-#pragma unroll
-            for (int sub = 0; sub < NSUB; sub += KG)
-                if (v + sub + kg < stop) compute(v + sub + kg, buf, sub + kg);
-            if (v + NSUB < stop) stage_store(v + NSUB, stop, buf ^ 1);
-            buf ^= 1;
+        stop = min(v1, g + kListed);
+        const int steps = (stop - g + NSUB - 1) / NSUB;
+        barrier_lds();
+        if (tid == 0) lds.lost = 0;
+        barrier_lds();
+        for (int e = tid; e < 2 * (stop - g) + 4; e += NT) {
+            const int id = e < 2 * (stop - g) ? attn_page(a, b, range.tile(g + (e >> 1)) * 32 + 16 * (e & 1), s.len) : 0;
+            lds.ids[e] = id;
+            if (id < 0) lds.lost = 1;
         }
+        if (!Q8) {
+            for (int e = tid; e < stop - g; e += NT) lds.odd[e] = 0;
+            if (tid == 0) lds.any = 0;
+        }
+        __syncthreads();
+        constexpr int AHEAD = S::AHEAD;
+        lost = __builtin_amdgcn_readfirstlane(lds.lost) != 0;
+        for (int st = 0; st < min(AHEAD, steps); st++) stage_load(g + st * NSUB, st);
+        wait_step<S::LOADS>(min(AHEAD, steps) - 1);
+        if (Q8) convert(0, 0);
+        else take_out(g, 0);
+        barrier_lds();
+        if (Q8 && AHEAD < steps) stage_load(g + AHEAD * NSUB, 0);
+        if (g + kg < stop) scores(0, kg);
+        /* The scores of the next tile run beside the weights of this one. */
+        int buf = 0, r = 0;           /* this step's buffer; its place in the ring of codes */
+        for (int st = 0; st < steps; st++) {
+            const int next = buf == S::BUFS - 1 ? 0 : buf + 1;
+#pragma unroll
+            for (int sub = 0; sub < NSUB; sub += KG) {
+                const int v = g + st * NSUB + sub + kg;
+                const bool live = v < stop && look(v, buf, sub + kg);
+                const bool turn = sub + KG >= NSUB;
+                if (turn && st + 1 < steps) {
+                    /* This step's scores are all taken: on to the next step's buffer. */
+                    if (!Q8) {
+                        wait_step<S::LOADS>(min(steps - 2 - st, AHEAD - 2));
+                        take_out(g + (st + 1) * NSUB, next);
+                    } else {
+                        r ^= 1;
+                        wait_step<S::LOADS>(min(steps - 2 - st, AHEAD - 1));
+                        convert(r, next);
+                    }
+                    barrier_lds();
+                    if (!Q8 && st + AHEAD < steps) stage_load(g + (st + AHEAD) * NSUB, buf == 0 ? S::BUFS - 1 : buf - 1);
+                    if (Q8 && st + 1 + AHEAD < steps) stage_load(g + (st + 1 + AHEAD) * NSUB, r);
+                }
+                /* Past the last tile these are scores of whatever the buffer holds, used by nothing. */
+                const int nb = turn ? next : buf, ns = turn ? kg : sub + KG + kg;
+                if (live) tile(buf, sub + kg, nb, ns);
+                else scores(nb, ns);
+            }
+            buf = next;
+        }
+        if (!Q8 && lds.any)
+            for (int v = g; v < stop; v++)
+                if (lds.odd[v - g]) put_back(v);
     }
 
-    l += __shfl_xor(l, 32, 64);
+    l += l1;
+    l += xor_partner<32>(l);
     /* Join the token groups: the upper half of them hands its sums over, lane by lane. */
 #pragma unroll
     for (int h = KG / 2; h >= 1; h >>= 1) {
-        attn_f4 *box = (attn_f4 *)lds.k + ((size_t)rg + RG * (kg % h)) * (64 * NC * 4);
+        attn_f4 *box = (attn_f4 *)lds.buf + ((size_t)rg + RG * (kg % h)) * (64 * NC * 4);
         float *mlbox = (float *)lds.ids + 128 * (rg + RG * (kg % h));
-        static_assert(sizeof(attn_f4) * RG * (KG / 2) * 64 * NC * 4 <= sizeof(lds.k) + sizeof(lds.v), "join space");
+        static_assert(sizeof(attn_f4) * RG * (KG / 2) * 64 * NC * 4 <= sizeof(lds.buf), "join space");
         static_assert(sizeof(float) * RG * (KG / 2) * 128 <= sizeof(lds.ids), "join space");
         __syncthreads();
         if (kg >= h && kg < 2 * h) {
@@ -393,7 +547,7 @@ template <int TYPE, typename T, int D>
 void tile_rg(const kv_args &a, const attn_args &t, const attn_plan &p, hipStream_t s) {
     if (p.columns == 256) tile_go<TYPE, T, D, 8, 1>(a, t, p, s);
     else if (p.columns == 128) tile_go<TYPE, T, D, 4, 2>(a, t, p, s);
-    else tile_go<TYPE, T, D, 2, 4>(a, t, p, s);
+    else tile_go<TYPE, T, D, 2, 2>(a, t, p, s);
 }
 
 template <int TYPE, typename T>

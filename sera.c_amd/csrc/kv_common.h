@@ -80,8 +80,8 @@ __device__ __forceinline__ int kv_find(const kv_args &a, int slot, int per, int 
         if (step == 1) break;
         span = min(step, a.sequences - lo);
     }
-    *unit = slot - base;
-    if (slot < base) return -1;
+    *unit = __builtin_amdgcn_readfirstlane(slot - base);
+    if (*unit < 0) return -1;
     return __builtin_amdgcn_readfirstlane(lo);
 }
 
