@@ -4,12 +4,11 @@
  * stands for.
  *
  * Both move data once and are bound by memory (or, for a few tokens, by the
- * launch). A wave takes one kv head of one 16-token block of a sequence,
- * lane l the channels E*l .. E*l+E-1 (E = head_dim / 64) of all 16 tokens:
- * row accesses are whole rows across the wave, and a lane ends with 16
- * tokens of its own channels, which is the order V is stored in, so nothing
- * passes through LDS. The block's loads are independent (up to 32 in flight
- * per lane).
+ * launch and three dependent loads: sequence, page, data). A wave takes K or V
+ * of one kv head of one 16-token block of a sequence. Rows are accessed in 16-byte
+ * pieces (D / VEC lanes to a row, several rows to an access); K's place in the cache is
+ * the same order. V's is not: 16 tokens of a channel lie side by side, so a wave
+ * turns its block in LDS of its own, in dwords that are unpacked by byte permutes.
  *
  * 8-bit quantizer: scale d = max|x| / 127 over the vector (an exact maximum,
  * one IEEE division), code = x / d rounded half to even, as the exact
@@ -19,6 +18,7 @@
  * with d / 2 puts q0 right, without a division per element.
  */
 #include "attn_common.h"
+#include "sera_dpp.h"
 #include "sera_launch.h"
 
 #pragma clang fp contract(off)
@@ -43,37 +43,47 @@ __device__ __forceinline__ kv_unit kv_unit_of(const kv_seq &s, int unit) {
     return u;
 }
 
-__device__ __forceinline__ float kv_wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    return v;
+/* N consecutive elements. */
+template <typename T, int N>
+struct __attribute__((aligned(sizeof(T) * N))) kv_vec {
+    T v[N];
+};
+
+/* How a wave accesses 16 rows of D elements, 16 bytes of T at a time. */
+template <typename T, int D>
+struct kv_rows {
+    static constexpr int VEC = 16 / (int)sizeof(T), LANES = D / VEC, ROWS = 64 / LANES, N = kBlock / ROWS;
+    /* token and first channel of access i of a lane */
+    static __device__ __forceinline__ int token(int i, int lane) { return i * ROWS + lane / LANES; }
+    static __device__ __forceinline__ int channel(int lane) { return lane % LANES * VEC; }
+};
+
+/* The largest of m over the lanes that share a row. */
+template <int LANES>
+__device__ __forceinline__ float kv_row_max(float m) {
+    m = fmaxf(m, xor_partner<1>(m));
+    m = fmaxf(m, xor_partner<2>(m));
+    m = fmaxf(m, xor_partner<4>(m));
+    if constexpr (LANES >= 16) m = fmaxf(m, xor_partner<8>(m));
+    if constexpr (LANES >= 32) m = fmaxf(m, xor_partner<16>(m));
+    return m;
 }
 
-/* E consecutive elements of a row. */
-template <typename T, int E>
-struct kv_vec {
-    T v[E];
-} __attribute__((aligned(sizeof(T) * E)));
-
-/* Scale of a vector spread over the wave (NaN if an element is not finite),
- * and the factors for its codes: `up` lifts vectors so small that 1 / d
- * would overflow (both factors are powers of two, exact). */
+/* Scale of a row (NaN if an element is not finite), and the factors for its
+ * codes: `up` lifts vectors so small that 1 / d would overflow (both factors
+ * are powers of two, exact). */
 struct kv_scale {
     float d, up, du, inv, half;
 };
 
-template <int E>
+template <int VEC, int LANES>
 __device__ __forceinline__ kv_scale kv_vector_scale(const float *x) {
     float m = 0.0f;
-    bool odd = false;
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-        m = fmaxf(m, fabsf(x[e]));
-        odd |= !(fabsf(x[e]) <= 3.402823466e38f);
-    }
-    m = kv_wave_max(m);
+    for (int e = 0; e < VEC; e++) m = fmaxf(m, x[e] == x[e] ? fabsf(x[e]) : INFINITY);
+    m = kv_row_max<LANES>(m);
     kv_scale s;
-    s.d = __ballot(odd) ? __builtin_nanf("") : m / 127.0f;
+    s.d = m <= 3.402823466e38f ? m / 127.0f : __builtin_nanf("");
     s.up = m < 0x1p-60f ? 0x1p64f : 1.0f;
     s.du = s.d * s.up;
     s.inv = 1.0f / s.du;
@@ -97,104 +107,103 @@ __device__ __forceinline__ int kv_code(float x, const kv_scale &s) {
 template <int TYPE, typename T, int D>
 __global__ __launch_bounds__(256) void sera_kv_write_kernel(kv_args a, const T *__restrict__ k, int64_t k_stride,
                                                             const T *__restrict__ v, int64_t v_stride) {
-    constexpr int E = D / 64;
-    const int lane = threadIdx.x & 63;
-    const int head = (int)blockIdx.y * 4 + (int)(threadIdx.x >> 6);
+    using R = kv_rows<T, D>;
+    constexpr bool Q8 = TYPE == (int)SERA_KV_Q8;
+    constexpr int VEC = R::VEC, N = R::N, ES = Q8 ? 1 : 2, ROW = D * ES / 4;      /* dwords of a row in LDS */
+    __shared__ uint32_t turn[4][kBlock][ROW];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int item = (int)blockIdx.y * 4 + wave, head = item >> 1;
+    const bool is_v = item & 1;
     int unit;
-    const int b = kv_find(a, (int)blockIdx.x, kBlock, 2, &unit);
-    if (b < 0 || head >= a.kv_heads) return;
-    const kv_seq s = kv_sequence(a, b);
-    if (s.bad) return;
+    const kv_seq s = kv_find_sequence(a, (int)blockIdx.x, kBlock, 2, &unit);
+    if (s.b < 0 || head >= a.kv_heads || s.bad) return;
     const kv_unit u = kv_unit_of(s, unit);
     if (u.t0 >= u.t1) return;
-    const int page = a.table[(size_t)b * a.table_stride + (u.pos0 >> a.page_shift)];
+    const int page = a.table[(size_t)s.b * a.table_stride + (u.pos0 >> a.page_shift)];
     if (page < 0 || page >= a.pages) return;
+    const size_t kv_bytes = ((size_t)D << a.page_shift) * ES;
     uint8_t *run = a.data + (size_t)page * a.page_bytes + (size_t)head * a.head_bytes;
     const int slot = u.pos0 & ((1 << a.page_shift) - 1);
-    const size_t kv_elems = (size_t)D << a.page_shift;
+    const int64_t stride = is_v ? v_stride : k_stride;
     /* row of the block's token 0; only tokens t0 .. t1-1 have one */
     const int64_t row = (int64_t)s.row0 + u.pos0 - (s.len - s.n);
-    const int d0 = E * lane;
-    const T *kp = k + row * k_stride + (int64_t)head * D + d0, *vp = v + row * v_stride + (int64_t)head * D + d0;
-    const bool full = u.t0 == 0 && u.t1 == kBlock;
+    const int d0 = R::channel(lane);
+    const T *from = (is_v ? v : k) + row * stride + (int64_t)head * D + d0;
+    uint8_t *to = run + (is_v ? kv_bytes : 0) + (size_t)slot * (D * ES);
 
-    kv_vec<T, E> kx[kBlock], vx[kBlock];
+    kv_vec<T, VEC> in[N];
 #pragma unroll
-    for (int t = 0; t < kBlock; t++)
-        if (t >= u.t0 && t < u.t1) {
-            kx[t] = *(const kv_vec<T, E> *)(kp + t * k_stride);
-            vx[t] = *(const kv_vec<T, E> *)(vp + t * v_stride);
+    for (int i = 0; i < N; i++) {
+        const int t = R::token(i, lane);
+#pragma unroll
+        for (int e = 0; e < VEC; e++) in[i].v[e] = (T)0.0f;
+        if (t >= u.t0 && t < u.t1) in[i] = *(const kv_vec<T, VEC> *)(from + t * stride);
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const int t = R::token(i, lane);
+        const bool new_row = t >= u.t0 && t < u.t1;
+        float x[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; e++) x[e] = kv_to_f32(in[i].v[e]);
+        if constexpr (Q8) {
+            const kv_scale sc = kv_vector_scale<VEC, R::LANES>(x);
+            kv_vec<int8_t, VEC> o;
+#pragma unroll
+            for (int e = 0; e < VEC; e++) o.v[e] = (int8_t)kv_code(x[e], sc);
+            if (new_row && d0 == 0)
+                ((float *)(run + 2 * kv_bytes))[((size_t)is_v << a.page_shift) + slot + t] = sc.d;
+            if (is_v) *(kv_vec<int8_t, VEC> *)((int8_t *)turn[wave][t] + d0) = o;
+            else if (new_row) *(kv_vec<int8_t, VEC> *)(to + t * D + d0) = o;
         } else {
+            kv_vec<_Float16, VEC> o;
 #pragma unroll
-            for (int e = 0; e < E; e++) kx[t].v[e] = vx[t].v[e] = (T)0.0f;
+            for (int e = 0; e < VEC; e++) o.v[e] = (_Float16)x[e];
+            if (is_v) *(kv_vec<_Float16, VEC> *)((_Float16 *)turn[wave][t] + d0) = o;
+            else if (new_row) *(kv_vec<_Float16, VEC> *)(to + (t * D + d0) * 2) = o;
         }
-
-    if (TYPE == (int)SERA_KV_F16) {
-        _Float16 *ko = (_Float16 *)run + (size_t)slot * D + d0;
-        _Float16 *vo = (_Float16 *)run + kv_elems + (size_t)slot * D + (size_t)d0 * 16;
-#pragma unroll
-        for (int t = 0; t < kBlock; t++)
-            if (t >= u.t0 && t < u.t1) {
-                kv_vec<_Float16, E> o;
-#pragma unroll
-                for (int e = 0; e < E; e++) o.v[e] = (_Float16)kv_to_f32(kx[t].v[e]);
-                *(kv_vec<_Float16, E> *)(ko + t * D) = o;
+    }
+    if (!is_v) return;
+    asm volatile("" ::: "memory");          /* the wave's own LDS, which it accesses in order */
+    if (u.t0 > 0 || u.t1 < kBlock) {        /* some of the block's tokens: one element at a time */
+        for (int t = u.t0; t < u.t1; t++)
+            for (int d = lane; d < D; d += 64) {
+                if (Q8) to[16 * d + t] = ((const uint8_t *)turn[wave][t])[d];
+                else ((uint16_t *)to)[16 * d + t] = ((const uint16_t *)turn[wave][t])[d];
             }
+        return;
+    }
+    if constexpr (Q8) {                     /* dword column c: channels 4c .. 4c+3; a lane takes D / 64 of them */
+        const int c = lane * (D / 64) / 4, j = lane * (D / 64) % 4;
+        uint32_t w[kBlock];
 #pragma unroll
-        for (int e = 0; e < E; e++) {
-            if (full) {
+        for (int t = 0; t < kBlock; t++) w[t] = turn[wave][t][c];
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    kv_vec<_Float16, 8> o;
+        for (int e = 0; e < D / 64; e++) {
+            kv_vec<uint32_t, 4> o;
+            const uint32_t pick = 0x0c0c0400u + (uint32_t)(j + e) * 0x0101u;       /* byte j + e of two dwords */
 #pragma unroll
-                    for (int t = 0; t < 8; t++) o.v[t] = (_Float16)kv_to_f32(vx[8 * h + t].v[e]);
-                    *(kv_vec<_Float16, 8> *)(vo + 16 * e + 8 * h) = o;
-                }
-            } else {
-#pragma unroll
-                for (int t = 0; t < kBlock; t++)
-                    if (t >= u.t0 && t < u.t1) vo[16 * e + t] = (_Float16)kv_to_f32(vx[t].v[e]);
-            }
+            for (int q = 0; q < 4; q++)
+                o.v[q] = __builtin_amdgcn_perm(w[4 * q + 1], w[4 * q], pick) |
+                         __builtin_amdgcn_perm(w[4 * q + 3], w[4 * q + 2], pick) << 16;
+            *(kv_vec<uint32_t, 4> *)(to + 16 * (lane * (D / 64) + e)) = o;
         }
-    } else {
-        int8_t *ko = (int8_t *)run + (size_t)slot * D + d0;
-        int8_t *vo = (int8_t *)run + kv_elems + (size_t)slot * D + (size_t)d0 * 16;
-        float *ks = (float *)(run + 2 * kv_elems) + slot, *vs = ks + ((size_t)1 << a.page_shift);
-        kv_vec<int8_t, 16> vq[E];
+    } else {                                /* dword column c: channels 2c, 2c+1; a lane takes both (D 128) or half of the tokens */
+        constexpr int TOKENS = D / 8;
+        const int c = lane % (D / 2), t0 = lane / (D / 2) * TOKENS;
+        uint32_t w[TOKENS];
 #pragma unroll
-        for (int t = 0; t < kBlock; t++) {
-            const bool in = t >= u.t0 && t < u.t1;
-            float x[E], y[E];
+        for (int t = 0; t < TOKENS; t++) w[t] = turn[wave][t0 + t][c];
 #pragma unroll
-            for (int e = 0; e < E; e++) {
-                x[e] = kv_to_f32(kx[t].v[e]);
-                y[e] = kv_to_f32(vx[t].v[e]);
+        for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int h = 0; h < TOKENS / 8; h++) {
+                kv_vec<uint32_t, 4> o;
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+                    o.v[q] = __builtin_amdgcn_perm(w[8 * h + 2 * q + 1], w[8 * h + 2 * q], e ? 0x07060302u : 0x05040100u);
+                *(kv_vec<uint32_t, 4> *)(to + 32 * (2 * c + e) + 2 * (t0 + 8 * h)) = o;
             }
-            const kv_scale sx = kv_vector_scale<E>(x), sy = kv_vector_scale<E>(y);
-            kv_vec<int8_t, E> o;
-#pragma unroll
-            for (int e = 0; e < E; e++) {
-                o.v[e] = (int8_t)kv_code(x[e], sx);
-                vq[e].v[t] = (int8_t)kv_code(y[e], sy);
-            }
-            if (in) {
-                *(kv_vec<int8_t, E> *)(ko + t * D) = o;
-                if (lane == 0) {
-                    ks[t] = sx.d;
-                    vs[t] = sy.d;
-                }
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-            if (full) {
-                *(kv_vec<int8_t, 16> *)(vo + 16 * e) = vq[e];
-            } else {
-#pragma unroll
-                for (int t = 0; t < kBlock; t++)
-                    if (t >= u.t0 && t < u.t1) vo[16 * e + t] = vq[e].v[t];
-            }
-        }
     }
 }
 
@@ -203,92 +212,97 @@ __global__ __launch_bounds__(256) void sera_kv_write_kernel(kv_args a, const T *
 template <int TYPE, typename T, int D>
 __global__ __launch_bounds__(256) void sera_kv_read_kernel(kv_args a, T *__restrict__ k, int64_t k_stride,
                                                            T *__restrict__ v, int64_t v_stride) {
-    constexpr int E = D / 64;
-    const int lane = threadIdx.x & 63;
-    const int head = (int)blockIdx.y * 4 + (int)(threadIdx.x >> 6);
+    using R = kv_rows<T, D>;
+    constexpr bool Q8 = TYPE == (int)SERA_KV_Q8;
+    constexpr int VEC = R::VEC, N = R::N, ES = Q8 ? 1 : 2;
+    __shared__ kv_vec<uint32_t, 4> turn[4][D * ES];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int item = (int)blockIdx.y * 4 + wave, head = item >> 1;
+    const bool is_v = item & 1;
     int unit;
-    const int b = kv_find(a, (int)blockIdx.x, kBlock, 2, &unit);
-    if (b < 0 || head >= a.kv_heads) return;
-    const kv_seq s = kv_sequence(a, b);
-    const int d0 = E * lane;
-    const int64_t col = (int64_t)head * D + d0;
+    const kv_seq s = kv_find_sequence(a, (int)blockIdx.x, kBlock, 2, &unit);
+    if (s.b < 0 || head >= a.kv_heads) return;
+    const int64_t stride = is_v ? v_stride : k_stride;
+    T *out = (is_v ? v : k) + (int64_t)head * D;
     const int before = s.bad ? s.n : min(max(s.n - s.len, 0), s.n);
     if (unit == 0 && before > 0) {
-        kv_vec<T, E> o;
+        kv_vec<T, VEC> o;
 #pragma unroll
-        for (int e = 0; e < E; e++) o.v[e] = kv_from_f32<T>(s.bad ? __builtin_nanf("") : 0.0f);
-        for (int64_t r = s.row0; r < s.row0 + before; r++) {
-            *(kv_vec<T, E> *)(k + r * k_stride + col) = o;
-            *(kv_vec<T, E> *)(v + r * v_stride + col) = o;
-        }
+        for (int e = 0; e < VEC; e++) o.v[e] = kv_from_f32<T>(s.bad ? __builtin_nanf("") : 0.0f);
+        for (int64_t r = s.row0 + lane / R::LANES; r < s.row0 + before; r += R::ROWS)
+            *(kv_vec<T, VEC> *)(out + r * stride + R::channel(lane)) = o;
     }
     if (s.bad) return;
     const kv_unit u = kv_unit_of(s, unit);
     if (u.t0 >= u.t1) return;
-    const int page = a.table[(size_t)b * a.table_stride + (u.pos0 >> a.page_shift)];
+    const int page = a.table[(size_t)s.b * a.table_stride + (u.pos0 >> a.page_shift)];
     const bool lost = page < 0 || page >= a.pages;
+    const size_t kv_bytes = ((size_t)D << a.page_shift) * ES;
     const uint8_t *run = a.data + (lost ? 0 : (size_t)page * a.page_bytes) + (size_t)head * a.head_bytes;
     const int slot = u.pos0 & ((1 << a.page_shift) - 1);
-    const size_t kv_elems = (size_t)D << a.page_shift;
-    const int64_t row = (int64_t)s.row0 + u.pos0 - (s.len - s.n);
-    T *kp = k + row * k_stride + col, *vp = v + row * v_stride + col;
+    const uint8_t *from = run + (is_v ? kv_bytes : 0) + (size_t)slot * (D * ES);
+    out += ((int64_t)s.row0 + u.pos0 - (s.len - s.n)) * stride;      /* of the block's token 0 */
+    float scale = lost ? __builtin_nanf("") : 1.0f;                  /* of token `lane` */
+    if (Q8 && lane < kBlock && !lost)
+        scale = ((const float *)(run + 2 * kv_bytes))[((size_t)is_v << a.page_shift) + slot + lane];
 
-    float kx[kBlock][E], vx[kBlock][E];
-    if (TYPE == (int)SERA_KV_F16) {
-        const _Float16 *ki = (const _Float16 *)run + (size_t)slot * D + d0;
-        const _Float16 *vi = (const _Float16 *)run + kv_elems + (size_t)slot * D + (size_t)d0 * 16;
-        kv_vec<_Float16, E> kr[kBlock];
-        kv_vec<_Float16, 8> vr[E][2];
+    if (!is_v) {
+        kv_vec<uint8_t, VEC * ES> in[N];
 #pragma unroll
-        for (int t = 0; t < kBlock; t++) kr[t] = *(const kv_vec<_Float16, E> *)(ki + t * D);
+        for (int i = 0; i < N; i++)
+            in[i] = *(const kv_vec<uint8_t, VEC * ES> *)(from + (R::token(i, lane) * D + R::channel(lane)) * ES);
 #pragma unroll
-        for (int e = 0; e < E; e++)
+        for (int i = 0; i < N; i++) {
+            const int t = R::token(i, lane);
+            const float f = __shfl(scale, t, 64);
+            kv_vec<T, VEC> o;
 #pragma unroll
-            for (int h = 0; h < 2; h++) vr[e][h] = *(const kv_vec<_Float16, 8> *)(vi + 16 * e + 8 * h);
-#pragma unroll
-        for (int t = 0; t < kBlock; t++)
-#pragma unroll
-            for (int e = 0; e < E; e++) {
-                kx[t][e] = (float)kr[t].v[e];
-                vx[t][e] = (float)vr[e][t >> 3].v[t & 7];
+            for (int e = 0; e < VEC; e++) {
+                const float x = Q8 ? (float)(int8_t)in[i].v[e]
+                                   : (float)__builtin_bit_cast(_Float16, (uint16_t)(in[i].v[e * ES] | in[i].v[e * ES + ES - 1] << 8));
+                o.v[e] = kv_from_f32<T>(x * f);
             }
-    } else {
-        const int8_t *ki = (const int8_t *)run + (size_t)slot * D + d0;
-        const int8_t *vi = (const int8_t *)run + kv_elems + (size_t)slot * D + (size_t)d0 * 16;
-        const float *ks = (const float *)(run + 2 * kv_elems) + slot, *vs = ks + ((size_t)1 << a.page_shift);
-        kv_vec<int8_t, E> kr[kBlock];
-        kv_vec<int8_t, 16> vr[E];
-#pragma unroll
-        for (int t = 0; t < kBlock; t++) kr[t] = *(const kv_vec<int8_t, E> *)(ki + t * D);
-#pragma unroll
-        for (int e = 0; e < E; e++) vr[e] = *(const kv_vec<int8_t, 16> *)(vi + 16 * e);
-#pragma unroll
-        for (int t = 0; t < kBlock; t++)
-#pragma unroll
-            for (int e = 0; e < E; e++) {
-                kx[t][e] = (float)kr[t].v[e] * ks[t];
-                vx[t][e] = (float)vr[e].v[t] * vs[t];
-            }
-    }
-#pragma unroll
-    for (int t = 0; t < kBlock; t++)
-        if (t >= u.t0 && t < u.t1) {
-            kv_vec<T, E> ko, vo;
-#pragma unroll
-            for (int e = 0; e < E; e++) {
-                ko.v[e] = kv_from_f32<T>(lost ? __builtin_nanf("") : kx[t][e]);
-                vo.v[e] = kv_from_f32<T>(lost ? __builtin_nanf("") : vx[t][e]);
-            }
-            *(kv_vec<T, E> *)(kp + t * k_stride) = ko;
-            *(kv_vec<T, E> *)(vp + t * v_stride) = vo;
+            if (t >= u.t0 && t < u.t1) *(kv_vec<T, VEC> *)(out + t * stride + R::channel(lane)) = o;
         }
+        return;
+    }
+    /* V: channels 4c .. 4c+3 lie D / 4 places apart in LDS, so that lanes of consecutive c read side by side. */
+    kv_vec<uint32_t, 4> in[D * ES / 64];
+#pragma unroll
+    for (int i = 0; i < D * ES / 64; i++) in[i] = ((const kv_vec<uint32_t, 4> *)from)[64 * i + lane];
+#pragma unroll
+    for (int i = 0; i < D * ES / 64; i++) {
+        const int at = 64 * i + lane, ch = at / ES;
+        turn[wave][(ch % 4 * (D / 4) + ch / 4) * ES + at % ES] = in[i];
+    }
+    asm volatile("" ::: "memory");
+    constexpr int PER = 4 / ES;             /* tokens of a dword */
+#pragma unroll
+    for (int i = 0; i < D * kBlock / (4 * PER * 64); i++) {
+        const int x = 64 * i + lane, c = x % (D / 4), q = x / (D / 4);    /* tokens PER * q .. of channels 4c .. */
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[j] = turn[wave][(j * (D / 4) + c) * ES + q / 4].v[q % 4];
+#pragma unroll
+        for (int z = 0; z < PER; z++) {
+            const int t = PER * q + z;
+            const float f = __shfl(scale, t, 64);
+            kv_vec<T, 4> o;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float y = Q8 ? (float)(int8_t)(w[j] >> (8 * z)) : (float)__builtin_bit_cast(_Float16, (uint16_t)(w[j] >> (16 * z)));
+                o.v[j] = kv_from_f32<T>(y * f);
+            }
+            if (t >= u.t0 && t < u.t1) *(kv_vec<T, 4> *)(out + t * stride + 4 * c) = o;
+        }
+    }
 }
 
 namespace {
 
 template <int TYPE, typename T, int D>
 hipError_t kv_move(bool write, const kv_args &a, void *k, int64_t ks, void *v, int64_t vs, hipStream_t s) {
-    const dim3 grid((unsigned)kv_slots(a.rows, a.sequences, kBlock, 2), (unsigned)((a.kv_heads + 3) / 4));
+    const dim3 grid((unsigned)kv_slots(a.rows, a.sequences, kBlock, 2), (unsigned)((2 * a.kv_heads + 3) / 4));
     if (write)
         hipLaunchKernelGGL((sera_kv_write_kernel<TYPE, T, D>), grid, dim3(256), 0, s, a, (const T *)k, ks,
                            (const T *)v, vs);

@@ -41,16 +41,19 @@ struct kv_seq {
     bool bad;       /* rows or length outside the bounds */
 };
 
-__device__ __forceinline__ kv_seq kv_sequence(const kv_args &a, int b) {
+__device__ __forceinline__ kv_seq kv_sequence_of(const kv_args &a, int b, int r0, int r1, int len) {
     kv_seq s;
     s.b = b;
-    const int r0 = a.row_start[b], r1 = a.row_start[b + 1], len = a.kv_len[b];
     s.bad = r0 < 0 || r1 < r0 || r1 > a.rows || r1 - r0 > a.max_new || len < 0 || len > a.max_kv;
     const int lo = min(max(r0, 0), a.rows), hi = min(max(r1, lo), a.rows);
     s.row0 = lo;
     s.n = hi - lo;
     s.len = len;
     return s;
+}
+
+__device__ __forceinline__ kv_seq kv_sequence(const kv_args &a, int b) {
+    return kv_sequence_of(a, b, a.row_start[b], a.row_start[b + 1], a.kv_len[b]);
 }
 
 /* Grids over (sequence, unit of `per` rows) when only the packed rows' count
@@ -83,6 +86,26 @@ __device__ __forceinline__ int kv_find(const kv_args &a, int slot, int per, int 
     *unit = __builtin_amdgcn_readfirstlane(slot - base);
     if (*unit < 0) return -1;
     return __builtin_amdgcn_readfirstlane(lo);
+}
+
+/* kv_find and the sequence found (b -1: none). Up to 63 sequences the lanes hold all of row_start and kv_len after
+ * one round of loads; otherwise the sequence is read after the search. */
+__device__ __forceinline__ kv_seq kv_find_sequence(const kv_args &a, int slot, int per, int extra, int *unit) {
+    kv_seq s;
+    s.b = -1;
+    if (a.sequences > 63) {
+        const int b = kv_find(a, slot, per, extra, unit);
+        return b < 0 ? s : kv_sequence(a, b);
+    }
+    const int lane = (int)(threadIdx.x & 63);
+    const int r = lane <= a.sequences ? a.row_start[lane] : 0, len = lane < a.sequences ? a.kv_len[lane] : 0;
+    const int key = lane < a.sequences ? min(max(r, 0), a.rows) / per + extra * lane : 0x7fffffff;
+    const int b = __popcll(__ballot(key <= slot)) - 1;
+    if (b < 0) return s;
+    *unit = slot - __builtin_amdgcn_readlane(key, b);
+    if (*unit < 0) return s;
+    return kv_sequence_of(a, b, __builtin_amdgcn_readlane(r, b), __builtin_amdgcn_readlane(r, b + 1),
+                          __builtin_amdgcn_readlane(len, b));
 }
 
 static inline int64_t kv_slots(int rows, int sequences, int per, int extra) {
