@@ -20,21 +20,23 @@ constexpr int kMaxSplits = 64;
  * shortens the chunks. */
 attn_plan plan_of(uint32_t cache_type, const kv_args &a, int heads, int cus) {
     attn_plan p = {};
+    p.shift = 5;
     const int group = heads / a.kv_heads;
     const int64_t columns = (int64_t)a.max_new * group;
     int64_t want;
     int least;           /* tiles of a chunk, at least */
     if (columns <= 32) {
-        p.columns = columns <= 16 ? 16 : 32;
+        p.columns = columns <= 8 ? 8 : columns <= 16 ? 16 : 32;
         p.waves = 4;
         p.slots = a.sequences;
-        p.shift = cache_type == SERA_KV_Q8 ? 6 : 5;
-        /* Two workgroups per CU are resident at once: more of them only repeat the start. */
-        want = 2 * (int64_t)cus / ((int64_t)a.sequences * a.kv_heads);
+        /* Split contexts only as far as there are CUs without a workgroup: joining costs a launch, and more workgroups a
+         * CU repeat the start (32 windows of 1024 tokens, 256 workgroups: 34 us whole, 40 in two; 24 contexts of 1050-2100
+         * tokens, 192 workgroups: 32 us whole, 33 in two, 31 in four; one context of 8000, 8 workgroups whole: 17 us in 32,
+         * 18 in 63). */
+        want = (int64_t)cus / ((int64_t)a.sequences * a.kv_heads);
         least = p.waves;                      /* a tile for every wave */
     } else {
         p.waves = 8;
-        p.shift = 5;
         const int64_t all = (int64_t)a.rows * group;
         /* 256 rows a workgroup load each key and value for the most rows, if that leaves every CU one. If not, 128
          * rows (two groups of waves over the tokens) for contexts up to 8192 tokens, where partial sums cost more
@@ -49,7 +51,7 @@ attn_plan plan_of(uint32_t cache_type, const kv_args &a, int heads, int cus) {
         least = 8;
     }
     const int tiles = (a.max_kv + (1 << p.shift) - 1) >> p.shift;
-    if (want > tiles / least) want = tiles / least;
+    if (want > (tiles + least - 1) / least) want = (tiles + least - 1) / least;
     if (want > kMaxSplits) want = kMaxSplits;
     p.splits = want < 1 ? 1 : (int)want;
     p.chunk = (tiles + p.splits - 1) / p.splits;
@@ -64,14 +66,12 @@ template <typename T, int D>
 __global__ __launch_bounds__(256) void sera_attn_join_kernel(kv_args a, attn_args t, int per, int splits, int chunk,
                                                              int shift) {
     constexpr int E = D / 64;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int i;
-    const int b = kv_find(a, (int)blockIdx.x, 1, 0, &i);
-    if (b < 0) return;
-    const kv_seq s = kv_sequence(a, b);
-    if (s.bad || i >= s.n) return;
+    const kv_seq s = kv_find_sequence(a, (int)blockIdx.x, 1, 0, &i);
+    if (s.b < 0 || s.bad || i >= s.n) return;
     const int first = s.len - s.n, rows = s.n * t.group, unit_rows = per ? per : a.max_new * t.group;
-    const int tile0 = per ? attn_first_tile(a, t.group, per, b, s.row0) : 0;
+    const int tile0 = per ? attn_first_tile(a, t.group, per, s.b, s.row0) : 0;
     for (int h = (int)blockIdx.y * 4 + wave; h < t.heads; h += (int)gridDim.y * 4) {
         const int head = h / t.group, row = i * t.group + h % t.group, unit = row / unit_rows;
         const int r = row - unit * unit_rows, last = min((unit + 1) * unit_rows, rows) - 1;
@@ -79,27 +79,47 @@ __global__ __launch_bounds__(256) void sera_attn_join_kernel(kv_args a, attn_arg
                                                first + last / t.group + 1, shift);
         const int used = max((range.count + chunk - 1) / chunk, 1);
         const size_t step = attn_partial_floats(unit_rows, D);
-        const int slot = per ? tile0 + unit : b;
+        const int slot = per ? tile0 + unit : s.b;
         const float *part = t.workspace + ((size_t)slot * a.kv_heads + head) * splits * step;
+        const float *from = part + (size_t)r * D + E * lane;
+        /* sums are loaded 16 splits at a time, the first together with the maxima that weigh them */
+        constexpr int BATCH = 16;
+        attn_vec<float, E> x[BATCH];
+#pragma unroll
+        for (int k = 0; k < BATCH; k++) x[k] = *(const attn_vec<float, E> *)(from + min(k, used - 1) * step);
         float m = kAttnLowest, l = 0.0f;
         if (lane < used) {
-            const attn_f2 x = *(const attn_f2 *)(part + lane * step + (size_t)unit_rows * D + 2 * r);
-            m = x[0];
-            l = x[1];
+            const attn_f2 ml = *(const attn_f2 *)(part + lane * step + (size_t)unit_rows * D + 2 * r);
+            m = ml[0];
+            l = ml[1];
         }
         float top = m;
-#pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+        top = fmaxf(top, xor_partner<1>(top));
+        top = fmaxf(top, xor_partner<2>(top));
+        top = fmaxf(top, xor_partner<4>(top));
+        top = fmaxf(top, xor_partner<8>(top));
+        top = fmaxf(top, xor_partner<16>(top));
+        top = fmaxf(top, xor_partner<32>(top));
         const float f = lane < used ? attn_exp2(m - top) : 0.0f;
         l *= f;
-#pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) l += __shfl_xor(l, o, 64);
+        l += xor_partner<1>(l);
+        l += xor_partner<2>(l);
+        l += xor_partner<4>(l);
+        l += xor_partner<8>(l);
+        l += xor_partner<16>(l);
+        l += xor_partner<32>(l);
         float y[E] = {};
-        for (int k = 0; k < used; k++) {
-            const attn_vec<float, E> x = *(const attn_vec<float, E> *)(part + k * step + (size_t)r * D + E * lane);
-            const float w = __shfl(f, k, 64);
+        for (int base = 0; base < used; base += BATCH) {
+            if (base > 0)
 #pragma unroll
-            for (int e = 0; e < E; e++) y[e] = fmaf(x.v[e], w, y[e]);
+                for (int k = 0; k < BATCH; k++)
+                    x[k] = *(const attn_vec<float, E> *)(from + min(base + k, used - 1) * step);
+#pragma unroll
+            for (int k = 0; k < BATCH; k++) {
+                const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), (base + k) & 63));
+#pragma unroll
+                for (int e = 0; e < E; e++) y[e] = base + k < used ? fmaf(x[k].v[e], w, y[e]) : y[e];
+            }
         }
         attn_vec<T, E> o;
 #pragma unroll

@@ -14,6 +14,9 @@
  * product: nothing moves between lanes but the maximum (two steps) and, at the end,
  * the sum of the weights.
  *
+ * Up to 8 rows of fp32 (PAIR) have both parts of their split in one operand, the high ones in columns 0..7, the low
+ * ones in 8..15, whose products are added: half of the MFMAs and of the registers for them.
+ *
  * A workgroup has the rows of one sequence and kv head (up to 16 * CT
  * columns) and a range of tiles; its waves take tiles in turn, each with a
  * running maximum of its own, and join through LDS at the end. Long contexts are
@@ -26,28 +29,32 @@ namespace {
 
 constexpr int kMaxTiles = 512;    /* whose page ids are in LDS at a time */
 
-/* Tile geometry. fp16: 32 tokens, 16-byte pieces of 8 channels (K) or of 8
- * tokens (V). 8 bits: 64 tokens, 16-byte pieces of 16 channels or 16 tokens,
- * so a piece feeds two MFMAs and a wave has as many bytes on the way. */
+/* Tile geometry: 32 tokens. A lane loads 16-byte pieces of K rows (8 fp16
+ * channels, or 16 codes, which feed two MFMAs), and of V 8 tokens of a
+ * channel (16 bytes of fp16, 8 of codes). */
 template <int TYPE, int D>
 struct few_shape {
     static constexpr bool Q8 = TYPE == (int)SERA_KV_Q8;
-    static constexpr int TT = Q8 ? 64 : 32, SHIFT = Q8 ? 6 : 5;
+    static constexpr int TT = 32, SHIFT = 5;
     static constexpr int QT = TT / 4;             /* tokens of a lane quarter, consecutive */
     static constexpr int NS = TT / 16;            /* 16-token A operands */
     static constexpr int KC = D / 32;             /* MFMA steps over the channels */
     static constexpr int KP = Q8 ? KC / 2 : KC;   /* 16-byte pieces of a K row per lane */
     static constexpr int NC = D / 16;             /* channel blocks */
-    static constexpr int PC = TT / 32;            /* MFMA steps over the tokens */
 };
+
+template <int TYPE>
+struct few_piece { typedef attn_u4 v; };
+template <>
+struct few_piece<(int)SERA_KV_Q8> { typedef attn_u2 v; };
 
 }  // namespace
 
-template <int TYPE, typename T, int D, int CT, int NW, int OCC>
+template <int TYPE, typename T, int D, int CT, int NW, int OCC, bool PAIR>
 __global__ __launch_bounds__(64 * NW, OCC) void sera_attn_few_kernel(kv_args a, attn_args t, int splits, int chunk) {
     using F = few_shape<TYPE, D>;
-    constexpr bool Q8 = F::Q8, TWO = sizeof(T) == 4;
-    constexpr int TT = F::TT, QT = F::QT, NS = F::NS, KC = F::KC, KP = F::KP, NC = F::NC, PC = F::PC;
+    constexpr bool Q8 = F::Q8, TWO = sizeof(T) == 4 && !PAIR;      /* a second fragment for the low parts */
+    constexpr int TT = F::TT, QT = F::QT, NS = F::NS, KC = F::KC, KP = F::KP, NC = F::NC;
     constexpr int RS = D + 4;                     /* row stride in LDS: rows start 4 banks apart */
     __shared__ int ids[kMaxTiles * (TT / 16)];
     __shared__ float red[NW][16][RS];
@@ -56,9 +63,15 @@ __global__ __launch_bounds__(64 * NW, OCC) void sera_attn_few_kernel(kv_args a, 
     const int b = (int)(blockIdx.z * gridDim.y + blockIdx.y);
     if (b >= a.sequences) return;
     const int head = (int)blockIdx.x % a.kv_heads, split = (int)blockIdx.x / a.kv_heads;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 15, quarter = lane >> 4, v0 = split * chunk;
+    /* Without a window a split's first table entries are known before the sequence is: their load goes along with the
+     * sequence's (max_kv bounds the table, whatever the length). */
+    const int64_t early = (int64_t)v0 * TT + 16 * tid;
+    int early_id = 0;
+    if (t.window == 0 && early < a.max_kv) early_id = a.table[(size_t)b * a.table_stride + (early >> a.page_shift)];
     const kv_seq s = kv_sequence(a, b);
     if (s.n == 0) return;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, quarter = lane >> 4;
     const int64_t q0 = (int64_t)head * t.group * D;
     if (s.bad) {
         if (split == 0)
@@ -69,13 +82,18 @@ __global__ __launch_bounds__(64 * NW, OCC) void sera_attn_few_kernel(kv_args a, 
     }
     const int pn = s.len - 1, p0 = max(s.len - s.n, 0), rows = s.n * t.group;
     const attn_range range = attn_range_of(t, p0, s.len, F::SHIFT);
-    const int v0 = split * chunk, v1 = min(v0 + chunk, range.count);
+    const int v1 = min(v0 + chunk, range.count);
     if (split > 0 && v0 >= range.count) return;
 
     /* Page ids of tiles g .. g + kMaxTiles, and from there the wave's tiles. */
     auto list_pages = [&](int g) {
-        for (int e = tid; e < min(v1 - g, kMaxTiles) * (TT / 16); e += 64 * NW)
-            ids[e] = attn_page(a, b, range.tile(g + e / (TT / 16)) * TT + e % (TT / 16) * 16, s.len);
+        for (int e = tid; e < min(v1 - g, kMaxTiles) * (TT / 16); e += 64 * NW) {
+            const int at = range.tile(g + e / (TT / 16)) * TT + e % (TT / 16) * 16;
+            if (t.window == 0 && g == v0 && e == tid)
+                ids[e] = at >= s.len ? 0 : early_id < 0 || early_id >= a.pages ? -1 : early_id;
+            else
+                ids[e] = attn_page(a, b, at, s.len);
+        }
     };
     list_pages(v0);
 
@@ -87,7 +105,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void sera_attn_few_kernel(kv_args a, 
     const float sign = t.scale_log2 < 0.0f ? -1.0f : 1.0f;
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
-        const int r = min(ct * 16 + col, rows - 1), i = r / t.group;
+        const int r = min(ct * 16 + (PAIR ? col & 7 : col), rows - 1), i = r / t.group;
         pos[ct] = s.len - s.n + i;
         const T *q = (const T *)t.q + (s.row0 + i) * t.q_stride + q0 + (r - i * t.group) * D;
         float x[KC][8], top = 0.0f;
@@ -97,8 +115,8 @@ __global__ __launch_bounds__(64 * NW, OCC) void sera_attn_few_kernel(kv_args a, 
 #pragma unroll
             for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(x[k][j]));
         }
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        top = fmaxf(top, xor_partner<16>(top));
+        top = fmaxf(top, xor_partner<32>(top));
         const int e = attn_q_exponent(top);
         const float up = ldexpf(sign, e);
         c[ct] = ldexpf(fabsf(t.scale_log2), -e);
@@ -107,8 +125,9 @@ __global__ __launch_bounds__(64 * NW, OCC) void sera_attn_few_kernel(kv_args a, 
 #pragma unroll
             for (int j = 0; j < 8; j++) x[k][j] *= up;
             attn_h8 lo;
-            attn_split<TWO>(x[k], qh[ct][k], lo);
+            attn_split<TWO || PAIR>(x[k], qh[ct][k], lo);
             if (TWO) ql[ct][k] = lo;
+            if (PAIR) qh[ct][k] = col < 8 ? qh[ct][k] : lo;
         }
     }
 
@@ -129,12 +148,14 @@ __global__ __launch_bounds__(64 * NW, OCC) void sera_attn_few_kernel(kv_args a, 
     /* Tokens of this lane: A row `col` of operand u is token QT * (col / 4) + 4 u + col % 4; its scores are
      * the tokens QT * quarter + 4 u + i. V pieces are those same tokens of one channel. */
     const int k_token = QT * (col >> 2) + (col & 3), v_token = QT * quarter;
-    attn_u4 kr[NS][KP], vr[NC];
+    attn_u4 kr[NS][KP];
+    typename few_piece<TYPE>::v vr[NC];
     attn_f4 ks[Q8 ? NS : 1], vs[Q8 ? NS : 1];
     int v_id = 0;
 
     /* The pieces of a tile. A lost page reads page 0 in its place (in the pool; its scores become NaN). */
     int g = v0;
+    bool odd = false;       /* this lane took values that are not finite out of a tile */
     auto load_k = [&](int v) {
         const int j = range.tile(v) * TT, *id = ids + (v - g) * (TT / 16);
         const uint8_t *run = base + (size_t)max(id[k_token >> 4], 0) * a.page_bytes;
@@ -158,9 +179,9 @@ __global__ __launch_bounds__(64 * NW, OCC) void sera_attn_few_kernel(kv_args a, 
         v_id = ids[(v - g) * (TT / 16) + (v_token >> 4)];
         const uint8_t *p = base + (size_t)max(v_id, 0) * a.page_bytes + kv_bytes +
                            (size_t)((j + v_token) & mask & ~15) * (D * (Q8 ? 1 : 2)) +
-                           (Q8 ? 16 * col : 32 * col + (v_token & 15) * 2);
+                           (16 * col + (v_token & 15)) * (Q8 ? 1 : 2);
 #pragma unroll
-        for (int k = 0; k < NC; k++) vr[k] = *(const attn_u4 *)(p + (Q8 ? 256 : 512) * k);
+        for (int k = 0; k < NC; k++) vr[k] = *(const typename few_piece<TYPE>::v *)(p + (Q8 ? 256 : 512) * k);
     };
 
     for (; g < v1; g += kMaxTiles) {
@@ -196,6 +217,11 @@ __global__ __launch_bounds__(64 * NW, OCC) void sera_attn_few_kernel(kv_args a, 
                         if (TWO) acc[ct][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[ct][k], acc[ct][u], 0, 0, 0);
                     }
                 }
+            if (PAIR)
+#pragma unroll
+                for (int u = 0; u < NS; u++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[0][u][i] += xor_partner<8>(acc[0][u][i]);
             attn_f4 vsn[Q8 ? NS : 1];
             float lv[Q8 ? NS : 1][4];
             if (Q8)
@@ -209,7 +235,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void sera_attn_few_kernel(kv_args a, 
                 }
             if (v + NW < end) load_k(v + NW);
 
-            attn_h8 ph[CT][PC], pl[CT][TWO ? PC : 1];
+            attn_h8 ph[CT], pl[CT];
     #pragma unroll
             for (int ct = 0; ct < CT; ct++) {
                 float x[4 * NS], top = kAttnLowest;
@@ -232,8 +258,8 @@ __global__ __launch_bounds__(64 * NW, OCC) void sera_attn_few_kernel(kv_args a, 
                 for (int u = 0; u < NS; u++)
     #pragma unroll
                     for (int i = 0; i < 4; i++) top = fmaxf(top, Q8 ? x[4 * u + i] + lv[u % (Q8 ? NS : 1)][i] : x[4 * u + i]);
-                top = fmaxf(top, __shfl_xor(top, 16, 64));
-                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                top = fmaxf(top, xor_partner<16>(top));
+                top = fmaxf(top, xor_partner<32>(top));
                 if (__ballot(top > m[ct] + kAttnLag)) {
                     const float f = attn_exp2(m[ct] - fmaxf(top, m[ct]));
                     m[ct] = fmaxf(top, m[ct]);
@@ -254,49 +280,66 @@ __global__ __launch_bounds__(64 * NW, OCC) void sera_attn_few_kernel(kv_args a, 
                         }
                         x[4 * u + i] = w;
                     }
-    #pragma unroll
-                for (int k = 0; k < PC; k++) {
-                    attn_h8 lo;
-                    attn_split<TWO>(x + 8 * k, ph[ct][k], lo);
-                    if (TWO) pl[ct][k] = lo;
+                    attn_split<TWO || PAIR>(x, ph[ct], pl[ct]);
+                if (PAIR) ph[ct] = col < 8 ? ph[ct] : pl[ct];
+            }
+#pragma unroll
+            for (int n = 0; n < NC; n++) {
+                attn_h8 vf;
+                if constexpr (Q8) vf = attn_codes(vr[n][0], vr[n][1]);
+                else vf = __builtin_bit_cast(attn_h8, vr[n]);
+                if (!Q8 && !seen) {
+                    attn_h8 bad;
+                    odd |= attn_take_odd(vf, bad);
+                }
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++) {
+                    o[ct][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[ct], o[ct][n], 0, 0, 0);
+                    if (TWO) o[ct][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[ct], o[ct][n], 0, 0, 0);
                 }
             }
-    #pragma unroll
-            for (int n = 0; n < NC; n++)
-    #pragma unroll
-                for (int k = 0; k < PC; k++) {
-                    attn_h8 vf = Q8 ? attn_codes(vr[n][2 * k], vr[n][2 * k + 1]) : __builtin_bit_cast(attn_h8, vr[n]);
-                    if (!Q8 && !seen) {
-                        /* fp16 values that are not finite: rows that see them get NaN in their channels, others nothing */
-                        attn_h8 odd;
-                        if (__ballot(attn_take_odd(vf, odd)))
-    #pragma unroll
-                            for (int ct = 0; ct < CT; ct++) {
-                                attn_h8 sees;
-    #pragma unroll
-                                for (int i = 0; i < 8; i++) 
-                                    sees[i] = attn_sees(t, pos[ct], j0 + i) ? (_Float16)1.0f : (_Float16)0.0f;
-                                attn_f4 hit = {0.0f, 0.0f, 0.0f, 0.0f};
-                                hit = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, sees, hit, 0, 0, 0);
-    #pragma unroll
-                                for (int i = 0; i < 4; i++) o[ct][n][i] = hit[i] > 0.0f ? __builtin_nanf("") : o[ct][n][i];
-                            }
-                    }
-    #pragma unroll
-                    for (int ct = 0; ct < CT; ct++) {
-                        o[ct][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[ct][k], o[ct][n], 0, 0, 0);
-                        if (TWO) o[ct][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[ct][k], o[ct][n], 0, 0, 0);
+            if (v + NW < end) load_v(v + NW);
+        }
+        /* fp16 values that are not finite, in tiles that a row does not see whole, were taken out: a product would
+         * carry them into rows that do not see them (0 * inf). The rows that do get NaN in their channels. */
+        if (!Q8 && __ballot(odd)) {
+            for (v = g + wave; v < end; v += NW) {
+                const int j = range.tile(v) * TT;
+                if (attn_all_seen(t, j, TT, p0, pn) && s.n <= s.len) continue;
+                load_v(v);
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++) {
+                    attn_h8 sees;
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        sees[i] = attn_sees(t, pos[ct], j + v_token + i) ? (_Float16)1.0f : (_Float16)0.0f;
+#pragma unroll
+                    for (int n = 0; n < NC; n++) {
+                        attn_h8 w, bad;
+                        if constexpr (!Q8) w = __builtin_bit_cast(attn_h8, vr[n]);
+                        attn_take_odd(w, bad);
+                        attn_f4 hit = {0.0f, 0.0f, 0.0f, 0.0f};
+                        hit = __builtin_amdgcn_mfma_f32_16x16x32_f16(bad, sees, hit, 0, 0, 0);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) o[ct][n][i] = hit[i] > 0.0f ? __builtin_nanf("") : o[ct][n][i];
+                        __builtin_amdgcn_sched_barrier(0);      /* one at a time: few registers */
                     }
                 }
-            if (v + NW < end) load_v(v + NW);
+            }
+            odd = false;
         }
     }
 
+    if (PAIR)
+#pragma unroll
+        for (int n = 0; n < NC; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[0][n][i] += xor_partner<8>(o[0][n][i]);
     /* Join the waves: columns of 16 rows at a time. */
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
-        l[ct] += __shfl_xor(l[ct], 16, 64);
-        l[ct] += __shfl_xor(l[ct], 32, 64);
+        l[ct] += xor_partner<16>(l[ct]);
+        l[ct] += xor_partner<32>(l[ct]);
         if (quarter == 0) {
             ml[wave][0][ct * 16 + col] = m[ct];
             ml[wave][1][ct * 16 + col] = l[ct];
@@ -347,10 +390,10 @@ __global__ __launch_bounds__(64 * NW, OCC) void sera_attn_few_kernel(kv_args a, 
 
 namespace {
 
-template <int TYPE, typename T, int D, int CT, int NW, int OCC>
+template <int TYPE, typename T, int D, int CT, int NW, int OCC, bool PAIR>
 void few_go(const kv_args &a, const attn_args &t, const attn_plan &p, hipStream_t s) {
     const int y = a.sequences < 32768 ? a.sequences : 32768;
-    hipLaunchKernelGGL((sera_attn_few_kernel<TYPE, T, D, CT, NW, OCC>),
+    hipLaunchKernelGGL((sera_attn_few_kernel<TYPE, T, D, CT, NW, OCC, PAIR>),
                        dim3((unsigned)(a.kv_heads * p.splits), (unsigned)y, (unsigned)((a.sequences + y - 1) / y)),
                        dim3(64 * NW), 0, s, a, t, p.splits, p.chunk);
 }
@@ -360,9 +403,11 @@ template <int TYPE, typename T, int D>
 void few_ct(const kv_args &a, const attn_args &t, const attn_plan &p, hipStream_t s) {
     constexpr bool Q8 = TYPE == (int)SERA_KV_Q8, F32 = sizeof(T) == 4;
     if (p.columns == 32)
-        few_go<TYPE, T, D, 2, 4, Q8 || (F32 && D == 128) ? 1 : 2>(a, t, p, s);
+        few_go<TYPE, T, D, 2, 4, F32 && D == 128 ? 1 : 2, false>(a, t, p, s);
+    else if (F32 && p.columns == 8)
+        few_go<TYPE, T, D, 1, 4, Q8 ? 3 : D == 128 ? 2 : 4, F32>(a, t, p, s);
     else
-        few_go<TYPE, T, D, 1, 4, D == 128 || Q8 ? 2 : 3>(a, t, p, s);
+        few_go<TYPE, T, D, 1, 4, D == 128 ? Q8 && !F32 ? 3 : 2 : Q8 || F32 ? 3 : 4, false>(a, t, p, s);
 }
 
 template <int TYPE, typename T>

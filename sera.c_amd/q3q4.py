@@ -209,9 +209,13 @@ def _ptr(t):
 
 
 def _stream(stream=None):
+    """The handle of a stream, by default of the current one (asked for as a number where torch has that: a Stream
+    object costs 3 us of a call)."""
+    if stream is not None:
+        return stream.cuda_stream
     import torch
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return ctypes.c_void_p(s.cuda_stream)
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(torch.cuda.current_device()) if raw else torch.cuda.current_stream().cuda_stream
 
 
 def _check(rc, what):
@@ -555,19 +559,21 @@ def linear_group(geometries, weights, outputs, x, x2=None, gamma=None, eps=0.0, 
 
 KV_F16 = 1      # SERA_KV_F16
 KV_Q8 = 264     # SERA_KV_Q8: int8 codes, one float scale per token and kv head
-_ROW_TYPES = None
+_ROW_TYPES = {}
 
 
-def _row_type(t):
-    """(type id, data pointer, row stride) of rows [n, width]."""
-    global _ROW_TYPES
-    if _ROW_TYPES is None:
+def _rows(t, n, width):
+    """(type id, data pointer, row stride) of rows [n or more, width]."""
+    if not _ROW_TYPES:
         import torch
-        _ROW_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
-    if t.dtype not in _ROW_TYPES or t.dim() != 2 or t.stride(1) != 1 or not t.is_cuda:
+        _ROW_TYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 30})
+    ty, shape, stride = _ROW_TYPES.get(t.dtype), t.shape, t.stride()
+    if ty is None or len(shape) != 2 or stride[1] != 1 or not t.is_cuda:
         raise Q3Q4Error("rows must be a 2-d float32, float16 or bfloat16 device tensor with contiguous rows, "
                         f"got {tuple(t.shape)} {t.dtype} strides {t.stride()}")
-    return _ROW_TYPES[t.dtype], t.data_ptr(), t.stride(0)
+    if shape[0] < n or shape[1] != width:
+        raise Q3Q4Error(f"rows must be [{n}, {width}], got {tuple(t.shape)}")
+    return ty, t.data_ptr(), stride[0]
 
 
 def kv_page_bytes(type, page_tokens, kv_heads, head_dim):
@@ -589,7 +595,7 @@ class KVCache:
         if data.dtype != torch.uint8 or not data.is_contiguous() or data.numel() < pages * self.page_bytes:
             raise Q3Q4Error(f"the cache's data must be {pages * self.page_bytes} contiguous uint8")
         self.type, self.pages, self.page_tokens = type, pages, page_tokens
-        self.kv_heads, self.head_dim, self.data = kv_heads, head_dim, data
+        self.kv_heads, self.head_dim, self.data, self.width = kv_heads, head_dim, data, kv_heads * head_dim
         self.args = KVCacheArgs(type, page_tokens, kv_heads, head_dim, pages, data.data_ptr())
         self.ref = ctypes.addressof(self.args)
 
@@ -620,26 +626,26 @@ class KVBatch:
         self.ref = ctypes.addressof(self.args)
 
 
-def _kv_rows(cache, batch, width, *tensors):
-    """(type, pointers and strides) of row operands, checked against the batch."""
+def _pair(cache, batch, width, x, y):
+    """Two row operands of one type, checked against the batch: (type, pointer, stride, pointer, stride)."""
     if batch.max_kv > batch.entries * cache.page_tokens:
         raise Q3Q4Error(f"max_kv={batch.max_kv} is more than {batch.entries} pages of {cache.page_tokens} hold")
-    got = [_row_type(t) for t in tensors]
-    for t, g in zip(tensors, got):
-        if t.shape[0] < batch.rows or t.shape[1] != width or g[0] != got[0][0]:
-            raise Q3Q4Error(f"rows must be [{batch.rows}, {width}] of one type, got {tuple(t.shape)} {t.dtype}")
-    return got
+    ty, xp, xs = _rows(x, batch.rows, width)
+    ty2, yp, ys = _rows(y, batch.rows, width)
+    if ty != ty2:
+        raise Q3Q4Error(f"rows must be of one type, got {x.dtype} and {y.dtype}")
+    return ty, xp, xs, yp, ys
 
 
 def kv_write(cache, batch, k, v, stream=None):
     """k, v [rows, kv_heads * head_dim] into the cache."""
-    (ty, kp, ks), (_, vp, vs) = _kv_rows(cache, batch, cache.kv_heads * cache.head_dim, k, v)
+    ty, kp, ks, vp, vs = _pair(cache, batch, cache.width, k, v)
     _check(load().sera_kv_write(cache.ref, batch.ref, ty, kp, ks, vp, vs, _stream(stream)), "sera_kv_write")
 
 
 def kv_read(cache, batch, k, v, stream=None):
     """The cached values of the batch's rows into k, v [rows, kv_heads * head_dim]."""
-    (ty, kp, ks), (_, vp, vs) = _kv_rows(cache, batch, cache.kv_heads * cache.head_dim, k, v)
+    ty, kp, ks, vp, vs = _pair(cache, batch, cache.width, k, v)
     _check(load().sera_kv_read(cache.ref, batch.ref, ty, kp, ks, vp, vs, _stream(stream)), "sera_kv_read")
 
 
@@ -654,7 +660,7 @@ def attention(cache, batch, q, out, scale, window=0, sinks=0, workspace=None, st
     """out[row] = attention of q[row] over its sequence's cache; q, out
     [rows, heads * head_dim] of one type. window 0: the whole context."""
     width = q.shape[1]
-    (ty, qp, qs), (_, op, os_) = _kv_rows(cache, batch, width, q, out)
+    ty, qp, qs, op, os_ = _pair(cache, batch, width, q, out)
     if width % cache.head_dim:
         raise Q3Q4Error(f"rows of {width} are no heads of {cache.head_dim}")
     wp, wb = (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if workspace is not None else (0, 0)
