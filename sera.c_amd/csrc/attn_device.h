@@ -194,8 +194,9 @@ __device__ __forceinline__ int attn_find_tile(const kv_args &a, int group, int p
     int n[kAttnCounted / 64], upto[kAttnCounted / 64], total = 0;
 #pragma unroll
     for (int i = 0; i < kAttnCounted / 64; i++) {
-        n[i] = 64 * i < a.sequences ? attn_tiles_of(a, 64 * i + lane, group, per) : 0;
-        upto[i] = n[i];
+        n[i] = upto[i] = 0;
+        if (64 * i >= a.sequences) continue;
+        upto[i] = n[i] = attn_tiles_of(a, 64 * i + lane, group, per);
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const int x = __shfl_up(upto[i], o, 64);

@@ -49,11 +49,29 @@ struct tile_lds {
     attn_u4 raw[S::Q8 ? S::RING : 1][S::Q8 ? S::PIECES * S::NT : 1];
     float raw_scale[S::Q8 ? S::RING : 1][S::Q8 ? S::NT : 1];
     float scale[S::Q8 ? 3 : 1][S::NSUB][3][32];                /* K scale, V scale, log2 of the V scale */
+    float row_scale[S::NW][32];                                /* of q's rows, at the start */
     alignas(16) int ids[2 * kListed + 4];
     int lost;                                                  /* a page of those is lost */
     int any;                                                    /* tiles with values taken out, and which */
     uint8_t odd[S::Q8 ? 4 : kListed];
 };
+
+/* 32 rows of D elements, 16 bytes of T a lane. */
+template <typename T, int D>
+struct tile_rows {
+    static constexpr int VEC = 16 / (int)sizeof(T), LANES = D / VEC, ROWS = 64 / LANES, N = 32 / ROWS;
+};
+
+/* The largest of m over LANES lanes that share a row. */
+template <int LANES>
+__device__ __forceinline__ float tile_row_max(float m) {
+    m = fmaxf(m, xor_partner<1>(m));
+    m = fmaxf(m, xor_partner<2>(m));
+    m = fmaxf(m, xor_partner<4>(m));
+    if constexpr (LANES >= 16) m = fmaxf(m, xor_partner<8>(m));
+    if constexpr (LANES >= 32) m = fmaxf(m, xor_partner<16>(m));
+    return m;
+}
 
 typedef const __attribute__((address_space(1))) void attn_global;
 typedef __attribute__((address_space(3))) void attn_local;
@@ -113,8 +131,18 @@ __global__ __launch_bounds__(64 * RG * KG, RG * KG / 4) void sera_attn_tile_kern
 
     /* This wave's rows, and where they end. */
     const int rg = wave % RG, kg = wave / RG;
-    const int w0 = r0 + 32 * rg, row = min(w0 + col, rows - 1), at = row / t.group;
-    const int pos = first + at;
+    const int w0 = r0 + 32 * rg;
+    /* Token and head of the workgroup's row `local`, without a division: (x + 1/2) / group is a 1/(2 group) or more
+     * from every whole number, its error in fp32 below (1 + 256 / group) 2^-22. */
+    const int at0 = r0 / t.group, rem0 = r0 - at0 * t.group;
+    const float inv_group = 1.0f / (float)t.group;
+    auto place = [&](int local, int &h) {
+        const int x = rem0 + min(local, rows - 1 - r0), q = (int)(((float)x + 0.5f) * inv_group);
+        h = x - q * t.group;
+        return at0 + q;
+    };
+    int unused;
+    const int pos = first + place(32 * rg + col, unused);
     const int pw0 = first + min(w0, rows - 1) / t.group, pw1 = first + min(w0 + 31, rows - 1) / t.group;
     const attn_whole whole = attn_whole_of(t, range, first < 0 ? -1 : pw0, pw1, 5);                /* of this wave */
     const attn_whole all = attn_whole_of(t, range, max(first + r0 / t.group, 0), end - 1, 5);      /* of all waves */
@@ -122,41 +150,19 @@ __global__ __launch_bounds__(64 * RG * KG, RG * KG / 4) void sera_attn_tile_kern
     const int last = w0 >= rows ? 0 : (pw1 >= 0 ? pw1 >> 5 : -1) + 1 + range.sink_tiles - range.low;
     const int from = t.window > 0 ? (max(pw0 - t.window + 1, 0) >> 5) + range.sink_tiles - range.low : 0;
 
-    attn_h8 qh[KC], ql[TWO ? KC : 1];
-    float c;
-    {
-        const T *q = (const T *)t.q + (s.row0 + at) * t.q_stride + q0 + (row - at * t.group) * D + 8 * half;
-        float top = 0.0f;
-        /* twice over the row (the second time from cache): its size first, then the fragments */
+    /* This wave's rows of q, on their way while pages are looked up. */
+    using R = tile_rows<T, D>;
+    const int part = lane % R::LANES * R::VEC, part_row = 32 * rg + lane / R::LANES;
+    attn_vec<T, R::VEC> q_in[R::N];
 #pragma unroll
-        for (int k = 0; k < KC; k++) {
-            float x[8];
-            attn_load8(q + 16 * k, x);
-#pragma unroll
-            for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(x[j]));
-        }
-        top = fmaxf(top, xor_partner<32>(top));
-        const int e = attn_q_exponent(top);
-        const float up = ldexpf(t.scale_log2 < 0.0f ? -1.0f : 1.0f, e);
-        c = fmaxf(ldexpf(fabsf(t.scale_log2), -e), 1.17549435e-38f);   /* not 0: a masked score is -inf * c */
-#pragma unroll
-        for (int k = 0; k < KC; k++) {
-            float x[8];
-            attn_load8(q + 16 * k, x);
-#pragma unroll
-            for (int j = 0; j < 8; j++) x[j] *= up;
-            attn_h8 lo;
-            attn_split<TWO>(x, qh[k], lo);
-            if (TWO) ql[k] = lo;
-        }
+    for (int i = 0; i < R::N; i++) {
+        int h;
+        const int at = place(part_row + i * R::ROWS, h);
+        q_in[i] = *(const attn_vec<T, R::VEC> *)((const T *)t.q + (s.row0 + at) * t.q_stride + q0 + h * D + part);
     }
 
-    float m = kAttnLowest, l = 0.0f, l1 = 0.0f;
-    attn_f16 o[NC];
-#pragma unroll
-    for (int n = 0; n < NC; n++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) o[n][i] = 0.0f;
+    attn_h8 qh[KC], ql[TWO ? KC : 1];
+    float c = 0.0f, m = kAttnLowest, l = 0.0f, l1 = 0.0f;
 
     const int mask = (1 << a.page_shift) - 1;
     const size_t kv_bytes = ((size_t)D << a.page_shift) * ES;
@@ -228,6 +234,95 @@ __global__ __launch_bounds__(64 * RG * KG, RG * KG / 4) void sera_attn_tile_kern
             if (half) p[2][col] = attn_log_scale(x);
         }
     };
+
+    constexpr int AHEAD = S::AHEAD;
+    /* The pages of the tiles from g on, and the first loads. */
+    auto begin = [&]() {
+        stop = min(v1, g + kListed);
+        const int steps = (stop - g + NSUB - 1) / NSUB;
+        barrier_lds();
+        if (tid == 0) lds.lost = 0;
+        barrier_lds();
+        for (int e = tid; e < 2 * (stop - g) + 4; e += NT) {
+            const int id = e < 2 * (stop - g) ? attn_page(a, b, range.tile(g + (e >> 1)) * 32 + 16 * (e & 1), s.len) : 0;
+            lds.ids[e] = id;
+            if (id < 0) lds.lost = 1;
+        }
+        if (!Q8) {
+            for (int e = tid; e < stop - g; e += NT) lds.odd[e] = 0;
+            if (tid == 0) lds.any = 0;
+        }
+        __syncthreads();
+        lost = __builtin_amdgcn_readfirstlane(lds.lost) != 0;
+        for (int st = 0; st < min(AHEAD, steps); st++) stage_load(g + st * NSUB, st);
+    };
+
+    /* q's rows, scaled, as fragments: through LDS in the buffer that is loaded last, half of the channels of the high
+     * and then of the low parts at a time. Loading fragments straight from memory touches 64 places an access and
+     * cost 15 us a workgroup. */
+    auto fragments_of_q = [&]() {
+        uint8_t *box = (uint8_t *)lds.buf[S::BUFS - 1] + wave * (32 * D);
+        static_assert(S::NW * 32 * D <= sizeof(lds.buf[0]), "room for q");
+        attn_vec<_Float16, R::VEC> hi[R::N], lo[R::N];
+        float minus = -1.0f;
+        asm("" : "+s"(minus));
+#pragma unroll
+        for (int i = 0; i < R::N; i++) {
+            float x[R::VEC], most = 0.0f;
+#pragma unroll
+            for (int z = 0; z < R::VEC; z++) {
+                x[z] = kv_to_f32(q_in[i].v[z]);
+                most = fmaxf(most, fabsf(x[z]));
+            }
+            const int e = attn_q_exponent(tile_row_max<R::LANES>(most));
+            const float up = ldexpf(t.scale_log2 < 0.0f ? -1.0f : 1.0f, e);
+            /* not 0: a masked score is -inf * c */
+            if (part == 0)
+                lds.row_scale[wave][i * R::ROWS + lane / R::LANES] = fmaxf(ldexpf(fabsf(t.scale_log2), -e), 1.17549435e-38f);
+#pragma unroll
+            for (int z = 0; z < R::VEC; z += 2) {
+                const float a0 = x[z] * up, a1 = x[z + 1] * up;
+                const attn_h2 h = attn_pack(a0, a1);
+                hi[i].v[z] = h[0];
+                hi[i].v[z + 1] = h[1];
+                if (TWO) {
+                    lo[i].v[z] = (_Float16)fmaf((float)h[0], minus, a0);
+                    lo[i].v[z + 1] = (_Float16)fmaf((float)h[1], minus, a1);
+                }
+            }
+        }
+        constexpr int UNITS_OF_HALF = D / 16;
+#pragma unroll
+        for (int turn = 0; turn < (TWO ? 4 : 2); turn++) {
+            const int first_channel = turn % 2 * (D / 2);
+            asm volatile("" ::: "memory");         /* the wave's own LDS, which it accesses in order */
+            if (part >= first_channel && part < first_channel + D / 2)
+#pragma unroll
+                for (int i = 0; i < R::N; i++) {
+                    const int r = i * R::ROWS + lane / R::LANES, byte = 2 * (part - first_channel);
+                    *(attn_vec<_Float16, R::VEC> *)(box + r * D + (((byte >> 4) ^ (r & (UNITS_OF_HALF - 1))) << 4) + (byte & 15)) =
+                        turn < 2 ? hi[i] : lo[i];
+                }
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int k = 0; k < KC / 2; k++) {
+                const attn_h8 f = *(const attn_h8 *)(box + col * D + (((2 * k + half) ^ (col & (UNITS_OF_HALF - 1))) << 4));
+                if (turn < 2) qh[turn * (KC / 2) + k] = f;
+                else if (TWO) ql[TWO ? (turn - 2) * (KC / 2) + k : 0] = f;
+            }
+        }
+        c = lds.row_scale[wave][col];
+    };
+
+    if (v0 < v1) {
+        begin();
+        fragments_of_q();
+    }
+    attn_f16 o[NC];
+#pragma unroll
+    for (int n = 0; n < NC; n++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[n][i] = 0.0f;
 
     attn_f16 x;                        /* scores: score i is of token 16 * (i / 8) + 8 * half + i % 8 */
     attn_f4 vs[Q8 ? 4 : 1];            /* and the scales of those tokens' values */
@@ -412,24 +507,8 @@ __global__ __launch_bounds__(64 * RG * KG, RG * KG / 4) void sera_attn_tile_kern
     };
 
     for (; g < v1; g += kListed) {
-        stop = min(v1, g + kListed);
+        if (g > v0) begin();
         const int steps = (stop - g + NSUB - 1) / NSUB;
-        barrier_lds();
-        if (tid == 0) lds.lost = 0;
-        barrier_lds();
-        for (int e = tid; e < 2 * (stop - g) + 4; e += NT) {
-            const int id = e < 2 * (stop - g) ? attn_page(a, b, range.tile(g + (e >> 1)) * 32 + 16 * (e & 1), s.len) : 0;
-            lds.ids[e] = id;
-            if (id < 0) lds.lost = 1;
-        }
-        if (!Q8) {
-            for (int e = tid; e < stop - g; e += NT) lds.odd[e] = 0;
-            if (tid == 0) lds.any = 0;
-        }
-        __syncthreads();
-        constexpr int AHEAD = S::AHEAD;
-        lost = __builtin_amdgcn_readfirstlane(lds.lost) != 0;
-        for (int st = 0; st < min(AHEAD, steps); st++) stage_load(g + st * NSUB, st);
         wait_step<S::LOADS>(min(AHEAD, steps) - 1);
         if (Q8) convert(0, 0);
         else take_out(g, 0);
@@ -505,32 +584,42 @@ __global__ __launch_bounds__(64 * RG * KG, RG * KG / 4) void sera_attn_tile_kern
                 }
         }
     }
-    if (kg > 0 || w0 + col >= rows) return;
-    if (splits > 1) {
-        float *part = t.workspace + (((size_t)slot * a.kv_heads + head) * splits + split) * attn_partial_floats(BR, D);
-        const int r = 32 * rg + col;
-#pragma unroll
-        for (int n = 0; n < NC; n++)
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                *(attn_f4 *)(part + (size_t)r * D + 32 * n + 8 * i + 4 * half) =
-                    attn_f4{o[n][4 * i], o[n][4 * i + 1], o[n][4 * i + 2], o[n][4 * i + 3]};
-        if (half == 0) {
-            part[(size_t)BR * D + 2 * r] = m;
-            part[(size_t)BR * D + 2 * r + 1] = l;
-        }
-        return;
-    }
-    T *out = (T *)t.out + (s.row0 + at) * t.out_stride + q0 + (row - at * t.group) * D + 4 * half;
+    /* The result by rows, through LDS: a lane has 16 bytes of two rows' pieces in turn, stores are whole rows. */
+    __syncthreads();
+    if (kg > 0) return;
+    float *box = (float *)lds.buf + rg * (32 * D);
+    static_assert(RG * 32 * D * sizeof(float) <= sizeof(lds.buf) + sizeof(lds.raw), "room for the result");
+    const float scale = splits > 1 ? 1.0f : 1.0f / l;
 #pragma unroll
     for (int n = 0; n < NC; n++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            float y[4];
+            attn_f4 y;
 #pragma unroll
-            for (int z = 0; z < 4; z++) y[z] = pos < 0 ? 0.0f : o[n][4 * i + z] / l;
-            attn_store4(out + 32 * n + 8 * i, y);
+            for (int z = 0; z < 4; z++) y[z] = splits == 1 && pos < 0 ? 0.0f : o[n][4 * i + z] * scale;
+            *(attn_f4 *)(box + col * D + (((8 * n + 2 * i + half) ^ (col & (D / 4 - 1))) << 2)) = y;
         }
+    asm volatile("" ::: "memory");
+    float *partial = t.workspace + (((size_t)slot * a.kv_heads + head) * splits + split) * attn_partial_floats(BR, D);
+    if (splits > 1 && half == 0 && w0 + col < rows) {
+        const int r = 32 * rg + col;
+        partial[(size_t)BR * D + 2 * r] = m;
+        partial[(size_t)BR * D + 2 * r + 1] = l;
+    }
+    constexpr int ROWS = 64 / (D / 4);
+#pragma unroll 4
+    for (int i = 0; i < 32 / ROWS; i++) {
+        const int r = i * ROWS + lane / (D / 4), u = lane % (D / 4);
+        if (w0 + r >= rows) break;
+        const attn_f4 y = *(const attn_f4 *)(box + r * D + ((u ^ (r & (D / 4 - 1))) << 2));
+        if (splits > 1) {
+            *(attn_f4 *)(partial + (size_t)(32 * rg + r) * D + 4 * u) = y;
+        } else {
+            int h;
+            const int at = place(32 * rg + r, h);
+            attn_store4((T *)t.out + (s.row0 + at) * t.out_stride + q0 + h * D + 4 * u, (const float *)&y);
+        }
+    }
 }
 
 namespace {
