@@ -93,8 +93,15 @@ __device__ __forceinline__ void barrier_lds() { asm volatile("s_waitcnt lgkmcnt(
 
 }  // namespace
 
+/* Waves per SIMD: 8 waves of 128 channels take a CU's registers and LDS; two workgroups of 64 channels fit where their
+ * registers do (a ragged window prefill of fp16 rows: 43 us, 57 us with one). */
 template <int TYPE, typename T, int D, int RG, int KG>
-__global__ __launch_bounds__(64 * RG * KG, RG * KG / 4) void sera_attn_tile_kernel(kv_args a, attn_args t, int slots, int splits,
+constexpr int tile_occupancy() {
+    return RG * KG / 4 * (D == 64 && RG * KG == 8 && TYPE == (int)SERA_KV_F16 && sizeof(T) == 2 ? 2 : 1);
+}
+
+template <int TYPE, typename T, int D, int RG, int KG>
+__global__ __launch_bounds__(64 * RG * KG, (tile_occupancy<TYPE, T, D, RG, KG>())) void sera_attn_tile_kernel(kv_args a, attn_args t, int slots, int splits,
                                                                          int chunk) {
     using S = tile_shape<TYPE, D, RG, KG>;
     constexpr bool Q8 = S::Q8, TWO = sizeof(T) == 4;
@@ -360,11 +367,13 @@ __global__ __launch_bounds__(64 * RG * KG, RG * KG / 4) void sera_attn_tile_kern
         if (!Q8) top *= c;
     };
     auto scores = [&](int buf, int sub) {
+        uint32_t kt = (buf * NSUB + sub) * 2 * TILE_BYTES;
+        asm volatile("" : "+s"(kt));          /* the addresses are made here, not kept */
 #pragma unroll
         for (int i = 0; i < 16; i++) x[i] = 0.0f;
 #pragma unroll
         for (int k = 0; k < KC; k++) {
-            const attn_h8 f = fragment(2 * NC + k, (buf * NSUB + sub) * 2 * TILE_BYTES, 0);
+            const attn_h8 f = fragment(2 * NC + k, kt, 0);
             x = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, qh[k], x, 0, 0, 0);
             if (TWO) x = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, ql[TWO ? k : 0], x, 0, 0, 0);
         }
@@ -405,7 +414,8 @@ __global__ __launch_bounds__(64 * RG * KG, RG * KG / 4) void sera_attn_tile_kern
      * stages of one fragment's MFMAs each, in a fixed order, with the fragments read DEPTH stages ahead. The second
      * half of the weights is made under the MFMAs of the first. */
     auto tile = [&](int buf, int sub, int nb, int ns) {
-        constexpr int DEPTH = 2, STAGES = KC + 2 * NC;
+        constexpr int DEPTH = D == 64 ? 1 : 2, STAGES = KC + 2 * NC;
+        __builtin_amdgcn_s_setprio(1);       /* a wave in its products goes before one that is not */
         const float shift = kAttnBias - m;
         float minus = -1.0f;
         asm("" : "+s"(minus));
@@ -454,6 +464,7 @@ __global__ __launch_bounds__(64 * RG * KG, RG * KG / 4) void sera_attn_tile_kern
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
+        __builtin_amdgcn_s_setprio(0);
         finish(nb, ns);
     };
 
