@@ -13,74 +13,92 @@
 
 namespace {
 
-constexpr int kMaxSplits = 64;
+constexpr int kMaxSplits = 64, kFewColumns = 32;
+
+void split_of(attn_plan &p, const kv_args &a, int64_t want, int least) {
+    const int tiles = (a.max_kv + (1 << kAttnShift) - 1) >> kAttnShift, most = (tiles + least - 1) / least;
+    if (want > most) want = most;
+    if (want > kMaxSplits) want = kMaxSplits;
+    p.splits = want < 1 ? 1 : (int)want;
+    p.chunk = (tiles + p.splits - 1) / p.splits;
+}
+
+struct attn_plans {
+    attn_plan few, tile;
+    int few_columns, few_rows;
+    size_t few_bytes, bytes;     /* workspace: partial sums of the few-row kernel, then of the tiles */
+};
 
 /* The workspace has no window in its size (it is asked for before the call
  * that names one), so the split is chosen without it and a window only
  * shortens the chunks. */
-attn_plan plan_of(uint32_t cache_type, const kv_args &a, int heads, int cus) {
-    attn_plan p = {};
-    p.shift = 5;
+attn_plans plan_of(const kv_args &a, int dim, int heads, int cus) {
+    attn_plans p = {};
     const int group = heads / a.kv_heads;
     const int64_t columns = (int64_t)a.max_new * group;
-    int64_t want;
-    int least;           /* tiles of a chunk, at least */
-    if (columns <= 32) {
-        p.columns = columns <= 8 ? 8 : columns <= 16 ? 16 : 32;
-        p.waves = 4;
-        p.slots = a.sequences;
+    /* One kernel takes all sequences, unless they differ much: where they have less than half of the longest one's
+     * rows on average, those of a token or so (a group's rows, rounded up to what the few-row kernel holds) go to it and the
+     * others to the tiles, in two launches (a chunk of 512 rows over 4096 positions and 31 tokens over 3000 each: 239 us,
+     * 279 all in tiles; from an 8-bit cache 228 and 314). */
+    if (columns <= kFewColumns) p.few_columns = 0x7fffffff;
+    else if (group <= kFewColumns && 2ll * a.rows < (int64_t)a.sequences * a.max_new)
+        p.few_columns = group <= 8 ? 8 : group <= 16 ? 16 : 32;
+    if (p.few_columns) {
+        const int most = columns < p.few_columns ? (int)columns : p.few_columns;
+        p.few.columns = most <= 8 ? 8 : most <= 16 ? 16 : 32;
+        p.few_rows = columns <= kFewColumns ? (int)columns : p.few_columns / group * group;
         /* Split contexts only as far as there are CUs without a workgroup: joining costs a launch, and more workgroups a
          * CU repeat the start (32 windows of 1024 tokens, 256 workgroups: 34 us whole, 40 in two; 24 contexts of 1050-2100
          * tokens, 192 workgroups: 32 us whole, 33 in two, 31 in four; one context of 8000, 8 workgroups whole: 17 us in 32,
-         * 18 in 63). */
-        want = (int64_t)cus / ((int64_t)a.sequences * a.kv_heads);
-        least = p.waves;                      /* a tile for every wave */
-    } else {
-        p.waves = 8;
+         * 18 in 63). At least a tile for each of the four waves. */
+        split_of(p.few, a, (int64_t)cus / ((int64_t)a.sequences * a.kv_heads), 4);
+    }
+    if (columns > kFewColumns) {
         const int64_t all = (int64_t)a.rows * group;
         /* 256 rows a workgroup load each key and value for the most rows, if that leaves every CU one. If not, 128
          * rows (two groups of waves over the tokens) for contexts up to 8192 tokens, where partial sums cost more
          * than they give: 16 branches of 256 rows over 1568 tokens take 74 us so and 93 us as 256 rows split in two;
          * 512 rows x 8 over 32768 tokens 1175 us so and 1031 us split. */
-        p.columns = 256;
-        while (p.columns > 64 && columns <= p.columns / 2) p.columns /= 2;
-        if (p.columns == 256 && (all + 255) / 256 * a.kv_heads < cus && a.max_kv <= 8192) p.columns = 128;
-        p.slots = (int)(all / p.columns + a.sequences);
-        const int64_t units = (all + p.columns - 1) / p.columns * a.kv_heads;
-        want = cus / units;
-        least = 8;
+        p.tile.columns = 256;
+        while (p.tile.columns > 64 && columns <= p.tile.columns / 2) p.tile.columns /= 2;
+        if (p.tile.columns == 256 && (all + 255) / 256 * a.kv_heads < cus && a.max_kv <= 8192) p.tile.columns = 128;
+        p.tile.slots = (int)(all / p.tile.columns + a.sequences);
+        split_of(p.tile, a, cus / ((all + p.tile.columns - 1) / p.tile.columns * a.kv_heads), 8);
     }
-    const int tiles = (a.max_kv + (1 << p.shift) - 1) >> p.shift;
-    if (want > (tiles + least - 1) / least) want = (tiles + least - 1) / least;
-    if (want > kMaxSplits) want = kMaxSplits;
-    p.splits = want < 1 ? 1 : (int)want;
-    p.chunk = (tiles + p.splits - 1) / p.splits;
+    const size_t row = (size_t)a.kv_heads * (dim + 2) * sizeof(float);
+    if (p.few.splits > 1) p.few_bytes = ((size_t)a.sequences * p.few.splits * p.few_rows * row + 15) & ~(size_t)15;
+    p.bytes = p.few_bytes;
+    if (p.tile.splits > 1) p.bytes += (size_t)p.tile.slots * p.tile.splits * p.tile.columns * row;
     return p;
 }
 
 }  // namespace
 
-/* Joins the partial sums of a row: a wave for each (row, query head).
- * per 0: a unit of partial sums has a sequence's rows (all max_new); otherwise `per` rows of the tile kernel. */
+/* Joins the partial sums of a row: a wave for each (row, query head). A unit of the few-row kernel's sums has a
+ * sequence's rows, one of the tile kernel's `columns` of them. */
 template <typename T, int D>
-__global__ __launch_bounds__(256) void sera_attn_join_kernel(kv_args a, attn_args t, int per, int splits, int chunk,
-                                                             int shift) {
+__global__ __launch_bounds__(256) void sera_attn_join_kernel(kv_args a, attn_args t, attn_plan few, attn_plan tile,
+                                                             size_t tile_sums) {
     constexpr int E = D / 64;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int i;
     const kv_seq s = kv_find_sequence(a, (int)blockIdx.x, 1, 0, &i);
     if (s.b < 0 || s.bad || i >= s.n) return;
-    const int first = s.len - s.n, rows = s.n * t.group, unit_rows = per ? per : a.max_new * t.group;
-    const int tile0 = per ? attn_first_tile(a, t.group, per, s.b, s.row0) : 0;
+    const int first = s.len - s.n, rows = s.n * t.group;
+    const bool is_few = rows <= t.few_columns;
+    const int splits = is_few ? few.splits : tile.splits, chunk = is_few ? few.chunk : tile.chunk;
+    if (splits < 2) return;
+    const int unit_rows = is_few ? t.few_rows : tile.columns;
+    const int tile0 = is_few ? 0 : attn_first_tile(a, t, unit_rows, s.b, s.row0);
     for (int h = (int)blockIdx.y * 4 + wave; h < t.heads; h += (int)gridDim.y * 4) {
         const int head = h / t.group, row = i * t.group + h % t.group, unit = row / unit_rows;
         const int r = row - unit * unit_rows, last = min((unit + 1) * unit_rows, rows) - 1;
         const attn_range range = attn_range_of(t, max(first + unit * unit_rows / t.group, 0),
-                                               first + last / t.group + 1, shift);
+                                               first + last / t.group + 1, kAttnShift);
         const int used = max((range.count + chunk - 1) / chunk, 1);
         const size_t step = attn_partial_floats(unit_rows, D);
-        const int slot = per ? tile0 + unit : s.b;
-        const float *part = t.workspace + ((size_t)slot * a.kv_heads + head) * splits * step;
+        const int slot = is_few ? s.b : tile0 + unit;
+        const float *part = t.workspace + (is_few ? 0 : tile_sums) + ((size_t)slot * a.kv_heads + head) * splits * step;
         const float *from = part + (size_t)r * D + E * lane;
         /* sums are loaded 16 splits at a time, the first together with the maxima that weigh them */
         constexpr int BATCH = 16;
@@ -131,37 +149,45 @@ __global__ __launch_bounds__(256) void sera_attn_join_kernel(kv_args a, attn_arg
 namespace {
 
 template <typename T>
-void join_t(int dim, const kv_args &a, const attn_args &t, const attn_plan &p, hipStream_t s) {
+void join_t(int dim, const kv_args &a, const attn_args &t, const attn_plans &p, hipStream_t s) {
     const dim3 grid((unsigned)a.rows, (unsigned)((t.heads + 3) / 4));
-    const int per = p.columns > 32 ? p.columns : 0;
+    const size_t at = p.few_bytes / sizeof(float);
     if (dim == 64)
-        hipLaunchKernelGGL((sera_attn_join_kernel<T, 64>), grid, dim3(256), 0, s, a, t, per, p.splits, p.chunk, p.shift);
+        hipLaunchKernelGGL((sera_attn_join_kernel<T, 64>), grid, dim3(256), 0, s, a, t, p.few, p.tile, at);
     else
-        hipLaunchKernelGGL((sera_attn_join_kernel<T, 128>), grid, dim3(256), 0, s, a, t, per, p.splits, p.chunk, p.shift);
+        hipLaunchKernelGGL((sera_attn_join_kernel<T, 128>), grid, dim3(256), 0, s, a, t, p.few, p.tile, at);
+}
+
+/* A window's rows see fewer tiles than a whole context has. */
+void shorten(attn_plan &p, const kv_args &a, const attn_args &t) {
+    if (!p.columns || t.window == 0) return;
+    const int64_t tile = 1 << kAttnShift, sinks = t.sinks < a.max_kv ? t.sinks : a.max_kv;
+    const int64_t tiles = (sinks + tile - 1) / tile + ((int64_t)t.window + a.max_new + tile - 2) / tile + 1;
+    const int64_t chunk = (tiles + p.splits - 1) / p.splits;
+    if (chunk < p.chunk) p.chunk = (int)chunk;
 }
 
 }  // namespace
 
-size_t sera_attn_workspace(uint32_t cache_type, const kv_args &a, int dim, int heads, int cus) {
-    const attn_plan p = plan_of(cache_type, a, heads, cus);
-    if (p.splits < 2) return 0;
-    const size_t rows = p.columns > 32 ? (size_t)p.columns : (size_t)a.max_new * (heads / a.kv_heads);
-    return (size_t)p.slots * a.kv_heads * p.splits * rows * (dim + 2) * sizeof(float);
-}
+size_t sera_attn_workspace(const kv_args &a, int dim, int heads, int cus) { return plan_of(a, dim, heads, cus).bytes; }
 
 /* Arguments are checked by the caller (sera_attn_runtime.hip). */
-hipError_t sera_launch_attn(uint32_t cache_type, uint32_t type, int dim, const kv_args &a, const attn_args &t,
+hipError_t sera_launch_attn(uint32_t cache_type, uint32_t type, int dim, const kv_args &a, const attn_args &args,
                             hipStream_t s) {
-    attn_plan p = plan_of(cache_type, a, t.heads, t.cus);
-    if (t.window > 0) {
-        const int64_t tile = 1 << p.shift, sinks = t.sinks < a.max_kv ? t.sinks : a.max_kv;
-        const int64_t tiles = (sinks + tile - 1) / tile + ((int64_t)t.window + a.max_new + tile - 2) / tile + 1;
-        const int64_t chunk = (tiles + p.splits - 1) / p.splits;
-        if (chunk < p.chunk) p.chunk = (int)chunk;
+    attn_plans p = plan_of(a, dim, args.heads, args.cus);
+    attn_args t = args;
+    t.few_columns = p.few_columns;
+    t.few_rows = p.few_rows;
+    shorten(p.few, a, t);
+    shorten(p.tile, a, t);
+    hipError_t e = hipSuccess;
+    if (p.tile.columns) {
+        attn_args u = t;
+        u.workspace += p.few_bytes / sizeof(float);
+        e = sera_launch_attn_tile(cache_type, type, dim, a, u, p.tile, s);
     }
-    hipError_t e = p.columns > 32 ? sera_launch_attn_tile(cache_type, type, dim, a, t, p, s)
-                                  : sera_launch_attn_few(cache_type, type, dim, a, t, p, s);
-    if (e != hipSuccess || p.splits < 2) return e;
+    if (e == hipSuccess && p.few.columns) e = sera_launch_attn_few(cache_type, type, dim, a, t, p.few, s);
+    if (e != hipSuccess || !p.bytes) return e;
     if (type == SERA_TYPE_F32) join_t<float>(dim, a, t, p, s);
     else if (type == SERA_TYPE_F16) join_t<_Float16>(dim, a, t, p, s);
     else join_t<__bf16>(dim, a, t, p, s);

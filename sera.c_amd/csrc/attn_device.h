@@ -170,33 +170,34 @@ __device__ __forceinline__ void attn_store4(T *p, const float *x) {
     *(attn_vec<T, 4> *)p = o;
 }
 
-/* Row tiles of `per` rows (tokens x heads of a group), numbered through the sequences without gaps: a workgroup
+/* Row tiles of `per` rows (tokens x heads of a group) of the tile kernel's sequences, numbered through the sequences without gaps: a workgroup
  * that finds no rows still takes a turn on a compute unit, and where every second one does (sequences of one tile
  * each, with slots for two), half of the units get nothing but those: 16 sequences of 256 rows took as long as 32. Up to
  * kAttnCounted sequences are counted, one load of a wave for 64 of them; beyond, kv_find's gaps are few against the rest. */
 constexpr int kAttnCounted = 256;
 
-__device__ __forceinline__ int attn_tiles_of(const kv_args &a, int b, int group, int per) {
+__device__ __forceinline__ int attn_tiles_of(const kv_args &a, const attn_args &t, int b, int per) {
     if (b >= a.sequences) return 0;
     const int r0 = min(max(a.row_start[b], 0), a.rows), r1 = min(max(a.row_start[b + 1], r0), a.rows);
-    return ((r1 - r0) * group + per - 1) / per;
+    const int rows = (r1 - r0) * t.group;
+    return rows <= t.few_columns ? 0 : (rows + per - 1) / per;
 }
 
 /* Sequence and tile of it in place `slot`, counted from the last: late rows see most and start first. -1: none.
  * *place: the tile's number. */
-__device__ __forceinline__ int attn_find_tile(const kv_args &a, int group, int per, int slots, int slot, int *tile,
-                                              int *place) {
+__device__ __forceinline__ int attn_find_tile(const kv_args &a, const attn_args &t, int per, int slots, int slot,
+                                              int *tile, int *place) {
     const int lane = (int)(threadIdx.x & 63);
     if (a.sequences > kAttnCounted) {
         *place = slots - 1 - slot;
-        return kv_find(a, *place, per, 1, tile, group);
+        return kv_find(a, *place, per, 1, tile, t.group);
     }
     int n[kAttnCounted / 64], upto[kAttnCounted / 64], total = 0;
 #pragma unroll
     for (int i = 0; i < kAttnCounted / 64; i++) {
         n[i] = upto[i] = 0;
         if (64 * i >= a.sequences) continue;
-        upto[i] = n[i] = attn_tiles_of(a, 64 * i + lane, group, per);
+        upto[i] = n[i] = attn_tiles_of(a, t, 64 * i + lane, per);
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const int x = __shfl_up(upto[i], o, 64);
@@ -219,11 +220,11 @@ __device__ __forceinline__ int attn_find_tile(const kv_args &a, int group, int p
 }
 
 /* The number of sequence b's first tile, row0 its first row. */
-__device__ __forceinline__ int attn_first_tile(const kv_args &a, int group, int per, int b, int row0) {
-    if (a.sequences > kAttnCounted) return row0 * group / per + b;
+__device__ __forceinline__ int attn_first_tile(const kv_args &a, const attn_args &t, int per, int b, int row0) {
+    if (a.sequences > kAttnCounted) return row0 * t.group / per + b;
     const int lane = (int)(threadIdx.x & 63);
     int sum = 0;
-    for (int i = lane; i < b; i += 64) sum += attn_tiles_of(a, i, group, per);
+    for (int i = lane; i < b; i += 64) sum += attn_tiles_of(a, t, i, per);
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
     return sum;

@@ -71,7 +71,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void sera_attn_few_kernel(kv_args a, 
     int early_id = 0;
     if (t.window == 0 && early < a.max_kv) early_id = a.table[(size_t)b * a.table_stride + (early >> a.page_shift)];
     const kv_seq s = kv_sequence(a, b);
-    if (s.n == 0) return;
+    if (s.n == 0 || s.n * t.group > t.few_columns) return;
     const int64_t q0 = (int64_t)head * t.group * D;
     if (s.bad) {
         if (split == 0)
@@ -347,8 +347,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void sera_attn_few_kernel(kv_args a, 
     }
     __syncthreads();
     float *const part = t.workspace +
-        (((size_t)b * a.kv_heads + head) * splits + split) * attn_partial_floats(a.max_new * t.group, D);
-    const int part_rows = a.max_new * t.group;
+        (((size_t)b * a.kv_heads + head) * splits + split) * attn_partial_floats(t.few_rows, D);
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
         if (ct * 16 >= rows) break;
@@ -374,8 +373,8 @@ __global__ __launch_bounds__(64 * NW, OCC) void sera_attn_few_kernel(kv_args a, 
             if (splits > 1) {
                 *(attn_f4 *)(part + (size_t)rr * D + d) = sum;
                 if (d == 0) {
-                    part[(size_t)part_rows * D + 2 * rr] = mt;
-                    part[(size_t)part_rows * D + 2 * rr + 1] = lt;
+                    part[(size_t)t.few_rows * D + 2 * rr] = mt;
+                    part[(size_t)t.few_rows * D + 2 * rr + 1] = lt;
                 }
             } else {
                 const int i = rr / t.group;

@@ -113,11 +113,11 @@ __global__ __launch_bounds__(64 * RG * KG, (tile_occupancy<TYPE, T, D, RG, KG>()
     if (slot >= slots) return;
     const int head = (int)blockIdx.x % a.kv_heads, split = (int)blockIdx.x / a.kv_heads;
     int unit;
-    const int b = attn_find_tile(a, t.group, BR, slots, slot, &unit, &slot);
+    const int b = attn_find_tile(a, t, BR, slots, slot, &unit, &slot);
     if (b < 0) return;
     const kv_seq s = kv_sequence(a, b);
     const int rows = s.n * t.group, r0 = unit * BR;
-    if (r0 >= rows) return;
+    if (r0 >= rows || rows <= t.few_columns) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, half = lane >> 5;
     const int64_t q0 = (int64_t)head * t.group * D;

@@ -141,7 +141,7 @@ size_t sera_attention_workspace_bytes(const sera_kv_cache *cache, const sera_kv_
     if (batch->rows < 1 || batch->rows > kMaxRows || batch->sequences < 1 || batch->sequences > kMaxSequences ||
         batch->max_new < 1 || batch->max_new > batch->rows || batch->max_kv < 1 || batch->max_kv > kMaxPositions)
         return 0;
-    return sera_attn_workspace(cache->type, args_of(cache, batch), cache->head_dim, heads, device_cus());
+    return sera_attn_workspace(args_of(cache, batch), cache->head_dim, heads, device_cus());
 }
 
 int sera_attention(const sera_kv_cache *cache, const sera_kv_batch *batch, uint32_t type, const void *q,
@@ -162,7 +162,7 @@ int sera_attention(const sera_kv_cache *cache, const sera_kv_batch *batch, uint3
     if (check_rows(tag, "q", type, q, q_stride, width) || check_rows(tag, "out", type, out, out_stride, width))
         return -1;
     const kv_args a = args_of(cache, batch);
-    attn_args t;
+    attn_args t = {};
     t.q = q;
     t.out = out;
     t.q_stride = q_stride;
@@ -174,7 +174,7 @@ int sera_attention(const sera_kv_cache *cache, const sera_kv_batch *batch, uint3
     t.sinks = sinks;
     t.workspace = (float *)workspace;
     t.cus = device_cus();
-    const size_t need = sera_attn_workspace(cache->type, a, cache->head_dim, heads, t.cus);
+    const size_t need = sera_attn_workspace(a, cache->head_dim, heads, t.cus);
     if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15u)))
         return fail(-1, "%s: the workspace must be 16-byte aligned and hold %zu bytes (%zu given)", tag, need,
                     workspace ? workspace_bytes : (size_t)0);
