@@ -119,7 +119,12 @@ size_t sera_attention_workspace_bytes(const sera_kv_cache *cache, const sera_kv_
  * Products run on fp16 matrix instructions with fp32 sums: for fp16 and bf16
  * rows with q and the softmax weights rounded once to fp16, for fp32 rows
  * with both split into two fp16 terms (22 bits), so the result keeps fp32's
- * accuracy against the cached values.
+ * accuracy against the cached values. A value that is not finite makes the rows
+ * that see it not finite in its channel (an infinity may come out as NaN).
+ *
+ * Sequences may differ in rows: where most have a token or so and some have
+ * long chunks, both kinds run in the kernel that suits them. A call makes one
+ * to three launches.
  *
  * workspace: 16-byte aligned device scratch of at least
  * sera_attention_workspace_bytes(), used by one call at a time; its content

@@ -37,9 +37,9 @@ attn_plans plan_of(const kv_args &a, int dim, int heads, int cus) {
     const int group = heads / a.kv_heads;
     const int64_t columns = (int64_t)a.max_new * group;
     /* One kernel takes all sequences, unless they differ much: where they have less than half of the longest one's
-     * rows on average, those of a token or so (a group's rows, rounded up to what the few-row kernel holds) go to it and the
-     * others to the tiles, in two launches (a chunk of 512 rows over 4096 positions and 31 tokens over 3000 each: 239 us,
-     * 279 all in tiles; from an 8-bit cache 228 and 314). */
+     * rows on average, those of a token or so (a group's rows, rounded up to what the few-row kernel holds) go to it
+     * and the others to the tiles, in two launches (a chunk of 512 rows over 4096 positions and 31 tokens over 3000
+     * each: 239 us, 279 all in tiles; from an 8-bit cache 228 and 314). */
     if (columns <= kFewColumns) p.few_columns = 0x7fffffff;
     else if (group <= kFewColumns && 2ll * a.rows < (int64_t)a.sequences * a.max_new)
         p.few_columns = group <= 8 ? 8 : group <= 16 ? 16 : 32;
@@ -47,10 +47,10 @@ attn_plans plan_of(const kv_args &a, int dim, int heads, int cus) {
         const int most = columns < p.few_columns ? (int)columns : p.few_columns;
         p.few.columns = most <= 8 ? 8 : most <= 16 ? 16 : 32;
         p.few_rows = columns <= kFewColumns ? (int)columns : p.few_columns / group * group;
-        /* Split contexts only as far as there are CUs without a workgroup: joining costs a launch, and more workgroups a
-         * CU repeat the start (32 windows of 1024 tokens, 256 workgroups: 34 us whole, 40 in two; 24 contexts of 1050-2100
-         * tokens, 192 workgroups: 32 us whole, 33 in two, 31 in four; one context of 8000, 8 workgroups whole: 17 us in 32,
-         * 18 in 63). At least a tile for each of the four waves. */
+        /* Split contexts only as far as there are CUs without a workgroup: joining costs a launch, and more
+         * workgroups a CU repeat the start (32 windows of 1024 tokens, 256 workgroups: 34 us whole, 40 in two; 24
+         * contexts of 1050-2100 tokens, 192 workgroups: 32 us whole, 33 in two, 31 in four; one context of 8000, 8
+         * workgroups whole: 17 us in 32, 18 in 63). At least a tile for each of the four waves. */
         split_of(p.few, a, (int64_t)cus / ((int64_t)a.sequences * a.kv_heads), 4);
     }
     if (columns > kFewColumns) {
@@ -74,8 +74,10 @@ attn_plans plan_of(const kv_args &a, int dim, int heads, int cus) {
 
 }  // namespace
 
-/* Joins the partial sums of a row: a wave for each (row, query head). A unit of the few-row kernel's sums has a
- * sequence's rows, one of the tile kernel's `columns` of them. */
+/* Joins the partial sums of a row: a wave for each (row, query head). A unit of
+ * the few-row kernel's sums has a sequence's rows, one of the tile kernel's
+ * `columns` of them. Latency, mostly: sequence, then maxima and sums together
+ * (one context of 513 tokens in 5 splits: 3 us; 32768 rows in two: 27 us, 3.0 TB/s). */
 template <typename T, int D>
 __global__ __launch_bounds__(256) void sera_attn_join_kernel(kv_args a, attn_args t, attn_plan few, attn_plan tile,
                                                              size_t tile_sums) {
@@ -98,7 +100,8 @@ __global__ __launch_bounds__(256) void sera_attn_join_kernel(kv_args a, attn_arg
         const int used = max((range.count + chunk - 1) / chunk, 1);
         const size_t step = attn_partial_floats(unit_rows, D);
         const int slot = is_few ? s.b : tile0 + unit;
-        const float *part = t.workspace + (is_few ? 0 : tile_sums) + ((size_t)slot * a.kv_heads + head) * splits * step;
+        const float *part =
+            t.workspace + (is_few ? 0 : tile_sums) + ((size_t)slot * a.kv_heads + head) * splits * step;
         const float *from = part + (size_t)r * D + E * lane;
         /* sums are loaded 16 splits at a time, the first together with the maxima that weigh them */
         constexpr int BATCH = 16;
@@ -169,7 +172,9 @@ void shorten(attn_plan &p, const kv_args &a, const attn_args &t) {
 
 }  // namespace
 
-size_t sera_attn_workspace(const kv_args &a, int dim, int heads, int cus) { return plan_of(a, dim, heads, cus).bytes; }
+size_t sera_attn_workspace(const kv_args &a, int dim, int heads, int cus) {
+    return plan_of(a, dim, heads, cus).bytes;
+}
 
 /* Arguments are checked by the caller (sera_attn_runtime.hip). */
 hipError_t sera_launch_attn(uint32_t cache_type, uint32_t type, int dim, const kv_args &a, const attn_args &args,

@@ -48,7 +48,8 @@ struct attn_whole {
     int v0, v1;
 };
 
-__device__ __forceinline__ attn_whole attn_whole_of(const attn_args &t, const attn_range &r, int p0, int p1, int shift) {
+__device__ __forceinline__ attn_whole attn_whole_of(const attn_args &t, const attn_range &r, int p0, int p1,
+                                                    int shift) {
     attn_whole w;
     const int past = r.sink_tiles - r.low;       /* v - tile */
     const int from = t.window > 0 ? max(p1 - t.window + 1, 0) : 0;
@@ -170,10 +171,13 @@ __device__ __forceinline__ void attn_store4(T *p, const float *x) {
     *(attn_vec<T, 4> *)p = o;
 }
 
-/* Row tiles of `per` rows (tokens x heads of a group) of the tile kernel's sequences, numbered through the sequences without gaps: a workgroup
- * that finds no rows still takes a turn on a compute unit, and where every second one does (sequences of one tile
- * each, with slots for two), half of the units get nothing but those: 16 sequences of 256 rows took as long as 32. Up to
- * kAttnCounted sequences are counted, one load of a wave for 64 of them; beyond, kv_find's gaps are few against the rest. */
+/* Row tiles of `per` rows (tokens x heads of a group) of the tile kernel's
+ * sequences, numbered through the sequences without gaps: a workgroup that finds
+ * no rows still takes a turn on a compute unit, and where every second one does
+ * (sequences of one tile each, with slots for two), half of the units get
+ * nothing but those: 16 sequences of 256 rows took as long as 32. Up to
+ * kAttnCounted sequences are counted, one load of a wave for 64 of them;
+ * beyond, kv_find's gaps are few against the rest. */
 constexpr int kAttnCounted = 256;
 
 __device__ __forceinline__ int attn_tiles_of(const kv_args &a, const attn_args &t, int b, int per) {

@@ -8,12 +8,28 @@
  * on 32x32x16 fp16 MFMAs. A workgroup has 32 * RG rows of one sequence and kv
  * head (tokens x heads of the group, so all heads share what is loaded); its
  * waves are RG groups of rows times KG groups of tokens. K and V pass through LDS
- * as fp16 in 32-token tiles, two steps of buffers deep, already in the order that
- * the A operands are read in: K rows with the token bits 2 and 3 exchanged, so
- * that the scores a lane gets are its B operand of the second product, 16-byte
- * units of a row exchanged by the row (xor) against bank conflicts; V in units of
- * (16 tokens, 32 channels), read as one run. A lane's 16 scores belong to one
- * row, so the softmax is in the lane but for one step between the halves of a wave.
+ * as fp16 in steps of two 32-token tiles, which come by direct-to-LDS loads two to three
+ * steps ahead (8-bit codes into a ring of their own, from where they are
+ * converted once for all waves), already in the order that the A operands are
+ * read in: K rows with the token bits 2 and 3 exchanged, so that the scores a
+ * lane gets are its B operand of the second product, 16-byte units of a row
+ * exchanged by the row (xor) against bank conflicts; V in units of (16 tokens,
+ * 32 channels), read as one run. A lane's 16 scores belong to one row, so the
+ * softmax is in the lane but for one step between the halves of a wave.
+ *
+ * fp32 rows hold q and the weights as two fp16 terms each: twice the MFMAs,
+ * the same reads of K and V. What bounds it: a tile of a wave is 32 (fp32 rows; 16 otherwise)
+ * MFMAs of 32 cycles, about 100 VALU instructions, 16 fragment reads; the two
+ * waves of a SIMD overlap part of it, MFMAs are busy 40% of the time
+ * (prefill of 2048 tokens). Registers decide the rest: 64 for the sums and 64 for q
+ * (fp32 rows, 128 channels) leave room for one tile of scores, not for the
+ * next one's beside it, and a value spilled and reloaded in the loop waits for
+ * all loads on their way. 64 rows a wave at one wave per SIMD were slower
+ * (356 us against 178 for that prefill: nothing hides a wave's own latencies), and so
+ * was a strict turn-taking of the two waves by barriers (no gain).
+ * 2048 tokens x 64 heads: 164 us, 840 TFLOP/s of fp16 products (fp32 rows),
+ * 110 us, 620 (16-bit rows); a large matrix product reaches 1180 here. 512 rows over
+ * 32768 8-bit tokens: 1040 us, 1050 TFLOP/s.
  */
 #include "attn_device.h"
 #include "sera_launch.h"
@@ -93,16 +109,17 @@ __device__ __forceinline__ void barrier_lds() { asm volatile("s_waitcnt lgkmcnt(
 
 }  // namespace
 
-/* Waves per SIMD: 8 waves of 128 channels take a CU's registers and LDS; two workgroups of 64 channels fit where their
- * registers do (a ragged window prefill of fp16 rows: 43 us, 57 us with one). */
+/* Waves per SIMD: 8 waves of 128 channels take a CU's registers and LDS; two
+ * workgroups of 64 channels fit where their registers do (a ragged window
+ * prefill of fp16 rows: 42 us, 57 us with one). */
 template <int TYPE, typename T, int D, int RG, int KG>
 constexpr int tile_occupancy() {
     return RG * KG / 4 * (D == 64 && RG * KG == 8 && TYPE == (int)SERA_KV_F16 && sizeof(T) == 2 ? 2 : 1);
 }
 
 template <int TYPE, typename T, int D, int RG, int KG>
-__global__ __launch_bounds__(64 * RG * KG, (tile_occupancy<TYPE, T, D, RG, KG>())) void sera_attn_tile_kernel(kv_args a, attn_args t, int slots, int splits,
-                                                                         int chunk) {
+__global__ __launch_bounds__(64 * RG * KG, (tile_occupancy<TYPE, T, D, RG, KG>()))
+void sera_attn_tile_kernel(kv_args a, attn_args t, int slots, int splits, int chunk) {
     using S = tile_shape<TYPE, D, RG, KG>;
     constexpr bool Q8 = S::Q8, TWO = sizeof(T) == 4;
     constexpr int NT = S::NT, NSUB = S::NSUB, UNITS = S::UNITS, KC = S::KC, NC = S::NC, BR = 32 * RG;
@@ -178,8 +195,8 @@ __global__ __launch_bounds__(64 * RG * KG, (tile_occupancy<TYPE, T, D, RG, KG>()
     bool lost = false;
 
     /* The loads of a step are 16-token blocks of UB pieces, tile by tile: K's two, V's two. A wave's 64 pieces of
-     * round e are of block e * (NT / UB) + wave * 64 / UB; a thread has the same place in all its blocks, so one offset
-     * for K's and one for V's. */
+     * round e are of block e * (NT / UB) + wave * 64 / UB; a thread has the same place in all its blocks, so one
+     * offset for K's and one for V's. */
     constexpr int UB = D * ES, STEP_UNITS = NSUB * PER;
     int off_k, off_v;
     {
@@ -204,7 +221,8 @@ __global__ __launch_bounds__(64 * RG * KG, (tile_occupancy<TYPE, T, D, RG, KG>()
                                (size_t)((range.tile(v + sub) * 32 + 16 * odd) & mask) * (D * ES);
             asm("" : "+s"(p));     /* a scalar address and the thread's 32-bit offset, kept apart */
             attn_u4 *to = (Q8 ? lds.raw[0] : lds.buf[0][0][0]) + r * STEP_UNITS + e * NT + wave * 64;
-            __builtin_amdgcn_global_load_lds((attn_global *)(p + (uint32_t)(is_v ? off_v : off_k)), (attn_local *)to, 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((attn_global *)(p + (uint32_t)(is_v ? off_v : off_k)), (attn_local *)to,
+                                             16, 0, 0);
         }
         if (Q8) {      /* both scales of a tile; every wave loads some, those of the first NSUB are used */
             const int token = lane & 31, sub = wave % NSUB;
@@ -251,7 +269,8 @@ __global__ __launch_bounds__(64 * RG * KG, (tile_occupancy<TYPE, T, D, RG, KG>()
         if (tid == 0) lds.lost = 0;
         barrier_lds();
         for (int e = tid; e < 2 * (stop - g) + 4; e += NT) {
-            const int id = e < 2 * (stop - g) ? attn_page(a, b, range.tile(g + (e >> 1)) * 32 + 16 * (e & 1), s.len) : 0;
+            int id = 0;
+            if (e < 2 * (stop - g)) id = attn_page(a, b, range.tile(g + (e >> 1)) * 32 + 16 * (e & 1), s.len);
             lds.ids[e] = id;
             if (id < 0) lds.lost = 1;
         }
@@ -265,8 +284,7 @@ __global__ __launch_bounds__(64 * RG * KG, (tile_occupancy<TYPE, T, D, RG, KG>()
     };
 
     /* q's rows, scaled, as fragments: through LDS in the buffer that is loaded last, half of the channels of the high
-     * and then of the low parts at a time. Loading fragments straight from memory touches 64 places an access and
-     * cost 15 us a workgroup. */
+     * and then of the low parts at a time. (Fragments straight from memory would touch 64 places an access.) */
     auto fragments_of_q = [&]() {
         uint8_t *box = (uint8_t *)lds.buf[S::BUFS - 1] + wave * (32 * D);
         static_assert(S::NW * 32 * D <= sizeof(lds.buf[0]), "room for q");
@@ -285,7 +303,8 @@ __global__ __launch_bounds__(64 * RG * KG, (tile_occupancy<TYPE, T, D, RG, KG>()
             const float up = ldexpf(t.scale_log2 < 0.0f ? -1.0f : 1.0f, e);
             /* not 0: a masked score is -inf * c */
             if (part == 0)
-                lds.row_scale[wave][i * R::ROWS + lane / R::LANES] = fmaxf(ldexpf(fabsf(t.scale_log2), -e), 1.17549435e-38f);
+                lds.row_scale[wave][i * R::ROWS + lane / R::LANES] =
+                    fmaxf(ldexpf(fabsf(t.scale_log2), -e), 1.17549435e-38f);
 #pragma unroll
             for (int z = 0; z < R::VEC; z += 2) {
                 const float a0 = x[z] * up, a1 = x[z + 1] * up;
@@ -298,7 +317,7 @@ __global__ __launch_bounds__(64 * RG * KG, (tile_occupancy<TYPE, T, D, RG, KG>()
                 }
             }
         }
-        constexpr int UNITS_OF_HALF = D / 16;
+        constexpr int HALF_UNITS = D / 16;
 #pragma unroll
         for (int turn = 0; turn < (TWO ? 4 : 2); turn++) {
             const int first_channel = turn % 2 * (D / 2);
@@ -307,13 +326,14 @@ __global__ __launch_bounds__(64 * RG * KG, (tile_occupancy<TYPE, T, D, RG, KG>()
 #pragma unroll
                 for (int i = 0; i < R::N; i++) {
                     const int r = i * R::ROWS + lane / R::LANES, byte = 2 * (part - first_channel);
-                    *(attn_vec<_Float16, R::VEC> *)(box + r * D + (((byte >> 4) ^ (r & (UNITS_OF_HALF - 1))) << 4) + (byte & 15)) =
-                        turn < 2 ? hi[i] : lo[i];
+                    const int at = r * D + (((byte >> 4) ^ (r & (HALF_UNITS - 1))) << 4) + (byte & 15);
+                    *(attn_vec<_Float16, R::VEC> *)(box + at) = turn < 2 ? hi[i] : lo[i];
                 }
             asm volatile("" ::: "memory");
 #pragma unroll
             for (int k = 0; k < KC / 2; k++) {
-                const attn_h8 f = *(const attn_h8 *)(box + col * D + (((2 * k + half) ^ (col & (UNITS_OF_HALF - 1))) << 4));
+                const int at = col * D + (((2 * k + half) ^ (col & (HALF_UNITS - 1))) << 4);
+                const attn_h8 f = *(const attn_h8 *)(box + at);
                 if (turn < 2) qh[turn * (KC / 2) + k] = f;
                 else if (TWO) ql[TWO ? (turn - 2) * (KC / 2) + k : 0] = f;
             }
@@ -340,7 +360,8 @@ __global__ __launch_bounds__(64 * RG * KG, (tile_occupancy<TYPE, T, D, RG, KG>()
      * address bits that the fragment's number has to itself, so one address serves all. */
     constexpr uint32_t TILE_BYTES = UNITS * 16;
     const uint32_t lds_at = (uint32_t)(uintptr_t)(attn_local *)lds.buf;
-    const uint32_t k_at = lds_at + col * (D * 2) + ((half ^ (col & S::XOR)) << 4), v_at = lds_at + TILE_BYTES + lane * 16;
+    const uint32_t k_at = lds_at + col * (D * 2) + ((half ^ (col & S::XOR)) << 4);
+    const uint32_t v_at = lds_at + TILE_BYTES + lane * 16;
     auto fragment = [&](int i, uint32_t k_tile, uint32_t v_tile) {
         const uint32_t at = i < 2 * NC ? v_at + v_tile + (uint32_t)i * 1024u
                                        : (k_at + k_tile) ^ (uint32_t)((i - 2 * NC) << 5);
@@ -384,7 +405,8 @@ __global__ __launch_bounds__(64 * RG * KG, (tile_occupancy<TYPE, T, D, RG, KG>()
         if (v >= last || (v < from && range.tile(v) * 32 >= t.sinks)) return false;
         if (Q8)
 #pragma unroll
-            for (int i = 0; i < 4; i++) vs[i] = *(const attn_f4 *)&lds.scale[buf][sub][1][16 * (i / 2) + half8 + 4 * (i % 2)];
+            for (int i = 0; i < 4; i++)
+                vs[i] = *(const attn_f4 *)&lds.scale[buf][sub][1][16 * (i / 2) + half8 + 4 * (i % 2)];
         if (lost || v < whole.v0 || v >= whole.v1) {
             const int j = range.tile(v) * 32;
             const int id0 = lds.ids[2 * (v - g)], id1 = lds.ids[2 * (v - g) + 1];
@@ -512,7 +534,7 @@ __global__ __launch_bounds__(64 * RG * KG, (tile_occupancy<TYPE, T, D, RG, KG>()
                 hit = __builtin_amdgcn_mfma_f32_32x32x16_f16(bad, sees, hit, 0, 0, 0);
 #pragma unroll
                 for (int i = 0; i < 16; i++) o[n][i] = hit[i] > 0.0f ? __builtin_nanf("") : o[n][i];
-                __builtin_amdgcn_sched_barrier(0);         /* few registers: this must not spill what the loop holds */
+                __builtin_amdgcn_sched_barrier(0);      /* one at a time: this must not spill what the loop holds */
             }
         }
     };
@@ -546,7 +568,8 @@ __global__ __launch_bounds__(64 * RG * KG, (tile_occupancy<TYPE, T, D, RG, KG>()
                         convert(r, next);
                     }
                     barrier_lds();
-                    if (!Q8 && st + AHEAD < steps) stage_load(g + (st + AHEAD) * NSUB, buf == 0 ? S::BUFS - 1 : buf - 1);
+                    if (!Q8 && st + AHEAD < steps)
+                        stage_load(g + (st + AHEAD) * NSUB, buf == 0 ? S::BUFS - 1 : buf - 1);
                     if (Q8 && st + 1 + AHEAD < steps) stage_load(g + (st + 1 + AHEAD) * NSUB, r);
                 }
                 /* Past the last tile these are scores of whatever the buffer holds, used by nothing. */
@@ -576,7 +599,8 @@ __global__ __launch_bounds__(64 * RG * KG, (tile_occupancy<TYPE, T, D, RG, KG>()
             for (int n = 0; n < NC; n++)
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                    box[(n * 4 + i) * 64 + lane] = attn_f4{o[n][4 * i], o[n][4 * i + 1], o[n][4 * i + 2], o[n][4 * i + 3]};
+                    box[(n * 4 + i) * 64 + lane] =
+                        attn_f4{o[n][4 * i], o[n][4 * i + 1], o[n][4 * i + 2], o[n][4 * i + 3]};
             mlbox[lane] = m;
             mlbox[64 + lane] = l;
         }
