@@ -185,6 +185,11 @@ hipError_t sera_launch_attn(uint32_t cache_type, uint32_t type, int dim, const k
     t.few_rows = p.few_rows;
     shorten(p.few, a, t);
     shorten(p.tile, a, t);
+    /* Whole contexts, a CU to each workgroup: eight waves of an 8-bit cache, whose conversions they share (24 contexts of
+     * 1050-2100 tokens: 29 us, 32 with four). From fp16 the four are as fast (40 and 40), and split contexts
+     * have few tiles for more (one of 513 tokens: 11 us with four, 14 with eight). */
+    p.few.waves = cache_type == SERA_KV_Q8 && p.few.columns <= 16 && p.few.splits == 1 &&
+                  (int64_t)a.sequences * a.kv_heads <= args.cus ? 8 : 4;
     hipError_t e = hipSuccess;
     if (p.tile.columns) {
         attn_args u = t;

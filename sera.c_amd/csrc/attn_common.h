@@ -24,6 +24,7 @@ struct attn_args {
 /* How a kernel's part of a call is cut up, in 32-token tiles. */
 struct attn_plan {
     int columns;         /* rows of q (tokens x heads of a group) that a workgroup has; 0: the kernel has no part */
+    int waves;           /* few-row kernel: of a workgroup */
     int slots;           /* tile kernel: row tiles, of `columns` rows each, at most */
     int splits, chunk;   /* workgroups over a context, tiles of each */
 };

@@ -410,12 +410,15 @@ void few_go(const kv_args &a, const attn_args &t, const attn_plan &p, hipStream_
 template <int TYPE, typename T, int D>
 void few_ct(const kv_args &a, const attn_args &t, const attn_plan &p, hipStream_t s) {
     constexpr bool Q8 = TYPE == (int)SERA_KV_Q8, F32 = sizeof(T) == 4;
-    if (p.columns == 32)
-        few_go<TYPE, T, D, 2, 4, F32 && D == 128 ? 1 : 2, false>(a, t, p, s);
-    else if (F32 && p.columns == 8)
-        few_go<TYPE, T, D, 1, 4, Q8 ? 3 : D == 128 ? 2 : 4, F32>(a, t, p, s);
-    else
-        few_go<TYPE, T, D, 1, 4, D == 128 ? Q8 && !F32 ? 3 : 2 : Q8 || F32 ? 3 : 4, false>(a, t, p, s);
+    constexpr int PAIRED = Q8 ? 3 : D == 128 ? 2 : 4;
+    constexpr int PLAIN = D == 128 ? Q8 && !F32 ? 3 : 2 : Q8 || F32 ? 3 : 4;
+    if (p.columns == 32) return few_go<TYPE, T, D, 2, 4, F32 && D == 128 ? 1 : 2, false>(a, t, p, s);
+    if constexpr (Q8) {
+        if (p.waves == 8 && F32 && p.columns == 8) return few_go<TYPE, T, D, 1, 8, 2, F32>(a, t, p, s);
+        if (p.waves == 8) return few_go<TYPE, T, D, 1, 8, 2, false>(a, t, p, s);
+    }
+    if (F32 && p.columns == 8) return few_go<TYPE, T, D, 1, 4, PAIRED, F32>(a, t, p, s);
+    few_go<TYPE, T, D, 1, 4, PLAIN, false>(a, t, p, s);
 }
 
 template <int TYPE, typename T>

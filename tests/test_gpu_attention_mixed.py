@@ -103,3 +103,14 @@ def test_rows_of_the_smaller_tiles(torch, kind, new, group):  # noqa: F811
     print(f"case small tiles new={new} group={group} kind={kind}", flush=True)
     check(Setup(torch, kind, F32, [new, new - 2], [300, 41], heads=2 * group, kv_heads=2, page=16, seed=new))
     check(Setup(torch, kind, BF16, [new, new - 1], [77, 260], heads=2 * group, kv_heads=2, dim=64, page=16, seed=new))
+
+
+@pytest.mark.parametrize("kind", [ao.F16, ao.Q8])
+@pytest.mark.parametrize("io,heads", [(F32, 8), (F32, 13), (BF16, 16), (F16, 3)])
+def test_many_whole_contexts(torch, kind, io, heads):  # noqa: F811
+    """A workgroup for each of 150 sequences: contexts are not split, an 8-bit cache's workgroups have eight waves."""
+    print(f"case whole contexts kind={kind} io={io} heads={heads}", flush=True)
+    lens = [1 + (b * 37) % 600 for b in range(150)]
+    check(Setup(torch, kind, io, [1] * 150, lens, heads=heads, kv_heads=1, page=64, seed=heads))
+    check(Setup(torch, kind, io, [1] * 150, lens, heads=heads, kv_heads=1, dim=64, page=16, seed=heads), window=90,
+          sinks=5)
