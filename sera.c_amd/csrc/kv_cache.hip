@@ -5,13 +5,14 @@
  *
  * Both move data once and are bound by memory (or, for a few tokens, by the
  * launch and three dependent loads: sequence, page, data). A wave takes K or V
- * of one kv head of one 16-token block of a sequence. Rows are accessed in 16-byte
+ * of one kv head of one 16-token block of a sequence, a half of it to write (more
+ * waves for the quantizer: 2048 tokens into an 8-bit cache and back 17.6 us, 19.9
+ * with whole blocks). Rows are accessed in 16-byte
  * pieces (D / VEC lanes to a row, several rows to an access); K's place in the cache is
  * the same order. V's is not: 16 tokens of a channel lie side by side, so a wave
  * turns its block in LDS of its own, in dwords that are unpacked by byte
  * permutes. 24588 tokens out of an 8-bit cache as fp32 rows: 80-88 us, 4.4-4.9
- * TB/s (a large copy: 5.2); 2048 fp32 tokens into it and back: 13 + 8 us for
- * 38 MB, the dependent loads and few waves of the write more than its bytes.
+ * TB/s (a large copy: 5.2); ragged bf16 chunks into an fp16 cache 7 us for 15 MB.
  *
  * 8-bit quantizer: scale d = max|x| / 127 over the vector (an exact maximum,
  * one IEEE division), code = x / d rounded half to even, as the exact
@@ -123,15 +124,18 @@ __global__ __launch_bounds__(256) void sera_kv_write_kernel(kv_args a, const T *
                                                             const T *__restrict__ v, int64_t v_stride) {
     using R = kv_rows<T, D>;
     constexpr bool Q8 = TYPE == (int)SERA_KV_Q8;
-    constexpr int VEC = R::VEC, N = R::N, ES = Q8 ? 1 : 2, ROW = D * ES / 4;      /* dwords of a row in LDS */
-    __shared__ uint32_t turn[4][kBlock][ROW];
+    constexpr int VEC = R::VEC, N = R::N / 2, ES = Q8 ? 1 : 2, ROW = D * ES / 4;  /* dwords of a row in LDS */
+    constexpr int TOKENS = kBlock / 2;
+    __shared__ uint32_t turn[4][TOKENS][ROW];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int item = (int)blockIdx.y * 4 + wave, head = item >> 1;
-    const bool is_v = item & 1;
+    const int item = (int)blockIdx.y * 4 + wave, head = item >> 2, h0 = (item & 1) * TOKENS;
+    const bool is_v = item & 2;
     int unit;
     const kv_seq s = kv_find_sequence(a, (int)blockIdx.x, kBlock, 2, &unit);
     if (s.b < 0 || head >= a.kv_heads || s.bad) return;
-    const kv_unit u = kv_unit_of(s, unit);
+    kv_unit u = kv_unit_of(s, unit);
+    u.t0 = max(u.t0, h0);
+    u.t1 = min(u.t1, h0 + TOKENS);
     if (u.t0 >= u.t1) return;
     const int page = a.table[(size_t)s.b * a.table_stride + (u.pos0 >> a.page_shift)];
     if (page < 0 || page >= a.pages) return;
@@ -148,14 +152,14 @@ __global__ __launch_bounds__(256) void sera_kv_write_kernel(kv_args a, const T *
     kv_vec<T, VEC> in[N];
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        const int t = R::token(i, lane);
+        const int t = h0 + R::token(i, lane);
 #pragma unroll
         for (int e = 0; e < VEC; e++) in[i].v[e] = (T)0.0f;
         if (t >= u.t0 && t < u.t1) in[i] = *(const kv_vec<T, VEC> *)(from + t * stride);
     }
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        const int t = R::token(i, lane);
+        const int t = h0 + R::token(i, lane);
         const bool new_row = t >= u.t0 && t < u.t1;
         float x[VEC];
 #pragma unroll
@@ -167,58 +171,55 @@ __global__ __launch_bounds__(256) void sera_kv_write_kernel(kv_args a, const T *
             for (int e = 0; e < VEC; e++) o.v[e] = (int8_t)kv_code(x[e], sc);
             if (new_row && d0 == 0)
                 ((float *)(run + 2 * kv_bytes))[((size_t)is_v << a.page_shift) + slot + t] = sc.d;
-            if (is_v) *(kv_vec<int8_t, VEC> *)((int8_t *)turn[wave][t] + d0) = o;
+            if (is_v) *(kv_vec<int8_t, VEC> *)((int8_t *)turn[wave][t - h0] + d0) = o;
             else if (new_row) *(kv_vec<int8_t, VEC> *)(to + t * D + d0) = o;
         } else {
             kv_vec<_Float16, VEC> o;
 #pragma unroll
             for (int e = 0; e < VEC; e++) o.v[e] = (_Float16)x[e];
-            if (is_v) *(kv_vec<_Float16, VEC> *)((_Float16 *)turn[wave][t] + d0) = o;
+            if (is_v) *(kv_vec<_Float16, VEC> *)((_Float16 *)turn[wave][t - h0] + d0) = o;
             else if (new_row) *(kv_vec<_Float16, VEC> *)(to + (t * D + d0) * 2) = o;
         }
     }
     if (!is_v) return;
     asm volatile("" ::: "memory");          /* the wave's own LDS, which it accesses in order */
-    if (u.t0 > 0 || u.t1 < kBlock) {        /* some of the block's tokens: one element at a time */
+    if (u.t1 - u.t0 < TOKENS) {             /* some of the tokens: one element at a time */
         for (int t = u.t0; t < u.t1; t++)
             for (int d = lane; d < D; d += 64) {
-                if (Q8) to[16 * d + t] = ((const uint8_t *)turn[wave][t])[d];
-                else ((uint16_t *)to)[16 * d + t] = ((const uint16_t *)turn[wave][t])[d];
+                if (Q8) to[16 * d + t] = ((const uint8_t *)turn[wave][t - h0])[d];
+                else ((uint16_t *)to)[16 * d + t] = ((const uint16_t *)turn[wave][t - h0])[d];
             }
         return;
     }
     if constexpr (Q8) {                     /* dword column c: channels 4c .. 4c+3; a lane takes D / 64 of them */
         const int c = lane * (D / 64) / 4, j = lane * (D / 64) % 4;
-        uint32_t w[kBlock];
-#pragma unroll
-        for (int t = 0; t < kBlock; t++) w[t] = turn[wave][t][c];
-#pragma unroll
-        for (int e = 0; e < D / 64; e++) {
-            kv_vec<uint32_t, 4> o;
-            const uint32_t pick = 0x0c0c0400u + (uint32_t)(j + e) * 0x0101u;       /* byte j + e of two dwords */
-#pragma unroll
-            for (int q = 0; q < 4; q++)
-                o.v[q] = __builtin_amdgcn_perm(w[4 * q + 1], w[4 * q], pick) |
-                         __builtin_amdgcn_perm(w[4 * q + 3], w[4 * q + 2], pick) << 16;
-            *(kv_vec<uint32_t, 4> *)(to + 16 * (lane * (D / 64) + e)) = o;
-        }
-    } else {                                /* dword column c: channels 2c, 2c+1, of all or half of the tokens */
-        constexpr int TOKENS = D / 8;
-        const int c = lane % (D / 2), t0 = lane / (D / 2) * TOKENS;
         uint32_t w[TOKENS];
 #pragma unroll
-        for (int t = 0; t < TOKENS; t++) w[t] = turn[wave][t0 + t][c];
+        for (int t = 0; t < TOKENS; t++) w[t] = turn[wave][t][c];
 #pragma unroll
-        for (int e = 0; e < 2; e++)
+        for (int e = 0; e < D / 64; e++) {
+            kv_vec<uint32_t, 2> o;
+            const uint32_t pick = 0x0c0c0400u + (uint32_t)(j + e) * 0x0101u;       /* byte j + e of two dwords */
 #pragma unroll
-            for (int h = 0; h < TOKENS / 8; h++) {
-                kv_vec<uint32_t, 4> o;
+            for (int q = 0; q < 2; q++)
+                o.v[q] = __builtin_amdgcn_perm(w[4 * q + 1], w[4 * q], pick) |
+                         __builtin_amdgcn_perm(w[4 * q + 3], w[4 * q + 2], pick) << 16;
+            *(kv_vec<uint32_t, 2> *)(to + 16 * (lane * (D / 64) + e) + h0) = o;
+        }
+    } else {                                /* dword column c: channels 2c, 2c+1, of all or half of the tokens */
+        constexpr int MINE = D / 16;
+        const int c = lane % (D / 2), t0 = lane / (D / 2) * MINE;
+        uint32_t w[MINE];
 #pragma unroll
-                for (int q = 0; q < 4; q++)
-                    o.v[q] = __builtin_amdgcn_perm(w[8 * h + 2 * q + 1], w[8 * h + 2 * q],
-                                                   e ? 0x07060302u : 0x05040100u);
-                *(kv_vec<uint32_t, 4> *)(to + 32 * (2 * c + e) + 2 * (t0 + 8 * h)) = o;
-            }
+        for (int t = 0; t < MINE; t++) w[t] = turn[wave][t0 + t][c];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            kv_vec<uint32_t, MINE / 2> o;
+#pragma unroll
+            for (int q = 0; q < MINE / 2; q++)
+                o.v[q] = __builtin_amdgcn_perm(w[2 * q + 1], w[2 * q], e ? 0x07060302u : 0x05040100u);
+            *(kv_vec<uint32_t, MINE / 2> *)(to + 32 * (2 * c + e) + 2 * (h0 + t0)) = o;
+        }
     }
 }
 
@@ -318,7 +319,9 @@ namespace {
 
 template <int TYPE, typename T, int D>
 hipError_t kv_move(bool write, const kv_args &a, void *k, int64_t ks, void *v, int64_t vs, hipStream_t s) {
-    const dim3 grid((unsigned)kv_slots(a.rows, a.sequences, kBlock, 2), (unsigned)((2 * a.kv_heads + 3) / 4));
+    /* K and V of a head; written in halves of a block */
+    const dim3 grid((unsigned)kv_slots(a.rows, a.sequences, kBlock, 2),
+                    (unsigned)(write ? a.kv_heads : (2 * a.kv_heads + 3) / 4));
     if (write)
         hipLaunchKernelGGL((sera_kv_write_kernel<TYPE, T, D>), grid, dim3(256), 0, s, a, (const T *)k, ks,
                            (const T *)v, vs);
