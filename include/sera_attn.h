@@ -103,8 +103,9 @@ int sera_kv_read(const sera_kv_cache *cache, const sera_kv_batch *batch, uint32_
                  void *v, int64_t v_stride, void *stream);
 
 /* Scratch for sera_attention with these bounds and `heads` query heads on
- * the current device (0: none is needed, or the arguments are refused by
- * the call as well). */
+ * the current device (0: none is needed, or the arguments are refused by the
+ * call as well). It does not grow with the bounds: small batches split their
+ * contexts and need more than large ones. */
 size_t sera_attention_workspace_bytes(const sera_kv_cache *cache, const sera_kv_batch *batch, int heads);
 
 /* out[row][head] = softmax(scale * q . K^T) V of each new row over its

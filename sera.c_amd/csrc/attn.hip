@@ -77,7 +77,8 @@ attn_plans plan_of(const kv_args &a, int dim, int heads, int cus) {
 /* Joins the partial sums of a row: a wave for each (row, query head). A unit of
  * the few-row kernel's sums has a sequence's rows, one of the tile kernel's
  * `columns` of them. Latency, mostly: sequence, then maxima and sums together
- * (one context of 513 tokens in 5 splits: 3 us; 32768 rows in two: 27 us, 3.0 TB/s). */
+ * (one context of 513 tokens in 5 splits: 3 us; 32768 rows in two: 21 us for
+ * 50 MB, 28 when 16 splits were loaded for two). */
 template <typename T, int D>
 __global__ __launch_bounds__(256) void sera_attn_join_kernel(kv_args a, attn_args t, attn_plan few, attn_plan tile,
                                                              size_t tile_sums) {
@@ -103,11 +104,15 @@ __global__ __launch_bounds__(256) void sera_attn_join_kernel(kv_args a, attn_arg
         const float *part =
             t.workspace + (is_few ? 0 : tile_sums) + ((size_t)slot * a.kv_heads + head) * splits * step;
         const float *from = part + (size_t)r * D + E * lane;
-        /* sums are loaded 16 splits at a time, the first together with the maxima that weigh them */
+        /* sums are loaded 16 splits at a time (2, if there are no more), the first together with the maxima that weigh
+         * them */
         constexpr int BATCH = 16;
         attn_vec<float, E> x[BATCH];
+        x[0] = *(const attn_vec<float, E> *)from;
+        x[1] = *(const attn_vec<float, E> *)(from + min(1, used - 1) * step);
+        if (used > 2)
 #pragma unroll
-        for (int k = 0; k < BATCH; k++) x[k] = *(const attn_vec<float, E> *)(from + min(k, used - 1) * step);
+            for (int k = 2; k < BATCH; k++) x[k] = *(const attn_vec<float, E> *)(from + min(k, used - 1) * step);
         float m = kAttnLowest, l = 0.0f;
         if (lane < used) {
             const attn_f2 ml = *(const attn_f2 *)(part + lane * step + (size_t)unit_rows * D + 2 * r);
