@@ -71,7 +71,8 @@ typedef struct {
  * and max_kv are the host's, and hold for every such run. The host cannot
  * check the arrays, the kernels do: a sequence whose rows or length are
  * outside the bounds writes nothing and its rows (those inside [0, rows)) come
- * out as NaN; a page id outside [0, pages) is never followed: its tokens are
+ * out as NaN; where row_start decreases, sequences overlap and what the batch's
+ * rows come out as is not defined (some may be left as they are); a page id outside [0, pages) is never followed: its tokens are
  * not written, and read as NaN. Positions below zero (a sequence with more
  * rows than length) are not written, and read as zeros. */
 typedef struct {

@@ -101,6 +101,7 @@ __global__ __launch_bounds__(256) void sera_attn_join_kernel(kv_args a, attn_arg
         const int used = max((range.count + chunk - 1) / chunk, 1);
         const size_t step = attn_partial_floats(unit_rows, D);
         const int slot = is_few ? s.b : tile0 + unit;
+        if (!is_few && (unsigned)slot >= (unsigned)tile.slots) continue;      /* not run (attn_find_tile) */
         const float *part =
             t.workspace + (is_few ? 0 : tile_sums) + ((size_t)slot * a.kv_heads + head) * splits * step;
         const float *from = part + (size_t)r * D + E * lane;

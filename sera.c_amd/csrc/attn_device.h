@@ -188,7 +188,8 @@ __device__ __forceinline__ int attn_tiles_of(const kv_args &a, const attn_args &
 }
 
 /* Sequence and tile of it in place `slot`, counted from the last: late rows see most and start first. -1: none.
- * *place: the tile's number. */
+ * *place: the tile's number, below `slots`, for which the workspace has room. Where row_start decreases, sequences
+ * overlap and have more tiles than that together; those past the last slot are not run. */
 __device__ __forceinline__ int attn_find_tile(const kv_args &a, const attn_args &t, int per, int slots, int slot,
                                               int *tile, int *place) {
     const int lane = (int)(threadIdx.x & 63);
@@ -211,7 +212,7 @@ __device__ __forceinline__ int attn_find_tile(const kv_args &a, const attn_args 
         total = __builtin_amdgcn_readfirstlane(__shfl(upto[i], 63, 64));
     }
     *place = total - 1 - slot;
-    if (*place < 0) return -1;
+    if (*place < 0 || *place >= slots) return -1;
     for (int i = 0; i < kAttnCounted / 64; i++) {
         const unsigned long long past = __ballot(upto[i] > *place);
         if (past) {

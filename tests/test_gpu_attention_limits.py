@@ -1,0 +1,47 @@
+"""Attention at the limits of what a caller may pass: arrays on the device that break the rules, the largest arguments,
+offsets. Tolerances as in test_gpu_attention.
+"""
+import numpy as np
+import pytest
+
+import attn_oracle as ao
+import q3q4
+from test_gpu_attention import BF16, F16, F32, Setup, check, close, torch  # noqa: F401  (torch: the fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("kind", [ao.F16, ao.Q8])
+@pytest.mark.parametrize("starts,rows,max_new,max_kv", [
+    ([0, 64, 0, 64, 0, 64], 64, 64, 4096),
+    ([0, 200, 0, 200, 0, 200, 0, 200], 200, 200, 4096),
+    ([0, 900, 100, 1000], 1000, 900, 16384),
+    ([0, 1, 0, 200, 1, 2, 0, 200, 3, 4, 5, 6, 7, 8, 9, 10], 200, 200, 4096),
+])
+def test_overlapping_sequences_stay_inside_the_workspace(torch, kind, starts, rows, max_new, max_kv):  # noqa: F811
+    """row_start that decreases: sequences that lie inside the bounds one by one and have more row tiles together than
+    the batch has rows for. Nothing behind the workspace is written, and an ordered batch in the same workspace is
+    right afterwards."""
+    print(f"case overlapping kind={kind} {starts}", flush=True)
+    n = len(starts) - 1
+    s = Setup(torch, kind, F32, [40, 3], [1000, 700], heads=8, kv_heads=1, page=64)
+    cache, _ = s.device()
+    ints = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    # every entry is a page of the pool
+    table = ints(np.resize(s.table[0, :8], (n, max_kv // 64)))
+    batch = q3q4.KVBatch(ints(starts), ints([max_kv - 7 * b for b in range(n)]), table, rows, max_new, max_kv)
+    need = q3q4.load().sera_attention_workspace_bytes(cache.ref, batch.ref, 8)
+    assert need > 0, "the case is meant to leave partial sums"
+    ws = torch.full((need + (64 << 20),), 0xA5, dtype=torch.uint8, device="cuda")
+    q = torch.randn(rows, 1024, device="cuda")
+    out = torch.full((rows + 64, 1024), 7.0, device="cuda")
+    q3q4.attention(cache, batch, q, out[:rows], 0.1, workspace=ws)
+    torch.cuda.synchronize()
+    assert (ws[need:] == 0xA5).all(), "written behind the workspace"
+    assert (out[rows:] == 7.0).all(), "written behind the rows"
+    q, qv = s.rows_of(1024)
+    want, tol = s.expect(qv, 0.1)
+    o = torch.full_like(q, 7.0)
+    assert q3q4.load().sera_attention_workspace_bytes(cache.ref, s.batch.ref, 8) <= ws.numel()
+    q3q4.attention(cache, s.batch, q, o, 0.1, workspace=ws)
+    close(o, want, tol, "ordered")
