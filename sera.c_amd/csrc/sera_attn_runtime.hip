@@ -170,7 +170,9 @@ int sera_attention(const sera_kv_cache *cache, const sera_kv_batch *batch, uint3
     t.heads = heads;
     t.group = heads / cache->kv_heads;
     t.scale_log2 = (float)((double)scale * 1.4426950408889634);
-    t.window = window;
+    /* A window of all positions is none. Below that it is under kMaxPositions, so p - window stays inside an int for
+     * every position p of a row, those in front of a sequence's start (p >= -kMaxRows) among them. */
+    t.window = window < batch->max_kv ? window : 0;
     t.sinks = sinks;
     t.workspace = (float *)workspace;
     t.cus = device_cus();

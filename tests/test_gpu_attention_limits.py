@@ -45,3 +45,16 @@ def test_overlapping_sequences_stay_inside_the_workspace(torch, kind, starts, ro
     assert q3q4.load().sera_attention_workspace_bytes(cache.ref, s.batch.ref, 8) <= ws.numel()
     q3q4.attention(cache, s.batch, q, o, 0.1, workspace=ws)
     close(o, want, tol, "ordered")
+
+
+@pytest.mark.parametrize("kind", [ao.F16, ao.Q8])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 40, 2 ** 30, 129, 128])
+@pytest.mark.parametrize("news,lens", [([50, 33], [7, 40]), ([2, 1], [1, 128]), ([300], [128])])
+def test_windows_as_wide_as_the_context_are_none(torch, kind, window, news, lens):  # noqa: F811
+    """A window of every position or more, up to the largest int: the result is that of no window, bit for bit, also
+    where a sequence has rows in front of its start."""
+    s = Setup(torch, kind, F32, news, lens, heads=8, kv_heads=2, page=16)
+    print(f"case wide window kind={kind} window={window} {news} of {lens}", flush=True)
+    q, first = check(s)
+    for sinks in (0, 5, 2 ** 31 - 1):
+        assert torch.equal(s.attend(q, s.dim ** -0.5, window, sinks), first)
