@@ -141,13 +141,16 @@ __device__ __forceinline__ bool attn_take_odd(attn_h8 &v, attn_h8 &odd) {
     return any;
 }
 
-/* log2 of a V scale, held inside the range where weights and their sum stay
- * normal fp32 numbers: 8-bit caches take the running maximum over s +
+/* log2 of a V scale: 8-bit caches take the running maximum over s +
  * log2(V scale), so that weight * scale fits fp16 however far the scales are
- * apart. A NaN stays out of the maximum (fmaxf takes the other). */
+ * apart. It is held inside -84 .. 121, for weights and their sum to stay normal
+ * fp32 numbers: a weight is at most 2^(84 + kAttnBias + kAttnLag) = 2^99, the sum of 2^28 of them (all positions that a
+ * sequence can have) 2^127; values whose scales are all below 2^-84 lose bits, and
+ * vectors of zeros (scale 0) count as such. A NaN stays out of the maximum (fmaxf
+ * takes the other). */
 __device__ __forceinline__ float attn_log_scale(float vs) {
     const float l = __builtin_amdgcn_logf(fabsf(vs));
-    return l < -100.0f ? -100.0f : l > 121.0f ? 121.0f : l;
+    return l < -84.0f ? -84.0f : l > 121.0f ? 121.0f : l;
 }
 
 template <typename T>

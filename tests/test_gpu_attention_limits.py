@@ -58,3 +58,33 @@ def test_windows_as_wide_as_the_context_are_none(torch, kind, window, news, lens
     q, first = check(s)
     for sinks in (0, 5, 2 ** 31 - 1):
         assert torch.equal(s.attend(q, s.dim ** -0.5, window, sinks), first)
+
+
+@pytest.mark.parametrize("new", [40, 1])
+def test_long_runs_of_zero_values(torch, new):  # noqa: F811
+    """An 8-bit context whose values are zero vectors (scale 0) but for the last 128, with scores that rise by 7.9
+    binades (less than the running maximum follows) behind the first 256: a sum of 56000 weights whose values hold
+    none of them down. The result is the sum of the last values over all weights."""
+    sequences, heads, kv_heads, dim, page, length = 32, 64, 8, 128, 128, 56064
+    rng = np.random.default_rng(2)
+    pages = length // page
+    pool = np.zeros((pages, kv_heads, ao.head_bytes(ao.Q8, page, dim)), np.uint8)
+    k, v, ks, vs = ao.views(pool, ao.Q8, page, kv_heads, dim)
+    k[2:], ks[2:] = 100, 1e-4                  # 0.01 in each channel
+    v[-1], vs[-1] = rng.integers(60, 128, v[-1].shape), 1 / 80
+    ints = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    cache = q3q4.KVCache(ao.Q8, pages, page, kv_heads, dim, torch.from_numpy(pool.reshape(-1)).cuda())
+    table = ints(range(pages))[None].expand(sequences, -1).contiguous()
+    batch = q3q4.KVBatch(ints([new * b for b in range(sequences + 1)]), ints([length] * sequences), table,
+                         new * sequences, new, length)
+    scale = 7.9 * np.log(2) / (0.01 * dim)
+    out = torch.full((new * sequences, heads * dim), 7.0, device="cuda")
+    q3q4.attention(cache, batch, torch.ones_like(out), out, scale,
+                   workspace=q3q4.attention_workspace(cache, batch, heads))
+    K, V = ao.values(pool, ao.Q8, page, kv_heads, dim, [list(range(pages))], 0, length)
+    n = min(new, 4)                            # the last rows, of the first and the last head
+    want, tol = ao.attend(K[[0, -1]], V[[0, -1]], np.ones((n, 2, dim)), length, scale, 0, 0, ao.F32T)
+    assert want.min() > 20 * tol.max()
+    for b in (0, sequences - 1):
+        got = out[(b + 1) * new - n:(b + 1) * new].view(n, heads, dim)[:, [0, -1]]
+        close(got, want, tol, f"sequence {b}")
