@@ -562,15 +562,15 @@ KV_Q8 = 264     # SERA_KV_Q8: int8 codes, one float scale per token and kv head
 _ROW_TYPES = {}
 
 
-def _rows(t, n, width):
-    """(type id, data pointer, row stride) of rows [n or more, width]."""
+def _rows(t, n, width, device):
+    """(type id, data pointer, row stride) of rows [n or more, width] on a device, by its index."""
     if not _ROW_TYPES:
         import torch
         _ROW_TYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 30})
     ty, shape, stride = _ROW_TYPES.get(t.dtype), t.shape, t.stride()
-    if ty is None or len(shape) != 2 or stride[1] != 1 or not t.is_cuda:
-        raise Q3Q4Error("rows must be a 2-d float32, float16 or bfloat16 device tensor with contiguous rows, "
-                        f"got {tuple(t.shape)} {t.dtype} strides {t.stride()}")
+    if ty is None or len(shape) != 2 or stride[1] != 1 or t.get_device() != device:
+        raise Q3Q4Error("rows must be a 2-d float32, float16 or bfloat16 device tensor with contiguous rows on the "
+                        f"cache's device, got {tuple(t.shape)} {t.dtype} strides {t.stride()} on {t.device}")
     if shape[0] < n or shape[1] != width:
         raise Q3Q4Error(f"rows must be [{n}, {width}], got {tuple(t.shape)}")
     return ty, t.data_ptr(), stride[0]
@@ -594,6 +594,7 @@ class KVCache:
             data = torch.empty(pages * self.page_bytes, dtype=torch.uint8, device=f"cuda:{device}")
         if data.dtype != torch.uint8 or not data.is_contiguous() or data.numel() < pages * self.page_bytes:
             raise Q3Q4Error(f"the cache's data must be {pages * self.page_bytes} contiguous uint8")
+        self.device = data.get_device()      # -1: the host, which the calls refuse
         self.type, self.pages, self.page_tokens = type, pages, page_tokens
         self.kv_heads, self.head_dim, self.data, self.width = kv_heads, head_dim, data, kv_heads * head_dim
         self.args = KVCacheArgs(type, page_tokens, kv_heads, head_dim, pages, data.data_ptr())
@@ -612,6 +613,9 @@ class KVBatch:
         for t, shape in ((row_start, (n + 1,)), (kv_len, (n,)), (page_table, (n, page_table.shape[-1]))):
             if t.dtype != torch.int32 or tuple(t.shape) != shape or (t.numel() > 1 and t.stride(-1) != 1):
                 raise Q3Q4Error(f"batch tensors are int32 with contiguous rows, got {t.dtype} {tuple(t.shape)}")
+            if t.device != kv_len.device:
+                raise Q3Q4Error(f"batch tensors are on one device, got {t.device} and {kv_len.device}")
+        self.device = kv_len.get_device()    # -1: the host, which the calls refuse
         self.row_start, self.kv_len, self.page_table = row_start, kv_len, page_table
         self.rows, self.max_new, self.max_kv = rows, max_new, max_kv
         # one sequence's table may have any stride: it is never used
@@ -630,8 +634,11 @@ def _pair(cache, batch, width, x, y):
     """Two row operands of one type, checked against the batch: (type, pointer, stride, pointer, stride)."""
     if batch.max_kv > batch.entries * cache.page_tokens:
         raise Q3Q4Error(f"max_kv={batch.max_kv} is more than {batch.entries} pages of {cache.page_tokens} hold")
-    ty, xp, xs = _rows(x, batch.rows, width)
-    ty2, yp, ys = _rows(y, batch.rows, width)
+    if cache.device < 0 or batch.device != cache.device:
+        raise Q3Q4Error("the cache's data and the batch's tensors must be device tensors on one device, got "
+                        f"{cache.data.device} and {batch.kv_len.device}")
+    ty, xp, xs = _rows(x, batch.rows, width, cache.device)
+    ty2, yp, ys = _rows(y, batch.rows, width, cache.device)
     if ty != ty2:
         raise Q3Q4Error(f"rows must be of one type, got {x.dtype} and {y.dtype}")
     return ty, xp, xs, yp, ys
@@ -663,6 +670,11 @@ def attention(cache, batch, q, out, scale, window=0, sinks=0, workspace=None, st
     ty, qp, qs, op, os_ = _pair(cache, batch, width, q, out)
     if width % cache.head_dim:
         raise Q3Q4Error(f"rows of {width} are no heads of {cache.head_dim}")
-    wp, wb = (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if workspace is not None else (0, 0)
+    wp, wb = 0, 0
+    if workspace is not None:
+        if workspace.get_device() != cache.device or not workspace.is_contiguous():
+            raise Q3Q4Error("the workspace must be a contiguous tensor on the cache's device, got "
+                            f"{tuple(workspace.shape)} strides {workspace.stride()} on {workspace.device}")
+        wp, wb = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     _check(load().sera_attention(cache.ref, batch.ref, ty, qp, qs, op, os_, width // cache.head_dim, scale, window,
                                  sinks, wp, wb, _stream(stream)), "sera_attention")
