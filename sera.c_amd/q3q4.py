@@ -666,7 +666,7 @@ def attention_workspace(cache, batch, heads):
 def attention(cache, batch, q, out, scale, window=0, sinks=0, workspace=None, stream=None):
     """out[row] = attention of q[row] over its sequence's cache; q, out
     [rows, heads * head_dim] of one type. window 0: the whole context."""
-    width = q.shape[1]
+    width = q.shape[-1] if len(q.shape) else 0       # rows that are not 2-d are refused next
     ty, qp, qs, op, os_ = _pair(cache, batch, width, q, out)
     if width % cache.head_dim:
         raise Q3Q4Error(f"rows of {width} are no heads of {cache.head_dim}")

@@ -83,3 +83,12 @@ def test_a_batch_is_on_one_device(at):
     t[at] = ints(*t[at].shape, device="meta")
     with pytest.raises(q3q4.Q3Q4Error, match="one device"):
         q3q4.KVBatch(*t, 2, 1, 16)
+
+
+@pytest.mark.parametrize("shape", [(), (64,), (1, 2, 64)])
+def test_attention_of_rows_that_are_not_2d_is_refused(shape):
+    c, b = cache_and_batch(0, 0)
+    q = OnDevice(2, 64)
+    q.shape, q.stride = shape, lambda: (1,) * len(shape)
+    with pytest.raises(q3q4.Q3Q4Error, match="2-d"):
+        q3q4.attention(c, b, q, q, 0.1)
