@@ -105,8 +105,10 @@ int sera_kv_read(const sera_kv_cache *cache, const sera_kv_batch *batch, uint32_
 
 /* Scratch for sera_attention with these bounds and `heads` query heads on
  * the current device (0: none is needed, or the arguments are refused by the
- * call as well). It does not grow with the bounds: small batches split their
- * contexts and need more than large ones. */
+ * call as well): partial sums of contexts that are split over workgroups, which
+ * is done only as far as compute units would be idle. So it is bounded, by 39
+ * MB on 256 compute units, and not monotone in the batch: one that fills the device
+ * needs none, a smaller one may need more. */
 size_t sera_attention_workspace_bytes(const sera_kv_cache *cache, const sera_kv_batch *batch, int heads);
 
 /* out[row][head] = softmax(scale * q . K^T) V of each new row over its

@@ -62,21 +62,25 @@ attn_plans plan_of(const kv_args &a, int dim, int heads, int cus) {
         p.tile.columns = 256;
         while (p.tile.columns > 64 && columns <= p.tile.columns / 2) p.tile.columns /= 2;
         if (p.tile.columns == 256 && (all + 255) / 256 * a.kv_heads < cus && a.max_kv <= 8192) p.tile.columns = 128;
-        p.tile.slots = (int)(all / p.tile.columns + a.sequences);
+        /* A sequence has a ragged tile at most; of those counted one by one, only sequences of more than few_columns
+         * have any. */
+        const int64_t ragged = all / (p.few_columns + 1);
+        p.tile.slots = (int)(all / p.tile.columns +
+                             (a.sequences <= kAttnCounted && ragged < a.sequences ? ragged : a.sequences));
         split_of(p.tile, a, cus / ((all + p.tile.columns - 1) / p.tile.columns * a.kv_heads), 8);
     }
     const size_t row = (size_t)a.kv_heads * (dim + 2) * sizeof(float);
     if (p.few.splits > 1) p.few_bytes = ((size_t)a.sequences * p.few.splits * p.few_rows * row + 15) & ~(size_t)15;
     p.bytes = p.few_bytes;
-    if (p.tile.splits > 1) p.bytes += (size_t)p.tile.slots * p.tile.splits * p.tile.columns * row;
+    if (p.tile.splits > 1) p.bytes += (size_t)a.rows * group * p.tile.splits * row;
     return p;
 }
 
 }  // namespace
 
-/* Joins the partial sums of a row: a wave for each (row, query head). A unit of
- * the few-row kernel's sums has a sequence's rows, one of the tile kernel's
- * `columns` of them. Latency, mostly: sequence, then maxima and sums together
+/* Joins the partial sums of a row: a wave for each (row, query head). How many
+ * splits have any goes by unit: a sequence's rows in the few-row kernel, `columns`
+ * of them in the tile kernel. Latency, mostly: sequence, then maxima and sums together
  * (one context of 513 tokens in 5 splits: 3 us; 32768 rows in two: 21 us for
  * 50 MB, 28 when 16 splits were loaded for two). */
 template <typename T, int D>
@@ -92,31 +96,35 @@ __global__ __launch_bounds__(256) void sera_attn_join_kernel(kv_args a, attn_arg
     const int splits = is_few ? few.splits : tile.splits, chunk = is_few ? few.chunk : tile.chunk;
     if (splits < 2) return;
     const int unit_rows = is_few ? t.few_rows : tile.columns;
-    const int tile0 = is_few ? 0 : attn_first_tile(a, t, unit_rows, s.b, s.row0);
     for (int h = (int)blockIdx.y * 4 + wave; h < t.heads; h += (int)gridDim.y * 4) {
         const int head = h / t.group, row = i * t.group + h % t.group, unit = row / unit_rows;
-        const int r = row - unit * unit_rows, last = min((unit + 1) * unit_rows, rows) - 1;
+        const int last = min((unit + 1) * unit_rows, rows) - 1;
         const attn_range range = attn_range_of(t, max(first + unit * unit_rows / t.group, 0),
                                                first + last / t.group + 1, kAttnShift);
         const int used = max((range.count + chunk - 1) / chunk, 1);
-        const size_t step = attn_partial_floats(unit_rows, D);
-        const int slot = is_few ? s.b : tile0 + unit;
-        if (!is_few && (unsigned)slot >= (unsigned)tile.slots) continue;      /* not run (attn_find_tile) */
-        const float *part =
-            t.workspace + (is_few ? 0 : tile_sums) + ((size_t)slot * a.kv_heads + head) * splits * step;
-        const float *from = part + (size_t)r * D + E * lane;
+        /* sums, and maxima with their weights' sums, of this row's first split, and how far apart those of two splits
+         * are: in floats, of which the workspace has some 10^7 */
+        const int place = is_few ? s.b * a.kv_heads + head : (s.row0 + i) * t.heads + h;
+        const int step = is_few ? (int)attn_partial_floats(unit_rows, D) : D, ml_step = is_few ? step : 2;
+        const int sums = place * splits * step + (is_few ? row * D : 0);
+        const int ml_at = is_few ? sums - row * D + unit_rows * D + 2 * row
+                                 : (a.rows * t.heads * D + 2 * place) * splits;
+        const float *const base = t.workspace + (is_few ? 0 : tile_sums);
+        const auto sum_of = [&](int split) {
+            return *(const attn_vec<float, E> *)(base + (uint32_t)(sums + min(split, used - 1) * step + E * lane));
+        };
         /* sums are loaded 16 splits at a time (2, if there are no more), the first together with the maxima that weigh
          * them */
         constexpr int BATCH = 16;
         attn_vec<float, E> x[BATCH];
-        x[0] = *(const attn_vec<float, E> *)from;
-        x[1] = *(const attn_vec<float, E> *)(from + min(1, used - 1) * step);
+        x[0] = sum_of(0);
+        x[1] = sum_of(1);
         if (used > 2)
 #pragma unroll
-            for (int k = 2; k < BATCH; k++) x[k] = *(const attn_vec<float, E> *)(from + min(k, used - 1) * step);
+            for (int k = 2; k < BATCH; k++) x[k] = sum_of(k);
         float m = kAttnLowest, l = 0.0f;
         if (lane < used) {
-            const attn_f2 ml = *(const attn_f2 *)(part + lane * step + (size_t)unit_rows * D + 2 * r);
+            const attn_f2 ml = *(const attn_f2 *)(base + (uint32_t)(ml_at + lane * ml_step));
             m = ml[0];
             l = ml[1];
         }
@@ -136,16 +144,15 @@ __global__ __launch_bounds__(256) void sera_attn_join_kernel(kv_args a, attn_arg
         l += xor_partner<16>(l);
         l += xor_partner<32>(l);
         float y[E] = {};
-        for (int base = 0; base < used; base += BATCH) {
-            if (base > 0)
+        for (int split = 0; split < used; split += BATCH) {
+            if (split > 0)
 #pragma unroll
-                for (int k = 0; k < BATCH; k++)
-                    x[k] = *(const attn_vec<float, E> *)(from + min(base + k, used - 1) * step);
+                for (int k = 0; k < BATCH; k++) x[k] = sum_of(split + k);
 #pragma unroll
             for (int k = 0; k < BATCH; k++) {
-                const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), (base + k) & 63));
+                const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), (split + k) & 63));
 #pragma unroll
-                for (int e = 0; e < E; e++) y[e] = base + k < used ? fmaf(x[k].v[e], w, y[e]) : y[e];
+                for (int e = 0; e < E; e++) y[e] = split + k < used ? fmaf(x[k].v[e], w, y[e]) : y[e];
             }
         }
         attn_vec<T, E> o;

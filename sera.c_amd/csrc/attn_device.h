@@ -191,15 +191,12 @@ __device__ __forceinline__ int attn_tiles_of(const kv_args &a, const attn_args &
 }
 
 /* Sequence and tile of it in place `slot`, counted from the last: late rows see most and start first. -1: none.
- * *place: the tile's number, below `slots`, for which the workspace has room. Where row_start decreases, sequences
- * overlap and have more tiles than that together; those past the last slot are not run. */
+ * Where row_start decreases, sequences overlap and may have more tiles together than there are slots: the first
+ * ones are not run. */
 __device__ __forceinline__ int attn_find_tile(const kv_args &a, const attn_args &t, int per, int slots, int slot,
-                                              int *tile, int *place) {
+                                              int *tile) {
     const int lane = (int)(threadIdx.x & 63);
-    if (a.sequences > kAttnCounted) {
-        *place = slots - 1 - slot;
-        return kv_find(a, *place, per, 1, tile, t.group);
-    }
+    if (a.sequences > kAttnCounted) return kv_find(a, slots - 1 - slot, per, 1, tile, t.group);
     int n[kAttnCounted / 64], upto[kAttnCounted / 64], total = 0;
 #pragma unroll
     for (int i = 0; i < kAttnCounted / 64; i++) {
@@ -214,31 +211,24 @@ __device__ __forceinline__ int attn_find_tile(const kv_args &a, const attn_args 
         upto[i] += total;
         total = __builtin_amdgcn_readfirstlane(__shfl(upto[i], 63, 64));
     }
-    *place = total - 1 - slot;
-    if (*place < 0 || *place >= slots) return -1;
+    const int place = total - 1 - slot;
+    if (place < 0) return -1;
     for (int i = 0; i < kAttnCounted / 64; i++) {
-        const unsigned long long past = __ballot(upto[i] > *place);
+        const unsigned long long past = __ballot(upto[i] > place);
         if (past) {
             const int l = __builtin_ctzll(past);
-            *tile = __builtin_amdgcn_readfirstlane(*place - (__shfl(upto[i], l, 64) - __shfl(n[i], l, 64)));
-            return 64 * i + l;
+            const int own = __shfl(n[i], l, 64);
+            *tile = __builtin_amdgcn_readfirstlane(place - (__shfl(upto[i], l, 64) - own));
+            /* not one of its tiles: only where overlapping sequences' sum left an int */
+            return (unsigned)*tile < (unsigned)__builtin_amdgcn_readfirstlane(own) ? 64 * i + l : -1;
         }
     }
     return -1;
 }
 
-/* The number of sequence b's first tile, row0 its first row. */
-__device__ __forceinline__ int attn_first_tile(const kv_args &a, const attn_args &t, int per, int b, int row0) {
-    if (a.sequences > kAttnCounted) return row0 * t.group / per + b;
-    const int lane = (int)(threadIdx.x & 63);
-    int sum = 0;
-    for (int i = lane; i < b; i += 64) sum += attn_tiles_of(a, t, i, per);
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    return sum;
-}
-
-/* A partial result: rows of D sums, then (m, l) of every row. */
+/* Partial results of a split context, in the workspace. Few rows: a unit of `rows` rows for each sequence, kv head and
+ * split, rows of D sums and then (m, l) of every row. Tiles: by packed row, which stays inside the batch's rows
+ * whatever row_start holds: D sums for each (row, query head, split), and behind them all (m, l) in the same order. */
 __device__ __forceinline__ size_t attn_partial_floats(int rows, int dim) { return (size_t)rows * (dim + 2); }
 
 #endif

@@ -126,11 +126,11 @@ void sera_attn_tile_kernel(kv_args a, attn_args t, int slots, int splits, int ch
     constexpr int PER = S::PER, PIECES = S::PIECES, ES = Q8 ? 1 : 2;
     __shared__ tile_lds<TYPE, D, RG, KG> lds;
 
-    int slot = (int)(blockIdx.z * gridDim.y + blockIdx.y);
+    const int slot = (int)(blockIdx.z * gridDim.y + blockIdx.y);
     if (slot >= slots) return;
     const int head = (int)blockIdx.x % a.kv_heads, split = (int)blockIdx.x / a.kv_heads;
     int unit;
-    const int b = attn_find_tile(a, t, BR, slots, slot, &unit, &slot);
+    const int b = attn_find_tile(a, t, BR, slots, slot, &unit);
     if (b < 0) return;
     const kv_seq s = kv_sequence(a, b);
     const int rows = s.n * t.group, r0 = unit * BR;
@@ -635,11 +635,17 @@ void sera_attn_tile_kernel(kv_args a, attn_args t, int slots, int splits, int ch
             *(attn_f4 *)(box + col * D + (((8 * n + 2 * i + half) ^ (col & (D / 4 - 1))) << 2)) = y;
         }
     asm volatile("" ::: "memory");
-    float *partial = t.workspace + (((size_t)slot * a.kv_heads + head) * splits + split) * attn_partial_floats(BR, D);
+    /* Partial sums by packed row, query head and split; their maxima and sums behind them all. */
+    float *const ml = t.workspace + (size_t)a.rows * t.heads * splits * D;
+    auto partial = [&](int local) {
+        int h;
+        const int at = place(local, h);
+        return ((size_t)(s.row0 + at) * t.heads + head * t.group + h) * splits + split;
+    };
     if (splits > 1 && half == 0 && w0 + col < rows) {
-        const int r = 32 * rg + col;
-        partial[(size_t)BR * D + 2 * r] = m;
-        partial[(size_t)BR * D + 2 * r + 1] = l;
+        const size_t k = partial(32 * rg + col);
+        ml[2 * k] = m;
+        ml[2 * k + 1] = l;
     }
     constexpr int ROWS = 64 / (D / 4);
 #pragma unroll 4
@@ -648,7 +654,7 @@ void sera_attn_tile_kernel(kv_args a, attn_args t, int slots, int splits, int ch
         if (w0 + r >= rows) break;
         const attn_f4 y = *(const attn_f4 *)(box + r * D + ((u ^ (r & (D / 4 - 1))) << 2));
         if (splits > 1) {
-            *(attn_f4 *)(partial + (size_t)(32 * rg + r) * D + 4 * u) = y;
+            *(attn_f4 *)(t.workspace + partial(32 * rg + r) * D + 4 * u) = y;
         } else {
             int h;
             const int at = place(32 * rg + r, h);
