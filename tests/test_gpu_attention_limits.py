@@ -88,3 +88,30 @@ def test_long_runs_of_zero_values(torch, new):  # noqa: F811
     for b in (0, sequences - 1):
         got = out[(b + 1) * new - n:(b + 1) * new].view(n, heads, dim)[:, [0, -1]]
         close(got, want, tol, f"sequence {b}")
+
+
+@pytest.mark.parametrize("kind", [ao.F16, ao.Q8])
+def test_rows_more_than_two_to_the_31_elements_apart(torch, kind):  # noqa: F811
+    """Four rows 3 * 2^28 elements apart, the last 2.4e9 from the first, as keys and values in and out, q and result."""
+    stride, width = 3 << 28, 1024
+    buf = torch.empty(3 * stride + 4 * width, device="cuda")
+    far = [buf.as_strided((4, width), (stride, 1), width * i) for i in range(4)]
+    i = lambda *a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    cache = q3q4.KVCache(kind, 1, 16, 8, 128)
+    cache.data.zero_()
+    batch = q3q4.KVBatch(i(0, 4), i(4), i(0)[None], 4, 4, 16)
+    for f in far:
+        f.copy_(torch.randn(4, width, device="cuda"))
+    near = [f.clone() for f in far]
+    q3q4.kv_write(cache, batch, far[0], far[1])
+    pool = np.zeros((1, 8, ao.head_bytes(kind, 16, 128)), np.uint8)
+    ao.write(pool, kind, 16, 8, 128, [[0]], [0, 4], [4], *(t.cpu().numpy() for t in near[:2]))
+    assert np.array_equal(cache.data.cpu().numpy(), pool.reshape(-1))
+    q3q4.kv_read(cache, batch, far[0], far[1])
+    K, V = ao.values(pool, kind, 16, 8, 128, [[0]], 0, 4)
+    for f, x in ((far[0], K), (far[1], V)):
+        assert np.array_equal(f.cpu().numpy(), x.transpose(1, 0, 2).reshape(4, width).astype(np.float32))
+    assert torch.equal(far[2], near[2]) and torch.equal(far[3], near[3])
+    q3q4.attention(cache, batch, far[2], far[3], 0.1, workspace=q3q4.attention_workspace(cache, batch, 8))
+    want, tol = ao.attend(K, V, near[2].double().cpu().numpy().reshape(4, 8, 128), 4, 0.1, 0, 0, ao.F32T)
+    close(far[3], want.reshape(4, -1), tol.reshape(4, -1), "far rows")
