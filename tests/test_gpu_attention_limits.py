@@ -115,3 +115,29 @@ def test_rows_more_than_two_to_the_31_elements_apart(torch, kind):  # noqa: F811
     q3q4.attention(cache, batch, far[2], far[3], 0.1, workspace=q3q4.attention_workspace(cache, batch, 8))
     want, tol = ao.attend(K, V, near[2].double().cpu().numpy().reshape(4, 8, 128), 4, 0.1, 0, 0, ao.F32T)
     close(far[3], want.reshape(4, -1), tol.reshape(4, -1), "far rows")
+
+
+@pytest.mark.parametrize("kind", [ao.F16, ao.Q8])
+@pytest.mark.parametrize("sequences", [300, 70, 40])
+def test_overlapping_sequences_in_every_search(torch, kind, sequences):  # noqa: F811
+    """The same for as many sequences as take each of the searches over row_start, and for writes and reads: they end,
+    and nothing but the batch's rows, the workspace and the tables' pages is written."""
+    print(f"case overlapping kind={kind} sequences={sequences}", flush=True)
+    rows, pages, page, heads, width, pad = 100, 40, 64, 8, 128, 16
+    ints = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    cache = q3q4.KVCache(kind, pages, page, 1, 128)
+    cache.data.zero_()
+    starts = [(0, 90, 30, 100, 29)[b % 5] for b in range(sequences + 1)]
+    table = ints(np.resize(np.arange(3, 23), (sequences, 64)))
+    batch = q3q4.KVBatch(ints(starts), ints([4000 - b for b in range(sequences)]), table, rows, 95, 4096)
+    need = q3q4.load().sera_attention_workspace_bytes(cache.ref, batch.ref, heads)
+    ws = torch.full((need + (32 << 20),), 0xA5, dtype=torch.uint8, device="cuda")
+    k, q = torch.randn(rows, width, device="cuda"), torch.randn(rows, heads * width, device="cuda")
+    out, ko, vo = (torch.full((rows + pad, w), 7.0, device="cuda") for w in (heads * width, width, width))
+    q3q4.kv_write(cache, batch, k, k)
+    q3q4.kv_read(cache, batch, ko[:rows], vo[:rows])
+    q3q4.attention(cache, batch, q, out[:rows], 0.1, workspace=ws)
+    torch.cuda.synchronize()
+    assert (ws[need:] == 0xA5).all() and all((t[rows:] == 7.0).all() for t in (out, ko, vo))
+    held = cache.data.view(pages, -1)
+    assert not held[:3].any() and not held[23:].any() and held[3:23].any()
