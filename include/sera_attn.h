@@ -116,9 +116,10 @@ size_t sera_attention_workspace_bytes(const sera_kv_cache *cache, const sera_kv_
  * [heads * head_dim] of `type` with their own strides; query head h reads
  * kv head h / (heads / kv_heads). The row at position p sees the positions
  * j <= p; with window > 0 only j > p - window, and the first `sinks`
- * positions, which stay visible. (The new rows' keys and values are written
- * before, by sera_kv_write.) A position that a row does not see has no
- * effect on it, whatever it holds. A row that sees nothing comes out as zeros.
+ * positions, which stay visible (a window of max_kv or more hides none). (The
+ * new rows' keys and values are written before, by sera_kv_write.) A position
+ * that a row does not see has no effect on it, whatever it holds. A row that
+ * sees nothing comes out as zeros.
  *
  * Products run on fp16 matrix instructions with fp32 sums: for fp16 and bf16
  * rows with q and the softmax weights rounded once to fp16, for fp32 rows

@@ -39,7 +39,8 @@ attn_plans plan_of(const kv_args &a, int dim, int heads, int cus) {
     /* One kernel takes all sequences, unless they differ much: where they have less than half of the longest one's
      * rows on average, those of a token or so (a group's rows, rounded up to what the few-row kernel holds) go to it
      * and the others to the tiles, in two launches (a chunk of 512 rows over 4096 positions and 31 tokens over 3000
-     * each: 239 us, 279 all in tiles; from an 8-bit cache 228 and 314). */
+     * each: 235 us, 279 all in tiles; from an 8-bit cache 229 and 305; 64 rows and 63 tokens over 3000: 188 and 333,
+     * 132 and 352). */
     if (columns <= kFewColumns) p.few_columns = 0x7fffffff;
     else if (group <= kFewColumns && 2ll * a.rows < (int64_t)a.sequences * a.max_new)
         p.few_columns = group <= 8 ? 8 : group <= 16 ? 16 : 32;
@@ -48,17 +49,17 @@ attn_plans plan_of(const kv_args &a, int dim, int heads, int cus) {
         p.few.columns = most <= 8 ? 8 : most <= 16 ? 16 : 32;
         p.few_rows = columns <= kFewColumns ? (int)columns : p.few_columns / group * group;
         /* Split contexts only as far as there are CUs without a workgroup: joining costs a launch, and more
-         * workgroups a CU repeat the start (32 windows of 1024 tokens, 256 workgroups: 34 us whole, 40 in two; 24
-         * contexts of 1050-2100 tokens, 192 workgroups: 32 us whole, 33 in two, 31 in four; one context of 8000, 8
-         * workgroups whole: 17 us in 32, 18 in 63). At least a tile for each of the four waves. */
+         * workgroups a CU repeat the start (32 windows of 1024 tokens, 256 workgroups: 33 us whole, 38 in two; 24
+         * contexts of 1050-2100 tokens, 192 workgroups: 39 us whole, 44 in two, from an 8-bit cache 25 and 29; one
+         * context of 8000, 8 workgroups whole: 15 us in 32, 17 in 63). At least a tile for each of the four waves. */
         split_of(p.few, a, (int64_t)cus / ((int64_t)a.sequences * a.kv_heads), 4);
     }
     if (columns > kFewColumns) {
         const int64_t all = (int64_t)a.rows * group;
         /* 256 rows a workgroup load each key and value for the most rows, if that leaves every CU one. If not, 128
          * rows (two groups of waves over the tokens) for contexts up to 8192 tokens, where partial sums cost more
-         * than they give: 16 branches of 256 rows over 1568 tokens take 74 us so and 93 us as 256 rows split in two;
-         * 512 rows x 8 over 32768 tokens 1175 us so and 1031 us split. */
+         * than they give: 16 branches of 256 rows over 1568 tokens take 73 us so and 87 us as 256 rows split in two;
+         * 512 rows x 8 over 8192 tokens 276 us and 271 us, over 32768 (8 bits) 1160 us and 1035 us. */
         p.tile.columns = 256;
         while (p.tile.columns > 64 && columns <= p.tile.columns / 2) p.tile.columns /= 2;
         if (p.tile.columns == 256 && (all + 255) / 256 * a.kv_heads < cus && a.max_kv <= 8192) p.tile.columns = 128;
@@ -81,8 +82,8 @@ attn_plans plan_of(const kv_args &a, int dim, int heads, int cus) {
 /* Joins the partial sums of a row: a wave for each (row, query head). How many
  * splits have any goes by unit: a sequence's rows in the few-row kernel, `columns`
  * of them in the tile kernel. Latency, mostly: sequence, then maxima and sums together
- * (one context of 513 tokens in 5 splits: 3 us; 32768 rows in two: 21 us for
- * 50 MB, 28 when 16 splits were loaded for two). */
+ * (one context of 513 tokens in 5 splits: 4 us; 32768 rows in two: 22 us for
+ * 50 MB, 28 when the sums of a row tile lay together and not those of a row). */
 template <typename T, int D>
 __global__ __launch_bounds__(256) void sera_attn_join_kernel(kv_args a, attn_args t, attn_plan few, attn_plan tile,
                                                              size_t tile_sums) {
@@ -199,7 +200,7 @@ hipError_t sera_launch_attn(uint32_t cache_type, uint32_t type, int dim, const k
     shorten(p.few, a, t);
     shorten(p.tile, a, t);
     /* Whole contexts, a CU to each workgroup: eight waves of an 8-bit cache, whose conversions they share (24 contexts of
-     * 1050-2100 tokens: 29 us, 32 with four). From fp16 the four are as fast (40 and 40), and split contexts
+     * 1050-2100 tokens: 25.5 us, 28.7 with four). From fp16 the four are as fast (40 and 40), and split contexts
      * have few tiles for more (one of 513 tokens: 11 us with four, 14 with eight). */
     p.few.waves = cache_type == SERA_KV_Q8 && p.few.columns <= 16 && p.few.splits == 1 &&
                   (int64_t)a.sequences * a.kv_heads <= args.cus ? 8 : 4;

@@ -23,7 +23,7 @@
  * split over workgroups, joined by sera_attn_join_kernel.
  *
  * Bound by memory once contexts are long: 64 of 8192 tokens (2.15 GB of fp16) in
- * 370 us, 5.8 TB/s. A call costs about 9 us (fp16; 10 us 8 bits) beyond the bytes
+ * 352 us, 6.1 TB/s (368 us back to back in a graph). A call costs about 9 us (fp16; 10 us 8 bits) beyond the bytes
  * at that rate: launch, two rounds of dependent loads (sequence and pages; data),
  * the last tile's products and the joins. K's and V's registers are loaded again
  * as soon as a tile's products have taken them, 16 KB a wave on the way (8 KB of

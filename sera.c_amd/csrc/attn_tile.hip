@@ -27,9 +27,10 @@
  * all loads on their way. 64 rows a wave at one wave per SIMD were slower
  * (356 us against 178 for that prefill: nothing hides a wave's own latencies), and so
  * was a strict turn-taking of the two waves by barriers (no gain).
- * 2048 tokens x 64 heads: 164 us, 840 TFLOP/s of fp16 products (fp32 rows),
- * 110 us, 620 (16-bit rows); a large matrix product reaches 1180 here. 512 rows over
- * 32768 8-bit tokens: 1040 us, 1050 TFLOP/s.
+ * 2048 tokens x 64 heads: 150 us, 920 TFLOP/s of fp16 products (fp32 rows),
+ * 98 us, 700 (16-bit rows), in calls one after another; 168 and 111 us where a
+ * graph leaves no gap between them. A large matrix product reaches 1180 here. 512 rows over
+ * 32768 8-bit tokens: 1030 us, 1060 TFLOP/s.
  */
 #include "attn_device.h"
 #include "sera_launch.h"

@@ -11,8 +11,8 @@
  * pieces (D / VEC lanes to a row, several rows to an access); K's place in the cache is
  * the same order. V's is not: 16 tokens of a channel lie side by side, so a wave
  * turns its block in LDS of its own, in dwords that are unpacked by byte
- * permutes. 24588 tokens out of an 8-bit cache as fp32 rows: 80-88 us, 4.4-4.9
- * TB/s (a large copy: 5.2); ragged bf16 chunks into an fp16 cache 7 us for 15 MB.
+ * permutes. 37922 tokens out of an 8-bit cache as fp32 rows: 79-88 us, 4.4-5.0
+ * TB/s (a large copy: 5.2); ragged bf16 chunks into an fp16 cache 6 us for 15 MB.
  *
  * 8-bit quantizer: scale d = max|x| / 127 over the vector (an exact maximum,
  * one IEEE division), code = x / d rounded half to even, as the exact
@@ -56,8 +56,8 @@ struct __attribute__((aligned(sizeof(T) * N))) kv_vec {
 typedef uint32_t kv_u4 __attribute__((ext_vector_type(4)));
 typedef uint32_t kv_u2 __attribute__((ext_vector_type(2)));
 
-/* Stores past the caches: rows read back are larger than what they come from and only stream through (24588 tokens
- * out of an 8-bit cache take 80 us so, 100 us with ordinary stores). */
+/* Stores past the caches: rows read back are larger than what they come from and only stream through (37922 tokens
+ * out of an 8-bit cache take 80 us so, 94 us with ordinary stores; out of an fp16 cache 118 and 116). */
 template <typename T, int N>
 __device__ __forceinline__ void kv_store_past(T *p, const kv_vec<T, N> &v) {
     if constexpr (sizeof(v) == 16) __builtin_nontemporal_store(__builtin_bit_cast(kv_u4, v), (kv_u4 *)p);

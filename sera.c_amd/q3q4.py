@@ -605,7 +605,8 @@ class KVBatch:
     """The sequences of a call (sera_kv_batch): int32 device tensors
     row_start [sequences + 1], kv_len [sequences] and page_table
     [sequences, entries], which are read when the work runs, and the host's
-    bounds for them."""
+    bounds for them. A call takes a batch, rows and a workspace on its cache's
+    device."""
 
     def __init__(self, row_start, kv_len, page_table, rows, max_new, max_kv):
         import torch
