@@ -112,7 +112,8 @@ def draw(rng):
                      ragged=seqs > 1, **shape)
     if op == "evict":
         ctx = _log(rng, 64, 30000)
-        seqs = _log(rng, 1, min(64, max(1, 64 * 8192 * 1024 // (2 * ctx * row))))
+        most = 64 * 8192 * 1024 // (2 * ctx * row) // (2 if cache == "q8" else 1)      # those are read back, in 32 bits
+        seqs = _log(rng, 1, min(64, max(1, most)))
         keep = max(8, int(ctx * rng.uniform(0.1, 1.0)))
         sinks = rng.choice([0, 1, 4])
         return _evict("", cache, seqs, ctx, keep, int((keep - sinks) * rng.uniform(0, 0.6)), sinks, ragged=seqs > 1, **shape)
