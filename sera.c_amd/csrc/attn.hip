@@ -160,6 +160,7 @@ __global__ __launch_bounds__(256) void sera_attn_join_kernel(kv_args a, attn_arg
 #pragma unroll
         for (int e = 0; e < E; e++) o.v[e] = kv_from_f32<T>(first + i < 0 ? 0.0f : y[e] / l);
         *(attn_vec<T, E> *)((T *)t.out + (s.row0 + i) * t.out_stride + (int64_t)h * D + E * lane) = o;
+        if (t.lse && lane == 0) t.lse[(size_t)(s.row0 + i) * t.heads + h] = attn_lse(top, l);
     }
 }
 
@@ -211,9 +212,11 @@ hipError_t sera_launch_attn(uint32_t cache_type, uint32_t type, int dim, const k
         e = sera_launch_attn_tile(cache_type, type, dim, a, u, p.tile, s);
     }
     if (e == hipSuccess && p.few.columns) e = sera_launch_attn_few(cache_type, type, dim, a, t, p.few, s);
-    if (e != hipSuccess || !p.bytes) return e;
-    if (type == SERA_TYPE_F32) join_t<float>(dim, a, t, p, s);
-    else if (type == SERA_TYPE_F16) join_t<_Float16>(dim, a, t, p, s);
-    else join_t<__bf16>(dim, a, t, p, s);
-    return hipGetLastError();
+    if (e == hipSuccess && p.bytes) {
+        if (type == SERA_TYPE_F32) join_t<float>(dim, a, t, p, s);
+        else if (type == SERA_TYPE_F16) join_t<_Float16>(dim, a, t, p, s);
+        else join_t<__bf16>(dim, a, t, p, s);
+        e = hipGetLastError();
+    }
+    return e == hipSuccess && t.weights ? sera_launch_attn_weights(cache_type, type, dim, a, t, s) : e;
 }

@@ -19,6 +19,31 @@ struct attn_args {
     int few_rows;                   /* rows of one of its partial results */
     float *workspace;
     int cus;                        /* compute units of the device */
+    float *lse;                     /* log2 of each row's sum of 2^s', [rows][heads], for the weights; NULL: not wanted */
+    const float *before;            /* sums so far, or NULL */
+    float *weights;                 /* [sequences][kv_heads][weights_stride] */
+    int64_t weights_stride;
+};
+
+/* Norm and rotation of q's and k's heads. */
+struct rope_args {
+    const float *inv_freq, *q_gamma, *k_gamma;
+    const int32_t *positions;
+    float eps;
+    int half;                       /* pairs of channels that turn */
+    bool neighbours;
+    int heads;                      /* q's */
+};
+
+/* What shortening a cache takes beside it and the batch. */
+struct evict_args {
+    int keep, recent, sinks;
+    const float *weights;
+    float *new_weights;
+    int64_t weights_stride;
+    const int32_t *new_table;
+    int64_t new_stride;
+    int32_t *new_len, *kept;
 };
 
 /* How a kernel's part of a call is cut up, in 32-token tiles. */
@@ -39,5 +64,11 @@ hipError_t sera_launch_attn(uint32_t cache_type, uint32_t type, int dim, const k
                             hipStream_t s);
 hipError_t sera_launch_attn_tile(uint32_t cache_type, uint32_t type, int dim, const kv_args &a, const attn_args &t,
                                  const attn_plan &p, hipStream_t s);
+hipError_t sera_launch_attn_weights(uint32_t cache_type, uint32_t type, int dim, const kv_args &a, const attn_args &t,
+                                    hipStream_t s);
+hipError_t sera_launch_kv_rope(uint32_t cache_type, uint32_t type, int dim, const kv_args &a, const rope_args &r,
+                               const void *q, int64_t q_stride, void *q_out, int64_t q_out_stride, const void *k,
+                               int64_t k_stride, const void *v, int64_t v_stride, hipStream_t s);
+hipError_t sera_launch_kv_evict(uint32_t cache_type, int dim, const kv_args &a, const evict_args &t, hipStream_t s);
 
 #endif

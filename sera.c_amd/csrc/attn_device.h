@@ -78,6 +78,9 @@ __device__ __forceinline__ int attn_page(const kv_args &a, int b, int pos, int l
 
 __device__ __forceinline__ float attn_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
+/* log2 of a row's sum of 2^s' from its maximum and its sum of weights. */
+__device__ __forceinline__ float attn_lse(float m, float l) { return m - kAttnBias + __builtin_amdgcn_logf(l); }
+
 /* The power of two that brings the largest |q| of a row near 2^10 (products
  * and sums then stay clear of fp16's and fp32's borders whatever the rows' size),
  * as its exponent. */

@@ -17,7 +17,8 @@ LIB_PATH = os.path.join(HERE, "libsera_q4k.so")
 ROOT = os.path.dirname(HERE)
 HEADERS = [os.path.join(ROOT, "include", "q3_q4_linear.h"),
            os.path.join(ROOT, "include", "sera_q4k.h"),
-           os.path.join(ROOT, "include", "sera_attn.h")]
+           os.path.join(ROOT, "include", "sera_attn.h"),
+           os.path.join(ROOT, "include", "sera_logprobs.h")]
 
 QTYPE_Q4_K = 12
 QTYPE_Q6_K = 14
@@ -56,6 +57,12 @@ class KVBatchArgs(ctypes.Structure):
     _fields_ = [("sequences", ctypes.c_int32), ("rows", ctypes.c_int32), ("max_new", ctypes.c_int32),
                 ("max_kv", ctypes.c_int32), ("table_stride", ctypes.c_int64), ("row_start", ctypes.c_void_p),
                 ("kv_len", ctypes.c_void_p), ("page_table", ctypes.c_void_p)]
+
+
+class QKRopeArgs(ctypes.Structure):
+    """sera_qk_rope (include/sera_attn.h)."""
+    _fields_ = [("inv_freq", ctypes.c_void_p), ("q_gamma", ctypes.c_void_p), ("k_gamma", ctypes.c_void_p),
+                ("eps", ctypes.c_float), ("rotated", ctypes.c_int32), ("pairing", ctypes.c_int32)]
 
 
 class Q3Q4Error(RuntimeError):
@@ -181,6 +188,13 @@ def load():
         "sera_kv_read": ([P, P, U32, P, I64, P, I64, P], I),
         "sera_attention_workspace_bytes": ([P, P, I], SZ),
         "sera_attention": ([P, P, U32, P, I64, P, I64, I, ctypes.c_float, I, I, P, SZ, P], I),
+        "sera_kv_write_rope": ([P, P, P, U32, P, I64, P, I64, I, P, I64, P, I64, P, P], I),
+        "sera_attention_weights_workspace_bytes": ([P, P, I], SZ),
+        "sera_attention_weights": ([P, P, U32, P, I64, P, I64, I, ctypes.c_float, I, I, P, P, I64, P, SZ, P], I),
+        "sera_kv_evict": ([P, P, I, I, I, P, P, I64, P, I64, P, P, P], I),
+        # sera_logprobs.h
+        "sera_logprobs_workspace_bytes": ([I, I, I], SZ),
+        "sera_logprobs": ([U32, P, I64, I, I, P, I, P, P, I, P, P, P, SZ, P], I),
     }
     for name, (args, res) in sigs.items():
         fn = getattr(L, name)
@@ -671,11 +685,192 @@ def attention(cache, batch, q, out, scale, window=0, sinks=0, workspace=None, st
     ty, qp, qs, op, os_ = _pair(cache, batch, width, q, out)
     if width % cache.head_dim:
         raise Q3Q4Error(f"rows of {width} are no heads of {cache.head_dim}")
-    wp, wb = 0, 0
-    if workspace is not None:
-        if workspace.get_device() != cache.device or not workspace.is_contiguous():
-            raise Q3Q4Error("the workspace must be a contiguous tensor on the cache's device, got "
-                            f"{tuple(workspace.shape)} strides {workspace.stride()} on {workspace.device}")
-        wp, wb = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    wp, wb = _scratch(workspace, cache.device)
     _check(load().sera_attention(cache.ref, batch.ref, ty, qp, qs, op, os_, width // cache.head_dim, scale, window,
                                  sinks, wp, wb, _stream(stream)), "sera_attention")
+
+
+def _scratch(workspace, device):
+    """(pointer, bytes) of a workspace on a device, by its index."""
+    if workspace is None:
+        return 0, 0
+    if workspace.get_device() != device or not workspace.is_contiguous():
+        raise Q3Q4Error("the workspace must be a contiguous tensor on the cache's device, got "
+                        f"{tuple(workspace.shape)} strides {workspace.stride()} on {workspace.device}")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
+# ---------------------------------------------------------------------------
+# Norm and rotation on the way into the cache; a cache of bounded length
+# ---------------------------------------------------------------------------
+
+ROPE_HALVES = 0         # SERA_ROPE_HALVES: channels i and i + rotated / 2 turn together
+ROPE_NEIGHBOURS = 1     # SERA_ROPE_NEIGHBOURS: channels 2i and 2i + 1
+
+
+def _call(name, device, stream, *args):
+    """One library call on a device (by its index) and a stream of it, by default its current one."""
+    import torch
+    if stream is not None and stream.device.index != device:
+        raise Q3Q4Error(f"{name}: the tensors are on device {device}, the stream on {stream.device}")
+    fn = getattr(load(), name)
+    if torch.cuda.current_device() == device:
+        return _check(fn(*args, _stream(stream)), name)
+    with torch.cuda.device(device):
+        _check(fn(*args, _stream(stream)), name)
+
+
+def _flat(name, t, dtype, shape, device):
+    """The pointer of a contiguous tensor of this type and shape (None in it: any) on a device, by its index."""
+    ok = t.dtype == dtype and len(t.shape) == len(shape) and t.is_contiguous() and t.get_device() == device
+    if not ok or any(w is not None and w != n for n, w in zip(t.shape, shape)):
+        want = ", ".join("any" if n is None else str(n) for n in shape)
+        raise Q3Q4Error(f"{name} must be a contiguous {dtype} tensor [{want}] on device {device}, got {t.dtype} "
+                        f"{tuple(t.shape)} strides {t.stride()} on {t.device}")
+    return t.data_ptr()
+
+
+class Rope:
+    """What q's and k's heads go through (sera_qk_rope): RMSNorm with a gamma (float32 [head_dim], None: no norm), then a turn of the first 2 *
+    len(inv_freq) channels, pair i by position * inv_freq[i] (float32, None: no turn)."""
+
+    def __init__(self, inv_freq=None, q_gamma=None, k_gamma=None, eps=1e-6, pairing=ROPE_HALVES):
+        import torch
+        given = [t for t in (inv_freq, q_gamma, k_gamma) if t is not None]
+        self.device = given[0].get_device() if given else None      # None: any
+        for name, t in (("inv_freq", inv_freq), ("q_gamma", q_gamma), ("k_gamma", k_gamma)):
+            if t is not None:
+                _flat(name, t, torch.float32, (None,), self.device)
+        self.inv_freq, self.q_gamma, self.k_gamma = inv_freq, q_gamma, k_gamma
+        self.rotated = 2 * inv_freq.numel() if inv_freq is not None else 0
+        self.args = QKRopeArgs(*(t.data_ptr() if t is not None else None for t in (inv_freq, q_gamma, k_gamma)), eps,
+                               self.rotated, pairing)
+        self.ref = ctypes.addressof(self.args)
+
+
+def kv_write_rope(cache, batch, rope, q, q_out, k, v, positions=None, stream=None):
+    """kv_write of k normed and rotated, and q into q_out the same way (q_out may be q); k, v [rows, kv_heads * head_dim],
+    q, q_out [rows, heads * head_dim] of one type. positions: int32 [rows], by default each row's place in its sequence."""
+    import torch
+    ty, kp, ks, vp, vs = _pair(cache, batch, cache.width, k, v)
+    width = q.shape[-1] if len(q.shape) else 0
+    ty2, qp, qs, op, os_ = _pair(cache, batch, width, q, q_out)
+    if ty != ty2:
+        raise Q3Q4Error(f"rows must be of one type, got {k.dtype} and {q.dtype}")
+    if width % cache.head_dim:
+        raise Q3Q4Error(f"rows of {width} are no heads of {cache.head_dim}")
+    if rope.device is not None and rope.device != cache.device:
+        raise Q3Q4Error(f"inv_freq and gammas must be on device {cache.device}")
+    for t in (rope.q_gamma, rope.k_gamma):
+        if t is not None and t.numel() != cache.head_dim:
+            raise Q3Q4Error(f"a gamma of {t.numel()} for heads of {cache.head_dim}")
+    pp = 0
+    if positions is not None:
+        pp = _flat("positions", positions, torch.int32, (None,), cache.device)
+        if positions.numel() < batch.rows:
+            raise Q3Q4Error(f"{positions.numel()} positions of {batch.rows} rows")
+    _call("sera_kv_write_rope", cache.device, stream, cache.ref, batch.ref, rope.ref, ty, qp, qs, op, os_,
+          width // cache.head_dim, kp, ks, vp, vs, pp)
+
+
+def attention_weights_workspace(cache, batch, heads):
+    """Scratch for attention_weights() with this batch's bounds."""
+    import torch
+    with torch.cuda.device(cache.data.device):
+        n = load().sera_attention_weights_workspace_bytes(cache.ref, batch.ref, heads)
+    return torch.empty(n, dtype=torch.uint8, device=cache.data.device) if n else None
+
+
+def _sums(name, t, cache, batch):
+    """(pointer, stride) of weights [sequences, kv_heads, max_kv or more]."""
+    import torch
+    p = _flat(name, t, torch.float32, (batch.kv_len.numel(), cache.kv_heads, None), cache.device)
+    if t.shape[2] < batch.max_kv:
+        raise Q3Q4Error(f"{name} has {t.shape[2]} positions of {batch.max_kv}")
+    return p, t.shape[2]
+
+
+def attention_weights(cache, batch, q, out, scale, weights, before=None, window=0, sinks=0, workspace=None, stream=None):
+    """attention(), and weights [sequences, kv_heads, max_kv or more] (float32) = before + what each position got from the
+    new rows, summed over them and the query heads of its kv head. before: the same shape, may be weights; None: zero."""
+    width = q.shape[-1] if len(q.shape) else 0
+    ty, qp, qs, op, os_ = _pair(cache, batch, width, q, out)
+    if width % cache.head_dim:
+        raise Q3Q4Error(f"rows of {width} are no heads of {cache.head_dim}")
+    sp, stride = _sums("weights", weights, cache, batch)
+    bp = 0
+    if before is not None:
+        bp, stride2 = _sums("before", before, cache, batch)
+        if stride != stride2:
+            raise Q3Q4Error(f"before {tuple(before.shape)} and weights {tuple(weights.shape)} differ")
+    wp, wb = _scratch(workspace, cache.device)
+    _call("sera_attention_weights", cache.device, stream, cache.ref, batch.ref, ty, qp, qs, op, os_,
+          width // cache.head_dim, scale, window, sinks, bp, sp, stride, wp, wb)
+
+
+def kv_evict(cache, batch, keep, weights, new_table, new_len, new_weights, kept, recent=0, sinks=0, stream=None):
+    """Shortens each sequence to `keep` positions: the first `sinks`, the last `recent` and those of the largest weights, for every kv
+    head by itself; they move to the pages of new_table [sequences, entries] (int32). new_len [sequences] and kept
+    [sequences, kv_heads, keep] (int32) tell what stayed, new_weights (as weights) has their sums."""
+    import torch
+    n = batch.kv_len.numel()
+    if cache.device < 0 or batch.device != cache.device:
+        raise Q3Q4Error("the cache's data and the batch's tensors must be device tensors on one device, got "
+                        f"{cache.data.device} and {batch.kv_len.device}")
+    if batch.max_kv > batch.entries * cache.page_tokens:
+        raise Q3Q4Error(f"max_kv={batch.max_kv} is more than {batch.entries} pages of {cache.page_tokens} hold")
+    sp, stride = _sums("weights", weights, cache, batch)
+    np_, stride2 = _sums("new_weights", new_weights, cache, batch)
+    if stride != stride2:
+        raise Q3Q4Error(f"weights {tuple(weights.shape)} and new_weights {tuple(new_weights.shape)} differ")
+    tp = _flat("new_table", new_table, torch.int32, (n, None), cache.device)
+    lp = _flat("new_len", new_len, torch.int32, (n,), cache.device)
+    kp = _flat("kept", kept, torch.int32, (n, cache.kv_heads, keep), cache.device)
+    _call("sera_kv_evict", cache.device, stream, cache.ref, batch.ref, keep, recent, sinks, sp, np_, stride, tp,
+          new_table.shape[1], lp, kp)
+
+
+# ---------------------------------------------------------------------------
+# Log probabilities (include/sera_logprobs.h)
+# ---------------------------------------------------------------------------
+
+def logprobs_workspace(logits, top=0):
+    """Scratch for logprobs() of logits [rows, vocab] (None: none needed)."""
+    import torch
+    with torch.cuda.device(logits.device):
+        n = load().sera_logprobs_workspace_bytes(logits.shape[0], logits.shape[1], top)
+    return torch.empty(n, dtype=torch.uint8, device=logits.device) if n else None
+
+
+def logprobs(logits, tokens=None, token_logprobs=None, entropy=None, top_ids=None, top_logprobs=None, workspace=None,
+             stream=None):
+    """Of logits [rows, vocab] (float32, float16 or bfloat16): the log probabilities of tokens [rows, n] (int32) into
+    token_logprobs [rows, n], the entropy into entropy [rows], the most likely tokens into top_ids (int32) and top_logprobs
+    [rows, top]; float32 results. What is None is not computed."""
+    import torch
+    if len(logits.shape) != 2:
+        raise Q3Q4Error(f"logits must be [rows, vocab], got {tuple(logits.shape)}")
+    rows, vocab = logits.shape
+    device = logits.get_device()
+    if device < 0:
+        raise Q3Q4Error(f"logits must be a device tensor, got {logits.device}")
+    if rows and vocab == 0:
+        raise Q3Q4Error("logits of no tokens")
+    ty, xp, stride = _rows(logits, rows, vocab, device) if vocab else (0, 0, 0)
+    if rows < 2:
+        stride = max(stride, vocab)      # one row's stride is never used
+    if (tokens is None) != (token_logprobs is None) or (top_ids is None) != (top_logprobs is None):
+        raise Q3Q4Error("tokens go with token_logprobs, top_ids with top_logprobs")
+    n, tp, gp, ep, top, ip, op = 0, 0, 0, 0, 0, 0, 0
+    if tokens is not None:
+        tp = _flat("tokens", tokens, torch.int32, (rows, None), device)
+        n = tokens.shape[1]
+        gp = _flat("token_logprobs", token_logprobs, torch.float32, (rows, n), device)
+    if entropy is not None:
+        ep = _flat("entropy", entropy, torch.float32, (rows,), device)
+    if top_ids is not None:
+        ip = _flat("top_ids", top_ids, torch.int32, (rows, None), device)
+        top = top_ids.shape[1]
+        op = _flat("top_logprobs", top_logprobs, torch.float32, (rows, top), device)
+    wp, wb = _scratch(workspace, device)
+    _call("sera_logprobs", device, stream, ty, xp, stride, rows, vocab, tp, n, gp, ep or None, top, ip, op, wp, wb)
