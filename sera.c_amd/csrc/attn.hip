@@ -187,8 +187,22 @@ void shorten(attn_plan &p, const kv_args &a, const attn_args &t) {
 
 }  // namespace
 
-size_t sera_attn_workspace(const kv_args &a, int dim, int heads, int cus) {
-    return plan_of(a, dim, heads, cus).bytes;
+/* The workspace of a call that wants the weights' sums: partial results, each row's z, then what the sums need. */
+static size_t lse_at(const attn_plans &p) { return (p.bytes + 15) & ~(size_t)15; }
+static size_t sums_at(const attn_plans &p, const kv_args &a, int heads) {
+    return (lse_at(p) + (size_t)a.rows * heads * sizeof(float) + 15) & ~(size_t)15;
+}
+static attn_sums sums_of(const attn_plans &p, const kv_args &a, int heads, int cus, size_t *bytes) {
+    return sera_attn_sums_plan(a, p.few.columns ? p.few_rows : 0,
+                               p.tile.columns ? (int64_t)a.max_new * (heads / a.kv_heads) : 0, cus, bytes);
+}
+
+size_t sera_attn_workspace(const kv_args &a, int dim, int heads, int cus, bool weigh) {
+    const attn_plans p = plan_of(a, dim, heads, cus);
+    if (!weigh) return p.bytes;
+    size_t n;
+    sums_of(p, a, heads, cus, &n);
+    return sums_at(p, a, heads) + n;
 }
 
 /* Arguments are checked by the caller (sera_attn_runtime.hip). */
@@ -198,6 +212,17 @@ hipError_t sera_launch_attn(uint32_t cache_type, uint32_t type, int dim, const k
     attn_args t = args;
     t.few_columns = p.few_columns;
     t.few_rows = p.few_rows;
+    attn_sums sums = {};
+    if (t.weights) {
+        uint8_t *const ws = (uint8_t *)t.workspace;
+        size_t n;
+        sums = sums_of(p, a, t.heads, t.cus, &n);
+        sums.scores = (float *)(ws + sums_at(p, a, t.heads));
+        sums.partial = (float *)((uint8_t *)sums.scores + sums.scores_bytes);
+        t.lse = (float *)(ws + lse_at(p));
+        t.scores = sums.scores;
+        t.pitch = sums.pitch;
+    }
     shorten(p.few, a, t);
     shorten(p.tile, a, t);
     /* Whole contexts, a CU to each workgroup: eight waves of an 8-bit cache, whose conversions they share (24 contexts of
@@ -218,5 +243,6 @@ hipError_t sera_launch_attn(uint32_t cache_type, uint32_t type, int dim, const k
         else join_t<__bf16>(dim, a, t, p, s);
         e = hipGetLastError();
     }
-    return e == hipSuccess && t.weights ? sera_launch_attn_weights(cache_type, type, dim, a, t, s) : e;
+    if (e != hipSuccess || !t.weights) return e;
+    return sera_launch_attn_sums(cache_type, type, dim, a, t, sums, p.tile.columns != 0, s);
 }

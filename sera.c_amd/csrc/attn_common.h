@@ -20,9 +20,20 @@ struct attn_args {
     float *workspace;
     int cus;                        /* compute units of the device */
     float *lse;                     /* log2 of each row's sum of 2^s', [rows][heads], for the weights; NULL: not wanted */
+    float *scores;                  /* s' of the few-row kernel, [sequences][kv_heads][few_rows][pitch], or NULL */
+    size_t pitch;
     const float *before;            /* sums so far, or NULL */
     float *weights;                 /* [sequences][kv_heads][weights_stride] */
     int64_t weights_stride;
+};
+
+/* How the weights' sums are made. */
+struct attn_sums {
+    int few_rows;                   /* columns of a sequence in the few-row kernel, at most; 0: it has no part */
+    size_t pitch;                   /* floats from one row of scores (or sums) to the next */
+    int splits, chunk;              /* ranges of columns, and 32-column blocks of one, of all other sequences */
+    size_t scores_bytes;            /* of the workspace; the ranges' sums lie behind */
+    float *scores, *partial;
 };
 
 /* Norm and rotation of q's and k's heads. */
@@ -57,15 +68,16 @@ constexpr int kAttnShift = 5;       /* log2 of a tile's tokens */
 
 hipError_t sera_launch_kv_move(bool write, uint32_t cache_type, uint32_t type, int dim, const kv_args &a, void *k,
                                int64_t k_stride, void *v, int64_t v_stride, hipStream_t s);
-size_t sera_attn_workspace(const kv_args &a, int dim, int heads, int cus);
+size_t sera_attn_workspace(const kv_args &a, int dim, int heads, int cus, bool weigh);
 hipError_t sera_launch_attn_few(uint32_t cache_type, uint32_t type, int dim, const kv_args &a, const attn_args &t,
                                 const attn_plan &p, hipStream_t s);
 hipError_t sera_launch_attn(uint32_t cache_type, uint32_t type, int dim, const kv_args &a, const attn_args &t,
                             hipStream_t s);
 hipError_t sera_launch_attn_tile(uint32_t cache_type, uint32_t type, int dim, const kv_args &a, const attn_args &t,
                                  const attn_plan &p, hipStream_t s);
-hipError_t sera_launch_attn_weights(uint32_t cache_type, uint32_t type, int dim, const kv_args &a, const attn_args &t,
-                                    hipStream_t s);
+attn_sums sera_attn_sums_plan(const kv_args &a, int few_rows, int64_t columns, int cus, size_t *bytes);
+hipError_t sera_launch_attn_sums(uint32_t cache_type, uint32_t type, int dim, const kv_args &a, const attn_args &t,
+                                 const attn_sums &p, bool many, hipStream_t s);
 hipError_t sera_launch_kv_rope(uint32_t cache_type, uint32_t type, int dim, const kv_args &a, const rope_args &r,
                                const void *q, int64_t q_stride, void *q_out, int64_t q_out_stride, const void *k,
                                int64_t k_stride, const void *v, int64_t v_stride, hipStream_t s);

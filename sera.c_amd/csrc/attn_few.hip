@@ -57,7 +57,8 @@ struct few_piece<(int)SERA_KV_Q8> { typedef attn_u2 v; };
 
 }  // namespace
 
-template <int TYPE, typename T, int D, int CT, int NW, int OCC, bool PAIR>
+/* KEEP: the scores are left for the weights' sums. */
+template <int TYPE, typename T, int D, int CT, int NW, int OCC, bool PAIR, bool KEEP>
 __global__ __launch_bounds__(64 * NW, OCC) void sera_attn_few_kernel(kv_args a, attn_args t, int splits, int chunk) {
     using F = few_shape<TYPE, D>;
     constexpr bool Q8 = F::Q8, TWO = sizeof(T) == 4 && !PAIR;      /* a second fragment for the low parts */
@@ -262,6 +263,12 @@ __global__ __launch_bounds__(64 * NW, OCC) void sera_attn_few_kernel(kv_args a, 
     #pragma unroll
                         for (int i = 0; i < 4; i++)
                             x[4 * u + i] = attn_sees(t, pos[ct], j0 + 4 * u + i) ? x[4 * u + i] : -INFINITY;
+                if (KEEP && ct * 16 + col < rows && (!PAIR || col < 8)) {
+                    float *to = t.scores + ((size_t)(b * a.kv_heads + head) * t.few_rows + ct * 16 + col) * t.pitch + j0;
+    #pragma unroll
+                    for (int u = 0; u < NS; u++)
+                        *(attn_f4 *)(to + 4 * u) = attn_f4{x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]};
+                }
     #pragma unroll
                 for (int u = 0; u < NS; u++)
     #pragma unroll
@@ -403,9 +410,13 @@ namespace {
 template <int TYPE, typename T, int D, int CT, int NW, int OCC, bool PAIR>
 void few_go(const kv_args &a, const attn_args &t, const attn_plan &p, hipStream_t s) {
     const int y = a.sequences < 32768 ? a.sequences : 32768;
-    hipLaunchKernelGGL((sera_attn_few_kernel<TYPE, T, D, CT, NW, OCC, PAIR>),
-                       dim3((unsigned)(a.kv_heads * p.splits), (unsigned)y, (unsigned)((a.sequences + y - 1) / y)),
-                       dim3(64 * NW), 0, s, a, t, p.splits, p.chunk);
+    const dim3 grid((unsigned)(a.kv_heads * p.splits), (unsigned)y, (unsigned)((a.sequences + y - 1) / y));
+    if (t.scores)
+        hipLaunchKernelGGL((sera_attn_few_kernel<TYPE, T, D, CT, NW, OCC, PAIR, true>), grid, dim3(64 * NW), 0, s, a, t,
+                           p.splits, p.chunk);
+    else
+        hipLaunchKernelGGL((sera_attn_few_kernel<TYPE, T, D, CT, NW, OCC, PAIR, false>), grid, dim3(64 * NW), 0, s, a,
+                           t, p.splits, p.chunk);
 }
 
 /* Waves per SIMD: as many as the registers (no spills) leave. */

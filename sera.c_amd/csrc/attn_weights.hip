@@ -5,149 +5,346 @@
  *   w_j = sum over rows i, query heads of 2^(s'_ij - z_i),   z_i = log2(sum_j 2^(s'_ij))
  *
  * with s' = scale * q . k * log2(e), as attention has them, and z left by its
- * kernels. A wave has 32 positions of a kv head, their keys in registers as
- * A operand, and passes over the columns (rows of q times heads of the group), 16 at a
- * time; a lane sums the columns it sees, lanes are joined at the end.
+ * kernels (t.lse).
+ *
+ * Few rows: the kernel that streams the cache has the scores; it leaves them
+ * (4 bytes for each position and column), and what is left to do is one pass over those.
+ *
+ * Many rows: the products again, S^T = K Q^T on 32x32x16 MFMAs, the keys of 256 positions
+ * in a workgroup's registers (64 a wave, A operand) and the columns (rows of q times heads
+ * of the group) passing by in blocks of 32: loaded by rows, scaled, split into fp16 terms and
+ * laid into LDS in the order of B fragments by all waves, a block ahead of the products. A lane has one column of a
+ * block, so z is one number a lane, and its sums stay in the lane until the
+ * end. Columns are cut into ranges over workgroups (positions alone are few: 64
+ * workgroups for a prompt of 2048 and 8 kv heads), whose sums the last kernel adds in their
+ * order.
  */
 #include "attn_device.h"
 #include "sera_launch.h"
 
 namespace {
 
-constexpr int kWaves = 4, kTokens = 32;
+constexpr int kTokens = 256, kWaveTokens = 64;        /* positions of a workgroup and a wave */
+
+template <typename T, int D>
+struct sum_shape {
+    static constexpr bool TWO = sizeof(T) == 4;
+    static constexpr int KC = D / 16, NB = kWaveTokens / 32;
+    static constexpr int VEC = 16 / (int)sizeof(T);            /* elements of a 16-byte load */
+    static constexpr int LOADS = D / (8 * VEC);                /* of a thread, 8 threads to a column */
+    static constexpr int UNITS = KC * 2 * 32;                  /* 16-byte units of a block's high (or low) terms */
+};
+
+/* Place of unit u = 2 kc + half of column `col`: (u, col), columns exchanged so that the units that a row's threads write
+ * at once lie in different banks. */
+__device__ __forceinline__ int sum_unit(int u, int col) { return u * 32 + (col ^ (((u & 3) << 1) | ((u >> 2) & 1))); }
+
+/* Blocks of columns c0 .. c1-1 (of 32) that see any of the positions j .. j+n-1. */
+__device__ __forceinline__ void sum_range(const attn_args &t, int first, int rows, int j, int n, int *c0, int *c1) {
+    const int i0 = max(j - first, 0);                                       /* rows before it see nothing */
+    int end = rows;
+    if (t.window > 0 && j >= t.sinks) {
+        const int64_t past = (int64_t)j + n - 1 + t.window - first;         /* nor do those from here on */
+        end = (int)min((int64_t)rows, max(past, (int64_t)0) * t.group);
+    }
+    *c0 = (int)(((int64_t)i0 * t.group) / 32);
+    *c1 = (int)(((int64_t)end + 31) / 32);
+}
 
 }  // namespace
 
 template <int TYPE, typename T, int D>
-__global__ __launch_bounds__(64 * kWaves) void sera_attn_weights_kernel(kv_args a, attn_args t) {
-    constexpr bool Q8 = TYPE == (int)SERA_KV_Q8, TWO = sizeof(T) == 4;
-    constexpr int ES = Q8 ? 1 : 2, KC = D / 32, KP = Q8 ? KC / 2 : KC, NS = kTokens / 16;
+__global__ __launch_bounds__(256, 2) void sera_attn_columns_kernel(kv_args a, attn_args t, attn_sums p) {
+    using S = sum_shape<T, D>;
+    constexpr bool Q8 = TYPE == (int)SERA_KV_Q8, TWO = S::TWO;
+    constexpr int ES = Q8 ? 1 : 2, KC = S::KC, NB = S::NB, UNITS = S::UNITS, LOADS = S::LOADS, VEC = S::VEC;
+    __shared__ attn_u4 box[2][TWO ? 2 : 1][UNITS];
+    __shared__ float cz[2][2][32];                        /* each column's factor, and z */
+
     const int b = (int)(blockIdx.z * gridDim.y + blockIdx.y);
     if (b >= a.sequences) return;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int head = (int)blockIdx.x % a.kv_heads;
-    const int j0 = ((int)blockIdx.x / a.kv_heads * kWaves + wave) * kTokens;
-    const int col = lane & 15, quarter = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int head = (int)blockIdx.x % a.kv_heads, x0 = (int)blockIdx.x / a.kv_heads;
+    const int split = x0 % p.splits, tile0 = x0 / p.splits * kTokens, j0 = tile0 + wave * kWaveTokens;
     const kv_seq s = kv_sequence(a, b);
-    if (s.bad || j0 >= s.len) return;
-    const int first = s.len - s.n, rows = s.n * t.group, mask = (1 << a.page_shift) - 1;
-
-    /* Keys: A row `col` of operand u is token 16 u + col. */
-    const uint8_t *base = a.data + (size_t)head * a.head_bytes;
-    attn_h8 kf[NS][KC];
-    attn_f4 ks[NS];
-    bool lost[NS];
-#pragma unroll
-    for (int u = 0; u < NS; u++) {
-        const int id = attn_page(a, b, j0 + 16 * u, s.len);
-        lost[u] = id < 0;
-        const uint8_t *run = base + (size_t)max(id, 0) * a.page_bytes;
-        const int slot = (j0 + 16 * u) & mask;
-        const uint8_t *p = run + (size_t)(slot + col) * (D * ES) + 16 * quarter;
-#pragma unroll
-        for (int k = 0; k < KP; k++) {
-            const attn_u4 w = *(const attn_u4 *)(p + 64 * k);
-            if (Q8) {
-                kf[u][2 * k] = attn_codes(w[0], w[1]);
-                kf[u][2 * k + 1] = attn_codes(w[2], w[3]);
-            } else {
-                kf[u][k] = __builtin_bit_cast(attn_h8, w);
-            }
-        }
-        if (Q8)
-            ks[u] = *(const attn_f4 *)(run + 2 * ((size_t)D << a.page_shift) + 4 * (size_t)(slot + 4 * quarter));
+    const int rows = s.n * t.group;
+    if (s.bad || tile0 >= s.len || rows <= t.few_columns) return;
+    const int first = s.len - s.n, mask = (1 << a.page_shift) - 1, col = lane & 31, half = lane >> 5;
+    int c0, c1;
+    sum_range(t, first, rows, tile0, kTokens, &c0, &c1);
+    if (p.splits > 1) {
+        c0 = max(c0, split * p.chunk);
+        c1 = min(c1, (split + 1) * p.chunk);
+        if (c0 >= c1) return;
     }
 
-    float sum[NS][4] = {};
+    /* This thread's column of the block that comes next, and its loads: 8 threads to a column. */
+    const int my_col = tid >> 3, sub = tid & 7;
+    int at_r = 32 * c0 + my_col, at_i = at_r / t.group, at_g = at_r - at_i * t.group;
+    const int step_i = 32 / t.group, step_g = 32 - step_i * t.group;
+    attn_vec<T, VEC> in[LOADS];
+    float z = INFINITY;
+    const auto load = [&]() {
+        const bool there = at_r < rows;
+        const int i = there ? at_i : s.n - 1, h = head * t.group + (there ? at_g : t.group - 1);
+        const T *q = (const T *)t.q + (s.row0 + i) * t.q_stride + (int64_t)h * D + VEC * sub;
+#pragma unroll
+        for (int k = 0; k < LOADS; k++) in[k] = *(const attn_vec<T, VEC> *)(q + 8 * VEC * k);
+        /* past the last column: no weight */
+        z = there ? t.lse[(size_t)(s.row0 + i) * t.heads + h] : INFINITY;
+        at_r += 32;
+        at_i += step_i;
+        at_g += step_g;
+        if (at_g >= t.group) {
+            at_g -= t.group;
+            at_i++;
+        }
+    };
     const float sign = t.scale_log2 < 0.0f ? -1.0f : 1.0f;
-    /* rows in front of the first that sees position j0 see none of these, unless they are sinks' positions */
-    const int c0 = max(j0 - first, 0) * t.group / 16;
-    for (int c = c0; c < (rows + 15) / 16; c++) {
-        const int r = min(16 * c + col, rows - 1), i = r / t.group, h = head * t.group + r - i * t.group;
-        const T *q = (const T *)t.q + (s.row0 + i) * t.q_stride + (int64_t)h * D;
-        float x[KC][8], top = 0.0f;
+    const auto put = [&](int buf) {
+        float x[LOADS][VEC], top = 0.0f;
 #pragma unroll
-        for (int k = 0; k < KC; k++) {
-            attn_load8(q + (Q8 ? 64 * (k >> 1) + 16 * quarter + 8 * (k & 1) : 32 * k + 8 * quarter), x[k]);
+        for (int k = 0; k < LOADS; k++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[k][e]));
-        }
-        const float z = t.lse[(size_t)(s.row0 + i) * t.heads + h];
-        top = fmaxf(top, xor_partner<16>(top));
-        top = fmaxf(top, xor_partner<32>(top));
+            for (int e = 0; e < VEC; e++) {
+                x[k][e] = kv_to_f32(in[k].v[e]);
+                top = fmaxf(top, fabsf(x[k][e]));
+            }
+        top = fmaxf(top, xor_partner<1>(top));
+        top = fmaxf(top, xor_partner<2>(top));
+        top = fmaxf(top, xor_partner<4>(top));
         const int e2 = attn_q_exponent(top);
-        const float up = ldexpf(sign, e2), down = ldexpf(fabsf(t.scale_log2), -e2);
-        attn_f4 acc[NS];
+        const float up = ldexpf(sign, e2);
+        if (sub == 0) {
+            cz[buf][0][my_col] = ldexpf(fabsf(t.scale_log2), -e2);
+            cz[buf][1][my_col] = z;
+        }
+        float minus = -1.0f;
+        asm("" : "+s"(minus));
 #pragma unroll
-        for (int u = 0; u < NS; u++) acc[u] = attn_f4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int k = 0; k < LOADS; k++) {
+            attn_vec<_Float16, VEC> hi, lo;
 #pragma unroll
-        for (int k = 0; k < KC; k++) {
+            for (int e = 0; e < VEC; e += 2) {
+                const float y0 = x[k][e] * up, y1 = x[k][e + 1] * up;
+                const attn_h2 h = attn_pack(y0, y1);
+                hi.v[e] = h[0];
+                hi.v[e + 1] = h[1];
+                if (TWO) {
+                    lo.v[e] = (_Float16)fmaf((float)h[0], minus, y0);
+                    lo.v[e + 1] = (_Float16)fmaf((float)h[1], minus, y1);
+                }
+            }
+            const int ch = 8 * VEC * k + VEC * sub;
+            uint8_t *to = (uint8_t *)&box[buf][0][sum_unit(ch >> 3, my_col)] + (ch & 7) * 2;
+            *(attn_vec<_Float16, VEC> *)to = hi;
+            if (TWO) *(attn_vec<_Float16, VEC> *)(to + UNITS * 16) = lo;
+        }
+    };
+    if (c0 < c1) load();
+
+    /* Keys: row `col` of A operand n is position j0 + 32 n + col. */
+    const uint8_t *base = a.data + (size_t)head * a.head_bytes;
+    attn_h8 kf[NB][KC];
+    attn_f4 ks[NB][Q8 ? 4 : 1];       /* of the positions of this lane's scores: 8 (i / 4) + 4 half + i % 4 */
+    uint32_t lost[NB];
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[k][e] *= up;
-            attn_h8 qh, ql;
-            attn_split<TWO>(x[k], qh, ql);
+    for (int n = 0; n < NB; n++) {
+        const int j = j0 + 32 * n + col, id = attn_page(a, b, j & ~15, s.len);
+        lost[n] = (uint32_t)__ballot(id < 0);
+        const uint8_t *run = base + (size_t)max(id, 0) * a.page_bytes;
+        const uint8_t *k = run + (size_t)(j & mask) * (D * ES) + 8 * half * ES;
 #pragma unroll
-            for (int u = 0; u < NS; u++) {
-                acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[u][k], qh, acc[u], 0, 0, 0);
-                if (TWO) acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[u][k], ql, acc[u], 0, 0, 0);
+        for (int kc = 0; kc < KC; kc++) {
+            if constexpr (Q8) {
+                const attn_u2 w = *(const attn_u2 *)(k + 16 * kc);
+                kf[n][kc] = attn_codes(w[0], w[1]);
+            } else {
+                kf[n][kc] = *(const attn_h8 *)(k + 32 * kc);
             }
         }
+        if (Q8) {
+            const float scale = ((const float *)(run + 2 * ((size_t)D << a.page_shift)))[j & mask];
 #pragma unroll
-        for (int u = 0; u < NS; u++) {
-            if (Q8) acc[u] *= ks[u];
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int j = j0 + 16 * u + 4 * quarter + e;
-                const bool sees = 16 * c + col < rows && attn_sees(t, first + i, j);
-                const float w = lost[u] ? __builtin_nanf("") : attn_exp2(acc[u][e] * down - z);
-                sum[u][e] += sees ? w : 0.0f;
-            }
+            for (int i = 0; i < 16; i++) ks[n][i / 4][i % 4] = __shfl(scale, 8 * (i / 4) + 4 * half + i % 4, 64);
         }
     }
-    const size_t place = ((size_t)b * a.kv_heads + head) * (size_t)t.weights_stride;
+
+    float sum[NB][16];
 #pragma unroll
-    for (int u = 0; u < NS; u++)
+    for (int n = 0; n < NB; n++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            float w = sum[u][e];
+        for (int i = 0; i < 16; i++) sum[n][i] = 0.0f;
+    if (c0 < c1) put(c0 & 1);
+    __syncthreads();
+    for (int c = c0; c < c1; c++) {
+        if (c + 1 < c1) load();
+        /* positions of the block's first and last row */
+        const int p0 = first + 32 * c / t.group, p1 = first + min(32 * c + 31, rows - 1) / t.group;
+        const int buf = c & 1;
+        if (p1 >= j0) {
+            attn_f16 x[NB];
+#pragma unroll
+            for (int n = 0; n < NB; n++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) x[n][i] = 0.0f;
+#pragma unroll
+            for (int kc = 0; kc < KC; kc++) {
+                const int at = sum_unit(2 * kc + half, col);
+                const attn_h8 h = __builtin_bit_cast(attn_h8, box[buf][0][at]);
+#pragma unroll
+                for (int n = 0; n < NB; n++) x[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[n][kc], h, x[n], 0, 0, 0);
+                if (TWO) {
+                    const attn_h8 l = __builtin_bit_cast(attn_h8, box[buf][TWO ? 1 : 0][at]);
+#pragma unroll
+                    for (int n = 0; n < NB; n++) x[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[n][kc], l, x[n], 0, 0, 0);
+                }
+            }
+            const float f = cz[buf][0][col], zc = cz[buf][1][col];
+#pragma unroll
+            for (int n = 0; n < NB; n++) {
+                if (Q8)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) x[n][i] *= ks[n][i / 4][i % 4];
+                const int j = j0 + 32 * n;
+                if (attn_all_seen(t, j, 32, p0, p1) && !lost[n]) {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) sum[n][i] += attn_exp2(fmaf(x[n][i], f, -zc));
+                } else {
+                    const int r = 32 * c + col, pos = first + min(r, rows - 1) / t.group;
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const int at = 8 * (i / 4) + 4 * half + i % 4;
+                        const float w = lost[n] >> at & 1u ? __builtin_nanf("") : attn_exp2(fmaf(x[n][i], f, -zc));
+                        sum[n][i] += r < rows && attn_sees(t, pos, j + at) ? w : 0.0f;
+                    }
+                }
+            }
+        }
+        if (c + 1 < c1) put((c + 1) & 1);
+        __syncthreads();
+    }
+
+    const size_t place = (size_t)b * a.kv_heads + head;
+    float *const to = p.splits > 1 ? p.partial + ((size_t)split * a.sequences * a.kv_heads + place) * p.pitch
+                                   : t.weights + place * (size_t)t.weights_stride;
+    const float *const from = t.before ? t.before + place * (size_t)t.weights_stride : nullptr;
+#pragma unroll
+    for (int n = 0; n < NB; n++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            float w = sum[n][i];
             w += xor_partner<1>(w);
             w += xor_partner<2>(w);
             w += xor_partner<4>(w);
             w += xor_partner<8>(w);
-            const int j = j0 + 16 * u + 4 * quarter + e;
-            if (col == 0 && j < s.len)
-                t.weights[place + j] = (t.before && j < first ? t.before[place + j] : 0.0f) + w;
+            w += xor_partner<16>(w);
+            const int j = j0 + 32 * n + 8 * (i / 4) + 4 * half + i % 4;
+            if (col != 0 || j >= s.len) continue;
+            if (p.splits == 1 && from && j < first) w += from[j];
+            to[j] = w;
         }
+}
+
+/* The sums of few rows from their scores, and of many from the ranges' sums: four positions a thread. */
+__global__ __launch_bounds__(256) void sera_attn_sums_kernel(kv_args a, attn_args t, attn_sums p) {
+    const int b = (int)(blockIdx.z * gridDim.y + blockIdx.y);
+    if (b >= a.sequences) return;
+    const int head = (int)blockIdx.x % a.kv_heads, j0 = ((int)blockIdx.x / a.kv_heads * 256 + (int)threadIdx.x) * 4;
+    const kv_seq s = kv_sequence(a, b);
+    if (s.bad || j0 >= s.len) return;
+    const int first = s.len - s.n, rows = s.n * t.group;
+    const bool is_few = rows <= t.few_columns;
+    if (!is_few && p.splits == 1) return;
+    const size_t place = (size_t)b * a.kv_heads + head;
+    attn_f4 w = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (is_few) {
+        const float *x = p.scores + place * p.few_rows * p.pitch + j0;
+        for (int r = 0; r < rows; r++) {
+            const int i = r / t.group;
+            const float z = t.lse[(size_t)(s.row0 + i) * t.heads + head * t.group + r - i * t.group];
+            const attn_f4 y = *(const attn_f4 *)(x + (size_t)r * p.pitch);
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] += attn_sees(t, first + i, j0 + e) ? attn_exp2(y[e] - z) : 0.0f;
+        }
+    } else {
+        int c0, c1;
+        sum_range(t, first, rows, j0 & ~(kTokens - 1), kTokens, &c0, &c1);
+        if (c0 < c1)
+            for (int k = c0 / p.chunk; k <= (c1 - 1) / p.chunk; k++)
+                w += *(const attn_f4 *)(p.partial + ((size_t)k * a.sequences * a.kv_heads + place) * p.pitch + j0);
+    }
+    const size_t at = place * (size_t)t.weights_stride + j0;
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (j0 + e < s.len) t.weights[at + e] = (t.before && j0 + e < first ? t.before[at + e] : 0.0f) + w[e];
 }
 
 namespace {
 
 template <int TYPE, typename T, int D>
-void weights_go(const kv_args &a, const attn_args &t, hipStream_t s) {
+void columns_go(const kv_args &a, const attn_args &t, const attn_sums &p, hipStream_t s) {
     const int y = a.sequences < 32768 ? a.sequences : 32768;
-    const int64_t tiles = ((int64_t)a.max_kv + kWaves * kTokens - 1) / (kWaves * kTokens);
-    hipLaunchKernelGGL((sera_attn_weights_kernel<TYPE, T, D>),
-                       dim3((unsigned)(tiles * a.kv_heads), (unsigned)y, (unsigned)((a.sequences + y - 1) / y)),
-                       dim3(64 * kWaves), 0, s, a, t);
+    const int64_t tiles = ((int64_t)a.max_kv + kTokens - 1) / kTokens;
+    hipLaunchKernelGGL((sera_attn_columns_kernel<TYPE, T, D>),
+                       dim3((unsigned)(tiles * p.splits * a.kv_heads), (unsigned)y,
+                            (unsigned)((a.sequences + y - 1) / y)), dim3(256), 0, s, a, t, p);
 }
 
 template <int TYPE, typename T>
-void weights_d(int dim, const kv_args &a, const attn_args &t, hipStream_t s) {
-    dim == 64 ? weights_go<TYPE, T, 64>(a, t, s) : weights_go<TYPE, T, 128>(a, t, s);
+void columns_d(int dim, const kv_args &a, const attn_args &t, const attn_sums &p, hipStream_t s) {
+    dim == 64 ? columns_go<TYPE, T, 64>(a, t, p, s) : columns_go<TYPE, T, 128>(a, t, p, s);
 }
 
 template <int TYPE>
-void weights_t(uint32_t type, int dim, const kv_args &a, const attn_args &t, hipStream_t s) {
-    if (type == SERA_TYPE_F32) weights_d<TYPE, float>(dim, a, t, s);
-    else if (type == SERA_TYPE_F16) weights_d<TYPE, _Float16>(dim, a, t, s);
-    else weights_d<TYPE, __bf16>(dim, a, t, s);
+void columns_t(uint32_t type, int dim, const kv_args &a, const attn_args &t, const attn_sums &p, hipStream_t s) {
+    if (type == SERA_TYPE_F32) columns_d<TYPE, float>(dim, a, t, p, s);
+    else if (type == SERA_TYPE_F16) columns_d<TYPE, _Float16>(dim, a, t, p, s);
+    else columns_d<TYPE, __bf16>(dim, a, t, p, s);
 }
 
 }  // namespace
 
-hipError_t sera_launch_attn_weights(uint32_t cache_type, uint32_t type, int dim, const kv_args &a, const attn_args &t,
-                                    hipStream_t s) {
-    if (cache_type == SERA_KV_F16) weights_t<(int)SERA_KV_F16>(type, dim, a, t, s);
-    else weights_t<(int)SERA_KV_Q8>(type, dim, a, t, s);
+/* How the sums are made, with few_rows columns of each sequence at most in the kernel of few rows (0: none goes there) and
+ * `columns` at most elsewhere (0: none). Bytes of workspace in *bytes. */
+attn_sums sera_attn_sums_plan(const kv_args &a, int few_rows, int64_t columns, int cus, size_t *bytes) {
+    attn_sums p = {};
+    p.pitch = ((size_t)a.max_kv + 31) & ~(size_t)31;
+    p.few_rows = few_rows;
+    p.splits = 1;
+    const size_t arrays = (size_t)a.sequences * a.kv_heads;
+    if (columns > 0) {
+        /* Ranges of columns until there are some 8 workgroups for each CU (2 run at a time; the work of a position's
+         * range falls along a prompt), of 8 blocks at least. */
+        const int64_t tiles = ((int64_t)a.max_kv + kTokens - 1) / kTokens * a.kv_heads * a.sequences;
+        const int64_t blocks = (columns + 31) / 32, most = (blocks + 7) / 8;
+        int64_t want = (8ll * cus + tiles - 1) / tiles;
+        if (want > most) want = most;
+        if (want > 64) want = 64;
+        p.splits = want < 1 ? 1 : (int)want;
+        p.chunk = (int)((blocks + p.splits - 1) / p.splits);
+    }
+    p.scores_bytes = (few_rows * arrays * p.pitch * sizeof(float) + 15) & ~(size_t)15;
+    *bytes = p.scores_bytes + (p.splits > 1 ? p.splits * arrays * p.pitch * sizeof(float) : 0);
+    return p;
+}
+
+/* After attention (sera_launch_attn). many: some sequences are not the few-row kernel's. */
+hipError_t sera_launch_attn_sums(uint32_t cache_type, uint32_t type, int dim, const kv_args &a, const attn_args &args,
+                                 const attn_sums &p, bool many, hipStream_t s) {
+    attn_args t = args;
+    if (!p.few_rows) t.few_columns = -1;            /* sequences without rows are the others' too */
+    if (many) {
+        if (cache_type == SERA_KV_F16) columns_t<(int)SERA_KV_F16>(type, dim, a, t, p, s);
+        else columns_t<(int)SERA_KV_Q8>(type, dim, a, t, p, s);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    if (p.few_rows || p.splits > 1) {
+        const int y = a.sequences < 32768 ? a.sequences : 32768;
+        const int64_t tiles = ((int64_t)a.max_kv + 1023) / 1024;
+        hipLaunchKernelGGL(sera_attn_sums_kernel, dim3((unsigned)(tiles * a.kv_heads), (unsigned)y,
+                                                       (unsigned)((a.sequences + y - 1) / y)), dim3(256), 0, s, a, t, p);
+    }
     return hipGetLastError();
 }

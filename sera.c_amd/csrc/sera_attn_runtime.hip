@@ -158,10 +158,7 @@ size_t workspace_of(const sera_kv_cache *cache, const sera_kv_batch *batch, int 
     if (batch->rows < 1 || batch->rows > kMaxRows || batch->sequences < 1 || batch->sequences > kMaxSequences ||
         batch->max_new < 1 || batch->max_new > batch->rows || batch->max_kv < 1 || batch->max_kv > kMaxPositions)
         return 0;
-    const kv_args a = args_of(cache, batch);
-    size_t n = sera_attn_workspace(a, cache->head_dim, heads, device_cus());
-    if (weigh) n = ((n + 15) & ~(size_t)15) + (size_t)batch->rows * heads * sizeof(float);
-    return n;
+    return sera_attn_workspace(args_of(cache, batch), cache->head_dim, heads, device_cus(), weigh);
 }
 
 /* Attention; with `weigh`, the sums of its weights. */
@@ -177,7 +174,7 @@ int attend(const char *tag, const sera_kv_cache *cache, const sera_kv_batch *bat
     if (window < 0 || sinks < 0) return fail(-1, "%s: window=%d, sinks=%d below zero", tag, window, sinks);
     if (!isfinite(scale)) return fail(-1, "%s: the scale is not finite", tag);
     if (empty) return 0;
-    if ((int64_t)batch->rows * heads > 0x7fffffff)
+    if ((int64_t)batch->rows * heads > 0x7fffffff - (weigh ? 63 : 0))      /* the sums go by blocks of 32 columns */
         return fail(-1, "%s: %d rows of %d heads reach 2^31", tag, batch->rows, heads);
     const int64_t width = (int64_t)heads * cache->head_dim;
     if (check_rows(tag, "q", type, q, q_stride, width) || check_rows(tag, "out", type, out, out_stride, width))
@@ -208,7 +205,6 @@ int attend(const char *tag, const sera_kv_cache *cache, const sera_kv_batch *bat
         return fail(-1, "%s: the workspace must be 16-byte aligned and hold %zu bytes (%zu given)", tag, need,
                     workspace ? workspace_bytes : (size_t)0);
     if (weigh) {
-        t.lse = (float *)((uint8_t *)workspace + need) - (size_t)batch->rows * heads;
         t.before = before;
         t.weights = weights;
         t.weights_stride = weights_stride;
