@@ -35,6 +35,9 @@ struct sum_shape {
     static constexpr int UNITS = KC * 2 * 32;                  /* 16-byte units of a block's high (or low) terms */
 };
 
+typedef __attribute__((address_space(3))) attn_u4 sum_local_u4;
+typedef __attribute__((address_space(3))) void sum_local;
+
 /* Place of unit u = 2 kc + half of column `col`: (u, col), columns exchanged so that the units that a row's threads write
  * at once lie in different banks. */
 __device__ __forceinline__ int sum_unit(int u, int col) { return u * 32 + (col ^ (((u & 3) << 1) | ((u >> 2) & 1))); }
@@ -60,6 +63,7 @@ __global__ __launch_bounds__(256, 2) void sera_attn_columns_kernel(kv_args a, at
     constexpr int ES = Q8 ? 1 : 2, KC = S::KC, NB = S::NB, UNITS = S::UNITS, LOADS = S::LOADS, VEC = S::VEC;
     __shared__ attn_u4 box[2][TWO ? 2 : 1][UNITS];
     __shared__ float cz[2][2][32];                        /* each column's factor, and z */
+    __shared__ attn_f4 key_scale[Q8 ? kTokens / 4 : 1];
 
     const int b = (int)(blockIdx.z * gridDim.y + blockIdx.y);
     if (b >= a.sequences) return;
@@ -82,16 +86,16 @@ __global__ __launch_bounds__(256, 2) void sera_attn_columns_kernel(kv_args a, at
     const int my_col = tid >> 3, sub = tid & 7;
     int at_r = 32 * c0 + my_col, at_i = at_r / t.group, at_g = at_r - at_i * t.group;
     const int step_i = 32 / t.group, step_g = 32 - step_i * t.group;
-    attn_vec<T, VEC> in[LOADS];
-    float z = INFINITY;
-    const auto load = [&]() {
+    attn_vec<T, VEC> in[2][LOADS];
+    float z[2] = {INFINITY, INFINITY};
+    const auto load = [&](int place) {
         const bool there = at_r < rows;
         const int i = there ? at_i : s.n - 1, h = head * t.group + (there ? at_g : t.group - 1);
         const T *q = (const T *)t.q + (s.row0 + i) * t.q_stride + (int64_t)h * D + VEC * sub;
 #pragma unroll
-        for (int k = 0; k < LOADS; k++) in[k] = *(const attn_vec<T, VEC> *)(q + 8 * VEC * k);
+        for (int k = 0; k < LOADS; k++) in[place][k] = *(const attn_vec<T, VEC> *)(q + 8 * VEC * k);
         /* past the last column: no weight */
-        z = there ? t.lse[(size_t)(s.row0 + i) * t.heads + h] : INFINITY;
+        z[place] = there ? t.lse[(size_t)(s.row0 + i) * t.heads + h] : INFINITY;
         at_r += 32;
         at_i += step_i;
         at_g += step_g;
@@ -101,13 +105,13 @@ __global__ __launch_bounds__(256, 2) void sera_attn_columns_kernel(kv_args a, at
         }
     };
     const float sign = t.scale_log2 < 0.0f ? -1.0f : 1.0f;
-    const auto put = [&](int buf) {
+    const auto put = [&](int place, int buf) {
         float x[LOADS][VEC], top = 0.0f;
 #pragma unroll
         for (int k = 0; k < LOADS; k++)
 #pragma unroll
             for (int e = 0; e < VEC; e++) {
-                x[k][e] = kv_to_f32(in[k].v[e]);
+                x[k][e] = kv_to_f32(in[place][k].v[e]);
                 top = fmaxf(top, fabsf(x[k][e]));
             }
         top = fmaxf(top, xor_partner<1>(top));
@@ -117,7 +121,7 @@ __global__ __launch_bounds__(256, 2) void sera_attn_columns_kernel(kv_args a, at
         const float up = ldexpf(sign, e2);
         if (sub == 0) {
             cz[buf][0][my_col] = ldexpf(fabsf(t.scale_log2), -e2);
-            cz[buf][1][my_col] = z;
+            cz[buf][1][my_col] = z[place];
         }
         float minus = -1.0f;
         asm("" : "+s"(minus));
@@ -141,12 +145,12 @@ __global__ __launch_bounds__(256, 2) void sera_attn_columns_kernel(kv_args a, at
             if (TWO) *(attn_vec<_Float16, VEC> *)(to + UNITS * 16) = lo;
         }
     };
-    if (c0 < c1) load();
+    if (c0 < c1) load(0);
+    if (c0 + 1 < c1) load(1);
 
     /* Keys: row `col` of A operand n is position j0 + 32 n + col. */
     const uint8_t *base = a.data + (size_t)head * a.head_bytes;
     attn_h8 kf[NB][KC];
-    attn_f4 ks[NB][Q8 ? 4 : 1];       /* of the positions of this lane's scores: 8 (i / 4) + 4 half + i % 4 */
     uint32_t lost[NB];
 #pragma unroll
     for (int n = 0; n < NB; n++) {
@@ -165,65 +169,134 @@ __global__ __launch_bounds__(256, 2) void sera_attn_columns_kernel(kv_args a, at
         }
         if (Q8) {
             const float scale = ((const float *)(run + 2 * ((size_t)D << a.page_shift)))[j & mask];
-#pragma unroll
-            for (int i = 0; i < 16; i++) ks[n][i / 4][i % 4] = __shfl(scale, 8 * (i / 4) + 4 * half + i % 4, 64);
+            if (half == 0) ((float *)key_scale)[wave * kWaveTokens + 32 * n + col] = scale;
         }
     }
+
+    uint32_t at[4];                   /* addresses of units 2 kc + half, less 64 kc of them, by kc % 4 */
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+        at[k] = (uint32_t)(uintptr_t)(sum_local *)box + (uint32_t)(sum_unit(2 * k + half, col) - 64 * k) * 16u;
 
     float sum[NB][16];
 #pragma unroll
     for (int n = 0; n < NB; n++)
 #pragma unroll
         for (int i = 0; i < 16; i++) sum[n][i] = 0.0f;
-    if (c0 < c1) put(c0 & 1);
+    /* Row and head of the block's first and last column, without divisions. */
+    int i0 = 32 * c0 / t.group, g0 = 32 * c0 - i0 * t.group, i1 = (32 * c0 + 31) / t.group, g1 = 32 * c0 + 31 - i1 * t.group;
+    if (c0 < c1) put(0, 0);
     __syncthreads();
-    for (int c = c0; c < c1; c++) {
-        if (c + 1 < c1) load();
-        /* positions of the block's first and last row */
-        const int p0 = first + 32 * c / t.group, p1 = first + min(32 * c + 31, rows - 1) / t.group;
-        const int buf = c & 1;
-        if (p1 >= j0) {
-            attn_f16 x[NB];
+    /* Score i of a lane is of position 8 (i / 4) + 4 half + i % 4 of its 32. The weights of scores i .. i+3, which every row of the
+     * block sees, or those of 32 n + .. <= last... */
+    const auto key_scales = [&](int n, int i) {
+        return key_scale[Q8 ? wave * (kWaveTokens / 4) + 8 * n + 2 * (i / 4) + half : 0];
+    };
+    constexpr int PARTS = TWO ? 2 : 1, STAGES = KC * PARTS, DEPTH = STAGES < 6 ? STAGES - 1 : 6, PER = 16 / STAGES;
+    attn_f16 x[NB];
+    attn_f4 scales;
+    const auto weigh = [&](int n, int i, float up, float z, bool whole, int last) {
+        if (Q8 && i % 4 == 0) scales = key_scales(n, i);
+        const float w = attn_exp2(fmaf(Q8 ? x[n][i] * scales[i % 4] : x[n][i], up, -z));
+        if (whole) sum[n][i] += w;
+        else sum[n][i] += 32 * n + 8 * (i / 4) + i % 4 <= last ? w : 0.0f;
+    };
+    /* ... and all 16 with the mask, of block c. */
+    const auto weigh_masked = [&](int n, int c, float up, float z) {
+        int side = half;
+        asm volatile("" : "+v"(side));       /* nothing of this is kept through the loop */
+        const int r = 32 * c + col, pos = first + min(r, rows - 1) / t.group;
 #pragma unroll
-            for (int n = 0; n < NB; n++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) x[n][i] = 0.0f;
-#pragma unroll
-            for (int kc = 0; kc < KC; kc++) {
-                const int at = sum_unit(2 * kc + half, col);
-                const attn_h8 h = __builtin_bit_cast(attn_h8, box[buf][0][at]);
-#pragma unroll
-                for (int n = 0; n < NB; n++) x[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[n][kc], h, x[n], 0, 0, 0);
-                if (TWO) {
-                    const attn_h8 l = __builtin_bit_cast(attn_h8, box[buf][TWO ? 1 : 0][at]);
-#pragma unroll
-                    for (int n = 0; n < NB; n++) x[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[n][kc], l, x[n], 0, 0, 0);
-                }
-            }
-            const float f = cz[buf][0][col], zc = cz[buf][1][col];
-#pragma unroll
-            for (int n = 0; n < NB; n++) {
-                if (Q8)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) x[n][i] *= ks[n][i / 4][i % 4];
-                const int j = j0 + 32 * n;
-                if (attn_all_seen(t, j, 32, p0, p1) && !lost[n]) {
-#pragma unroll
-                    for (int i = 0; i < 16; i++) sum[n][i] += attn_exp2(fmaf(x[n][i], f, -zc));
-                } else {
-                    const int r = 32 * c + col, pos = first + min(r, rows - 1) / t.group;
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const int at = 8 * (i / 4) + 4 * half + i % 4;
-                        const float w = lost[n] >> at & 1u ? __builtin_nanf("") : attn_exp2(fmaf(x[n][i], f, -zc));
-                        sum[n][i] += r < rows && attn_sees(t, pos, j + at) ? w : 0.0f;
-                    }
-                }
-            }
+        for (int i = 0; i < 16; i++) {
+            if (Q8 && i % 4 == 0) scales = key_scales(n, i);
+            const int tok = 8 * (i / 4) + 4 * side + i % 4;
+            float w = attn_exp2(fmaf(Q8 ? x[n][i] * scales[i % 4] : x[n][i], up, -z));
+            w = lost[n] >> tok & 1u ? __builtin_nanf("") : w;
+            sum[n][i] += r < rows && attn_sees(t, pos, j0 + 32 * n + tok) ? w : 0.0f;
         }
-        if (c + 1 < c1) put((c + 1) & 1);
+    };
+    /* The scores of 32 positions and the block in `buf`, a fragment's MFMA a stage, with the fragments read DEPTH stages
+     * ahead and other work under them. */
+    const auto products = [&](int n, int buf, auto under) {
+        const auto fragment = [&](int st) {
+            const int kc = st / PARTS, part = st % PARTS;
+            return __builtin_bit_cast(attn_h8, *(const sum_local_u4 *)(uintptr_t)(
+                at[kc & 3] + (uint32_t)(buf * PARTS * UNITS * 16) + (uint32_t)((part * UNITS + 64 * kc) * 16)));
+        };
+        attn_h8 f[DEPTH + 1];
+#pragma unroll
+        for (int st = 0; st < DEPTH; st++) f[st] = fragment(st);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int st = 0; st < STAGES; st++) {
+            const attn_f16 none = {};
+            const attn_h8 w = f[st % (DEPTH + 1)];
+            if (st + DEPTH < STAGES) f[(st + DEPTH) % (DEPTH + 1)] = fragment(st + DEPTH);
+            x[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[n][st / PARTS], w, st ? x[n] : none, 0, 0, 0);
+            under(st);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    /* Block c is in buffer `buf`, block c + 1 in registers `buf ^ 1`, block c + 2 comes into `buf`. The weights of the
+     * first 32 positions are made under the products of the others, theirs under those of the next block's first. */
+    float up1 = 0.0f, z1 = 0.0f;      /* of the block whose x[1] waits */
+    int last1 = 0;
+    bool waits = false, plain1 = false, whole1 = false;
+    const bool simple = !(lost[0] | lost[1]) && t.window == 0;     /* the mask is the order of positions alone */
+    const auto step = [&](int c, int buf) {
+        if (c + 2 < c1) load(buf);
+        const int p0 = first + i0, p1 = min(first + i1, s.len - 1);
+        /* blocks in front of this wave's positions see none of them */
+        if (p1 >= j0) {
+            const bool whole = attn_all_seen(t, j0, kWaveTokens, p0, p1) && !(lost[0] | lost[1]), plain = whole || simple;
+            if (waits && plain1) {
+                products(0, buf, [&](int st) {
+#pragma unroll
+                    for (int e = 0; e < PER; e++) weigh(1, st * PER + e, up1, z1, whole1, last1);
+                });
+            } else {
+                if (waits) weigh_masked(1, c - 1, up1, z1);
+                products(0, buf, [](int) {});
+            }
+            up1 = cz[buf][0][col];
+            z1 = cz[buf][1][col];
+            whole1 = whole;
+            if (!whole) {       /* the last of the wave's positions that this lane's column sees, less the lane's first */
+                const int r = 32 * c + col;
+                last1 = r < rows ? first + r / t.group - j0 - 4 * half : -1;
+            }
+            if (plain) {
+                products(1, buf, [&](int st) {
+#pragma unroll
+                    for (int e = 0; e < PER; e++) weigh(0, st * PER + e, up1, z1, whole, last1);
+                });
+            } else {
+                products(1, buf, [](int) {});
+                weigh_masked(0, c, up1, z1);
+            }
+            waits = true;
+            plain1 = plain;
+        }
+        i0 += step_i;
+        i1 += step_i;
+        g0 += step_g;
+        g1 += step_g;
+        if (g0 >= t.group) {
+            g0 -= t.group;
+            i0++;
+        }
+        if (g1 >= t.group) {
+            g1 -= t.group;
+            i1++;
+        }
+        if (c + 1 < c1) put(buf ^ 1, buf ^ 1);
         __syncthreads();
+    };
+    for (int c = c0; c < c1; c += 2) {
+        step(c, 0);
+        if (c + 1 < c1) step(c + 1, 1);
     }
+    if (waits) weigh_masked(1, c1 - 1, up1, z1);
 
     const size_t place = (size_t)b * a.kv_heads + head;
     float *const to = p.splits > 1 ? p.partial + ((size_t)split * a.sequences * a.kv_heads + place) * p.pitch
