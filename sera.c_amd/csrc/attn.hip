@@ -194,7 +194,7 @@ static size_t sums_at(const attn_plans &p, const kv_args &a, int heads) {
 }
 static attn_sums sums_of(const attn_plans &p, const kv_args &a, int heads, int cus, size_t *bytes) {
     return sera_attn_sums_plan(a, p.few.columns ? p.few_rows : 0,
-                               p.tile.columns ? (int64_t)a.max_new * (heads / a.kv_heads) : 0, cus, bytes);
+                               p.tile.columns ? heads / a.kv_heads : 0, cus, bytes);
 }
 
 size_t sera_attn_workspace(const kv_args &a, int dim, int heads, int cus, bool weigh) {

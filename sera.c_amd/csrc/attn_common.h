@@ -31,7 +31,9 @@ struct attn_args {
 struct attn_sums {
     int few_rows;                   /* columns of a sequence in the few-row kernel, at most; 0: it has no part */
     size_t pitch;                   /* floats from one row of scores (or sums) to the next */
-    int splits, chunk;              /* ranges of columns, and 32-column blocks of one, of all other sequences */
+    int groups, share;              /* of all other sequences: workgroups of a sequence and head at most, units (blocks of 32
+                                     * columns over 256 positions) of one */
+    size_t slots;                   /* places of 256 sums for a sequence and head */
     size_t scores_bytes;            /* of the workspace; the ranges' sums lie behind */
     float *scores, *partial;
 };
@@ -75,7 +77,7 @@ hipError_t sera_launch_attn(uint32_t cache_type, uint32_t type, int dim, const k
                             hipStream_t s);
 hipError_t sera_launch_attn_tile(uint32_t cache_type, uint32_t type, int dim, const kv_args &a, const attn_args &t,
                                  const attn_plan &p, hipStream_t s);
-attn_sums sera_attn_sums_plan(const kv_args &a, int few_rows, int64_t columns, int cus, size_t *bytes);
+attn_sums sera_attn_sums_plan(const kv_args &a, int few_rows, int group, int cus, size_t *bytes);
 hipError_t sera_launch_attn_sums(uint32_t cache_type, uint32_t type, int dim, const kv_args &a, const attn_args &t,
                                  const attn_sums &p, bool many, hipStream_t s);
 hipError_t sera_launch_kv_rope(uint32_t cache_type, uint32_t type, int dim, const kv_args &a, const rope_args &r,

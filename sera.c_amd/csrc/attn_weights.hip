@@ -42,16 +42,19 @@ typedef __attribute__((address_space(3))) void sum_local;
  * at once lie in different banks. */
 __device__ __forceinline__ int sum_unit(int u, int col) { return u * 32 + (col ^ (((u & 3) << 1) | ((u >> 2) & 1))); }
 
-/* Blocks of columns c0 .. c1-1 (of 32) that see any of the positions j .. j+n-1. */
-__device__ __forceinline__ void sum_range(const attn_args &t, int first, int rows, int j, int n, int *c0, int *c1) {
-    const int i0 = max(j - first, 0);                                       /* rows before it see nothing */
-    int end = rows;
-    if (t.window > 0 && j >= t.sinks) {
-        const int64_t past = (int64_t)j + n - 1 + t.window - first;         /* nor do those from here on */
-        end = (int)min((int64_t)rows, max(past, (int64_t)0) * t.group);
-    }
-    *c0 = (int)(((int64_t)i0 * t.group) / 32);
-    *c1 = (int)(((int64_t)end + 31) / 32);
+/* Blocks of 32 columns, c0 .. c1-1, that see any of a tile's positions. */
+struct sum_blocks {
+    int c0, c1;
+};
+__device__ __forceinline__ sum_blocks sum_blocks_of(const attn_args &t, const kv_seq &s, int tile) {
+    const int first = s.len - s.n, j = tile * kTokens;
+    int64_t end = s.n;
+    if (t.window > 0 && j >= t.sinks)                   /* rows from here on see nothing of it, nor do those in front */
+        end = min(end, max((int64_t)j + kTokens - 1 + t.window - first, (int64_t)0));
+    sum_blocks r;
+    r.c0 = (int)((int64_t)max(j - first, 0) * t.group / 32);
+    r.c1 = (int)((end * t.group + 31) / 32);
+    return r;
 }
 
 }  // namespace
@@ -68,24 +71,64 @@ __global__ __launch_bounds__(256, 2) void sera_attn_columns_kernel(kv_args a, at
     const int b = (int)(blockIdx.z * gridDim.y + blockIdx.y);
     if (b >= a.sequences) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int head = (int)blockIdx.x % a.kv_heads, x0 = (int)blockIdx.x / a.kv_heads;
-    const int split = x0 % p.splits, tile0 = x0 / p.splits * kTokens, j0 = tile0 + wave * kWaveTokens;
+    const int head = (int)blockIdx.x % a.kv_heads, group_index = (int)blockIdx.x / a.kv_heads;
     const kv_seq s = kv_sequence(a, b);
     const int rows = s.n * t.group;
-    if (s.bad || tile0 >= s.len || rows <= t.few_columns) return;
+    if (s.bad || rows <= t.few_columns) return;
     const int first = s.len - s.n, mask = (1 << a.page_shift) - 1, col = lane & 31, half = lane >> 5;
-    int c0, c1;
-    sum_range(t, first, rows, tile0, kTokens, &c0, &c1);
-    if (p.splits > 1) {
-        c0 = max(c0, split * p.chunk);
-        c1 = min(c1, (split + 1) * p.chunk);
-        if (c0 >= c1) return;
+
+    /* This workgroup's units: the tile that the first one is in, by counting 256 tiles at a time. */
+    const int tiles = (s.len + kTokens - 1) / kTokens;
+    const int64_t u0 = (int64_t)group_index * p.share;
+    int tile = -1, c_first = 0;
+    {
+        __shared__ int64_t ends[4];
+        __shared__ int found[2];
+        if (tid == 0) found[0] = -1;
+        int64_t before = 0;
+        for (int x = 0; x < tiles; x += 256) {
+            int n = 0;
+            sum_blocks r = {0, 0};
+            if (x + tid < tiles) {
+                r = sum_blocks_of(t, s, x + tid);
+                n = max(r.c1 - r.c0, 0);
+            }
+            int64_t upto = n;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int64_t y = __shfl_up(upto, o, 64);
+                upto += lane >= o ? y : 0;
+            }
+            if (lane == 63) ends[wave] = upto;
+            __syncthreads();
+            int64_t from = before;
+            for (int w = 0; w < wave; w++) from += ends[w];
+            before += ends[0] + ends[1] + ends[2] + ends[3];
+            from += upto - n;
+            if (u0 >= from && u0 < from + n) {
+                found[0] = x + tid;
+                found[1] = r.c0 + (int)(u0 - from);
+            }
+            __syncthreads();
+            if (found[0] >= 0) break;
+        }
+        tile = __builtin_amdgcn_readfirstlane(found[0]);
+        c_first = __builtin_amdgcn_readfirstlane(found[1]);
     }
+    if (tiles == 0 || tile < 0) return;
+    int left = p.share;
+    const float sign = t.scale_log2 < 0.0f ? -1.0f : 1.0f;
+    const int my_col = tid >> 3, sub = tid & 7, step_i = 32 / t.group, step_g = 32 - step_i * t.group;
+    const uint8_t *base = a.data + (size_t)head * a.head_bytes;
+    for (; tile < tiles && left > 0; tile++, c_first = -1) {
+    const int tile0 = tile * kTokens, j0 = tile0 + wave * kWaveTokens;
+    const sum_blocks range = sum_blocks_of(t, s, tile);
+    const int c0 = c_first < 0 ? range.c0 : c_first, c1 = min(range.c1, c0 + left);
+    if (c0 >= c1) continue;
+    left -= c1 - c0;
 
     /* This thread's column of the block that comes next, and its loads: 8 threads to a column. */
-    const int my_col = tid >> 3, sub = tid & 7;
     int at_r = 32 * c0 + my_col, at_i = at_r / t.group, at_g = at_r - at_i * t.group;
-    const int step_i = 32 / t.group, step_g = 32 - step_i * t.group;
     attn_vec<T, VEC> in[2][LOADS];
     float z[2] = {INFINITY, INFINITY};
     const auto load = [&](int place) {
@@ -104,7 +147,6 @@ __global__ __launch_bounds__(256, 2) void sera_attn_columns_kernel(kv_args a, at
             at_i++;
         }
     };
-    const float sign = t.scale_log2 < 0.0f ? -1.0f : 1.0f;
     const auto put = [&](int place, int buf) {
         float x[LOADS][VEC], top = 0.0f;
 #pragma unroll
@@ -123,21 +165,13 @@ __global__ __launch_bounds__(256, 2) void sera_attn_columns_kernel(kv_args a, at
             cz[buf][0][my_col] = ldexpf(fabsf(t.scale_log2), -e2);
             cz[buf][1][my_col] = z[place];
         }
-        float minus = -1.0f;
-        asm("" : "+s"(minus));
 #pragma unroll
         for (int k = 0; k < LOADS; k++) {
             attn_vec<_Float16, VEC> hi, lo;
 #pragma unroll
-            for (int e = 0; e < VEC; e += 2) {
-                const float y0 = x[k][e] * up, y1 = x[k][e + 1] * up;
-                const attn_h2 h = attn_pack(y0, y1);
-                hi.v[e] = h[0];
-                hi.v[e + 1] = h[1];
-                if (TWO) {
-                    lo.v[e] = (_Float16)fmaf((float)h[0], minus, y0);
-                    lo.v[e + 1] = (_Float16)fmaf((float)h[1], minus, y1);
-                }
+            for (int e = 0; e < VEC; e++) {            /* scaled and rounded in one mixed instruction each */
+                hi.v[e] = (_Float16)fmaf(x[k][e], up, 0.0f);
+                if (TWO) lo.v[e] = (_Float16)fmaf(x[k][e], up, -(float)hi.v[e]);
             }
             const int ch = 8 * VEC * k + VEC * sub;
             uint8_t *to = (uint8_t *)&box[buf][0][sum_unit(ch >> 3, my_col)] + (ch & 7) * 2;
@@ -145,11 +179,10 @@ __global__ __launch_bounds__(256, 2) void sera_attn_columns_kernel(kv_args a, at
             if (TWO) *(attn_vec<_Float16, VEC> *)(to + UNITS * 16) = lo;
         }
     };
-    if (c0 < c1) load(0);
+    load(0);
     if (c0 + 1 < c1) load(1);
 
     /* Keys: row `col` of A operand n is position j0 + 32 n + col. */
-    const uint8_t *base = a.data + (size_t)head * a.head_bytes;
     attn_h8 kf[NB][KC];
     uint32_t lost[NB];
 #pragma unroll
@@ -173,6 +206,12 @@ __global__ __launch_bounds__(256, 2) void sera_attn_columns_kernel(kv_args a, at
         }
     }
 
+    /* They have to have landed here: a wait for them in the loop would be one for the columns on their way. */
+#pragma unroll
+    for (int n = 0; n < NB; n++)
+#pragma unroll
+        for (int kc = 0; kc < KC; kc++) asm volatile("" : "+v"(kf[n][kc]));
+
     uint32_t at[4];                   /* addresses of units 2 kc + half, less 64 kc of them, by kc % 4 */
 #pragma unroll
     for (int k = 0; k < 4; k++)
@@ -185,7 +224,7 @@ __global__ __launch_bounds__(256, 2) void sera_attn_columns_kernel(kv_args a, at
         for (int i = 0; i < 16; i++) sum[n][i] = 0.0f;
     /* Row and head of the block's first and last column, without divisions. */
     int i0 = 32 * c0 / t.group, g0 = 32 * c0 - i0 * t.group, i1 = (32 * c0 + 31) / t.group, g1 = 32 * c0 + 31 - i1 * t.group;
-    if (c0 < c1) put(0, 0);
+    put(0, 0);
     __syncthreads();
     /* Score i of a lane is of position 8 (i / 4) + 4 half + i % 4 of its 32. The weights of scores i .. i+3, which every row of the
      * block sees, or those of 32 n + .. <= last... */
@@ -195,11 +234,14 @@ __global__ __launch_bounds__(256, 2) void sera_attn_columns_kernel(kv_args a, at
     constexpr int PARTS = TWO ? 2 : 1, STAGES = KC * PARTS, DEPTH = STAGES < 6 ? STAGES - 1 : 6, PER = 16 / STAGES;
     attn_f16 x[NB];
     attn_f4 scales;
-    const auto weigh = [&](int n, int i, float up, float z, bool whole, int last) {
+    const auto weigh = [&](int n, int i, float up, float z) {
+        if (Q8 && i % 4 == 0) scales = key_scales(n, i);
+        sum[n][i] += attn_exp2(fmaf(Q8 ? x[n][i] * scales[i % 4] : x[n][i], up, -z));
+    };
+    const auto weigh_to = [&](int n, int i, float up, float z, int last) {
         if (Q8 && i % 4 == 0) scales = key_scales(n, i);
         const float w = attn_exp2(fmaf(Q8 ? x[n][i] * scales[i % 4] : x[n][i], up, -z));
-        if (whole) sum[n][i] += w;
-        else sum[n][i] += 32 * n + 8 * (i / 4) + i % 4 <= last ? w : 0.0f;
+        sum[n][i] += 32 * n + 8 * (i / 4) + i % 4 <= last ? w : 0.0f;
     };
     /* ... and all 16 with the mask, of block c. */
     const auto weigh_masked = [&](int n, int c, float up, float z) {
@@ -249,10 +291,15 @@ __global__ __launch_bounds__(256, 2) void sera_attn_columns_kernel(kv_args a, at
         /* blocks in front of this wave's positions see none of them */
         if (p1 >= j0) {
             const bool whole = attn_all_seen(t, j0, kWaveTokens, p0, p1) && !(lost[0] | lost[1]), plain = whole || simple;
-            if (waits && plain1) {
+            if (waits && whole1) {
                 products(0, buf, [&](int st) {
 #pragma unroll
-                    for (int e = 0; e < PER; e++) weigh(1, st * PER + e, up1, z1, whole1, last1);
+                    for (int e = 0; e < PER; e++) weigh(1, st * PER + e, up1, z1);
+                });
+            } else if (waits && plain1) {
+                products(0, buf, [&](int st) {
+#pragma unroll
+                    for (int e = 0; e < PER; e++) weigh_to(1, st * PER + e, up1, z1, last1);
                 });
             } else {
                 if (waits) weigh_masked(1, c - 1, up1, z1);
@@ -265,10 +312,15 @@ __global__ __launch_bounds__(256, 2) void sera_attn_columns_kernel(kv_args a, at
                 const int r = 32 * c + col;
                 last1 = r < rows ? first + r / t.group - j0 - 4 * half : -1;
             }
-            if (plain) {
+            if (whole) {
                 products(1, buf, [&](int st) {
 #pragma unroll
-                    for (int e = 0; e < PER; e++) weigh(0, st * PER + e, up1, z1, whole, last1);
+                    for (int e = 0; e < PER; e++) weigh(0, st * PER + e, up1, z1);
+                });
+            } else if (plain) {
+                products(1, buf, [&](int st) {
+#pragma unroll
+                    for (int e = 0; e < PER; e++) weigh_to(0, st * PER + e, up1, z1, last1);
                 });
             } else {
                 products(1, buf, [](int) {});
@@ -298,10 +350,10 @@ __global__ __launch_bounds__(256, 2) void sera_attn_columns_kernel(kv_args a, at
     }
     if (waits) weigh_masked(1, c1 - 1, up1, z1);
 
-    const size_t place = (size_t)b * a.kv_heads + head;
-    float *const to = p.splits > 1 ? p.partial + ((size_t)split * a.sequences * a.kv_heads + place) * p.pitch
-                                   : t.weights + place * (size_t)t.weights_stride;
-    const float *const from = t.before ? t.before + place * (size_t)t.weights_stride : nullptr;
+    /* The tile's sums (or this workgroup's part of them) go to a place of their own, number group_index + tile: each next one
+     * of a sequence and head has the next workgroup, the next tile or both. */
+    float *const to = p.partial + (((size_t)b * a.kv_heads + head) * p.slots + group_index + tile) * kTokens +
+                      wave * kWaveTokens;
 #pragma unroll
     for (int n = 0; n < NB; n++)
 #pragma unroll
@@ -312,45 +364,74 @@ __global__ __launch_bounds__(256, 2) void sera_attn_columns_kernel(kv_args a, at
             w += xor_partner<4>(w);
             w += xor_partner<8>(w);
             w += xor_partner<16>(w);
-            const int j = j0 + 32 * n + 8 * (i / 4) + 4 * half + i % 4;
-            if (col != 0 || j >= s.len) continue;
-            if (p.splits == 1 && from && j < first) w += from[j];
-            to[j] = w;
+            if (col == 0) to[32 * n + 8 * (i / 4) + 4 * half + i % 4] = w;
         }
+    __syncthreads();        /* the next tile's first block goes where the last one's is read */
+    }
 }
 
-/* The sums of few rows from their scores, and of many from the ranges' sums: four positions a thread. */
+/* The sums of few rows from their scores, and of many from the workgroups' parts: four positions a thread, a tile a wave. */
 __global__ __launch_bounds__(256) void sera_attn_sums_kernel(kv_args a, attn_args t, attn_sums p) {
     const int b = (int)(blockIdx.z * gridDim.y + blockIdx.y);
     if (b >= a.sequences) return;
-    const int head = (int)blockIdx.x % a.kv_heads, j0 = ((int)blockIdx.x / a.kv_heads * 256 + (int)threadIdx.x) * 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int head = (int)blockIdx.x % a.kv_heads, tile = (int)blockIdx.x / a.kv_heads * 4 + wave;
+    const int j = tile * kTokens + 4 * lane;
     const kv_seq s = kv_sequence(a, b);
-    if (s.bad || j0 >= s.len) return;
+    if (s.bad || tile * kTokens >= s.len) return;
     const int first = s.len - s.n, rows = s.n * t.group;
-    const bool is_few = rows <= t.few_columns;
-    if (!is_few && p.splits == 1) return;
     const size_t place = (size_t)b * a.kv_heads + head;
+    constexpr int BATCH = 8;        /* loads on their way */
     attn_f4 w = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (is_few) {
-        const float *x = p.scores + place * p.few_rows * p.pitch + j0;
-        for (int r = 0; r < rows; r++) {
-            const int i = r / t.group;
-            const float z = t.lse[(size_t)(s.row0 + i) * t.heads + head * t.group + r - i * t.group];
-            const attn_f4 y = *(const attn_f4 *)(x + (size_t)r * p.pitch);
+    if (rows <= t.few_columns) {
+        const float *x = p.scores + place * p.few_rows * p.pitch + j;
+        const float *z = t.lse + (size_t)s.row0 * t.heads + head * t.group;
+        if (j < s.len)
+            for (int r = 0; r < rows; r += BATCH) {
+                attn_f4 y[BATCH];
+                float l[BATCH];
+                int pos[BATCH];
 #pragma unroll
-            for (int e = 0; e < 4; e++) w[e] += attn_sees(t, first + i, j0 + e) ? attn_exp2(y[e] - z) : 0.0f;
-        }
+                for (int k = 0; k < BATCH; k++) {
+                    const int rr = min(r + k, rows - 1), i = rr / t.group;
+                    y[k] = *(const attn_f4 *)(x + (size_t)rr * p.pitch);
+                    l[k] = z[(size_t)i * t.heads + rr - i * t.group];
+                    pos[k] = r + k < rows ? first + i : -1;
+                }
+#pragma unroll
+                for (int k = 0; k < BATCH; k++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        w[e] += pos[k] >= 0 && attn_sees(t, pos[k], j + e) ? attn_exp2(y[k][e] - l[k]) : 0.0f;
+            }
     } else {
-        int c0, c1;
-        sum_range(t, first, rows, j0 & ~(kTokens - 1), kTokens, &c0, &c1);
-        if (c0 < c1)
-            for (int k = c0 / p.chunk; k <= (c1 - 1) / p.chunk; k++)
-                w += *(const attn_f4 *)(p.partial + ((size_t)k * a.sequences * a.kv_heads + place) * p.pitch + j0);
+        /* units in front of the tile's */
+        int64_t u0 = 0;
+        for (int x = lane; x < tile; x += 64) {
+            const sum_blocks r = sum_blocks_of(t, s, x);
+            u0 += max(r.c1 - r.c0, 0);
+        }
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) u0 += __shfl_xor(u0, o, 64);
+        const sum_blocks range = sum_blocks_of(t, s, tile);
+        const int64_t u1 = u0 + max(range.c1 - range.c0, 0);
+        if (u0 < u1) {
+            const int g0 = (int)(u0 / p.share), g1 = (int)((u1 - 1) / p.share);
+            const float *x = p.partial + (place * p.slots + tile) * kTokens + 4 * lane;
+            for (int g = g0; g <= g1; g += BATCH) {
+                attn_f4 y[BATCH];
+#pragma unroll
+                for (int k = 0; k < BATCH; k++) y[k] = *(const attn_f4 *)(x + (size_t)min(g + k, g1) * kTokens);
+#pragma unroll
+                for (int k = 0; k < BATCH; k++)
+                    if (g + k <= g1) w += y[k];
+            }
+        }
     }
-    const size_t at = place * (size_t)t.weights_stride + j0;
+    const size_t at = place * (size_t)t.weights_stride + j;
 #pragma unroll
     for (int e = 0; e < 4; e++)
-        if (j0 + e < s.len) t.weights[at + e] = (t.before && j0 + e < first ? t.before[at + e] : 0.0f) + w[e];
+        if (j + e < s.len) t.weights[at + e] = (t.before && j + e < first ? t.before[at + e] : 0.0f) + w[e];
 }
 
 namespace {
@@ -358,10 +439,9 @@ namespace {
 template <int TYPE, typename T, int D>
 void columns_go(const kv_args &a, const attn_args &t, const attn_sums &p, hipStream_t s) {
     const int y = a.sequences < 32768 ? a.sequences : 32768;
-    const int64_t tiles = ((int64_t)a.max_kv + kTokens - 1) / kTokens;
     hipLaunchKernelGGL((sera_attn_columns_kernel<TYPE, T, D>),
-                       dim3((unsigned)(tiles * p.splits * a.kv_heads), (unsigned)y,
-                            (unsigned)((a.sequences + y - 1) / y)), dim3(256), 0, s, a, t, p);
+                       dim3((unsigned)(p.groups * a.kv_heads), (unsigned)y, (unsigned)((a.sequences + y - 1) / y)),
+                       dim3(256), 0, s, a, t, p);
 }
 
 template <int TYPE, typename T>
@@ -379,26 +459,36 @@ void columns_t(uint32_t type, int dim, const kv_args &a, const attn_args &t, con
 }  // namespace
 
 /* How the sums are made, with few_rows columns of each sequence at most in the kernel of few rows (0: none goes there) and
- * `columns` at most elsewhere (0: none). Bytes of workspace in *bytes. */
-attn_sums sera_attn_sums_plan(const kv_args &a, int few_rows, int64_t columns, int cus, size_t *bytes) {
+ * groups of `group` columns for each of max_new rows at most elsewhere (0: none). Bytes of workspace in *bytes. */
+attn_sums sera_attn_sums_plan(const kv_args &a, int few_rows, int group, int cus, size_t *bytes) {
     attn_sums p = {};
     p.pitch = ((size_t)a.max_kv + 31) & ~(size_t)31;
     p.few_rows = few_rows;
-    p.splits = 1;
     const size_t arrays = (size_t)a.sequences * a.kv_heads;
-    if (columns > 0) {
-        /* Ranges of columns until there are some 8 workgroups for each CU (2 run at a time; the work of a position's
-         * range falls along a prompt), of 8 blocks at least. */
-        const int64_t tiles = ((int64_t)a.max_kv + kTokens - 1) / kTokens * a.kv_heads * a.sequences;
-        const int64_t blocks = (columns + 31) / 32, most = (blocks + 7) / 8;
-        int64_t want = (8ll * cus + tiles - 1) / tiles;
-        if (want > most) want = most;
-        if (want > 64) want = 64;
-        p.splits = want < 1 ? 1 : (int)want;
-        p.chunk = (int)((blocks + p.splits - 1) / p.splits);
-    }
     p.scores_bytes = (few_rows * arrays * p.pitch * sizeof(float) + 15) & ~(size_t)15;
-    *bytes = p.scores_bytes + (p.splits > 1 ? p.splits * arrays * p.pitch * sizeof(float) : 0);
+    *bytes = p.scores_bytes;
+    if (!group) return p;
+    /* The units of a sequence of max_new rows over max_kv positions: of tile t those of rows behind it, of all rows at most. A
+     * block begun counts, so a shorter sequence has no more. */
+    const int64_t tiles = ((int64_t)a.max_kv + kTokens - 1) / kTokens;
+    const int64_t blocks = ((int64_t)a.max_new * group + 31) / 32;
+    const int64_t part = ((int64_t)a.max_kv - blocks * 32 / group) / kTokens;      /* tiles in front of all rows, about */
+    int64_t units = 0;
+    const int64_t whole = part < 0 ? 0 : part > tiles ? tiles : part;
+    units += whole * blocks;
+    for (int64_t x = whole; x < tiles; x++) {
+        const int64_t n = ((int64_t)a.max_kv - x * kTokens) * group / 32 + 2;
+        units += n < blocks ? n : blocks;
+    }
+    /* Two workgroups run on a CU; each has an equal share of all units, of 8 at least: the start of one costs some 5. */
+    const int64_t sequences = (a.rows + a.max_new - 1) / a.max_new;
+    int64_t share = (units * sequences * a.kv_heads + 2ll * cus - 1) / (2ll * cus);
+    if (share < 8) share = 8;
+    if (share > 0x3fffffff) share = 0x3fffffff;
+    p.share = (int)share;
+    p.groups = (int)((units + share - 1) / share);
+    p.slots = (size_t)(p.groups + tiles);
+    *bytes += arrays * p.slots * kTokens * sizeof(float);
     return p;
 }
 
@@ -413,11 +503,9 @@ hipError_t sera_launch_attn_sums(uint32_t cache_type, uint32_t type, int dim, co
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    if (p.few_rows || p.splits > 1) {
-        const int y = a.sequences < 32768 ? a.sequences : 32768;
-        const int64_t tiles = ((int64_t)a.max_kv + 1023) / 1024;
-        hipLaunchKernelGGL(sera_attn_sums_kernel, dim3((unsigned)(tiles * a.kv_heads), (unsigned)y,
-                                                       (unsigned)((a.sequences + y - 1) / y)), dim3(256), 0, s, a, t, p);
-    }
+    const int y = a.sequences < 32768 ? a.sequences : 32768;
+    const int64_t four = ((int64_t)a.max_kv + 4 * kTokens - 1) / (4 * kTokens);
+    hipLaunchKernelGGL(sera_attn_sums_kernel, dim3((unsigned)(four * a.kv_heads), (unsigned)y,
+                                                   (unsigned)((a.sequences + y - 1) / y)), dim3(256), 0, s, a, t, p);
     return hipGetLastError();
 }
