@@ -24,14 +24,15 @@
 
 namespace {
 
-constexpr int kTokens = 256, kWaveTokens = 64;        /* positions of a workgroup and a wave */
+constexpr int kWaves = 8, kWaveTokens = 64, kTokens = kWaves * kWaveTokens;      /* positions of a wave and a workgroup */
 
 template <typename T, int D>
 struct sum_shape {
     static constexpr bool TWO = sizeof(T) == 4;
     static constexpr int KC = D / 16, NB = kWaveTokens / 32;
     static constexpr int VEC = 16 / (int)sizeof(T);            /* elements of a 16-byte load */
-    static constexpr int LOADS = D / (8 * VEC);                /* of a thread, 8 threads to a column */
+    static constexpr int TPC = D / VEC < 16 ? D / VEC : 16;    /* threads to a column */
+    static constexpr int LOADS = D / (TPC * VEC);              /* of a thread */
     static constexpr int UNITS = KC * 2 * 32;                  /* 16-byte units of a block's high (or low) terms */
 };
 
@@ -60,10 +61,10 @@ __device__ __forceinline__ sum_blocks sum_blocks_of(const attn_args &t, const kv
 }  // namespace
 
 template <int TYPE, typename T, int D>
-__global__ __launch_bounds__(256, 2) void sera_attn_columns_kernel(kv_args a, attn_args t, attn_sums p) {
+__global__ __launch_bounds__(64 * kWaves, 2) void sera_attn_columns_kernel(kv_args a, attn_args t, attn_sums p) {
     using S = sum_shape<T, D>;
     constexpr bool Q8 = TYPE == (int)SERA_KV_Q8, TWO = S::TWO;
-    constexpr int ES = Q8 ? 1 : 2, KC = S::KC, NB = S::NB, UNITS = S::UNITS, LOADS = S::LOADS, VEC = S::VEC;
+    constexpr int ES = Q8 ? 1 : 2, KC = S::KC, NB = S::NB, UNITS = S::UNITS, LOADS = S::LOADS, VEC = S::VEC, TPC = S::TPC;
     __shared__ attn_u4 box[2][TWO ? 2 : 1][UNITS];
     __shared__ float cz[2][2][32];                        /* each column's factor, and z */
     __shared__ attn_f4 key_scale[Q8 ? kTokens / 4 : 1];
@@ -77,16 +78,16 @@ __global__ __launch_bounds__(256, 2) void sera_attn_columns_kernel(kv_args a, at
     if (s.bad || rows <= t.few_columns) return;
     const int first = s.len - s.n, mask = (1 << a.page_shift) - 1, col = lane & 31, half = lane >> 5;
 
-    /* This workgroup's units: the tile that the first one is in, by counting 256 tiles at a time. */
+    /* This workgroup's units: the tile that the first one is in, by counting as many tiles as there are threads at a time. */
     const int tiles = (s.len + kTokens - 1) / kTokens;
     const int64_t u0 = (int64_t)group_index * p.share;
     int tile = -1, c_first = 0;
     {
-        __shared__ int64_t ends[4];
+        __shared__ int64_t ends[kWaves];
         __shared__ int found[2];
         if (tid == 0) found[0] = -1;
         int64_t before = 0;
-        for (int x = 0; x < tiles; x += 256) {
+        for (int x = 0; x < tiles; x += 64 * kWaves) {
             int n = 0;
             sum_blocks r = {0, 0};
             if (x + tid < tiles) {
@@ -102,8 +103,10 @@ __global__ __launch_bounds__(256, 2) void sera_attn_columns_kernel(kv_args a, at
             if (lane == 63) ends[wave] = upto;
             __syncthreads();
             int64_t from = before;
-            for (int w = 0; w < wave; w++) from += ends[w];
-            before += ends[0] + ends[1] + ends[2] + ends[3];
+            for (int w = 0; w < kWaves; w++) {
+                from += w < wave ? ends[w] : 0;
+                before += ends[w];
+            }
             from += upto - n;
             if (u0 >= from && u0 < from + n) {
                 found[0] = x + tid;
@@ -118,7 +121,7 @@ __global__ __launch_bounds__(256, 2) void sera_attn_columns_kernel(kv_args a, at
     if (tiles == 0 || tile < 0) return;
     int left = p.share;
     const float sign = t.scale_log2 < 0.0f ? -1.0f : 1.0f;
-    const int my_col = tid >> 3, sub = tid & 7, step_i = 32 / t.group, step_g = 32 - step_i * t.group;
+    const int my_col = tid / TPC, sub = tid % TPC, step_i = 32 / t.group, step_g = 32 - step_i * t.group;
     const uint8_t *base = a.data + (size_t)head * a.head_bytes;
     for (; tile < tiles && left > 0; tile++, c_first = -1) {
     const int tile0 = tile * kTokens, j0 = tile0 + wave * kWaveTokens;
@@ -127,18 +130,20 @@ __global__ __launch_bounds__(256, 2) void sera_attn_columns_kernel(kv_args a, at
     if (c0 >= c1) continue;
     left -= c1 - c0;
 
-    /* This thread's column of the block that comes next, and its loads: 8 threads to a column. */
+    /* This thread's column of the block that comes next, and its loads (32 columns may need fewer threads than there are). */
     int at_r = 32 * c0 + my_col, at_i = at_r / t.group, at_g = at_r - at_i * t.group;
     attn_vec<T, VEC> in[2][LOADS];
-    float z[2] = {INFINITY, INFINITY};
+    float z[2];
+    bool there[2];                    /* not past the last column, which have no weight */
+    const bool loads = 32 * TPC == 64 * kWaves || my_col < 32;
     const auto load = [&](int place) {
-        const bool there = at_r < rows;
-        const int i = there ? at_i : s.n - 1, h = head * t.group + (there ? at_g : t.group - 1);
+        if (!loads) return;
+        there[place] = at_r < rows;
+        const int i = there[place] ? at_i : s.n - 1, h = head * t.group + (there[place] ? at_g : t.group - 1);
         const T *q = (const T *)t.q + (s.row0 + i) * t.q_stride + (int64_t)h * D + VEC * sub;
 #pragma unroll
-        for (int k = 0; k < LOADS; k++) in[place][k] = *(const attn_vec<T, VEC> *)(q + 8 * VEC * k);
-        /* past the last column: no weight */
-        z[place] = there ? t.lse[(size_t)(s.row0 + i) * t.heads + h] : INFINITY;
+        for (int k = 0; k < LOADS; k++) in[place][k] = *(const attn_vec<T, VEC> *)(q + TPC * VEC * k);
+        z[place] = t.lse[(size_t)(s.row0 + i) * t.heads + h];
         at_r += 32;
         at_i += step_i;
         at_g += step_g;
@@ -148,6 +153,7 @@ __global__ __launch_bounds__(256, 2) void sera_attn_columns_kernel(kv_args a, at
         }
     };
     const auto put = [&](int place, int buf) {
+        if (!loads) return;
         float x[LOADS][VEC], top = 0.0f;
 #pragma unroll
         for (int k = 0; k < LOADS; k++)
@@ -159,11 +165,12 @@ __global__ __launch_bounds__(256, 2) void sera_attn_columns_kernel(kv_args a, at
         top = fmaxf(top, xor_partner<1>(top));
         top = fmaxf(top, xor_partner<2>(top));
         top = fmaxf(top, xor_partner<4>(top));
+        if (TPC == 16) top = fmaxf(top, xor_partner<8>(top));
         const int e2 = attn_q_exponent(top);
         const float up = ldexpf(sign, e2);
         if (sub == 0) {
             cz[buf][0][my_col] = ldexpf(fabsf(t.scale_log2), -e2);
-            cz[buf][1][my_col] = z[place];
+            cz[buf][1][my_col] = there[place] ? z[place] : INFINITY;
         }
 #pragma unroll
         for (int k = 0; k < LOADS; k++) {
@@ -173,7 +180,7 @@ __global__ __launch_bounds__(256, 2) void sera_attn_columns_kernel(kv_args a, at
                 hi.v[e] = (_Float16)fmaf(x[k][e], up, 0.0f);
                 if (TWO) lo.v[e] = (_Float16)fmaf(x[k][e], up, -(float)hi.v[e]);
             }
-            const int ch = 8 * VEC * k + VEC * sub;
+            const int ch = TPC * VEC * k + VEC * sub;
             uint8_t *to = (uint8_t *)&box[buf][0][sum_unit(ch >> 3, my_col)] + (ch & 7) * 2;
             *(attn_vec<_Float16, VEC> *)to = hi;
             if (TWO) *(attn_vec<_Float16, VEC> *)(to + UNITS * 16) = lo;
@@ -285,8 +292,11 @@ __global__ __launch_bounds__(256, 2) void sera_attn_columns_kernel(kv_args a, at
     int last1 = 0;
     bool waits = false, plain1 = false, whole1 = false;
     const bool simple = !(lost[0] | lost[1]) && t.window == 0;     /* the mask is the order of positions alone */
+    const bool early = wave >= kWaves / 2;
     const auto step = [&](int c, int buf) {
         if (c + 2 < c1) load(buf);
+        /* Of the two waves of a SIMD one converts the next block before its products, the other behind them. */
+        if (early && c + 1 < c1) put(buf ^ 1, buf ^ 1);
         const int p0 = first + i0, p1 = min(first + i1, s.len - 1);
         /* blocks in front of this wave's positions see none of them */
         if (p1 >= j0) {
@@ -341,7 +351,7 @@ __global__ __launch_bounds__(256, 2) void sera_attn_columns_kernel(kv_args a, at
             g1 -= t.group;
             i1++;
         }
-        if (c + 1 < c1) put(buf ^ 1, buf ^ 1);
+        if (!early && c + 1 < c1) put(buf ^ 1, buf ^ 1);
         __syncthreads();
     };
     for (int c = c0; c < c1; c += 2) {
@@ -370,15 +380,15 @@ __global__ __launch_bounds__(256, 2) void sera_attn_columns_kernel(kv_args a, at
     }
 }
 
-/* The sums of few rows from their scores, and of many from the workgroups' parts: four positions a thread, a tile a wave. */
+/* The sums of few rows from their scores, and of many from the workgroups' parts: four positions a thread. */
 __global__ __launch_bounds__(256) void sera_attn_sums_kernel(kv_args a, attn_args t, attn_sums p) {
     const int b = (int)(blockIdx.z * gridDim.y + blockIdx.y);
     if (b >= a.sequences) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int head = (int)blockIdx.x % a.kv_heads, tile = (int)blockIdx.x / a.kv_heads * 4 + wave;
-    const int j = tile * kTokens + 4 * lane;
+    const int head = (int)blockIdx.x % a.kv_heads, w0 = ((int)blockIdx.x / a.kv_heads * 4 + wave) * 256;
+    const int j = w0 + 4 * lane, tile = w0 / kTokens;
     const kv_seq s = kv_sequence(a, b);
-    if (s.bad || tile * kTokens >= s.len) return;
+    if (s.bad || w0 >= s.len) return;
     const int first = s.len - s.n, rows = s.n * t.group;
     const size_t place = (size_t)b * a.kv_heads + head;
     constexpr int BATCH = 8;        /* loads on their way */
@@ -417,7 +427,7 @@ __global__ __launch_bounds__(256) void sera_attn_sums_kernel(kv_args a, attn_arg
         const int64_t u1 = u0 + max(range.c1 - range.c0, 0);
         if (u0 < u1) {
             const int g0 = (int)(u0 / p.share), g1 = (int)((u1 - 1) / p.share);
-            const float *x = p.partial + (place * p.slots + tile) * kTokens + 4 * lane;
+            const float *x = p.partial + (place * p.slots + tile) * kTokens + j % kTokens;
             for (int g = g0; g <= g1; g += BATCH) {
                 attn_f4 y[BATCH];
 #pragma unroll
@@ -441,7 +451,7 @@ void columns_go(const kv_args &a, const attn_args &t, const attn_sums &p, hipStr
     const int y = a.sequences < 32768 ? a.sequences : 32768;
     hipLaunchKernelGGL((sera_attn_columns_kernel<TYPE, T, D>),
                        dim3((unsigned)(p.groups * a.kv_heads), (unsigned)y, (unsigned)((a.sequences + y - 1) / y)),
-                       dim3(256), 0, s, a, t, p);
+                       dim3(64 * kWaves), 0, s, a, t, p);
 }
 
 template <int TYPE, typename T>
@@ -480,9 +490,9 @@ attn_sums sera_attn_sums_plan(const kv_args &a, int few_rows, int group, int cus
         const int64_t n = ((int64_t)a.max_kv - x * kTokens) * group / 32 + 2;
         units += n < blocks ? n : blocks;
     }
-    /* Two workgroups run on a CU; each has an equal share of all units, of 8 at least: the start of one costs some 5. */
+    /* A workgroup runs on a CU; each has an equal share of all units, of 8 at least: the start of one costs some 5. */
     const int64_t sequences = (a.rows + a.max_new - 1) / a.max_new;
-    int64_t share = (units * sequences * a.kv_heads + 2ll * cus - 1) / (2ll * cus);
+    int64_t share = (units * sequences * a.kv_heads + cus - 1) / cus;
     if (share < 8) share = 8;
     if (share > 0x3fffffff) share = 0x3fffffff;
     p.share = (int)share;
@@ -504,7 +514,7 @@ hipError_t sera_launch_attn_sums(uint32_t cache_type, uint32_t type, int dim, co
         if (e != hipSuccess) return e;
     }
     const int y = a.sequences < 32768 ? a.sequences : 32768;
-    const int64_t four = ((int64_t)a.max_kv + 4 * kTokens - 1) / (4 * kTokens);
+    const int64_t four = ((int64_t)a.max_kv + 1023) / 1024;
     hipLaunchKernelGGL(sera_attn_sums_kernel, dim3((unsigned)(four * a.kv_heads), (unsigned)y,
                                                    (unsigned)((a.sequences + y - 1) / y)), dim3(256), 0, s, a, t, p);
     return hipGetLastError();
