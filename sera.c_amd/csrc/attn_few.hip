@@ -156,6 +156,11 @@ __global__ __launch_bounds__(64 * NW, OCC) void sera_attn_few_kernel(kv_args a, 
     /* Tokens of this lane: A row `col` of operand u is token QT * (col / 4) + 4 u + col % 4; its scores are
      * the tokens QT * quarter + 4 u + i. V pieces are those same tokens of one channel. */
     const int k_token = QT * (col >> 2) + (col & 3), v_token = QT * quarter;
+    float *keep[CT];        /* rows of scores, as q's: columns past the last have its q and write its scores once more */
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++)
+        keep[ct] = KEEP ? t.scores + ((size_t)(b * a.kv_heads + head) * t.few_rows +
+                                      min(ct * 16 + (PAIR ? col & 7 : col), rows - 1)) * t.pitch : nullptr;
     attn_u4 kr[NS][KP];
     typename few_piece<TYPE>::v vr[NC];
     attn_f4 ks[Q8 ? NS : 1], vs[Q8 ? NS : 1];
@@ -263,8 +268,8 @@ __global__ __launch_bounds__(64 * NW, OCC) void sera_attn_few_kernel(kv_args a, 
     #pragma unroll
                         for (int i = 0; i < 4; i++)
                             x[4 * u + i] = attn_sees(t, pos[ct], j0 + 4 * u + i) ? x[4 * u + i] : -INFINITY;
-                if (KEEP && ct * 16 + col < rows && (!PAIR || col < 8)) {
-                    float *to = t.scores + ((size_t)(b * a.kv_heads + head) * t.few_rows + ct * 16 + col) * t.pitch + j0;
+                if (KEEP) {
+                    float *to = keep[ct] + j0;
     #pragma unroll
                     for (int u = 0; u < NS; u++)
                         *(attn_f4 *)(to + 4 * u) = attn_f4{x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]};
