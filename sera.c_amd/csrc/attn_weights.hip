@@ -397,16 +397,19 @@ __global__ __launch_bounds__(256) void sera_attn_sums_kernel(kv_args a, attn_arg
         const float *x = p.scores + place * p.few_rows * p.pitch + j;
         const float *z = t.lse + (size_t)s.row0 * t.heads + head * t.group;
         if (j < s.len)
-            for (int r = 0; r < rows; r += BATCH) {
+            for (int r = 0, i = 0, g = 0; r < rows; r += BATCH) {
                 attn_f4 y[BATCH];
                 float l[BATCH];
                 int pos[BATCH];
 #pragma unroll
                 for (int k = 0; k < BATCH; k++) {
-                    const int rr = min(r + k, rows - 1), i = rr / t.group;
-                    y[k] = *(const attn_f4 *)(x + (size_t)rr * p.pitch);
-                    l[k] = z[(size_t)i * t.heads + rr - i * t.group];
+                    y[k] = *(const attn_f4 *)(x + (size_t)min(r + k, rows - 1) * p.pitch);
+                    l[k] = z[(size_t)min(i, s.n - 1) * t.heads + g];
                     pos[k] = r + k < rows ? first + i : -1;
+                    if (++g == t.group) {
+                        g = 0;
+                        i++;
+                    }
                 }
 #pragma unroll
                 for (int k = 0; k < BATCH; k++)

@@ -3,42 +3,57 @@
  * stay, and their move to new pages.
  *
  * Choice: a workgroup for each sequence and kv head. Weights become whole numbers
- * of the same order; the smallest one that stays (of the middle positions) is built bit by
- * bit, each bit by counting how many are as large. Then each wave walks a run
- * of positions of its own and writes what stays behind what the runs before it
- * keep, which a count of each run says.
+ * of the same order; the smallest one that stays is built bit by bit, each bit by
+ * counting how many are as large. Then each wave walks a run of positions of its own, held in
+ * registers up to 32768 positions, and writes what stays behind what the
+ * runs before it keep, which a count of each run says.
  *
  * Move: a wave for K or V of 16 new places of a head. A K row is a run of
- * bytes; a V token is an element of each channel's 16.
+ * bytes. A V token is an element of each channel's 16, so whole blocks of 16 old tokens
+ * come as they lie, go through LDS, and the tokens that stay are picked from there.
  */
 #include "attn_common.h"
+#include "sera_dpp.h"
 #include "sera_launch.h"
 
 namespace {
 
-constexpr int kKeepWaves = 16;
+constexpr int kKeepWaves = 4;
 
-/* A weight as a whole number of the same order, at least 1; NaN is 0. */
+/* A weight as a whole number of the same order, from 2 on; NaN is 1. */
 __device__ __forceinline__ uint32_t keep_key(float w) {
     const uint32_t u = __float_as_uint(w + 0.0f);       /* -0 becomes 0 */
-    return w != w ? 0u : (u & 0x80000000u) ? ~u : u | 0x80000000u;
+    return w != w ? 1u : (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+
+/* The sum over a wave, wave-uniform. */
+__device__ __forceinline__ int keep_wave_sum(int n) {
+    n += xor_partner<1>(n);
+    n += xor_partner<2>(n);
+    n += xor_partner<4>(n);
+    n += xor_partner<8>(n);
+    n += xor_partner<16>(n);
+    n += xor_partner<32>(n);
+    return __builtin_amdgcn_readfirstlane(n);
 }
 
 typedef uint32_t move_u4 __attribute__((ext_vector_type(4)));
 
 }  // namespace
 
+/* R: 64-position rows of a wave's run that are held in registers (the run fits); 0: they are read again each time. */
+template <int R>
 __global__ __launch_bounds__(64 * kKeepWaves) void sera_kv_keep_kernel(kv_args a, evict_args t) {
-    __shared__ int part[2][kKeepWaves], part_eq[kKeepWaves];
+    __shared__ int part[2][kKeepWaves][4], part_eq[kKeepWaves];
     const int b = (int)(blockIdx.z * gridDim.y + blockIdx.y), head = (int)blockIdx.x;
     if (b >= a.sequences) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int len = a.kv_len[b];
     const bool bad = len < 0 || len > a.max_kv, all = !bad && len <= t.keep;
     const size_t place = (size_t)b * a.kv_heads + head;
-    int *kept = t.kept + place * t.keep;
-    const float *w = t.weights + place * t.weights_stride;
-    float *to = t.new_weights + place * t.weights_stride;
+    int *__restrict__ kept = t.kept + place * t.keep;
+    const float *__restrict__ w = t.weights + place * t.weights_stride;
+    float *__restrict__ to = t.new_weights + place * t.weights_stride;
     const int count = bad ? 0 : min(len, t.keep);
     if (head == 0 && tid == 0) t.new_len[b] = bad ? -1 : count;
     for (int x = count + tid; x < t.keep; x += 64 * kKeepWaves) kept[x] = -1;
@@ -50,72 +65,115 @@ __global__ __launch_bounds__(64 * kKeepWaves) void sera_kv_keep_kernel(kv_args a
         }
         return;
     }
-    const int lo = t.sinks, hi = len - t.recent, want = t.keep - t.sinks - t.recent;     /* hi - lo > want */
+    const int lo = t.sinks, hi = len - t.recent;
 
-    /* The want-th largest key of the middle (all ones if none is wanted), and how many are larger. */
-    uint32_t least = want > 0 ? 0u : 0xffffffffu;
-    int larger = 0, turn = 0;
-    const auto count_from = [&](uint32_t key) {
-        int n = 0;
-        for (int x = lo + 64 * wave; x < hi; x += 64 * kKeepWaves)
-            n += __popcll(__ballot(x + lane < hi && keep_key(w[min(x + lane, hi - 1)]) >= key));
-        turn ^= 1;
-        if (lane == 0) part[turn][wave] = n;
-        __syncthreads();
-        n = 0;
+    /* A wave's run of positions. Those outside the middle count as the largest there are, places behind the run as none. */
+    const int run = ((len + kKeepWaves - 1) / kKeepWaves + 63) & ~63, from = min(wave * run, len), end = min(from + run, len);
+    uint32_t key[R ? R : 1];
+    const auto key_of = [&](float v, int j) { return j >= end ? 0u : j < lo || j >= hi ? 0xffffffffu : keep_key(v); };
+    if (R) {
+        float v[R ? R : 1];
 #pragma unroll
-        for (int x = 0; x < kKeepWaves; x++) n += part[turn][x];
-        return n;
+        for (int r = 0; r < R; r++) v[r] = w[min(from + 64 * r + lane, len - 1)];
+#pragma unroll
+        for (int r = 0; r < R; r++) key[r] = key_of(v[r], from + 64 * r + lane);
+    }
+    /* For every row of the run: its first position and its keys. */
+    const auto rows = [&](auto each) {
+        if constexpr (R > 0) {
+#pragma unroll
+            for (int r = 0; r < R; r++) each(from + 64 * r, key[r]);
+        } else {
+            for (int x = from; x < end; x += 64) each(x, key_of(w[min(x + lane, len - 1)], x + lane));
+        }
     };
-    if (want > 0) {
-        for (int bit = 31; bit >= 0; bit--) {
-            const uint32_t key = least | 1u << bit;
-            const int n = count_from(key);
-            if (n >= want) least = key;
-            else larger = n;
+
+    /* Of all, those outside the middle among them, t.keep stay: those above `cut`, and the first `ties` of those equal to it. The cut is the
+     * t.keep-th largest, built bit by bit; as soon as exactly that many reach it, it is the number below. */
+    uint32_t cut = 0u;
+    int larger = 0, turn = 0;
+    bool exact = false;
+    for (int bit = 30; bit >= 0 && !exact; bit -= 2) {          /* two bits: three counts */
+        int n[3] = {0, 0, 0};
+        rows([&](int, uint32_t k) {
+#pragma unroll
+            for (int i = 0; i < 3; i++) n[i] += k >= (cut | (uint32_t)(i + 1) << bit);
+        });
+        turn ^= 1;
+#pragma unroll
+        for (int i = 0; i < 3; i++) {
+            n[i] = keep_wave_sum(n[i]);
+            if (lane == 0) part[turn][wave][i] = n[i];
+        }
+        __syncthreads();
+        const uint32_t base = cut;
+#pragma unroll
+        for (int i = 0; i < 3; i++) {
+            int all = 0;
+#pragma unroll
+            for (int x = 0; x < kKeepWaves; x++) all += part[turn][x][i];
+            /* the highest that as many reach; the one above it has fewer */
+            if (all >= t.keep) cut = base | (uint32_t)(i + 1) << bit;
+            else if (cut == (i ? base | (uint32_t)i << bit : base)) larger = all;
+            exact |= all == t.keep;
+            if (all <= t.keep) break;
         }
     }
-    const int ties = want - larger;      /* of those equal to `least`, the first ones */
-
-    /* Each wave's run of positions: what it keeps for sure, and its ties. */
-    const int run = ((len + kKeepWaves - 1) / kKeepWaves + 63) & ~63, from = min(wave * run, len), end = min(from + run, len);
-    int sure = 0, equal = 0;
-    for (int x = from; x < end; x += 64) {
-        const int j = x + lane;
-        const bool middle = j >= lo && j < hi;
-        const uint32_t key = j < end ? keep_key(w[j]) : 0u;
-        sure += __popcll(__ballot(j < end && (!middle || (want > 0 && key > least))));
-        equal += __popcll(__ballot(j < end && middle && want > 0 && key == least));
+    if (exact) {
+        cut--;
+        larger = t.keep;
     }
+    const int ties = t.keep - larger;
+
+    int sure = 0, equal = 0;
+    rows([&](int, uint32_t k) {
+        sure += k > cut;
+        equal += k == cut && k != 0u;
+    });
+    sure = keep_wave_sum(sure);
+    equal = keep_wave_sum(equal);
     __syncthreads();
     if (lane == 0) {
-        part[0][wave] = sure;
+        part[0][wave][0] = sure;
         part_eq[wave] = equal;
     }
     __syncthreads();
     int at = 0, seen = 0;
-    for (int x = 0; x < wave; x++) {
-        at += part[0][x] + max(min(ties - seen, part_eq[x]), 0);
-        seen += part_eq[x];
-    }
-    for (int x = from; x < end; x += 64) {
-        const int j = x + lane;
-        const bool middle = j >= lo && j < hi;
-        const float value = j < end ? w[j] : 0.0f;
-        const uint32_t key = keep_key(value);
-        const unsigned long long below = (1ull << lane) - 1ull;
-        const bool tie = j < end && middle && want > 0 && key == least;
+#pragma unroll
+    for (int x = 0; x < kKeepWaves; x++)
+        if (x < wave) {
+            at += part[0][x][0] + max(min(ties - seen, part_eq[x]), 0);
+            seen += part_eq[x];
+        }
+    const unsigned long long below = (1ull << lane) - 1ull;
+    const auto put = [&](int x, uint32_t k, float v) {
+        const bool tie = k == cut && k != 0u;
         const unsigned long long tied = __ballot(tie);
-        const bool stays = j < end && (!middle || (want > 0 && key > least) ||
-                                       (tie && seen + __popcll(tied & below) < ties));
+        const bool stays = k > cut || (tie && seen + __popcll(tied & below) < ties);
         const unsigned long long staying = __ballot(stays);
         if (stays) {
             const int p = at + __popcll(staying & below);
-            kept[p] = j;
-            to[p] = value;
+            kept[p] = x + lane;
+            to[p] = v;
         }
         at += __popcll(staying);
         seen += __popcll(tied);
+    };
+    if constexpr (R > 0) {
+        constexpr int BATCH = 8;        /* loads on their way */
+#pragma unroll
+        for (int r = 0; r < R; r += BATCH) {
+            float v[BATCH];
+#pragma unroll
+            for (int i = 0; i < BATCH; i++) v[i] = w[min(from + 64 * (r + i) + lane, len - 1)];
+#pragma unroll
+            for (int i = 0; i < BATCH; i++) put(from + 64 * (r + i), key[r + i], v[i]);
+        }
+    } else {
+        for (int x = from; x < end; x += 64) {
+            const float v = w[min(x + lane, len - 1)];
+            put(x, key_of(v, x + lane), v);
+        }
     }
 }
 
@@ -123,6 +181,8 @@ __global__ __launch_bounds__(64 * kKeepWaves) void sera_kv_keep_kernel(kv_args a
 template <int ES, int D>
 __global__ __launch_bounds__(256) void sera_kv_move_kernel(kv_args a, evict_args t, int blocks) {
     constexpr int ROW = D * ES, LANES = ROW / 16, ROWS = 64 / LANES, N = 16 / ROWS;
+    constexpr int DW = 4 * ES;                           /* dwords of a channel's 16 tokens */
+    __shared__ uint32_t turn[2][DW][D];                  /* of the waves that move V: a block, dword by dword of all channels */
     const int b = (int)(blockIdx.z * gridDim.y + blockIdx.y);
     if (b >= a.sequences) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -171,29 +231,47 @@ __global__ __launch_bounds__(256) void sera_kv_move_kernel(kv_args a, evict_args
         }
         return;
     }
-    for (int d = lane; d < D; d += 64) {
-        uint32_t w[4 * ES];
+    uint32_t w[D / 64][DW], (*const box)[D] = turn[wave >> 1];
 #pragma unroll
-        for (int i = 0; i < 4 * ES; i++) w[i] = 0u;
+    for (int i = 0; i < D / 64; i++)
 #pragma unroll
-        for (int y = 0; y < 16; y++) {
-            const int p = __builtin_amdgcn_readlane(page, y), at = __builtin_amdgcn_readlane(pos, y) & mask;
-            uint32_t v = lost & (ES == 2 ? 0xffffu : 0xffu);
-            if (p >= 0) {
-                const uint8_t *from = src + (size_t)p * a.page_bytes + kv_bytes + (size_t)(at & ~15) * ROW +
-                                      (16 * d + (at & 15)) * ES;
-                v = ES == 2 ? (uint32_t)*(const uint16_t *)from : (uint32_t)*from;
-            }
-            w[y * ES / 4] |= v << (y * ES % 4 * 8);
+        for (int k = 0; k < DW; k++) w[i][k] = 0u;
+    int there = -1;                                      /* the position of the block in LDS */
+#pragma unroll
+    for (int y = 0; y < 16; y++) {
+        const int p = __builtin_amdgcn_readlane(page, y), from = __builtin_amdgcn_readlane(pos, y), o = from & 15;
+        if (y < n && from - o != there) {
+            there = from - o;
+            const uint8_t *block = src + (size_t)max(p, 0) * a.page_bytes + kv_bytes + (size_t)(there & mask) * ROW;
+#pragma unroll
+            for (int i = 0; i < D / 64; i++)
+#pragma unroll
+                for (int k = 0; k < ES; k++) {
+                    move_u4 x = ((const move_u4 *)(block + (size_t)(64 * i + lane) * (16 * ES)))[k];
+                    if (p < 0) x = move_u4{lost, lost, lost, lost};
+#pragma unroll
+                    for (int e = 0; e < 4; e++) box[4 * k + e][64 * i + lane] = x[e];
+                }
+            asm volatile("" ::: "memory");               /* the wave's own LDS, which it accesses in order */
         }
-        uint8_t *to = dst + kv_bytes + (size_t)new_slot * ROW + 16 * d * ES;
+#pragma unroll
+        for (int i = 0; i < D / 64; i++) {
+            const uint32_t v = box[o * ES / 4][64 * i + lane] >> (o * ES % 4 * 8);
+            w[i][y * ES / 4] |= (v & (ES == 2 ? 0xffffu : 0xffu)) << (y * ES % 4 * 8);
+        }
+        asm volatile("" ::: "memory");
+    }
+#pragma unroll
+    for (int i = 0; i < D / 64; i++) {
+        uint8_t *to = dst + kv_bytes + (size_t)new_slot * ROW + 16 * (64 * i + lane) * ES;
         if (n == 16) {
 #pragma unroll
-            for (int i = 0; i < ES; i++) ((move_u4 *)to)[i] = move_u4{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+            for (int k = 0; k < ES; k++)
+                ((move_u4 *)to)[k] = move_u4{w[i][4 * k], w[i][4 * k + 1], w[i][4 * k + 2], w[i][4 * k + 3]};
         } else {
 #pragma unroll
             for (int y = 0; y < 16; y++) {
-                const uint32_t v = w[y * ES / 4] >> (y * ES % 4 * 8);
+                const uint32_t v = w[i][y * ES / 4] >> (y * ES % 4 * 8);
                 if (y < n) {
                     if (ES == 2) ((uint16_t *)to)[y] = (uint16_t)v;
                     else to[y] = (uint8_t)v;
@@ -207,7 +285,11 @@ __global__ __launch_bounds__(256) void sera_kv_move_kernel(kv_args a, evict_args
 hipError_t sera_launch_kv_evict(uint32_t cache_type, int dim, const kv_args &a, const evict_args &t, hipStream_t s) {
     const int y = a.sequences < 32768 ? a.sequences : 32768;
     const unsigned z = (unsigned)((a.sequences + y - 1) / y);
-    hipLaunchKernelGGL(sera_kv_keep_kernel, dim3((unsigned)a.kv_heads, (unsigned)y, z), dim3(64 * kKeepWaves), 0, s, a, t);
+    const dim3 heads((unsigned)a.kv_heads, (unsigned)y, z), threads(64 * kKeepWaves);
+    if (a.max_kv <= 16 * 64 * kKeepWaves) hipLaunchKernelGGL(sera_kv_keep_kernel<16>, heads, threads, 0, s, a, t);
+    else if (a.max_kv <= 32 * 64 * kKeepWaves) hipLaunchKernelGGL(sera_kv_keep_kernel<32>, heads, threads, 0, s, a, t);
+    else if (a.max_kv <= 128 * 64 * kKeepWaves) hipLaunchKernelGGL(sera_kv_keep_kernel<128>, heads, threads, 0, s, a, t);
+    else hipLaunchKernelGGL(sera_kv_keep_kernel<0>, heads, threads, 0, s, a, t);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const int most = t.keep < a.max_kv ? t.keep : a.max_kv, blocks = (most + 15) / 16;
