@@ -6,14 +6,24 @@
  *
  *   log p(x) = (x - m) - log s       H = log s - t / s
  *
- * A wave takes a piece of a row, 64 lanes x 16 bytes at a time. The top: a
+ * (x log2(e) - m log2(e) in one instruction instead of a difference and a product would leave an
+ * error of m's size: exponents of 2^20 and more come out wrong.)
+ *
+ * A wave takes a piece of a row, 16 elements of a lane at a time. The top: a
  * wave holds candidates in LDS as 64-bit keys, the logit as a whole number of the same order
  * above the inverted id, so no two are alike and equal logits are in the order of
- * their ids. An element that is below the top-th candidate of the last cut is passed over, which is
- * a comparison of a lane's largest one for almost all; the others are
- * appended, and a full list is cut to the top again. The four lists of a workgroup
- * are cut to one; a row that is split over workgroups leaves (m, s, t) and a
+ * their ids. The workgroup keeps the maximum of each lane number over its waves: the top-th largest of these 64
+ * bounds the top from below, and what is not below it has to be looked at. For almost
+ * all elements that is one comparison of the largest of 16. A step that has such elements
+ * reads them once more, out of the cache, so that the many others keep no registers for it. A
+ * full list is cut to its top, and so are at the end the four lists of a workgroup
+ * to one; a row that is split over workgroups leaves (m, s, t) and a
  * list of each, which a second launch joins in the same way.
+ *
+ * Bound by reading the logits, and of 16-bit ones by the vector instructions (8 an element and an
+ * exponential). 2047 rows of 151937 bf16 logits: 120 us without a top (5.2 TB/s, what a copy reaches), 159 us with the top 8;
+ * 1008 rows of 151936 fp32 logits with the top 8: 113 us (5.4 TB/s). 16 rows: 12 + 7 us, 1 row: 10 + 9 us, which is latency. A
+ * threshold of each wave by itself, its list's top-th, made the first 250 us: four times as many steps had something to look at.
  */
 #include "logprobs.h"
 #include "sera_dpp.h"
@@ -43,20 +53,30 @@ __device__ __forceinline__ float lp_least_value(lp_key k) {
     const uint32_t o = (uint32_t)(k >> 32);
     return o < 0x00800000u ? -INFINITY : lp_value(o);
 }
+/* A value that is less than all of this order and more (-0 is no less than 0); -inf below those of numbers. */
+__device__ __forceinline__ float lp_below(uint32_t o) {
+    return o < 0x00800001u ? -INFINITY : lp_value(o - (o == 0x80000000u ? 2 : 1));
+}
 
 /* Running sums of a lane. m is not -inf. */
 struct lp_sum {
     float m, s, t;
 };
 
-__device__ __forceinline__ void lp_join(lp_sum &a, const lp_sum &b) {
-    const float m = fmaxf(a.m, b.m);
-    /* differences beyond 200 have no weight left; held there, no product with 0 is undefined */
-    const float da = fmaxf(a.m - m, -200.0f), db = fmaxf(b.m - m, -200.0f);
-    const float fa = __builtin_amdgcn_exp2f(da * kLog2E), fb = __builtin_amdgcn_exp2f(db * kLog2E);
-    a.t = fa * (a.t + da * a.s) + fb * (b.t + db * b.s);
-    a.s = fa * a.s + fb * b.s;
+/* The sums around a maximum m that is as large or larger. */
+__device__ __forceinline__ void lp_raise(lp_sum &a, float m) {
+    const float d = fmaxf(a.m - m, -200.0f);      /* no weight is left beyond; held there, no product with 0 is undefined */
+    const float f = __builtin_amdgcn_exp2f(d * kLog2E);
+    a.t = f * fmaf(d, a.s, a.t);
+    a.s *= f;
     a.m = m;
+}
+__device__ __forceinline__ void lp_join(lp_sum &a, lp_sum b) {
+    const float m = fmaxf(a.m, b.m);
+    lp_raise(a, m);
+    lp_raise(b, m);
+    a.s += b.s;
+    a.t += b.t;
 }
 
 template <int OFF>
@@ -76,52 +96,74 @@ __device__ __forceinline__ void lp_join_wave(lp_sum &a) {
     lp_join_lane<32>(a);
 }
 
+/* The n-th largest of a wave's numbers, or one between it and the next smaller (so as many are as large); 0 if there are
+ * fewer than n above 0. Two bits at a time, as a bit's latency is a comparison, a count and a branch. *larger: how many are over it, if it
+ * is the number itself. */
+template <int N>
+__device__ __forceinline__ uint32_t lp_nth(const uint32_t (&k)[N], int n, bool *exact, int *larger) {
+    uint32_t at = 0;
+    *larger = 0;
+    for (int bit = 30; bit >= 0; bit -= 2) {
+        int count[3] = {0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < 3; j++)
+#pragma unroll
+            for (int i = 0; i < N; i++) count[j] += __popcll(__ballot(k[i] >= (at | (uint32_t)(j + 1) << bit)));
+        const int up = (count[0] >= n) + (count[1] >= n) + (count[2] >= n);
+        *larger = up == 0 ? count[0] : up == 1 ? count[1] : up == 2 ? count[2] : *larger;
+        at |= (uint32_t)up << bit;
+        if (count[0] == n || count[1] == n || count[2] == n) {
+            *exact = true;
+            return at;
+        }
+    }
+    *exact = false;
+    return at;
+}
+
+/* The same of 64-bit numbers. */
+template <int N>
+__device__ __forceinline__ lp_key lp_nth_key(const lp_key (&k)[N], int n) {
+    uint32_t part[N];
+    bool exact;
+    int larger;
+#pragma unroll
+    for (int i = 0; i < N; i++) part[i] = (uint32_t)(k[i] >> 32);
+    const uint32_t high = lp_nth(part, n, &exact, &larger);
+    if (exact || high == 0) return (lp_key)high << 32;
+#pragma unroll
+    for (int i = 0; i < N; i++) part[i] = (uint32_t)(k[i] >> 32) == high ? (uint32_t)k[i] : 0u;
+    return (lp_key)high << 32 | lp_nth(part, n - larger, &exact, &larger);
+}
+
 /* The candidates of a wave: n keys in LDS (wave-uniform), of which those below `least` need not be looked at. */
 struct lp_list {
     lp_key *keys;
     int n, top;
     lp_key least;
 
-    /* The `top` largest of the n keys to the front. */
-    __device__ __forceinline__ void cut(int lane) {
-        if (n <= top) return;
-        lp_key k[kRoom / 64];
+    /* The `top` largest of the n <= 64 N keys to the front. */
+    template <int N>
+    __device__ __forceinline__ void cut_of(int lane) {
+        lp_key k[N];
         asm volatile("" ::: "memory");          /* the wave's own LDS, which it accesses in order */
 #pragma unroll
-        for (int i = 0; i < kRoom / 64; i++) k[i] = 64 * i + lane < n ? keys[64 * i + lane] : 0;
-        /* the top-th largest, bit by bit; all bits of keys that are never alike: as soon as exactly `top` are as large,
-         * the rest of the bits do not matter */
-        lp_key least_of = 0;
-        for (int bit = 63; bit >= 0; bit--) {
-            const lp_key at = least_of | 1ull << bit;
-            int count = 0;
+        for (int i = 0; i < N; i++) k[i] = 64 * i + lane < n ? keys[64 * i + lane] : 0;
+        least = lp_nth_key(k, top);
+        n = 0;
 #pragma unroll
-            for (int i = 0; i < kRoom / 64; i++) count += __popcll(__ballot(k[i] >= at));
-            if (count >= top) least_of = at;
-            if (count == top) break;
-        }
-        int to = 0;
-#pragma unroll
-        for (int i = 0; i < kRoom / 64; i++) {
-            const bool stays = k[i] >= least_of && k[i] != 0;
-            const lp_key all = __ballot(stays);
-            if (stays) keys[to + __popcll(all & ((1ull << lane) - 1))] = k[i];
-            to += __popcll(all);
-        }
-        asm volatile("" ::: "memory");
-        n = to;
-        least = least_of;
+        for (int i = 0; i < N; i++) put(k[i], k[i] >= least && k[i] != 0, lane);
+    }
+    __device__ __forceinline__ void cut(int lane) {
+        if (n <= top) return;
+        if (n <= 128) cut_of<2>(lane);
+        else cut_of<kRoom / 64>(lane);
     }
 
-    /* Those of the lanes' keys that are not below the cut. 0: none. */
-    __device__ __forceinline__ void add(lp_key key, int lane) {
-        lp_key all = __ballot(key != 0 && key >= least);
-        if (!all) return;
-        if (n + __popcll(all) > kRoom) {
-            cut(lane);
-            all = __ballot(key != 0 && key >= least);
-        }
-        if (key != 0 && key >= least) keys[n + __popcll(all & ((1ull << lane) - 1))] = key;
+    /* The keys of some lanes behind the others; there is room. */
+    __device__ __forceinline__ void put(lp_key key, bool in, int lane) {
+        const lp_key all = __ballot(in);
+        if (in) keys[n + __popcll(all & ((1ull << lane) - 1))] = key;
         n += __popcll(all);
         asm volatile("" ::: "memory");
     }
@@ -129,6 +171,7 @@ struct lp_list {
     /* In falling order: the place of each (one a lane, n <= 64). */
     __device__ __forceinline__ int place(lp_key mine) const {
         int above = 0;
+#pragma unroll 8
         for (int i = 0; i < n; i++) above += keys[i] > mine;
         return above;
     }
@@ -136,6 +179,24 @@ struct lp_list {
 
 template <typename T>
 __device__ __forceinline__ float lp_f32(T x) { return (float)x; }
+
+/* 16 bytes of a row, kept as words so that nothing waits for them before their elements are wanted. */
+typedef uint32_t lp_words __attribute__((ext_vector_type(4)));
+typedef const lp_words __attribute__((address_space(1))) *lp_global;
+union lp_unit {
+    lp_words words;
+    uint32_t word[4];
+};
+template <typename T>
+__device__ __forceinline__ float lp_element(const lp_unit &u, int e) {
+    constexpr int PER = 4 / (int)sizeof(T), BITS = 8 * (int)sizeof(T);
+    const uint32_t bits = u.word[e / PER] >> BITS * (e % PER);
+    T x;
+    __builtin_memcpy(&x, &bits, sizeof(T));
+    return lp_f32(x);
+}
+/* What is read of a row that has no whole unit. */
+__device__ const lp_words lp_no_unit = {0u, 0u, 0u, 0u};
 
 }  // namespace
 
@@ -155,7 +216,7 @@ __device__ __forceinline__ void lp_join_group(lp_sum &a, lp_list &list, lp_key (
     for (int w = 1; w < kWaves; w++) {
         const lp_sum b = {sums[w][0], sums[w][1], sums[w][2]};
         lp_join(a, b);
-        list.add(lane < counts[w] ? keys[w][lane] : 0, lane);
+        list.put(keys[w][min(lane, max(counts[w] - 1, 0))], lane < counts[w], lane);
     }
     list.cut(lane);
 }
@@ -182,82 +243,113 @@ __device__ __forceinline__ void lp_finish(const logprobs_args &p, int64_t row, c
     }
 }
 
+/* 8 waves of a SIMD hold 2047 rows at once (159 us; with 7, 164); of fp32 logits the registers do not suffice, and memory is the
+ * bound. */
 template <typename T>
-__global__ __launch_bounds__(64 * kWaves) void sera_logprobs_kernel(logprobs_args p) {
-    constexpr int VEC = 16 / (int)sizeof(T), UNROLL = 4;
-    struct __attribute__((aligned(16))) vec { T v[VEC]; };
+__global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 7 : 8) void sera_logprobs_kernel(logprobs_args p) {
+    constexpr int VEC = 16 / (int)sizeof(T), UNROLL = 16 / VEC;
     __shared__ lp_key keys[kWaves][kRoom];
     __shared__ float sums[kWaves][3];
     __shared__ int counts[kWaves];
+    __shared__ uint32_t most[64], bound;            /* of the lanes' largest, and what follows from them */
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t row = blockIdx.x;
-    const int split = blockIdx.y;
+    const int split = blockIdx.y, piece = split * kWaves + wave, pieces = p.splits * kWaves;
     const T *x = (const T *)p.logits + row * p.stride;
-    /* 16-byte units of the row, from the one that holds its first element; the first and the last may be partly its */
-    const int skip = (int)((uintptr_t)x & 15u) / (int)sizeof(T);
-    const int units = (p.vocab + skip + VEC - 1) / VEC, pieces = p.splits * kWaves;
-    const int per = (units + pieces - 1) / pieces, u0 = (split * kWaves + wave) * per, u1 = min(u0 + per, units);
+    /* The row's whole 16-byte units, in equal shares; the elements in front of them are a step of the first wave, those
+     * behind them one of the last. */
+    const int front = min((int)(-(uintptr_t)x & 15u) / (int)sizeof(T), p.vocab);
+    const int units = (p.vocab - front) / VEC, back = p.vocab - front - units * VEC;
+    const int per = (units + pieces - 1) / pieces, u0 = min(piece * per, units), u1 = min(u0 + per, units);
+    const int steps = (u1 - u0 + 64 * UNROLL - 1) / (64 * UNROLL);
+    const int from = piece == 0 && front ? -1 : 0, to = steps + (piece == pieces - 1 && back);
 
     lp_list list;
     list.keys = keys[wave];
     list.n = 0;
     list.top = p.top;
     list.least = 0;
-    float least_value = -INFINITY;
     lp_sum a = {kLowest, 0.0f, 0.0f};
-    const auto load = [&](int u, vec *w) {
-        if (u * VEC >= skip && u + 64 * UNROLL <= u1 && (u + 64 * UNROLL) * VEC - skip <= p.vocab) {
-#pragma unroll
-            for (int i = 0; i < UNROLL; i++) w[i] = *(const vec *)(x + ((u + 64 * i + lane) * VEC - skip));
-        } else {
-#pragma unroll
-            for (int i = 0; i < UNROLL; i++)
-#pragma unroll
-                for (int e = 0; e < VEC; e++) {
-                    const int at = u + 64 * i + lane, id = at * VEC - skip + e;
-                    w[i].v[e] = at < u1 && id >= 0 && id < p.vocab ? x[id] : (T)-INFINITY;
-                }
+
+    /* Unit i of a step for a lane: the id of its first element, and how many of its elements there are. */
+    const auto unit = [&](int step, int i, int lane, int *id) {
+        if (step >= 0 && step < steps) {
+            const int at = u0 + 64 * (UNROLL * step + i) + lane;
+            *id = front + VEC * min(at, u1 - 1);
+            return at < u1 ? VEC : 0;
         }
+        const int n = step < 0 ? front : back;
+        *id = (step < 0 ? 0 : p.vocab - back) + min(lane, n - 1);
+        return i == 0 && lane < n ? 1 : 0;
     };
-    for (int u = u0; u < u1; u += 64 * UNROLL) {
-        vec in[UNROLL];
-        load(u, in);
-        float y[UNROLL][VEC], top = -INFINITY;
+    /* Always and in one way, so that nothing waits for a load before the next step; what a step has not got is taken out of it there. */
+    const lp_global first = (lp_global)(units ? (const lp_words *)(x + front) : &lp_no_unit);
+    const auto load = [&](int step, lp_unit *w) {
 #pragma unroll
         for (int i = 0; i < UNROLL; i++)
+            w[i].words = first[max(min(u0 + 64 * (UNROLL * step + i) + lane, u1 - 1), 0)];
+    };
+
+    /* What is not over `least` has no place in the top; but -inf has one until the list is as long. */
+    float least = p.top ? -INFINITY : INFINITY;
+    const auto look = [&](int step, float top) {
+        const uint32_t now = lp_order(top), had = atomicMax(&most[lane], now), mine[1] = {had > now ? had : now};
+        bool exact;
+        int larger;
+        const uint32_t nth = lp_nth(mine, p.top, &exact, &larger);
+        if (lane == 0) atomicMax(&bound, nth);
+        least = fmaxf(least, lp_below(nth));
+        const bool all = least == -INFINITY && list.n < p.top;
+        uint64_t lanes = __ballot(top > least || all);
+        while (lanes) {                             /* 4 lanes' elements at a time */
+            int of = 64;
 #pragma unroll
-            for (int e = 0; e < VEC; e++) y[i][e] = lp_f32(in[i].v[e]);
-#pragma unroll
-        for (int i = 0; i < UNROLL; i++)
-#pragma unroll
-            for (int e = 0; e < VEC; e++) top = fmaxf(top, y[i][e]);
-        if (__ballot(top > a.m)) {
-            const float m = fmaxf(a.m, top), d = fmaxf(a.m - m, -200.0f), f = __builtin_amdgcn_exp2f(d * kLog2E);
-            a.t = f * (a.t + d * a.s);
-            a.s *= f;
-            a.m = m;
-        }
-#pragma unroll
-        for (int i = 0; i < UNROLL; i++)
-#pragma unroll
-            for (int e = 0; e < VEC; e++) {
-                const float d = y[i][e] - a.m, w = __builtin_amdgcn_exp2f(d * kLog2E);
-                a.s += w;
-                a.t = fmaf(w, fmaxf(d, -200.0f), a.t);
+            for (int j = 0; j < 4; j++) {
+                if (lane >> 4 == j && lanes) of = __builtin_ctzll(lanes);
+                lanes &= lanes - 1;
             }
-        if (p.top && __ballot(top >= least_value)) {
-#pragma unroll
-            for (int i = 0; i < UNROLL; i++)
-#pragma unroll
-                for (int e = 0; e < VEC; e++) {
-                    const int at = u + 64 * i + lane, id = at * VEC - skip + e;
-                    const bool in = at < u1 && id >= 0 && id < p.vocab;
-                    if (__ballot(in && y[i][e] >= least_value)) {
-                        list.add(in ? (lp_key)lp_order(y[i][e]) << 32 | (uint32_t)~id : 0, lane);
-                        least_value = lp_least_value(list.least);
-                    }
-                }
+            int id;
+            const int n = unit(step, (lane & 15) / VEC, of, &id), e = (lane & 15) % VEC;
+            float y = -INFINITY;
+            if (of < 64 && e < n) y = lp_f32(x[id += e]);
+            const bool is = of < 64 && e < n && (y > least || all);
+            if (list.n > kRoom - 64) list.cut(lane);
+            list.put((lp_key)lp_order(y) << 32 | (uint32_t)~id, is && y == y, lane);
         }
+        /* The ids that follow are higher: equal logits come behind the list's. */
+        least = fmaxf(least, lp_least_value(list.least));
+    };
+
+    if (threadIdx.x < 64) most[lane] = 0;
+    if (threadIdx.x == 0) bound = 0;
+    lp_unit in[UNROLL];
+    load(from, in);
+    __syncthreads();
+    for (int step = from; step < to; step++) {
+        float y[16], top = -INFINITY;
+        least = fmaxf(least, lp_below(__hip_atomic_load(&bound, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP)));
+#pragma unroll
+        for (int k = 0; k < 16; k++) y[k] = lp_element<T>(in[k / VEC], k % VEC);
+        load(step + 1, in);
+        if (step < 0 || u0 + 64 * UNROLL * (step + 1) > u1) {
+#pragma unroll
+            for (int k = 0; k < 16; k++) {
+                int id;
+                const int n = unit(step, k / VEC, lane, &id);
+                if (k % VEC >= n) y[k] = -INFINITY;
+                else if (n < VEC) y[k] = lp_f32(x[id]);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 16; k++) top = fmaxf(top, y[k]);
+        if (__ballot(top > a.m)) lp_raise(a, fmaxf(a.m, top));
+#pragma unroll
+        for (int k = 0; k < 16; k++) {
+            const float d = y[k] - a.m, w = __builtin_amdgcn_exp2f(d * kLog2E);
+            a.s += w;
+            a.t = fmaf(w, fmaxf(d, -200.0f), a.t);
+        }
+        if (__ballot(top > least) || (least == -INFINITY && list.n < p.top)) look(step, top);
     }
     lp_join_group(a, list, keys, sums, counts, lane, wave);
     if (wave) return;
@@ -292,8 +384,19 @@ __global__ __launch_bounds__(64 * kWaves) void sera_logprobs_join_kernel(logprob
         const lp_sum b = {ws[3 * i], ws[3 * i + 1], ws[3 * i + 2]};
         lp_join(a, b);
     }
-    for (int i = 64 * wave; i < p.splits * p.top; i += 64 * kWaves)
-        list.add(i + lane < p.splits * p.top ? parts[i + lane] : 0, lane);
+    if (p.top) {
+        const int n = p.splits * p.top;
+        lp_key most = 0;
+#pragma unroll 4
+        for (int i = 64 * wave + lane; i < n; i += 64 * kWaves) most = parts[i] > most ? parts[i] : most;
+        const lp_key mine[1] = {most};
+        list.least = lp_nth_key(mine, p.top);
+        for (int i = 64 * wave; i < n; i += 64 * kWaves) {
+            if (list.n + 64 > kRoom) list.cut(lane);
+            const lp_key key = i + lane < n ? parts[i + lane] : 0;
+            list.put(key, key != 0 && key >= list.least, lane);
+        }
+    }
     lp_join_group(a, list, keys, sums, counts, lane, wave);
     if (wave == 0) lp_finish<T>(p, row, a, list, lane);
 }
@@ -317,10 +420,10 @@ hipError_t lp_go(const logprobs_args &p, hipStream_t s) {
 int sera_logprobs_splits(int rows, int vocab, int cus) {
     const int64_t most = vocab / 4 / kLeastUnits, want = 2ll * cus / rows;
     const int64_t n = most < want ? most : want;
-    return n < 1 ? 1 : n > 128 ? 128 : (int)n;
+    return n < 1 ? 1 : n > 64 ? 64 : (int)n;
 }
 
-/* Floats of the partial sums (even, the lists lie behind them), and bytes of all. */
+/* Floats of the partial sums (the lists lie behind them, 16-byte aligned). */
 size_t sera_logprobs_sums(int rows, int splits) { return ((size_t)rows * splits * 3 + 3) & ~(size_t)3; }
 
 hipError_t sera_launch_logprobs(uint32_t type, const logprobs_args &p, hipStream_t s) {
