@@ -5,7 +5,7 @@
  * Choice: a workgroup for each sequence and kv head. Weights become whole numbers
  * of the same order; the smallest one that stays is built bit by bit, each bit by
  * counting how many are as large. Then each wave walks a run of positions of its own, held in
- * registers up to 32768 positions, and writes what stays behind what the
+ * registers up to 16384 positions, and writes what stays behind what the
  * runs before it keep, which a count of each run says.
  *
  * Move: a wave for K or V of 16 new places of a head. A K row is a run of
@@ -288,7 +288,7 @@ hipError_t sera_launch_kv_evict(uint32_t cache_type, int dim, const kv_args &a, 
     const dim3 heads((unsigned)a.kv_heads, (unsigned)y, z), threads(64 * kKeepWaves);
     if (a.max_kv <= 16 * 64 * kKeepWaves) hipLaunchKernelGGL(sera_kv_keep_kernel<16>, heads, threads, 0, s, a, t);
     else if (a.max_kv <= 32 * 64 * kKeepWaves) hipLaunchKernelGGL(sera_kv_keep_kernel<32>, heads, threads, 0, s, a, t);
-    else if (a.max_kv <= 128 * 64 * kKeepWaves) hipLaunchKernelGGL(sera_kv_keep_kernel<128>, heads, threads, 0, s, a, t);
+    else if (a.max_kv <= 64 * 64 * kKeepWaves) hipLaunchKernelGGL(sera_kv_keep_kernel<64>, heads, threads, 0, s, a, t);
     else hipLaunchKernelGGL(sera_kv_keep_kernel<0>, heads, threads, 0, s, a, t);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
