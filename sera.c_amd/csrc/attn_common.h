@@ -46,6 +46,7 @@ struct rope_args {
     int half;                       /* pairs of channels that turn */
     bool neighbours;
     int heads;                      /* q's */
+    int cus;                        /* compute units of the device */
 };
 
 /* What shortening a cache takes beside it and the batch. */

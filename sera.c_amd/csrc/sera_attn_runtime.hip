@@ -293,6 +293,7 @@ int sera_kv_write_rope(const sera_kv_cache *cache, const sera_kv_batch *batch, c
     r.half = rope->rotated / 2;
     r.neighbours = rope->pairing == SERA_ROPE_NEIGHBOURS;
     r.heads = heads;
+    r.cus = device_cus();
     return sera_launch_kv_rope(cache->type, type, dim, args_of(cache, batch), r, q, q_stride, q_out, q_out_stride, k,
                                k_stride, v, v_stride, (hipStream_t)stream) == hipSuccess
                ? 0 : fail(-3, "%s: launch failed", tag);
