@@ -21,11 +21,12 @@
  * list of each, which a second launch joins in the same way.
  *
  * Bound by reading the logits, and of 16-bit ones by the vector instructions (8 an element and an
- * exponential). 2047 rows of 151937 bf16 logits: 120 us without a top (5.2 TB/s, what a copy reaches), 159 us with the top 8;
- * 1008 rows of 151936 fp32 logits with the top 8: 113 us (5.4 TB/s). 16 rows: 12 + 7 us, 1 row: 10 + 9 us, which is latency. A
+ * exponential). 2047 rows of 151937 bf16 logits: 119 us without a top (5.2 TB/s, what a copy reaches), 157 us with the top 8;
+ * 1008 rows of 151936 fp32 logits with the top 8: 112 us (5.5 TB/s). 16 rows: 11 + 4 us, 1 row: 8.5 + 6.5 us, which is latency. A
  * threshold of each wave by itself, its list's top-th, made the first 250 us: four times as many steps had something to look at.
  */
 #include "logprobs.h"
+#include "../../include/sera_logprobs.h"
 #include "sera_dpp.h"
 #include "sera_launch.h"
 
@@ -35,6 +36,7 @@
 namespace {
 
 constexpr int kWaves = 4, kRoom = 256;             /* candidates of a wave */
+constexpr int kMostSplits = 64;                    /* of a row */
 constexpr float kLowest = -3.402823466e38f, kLog2E = 1.4426950408889634f;
 
 typedef unsigned long long lp_key;
@@ -200,11 +202,10 @@ __device__ const lp_words lp_no_unit = {0u, 0u, 0u, 0u};
 
 }  // namespace
 
-/* Joins the waves of a workgroup, and its lists into that of wave 0. */
+/* Joins the waves of a workgroup: the sums for all of them, the lists into that of wave 0. */
 __device__ __forceinline__ void lp_join_group(lp_sum &a, lp_list &list, lp_key (*keys)[kRoom], float (*sums)[3],
                                               int *counts, int lane, int wave) {
     lp_join_wave(a);
-    list.cut(lane);
     if (lane == 0) {
         sums[wave][0] = a.m;
         sums[wave][1] = a.s;
@@ -212,30 +213,38 @@ __device__ __forceinline__ void lp_join_group(lp_sum &a, lp_list &list, lp_key (
         counts[wave] = list.n;
     }
     __syncthreads();
-    if (wave) return;
-    for (int w = 1; w < kWaves; w++) {
-        const lp_sum b = {sums[w][0], sums[w][1], sums[w][2]};
-        lp_join(a, b);
-        list.put(keys[w][min(lane, max(counts[w] - 1, 0))], lane < counts[w], lane);
+    int all = 0;
+    for (int w = 0; w < kWaves; w++) all += counts[w];
+    if (all > kRoom) {                  /* else one cut of them together does */
+        list.cut(lane);
+        __syncthreads();
+        if (lane == 0) counts[wave] = list.n;
+        __syncthreads();
     }
+    a = {sums[0][0], sums[0][1], sums[0][2]};
+    for (int w = 1; w < kWaves; w++) lp_join(a, {sums[w][0], sums[w][1], sums[w][2]});
+    if (wave) return;
+    for (int w = 1; w < kWaves; w++)
+        for (int i = lane, n = counts[w]; i - lane < n; i += 64) list.put(keys[w][min(i, n - 1)], i < n, lane);
     list.cut(lane);
 }
 
-/* What is asked of a row, from its sums and its list, by wave 0. */
+/* What is asked of a row, from its sums and its list: the top by wave 0, tokens and entropy by the others. */
 template <typename T>
 __device__ __forceinline__ void lp_finish(const logprobs_args &p, int64_t row, const lp_sum &a, const lp_list &list,
-                                          int lane) {
+                                          int lane, int wave) {
     const T *x = (const T *)p.logits + row * p.stride;
     const bool fine = a.s > 0.0f && a.s < INFINITY;
     const float nan = __builtin_nanf(""), log_s = logf(a.s);
-    for (int i = lane; i < p.per_row; i += 64) {
-        const int token = p.tokens[row * p.per_row + i];
-        float y = nan;
-        if (fine && token >= 0 && token < p.vocab) y = (lp_f32(x[token]) - a.m) - log_s;
-        p.token_logprobs[row * p.per_row + i] = y;
-    }
-    if (p.entropy && lane == 0) p.entropy[row] = fine ? log_s - a.t / a.s : nan;
-    if (lane < p.top) {
+    if (wave) {
+        for (int i = 64 * (wave - 1) + lane; i < p.per_row; i += 64 * (kWaves - 1)) {
+            const int token = p.tokens[row * p.per_row + i];
+            float y = nan;
+            if (fine && token >= 0 && token < p.vocab) y = (lp_f32(x[token]) - a.m) - log_s;
+            p.token_logprobs[row * p.per_row + i] = y;
+        }
+        if (p.entropy && threadIdx.x == 64) p.entropy[row] = fine ? log_s - a.t / a.s : nan;
+    } else if (lane < p.top) {
         const lp_key mine = lane < list.n ? list.keys[lane] : 0;
         const int at = fine && lane < list.n ? list.place(mine) : lane;
         p.top_ids[row * p.top + at] = fine ? (int)~(uint32_t)mine : -1;
@@ -243,7 +252,7 @@ __device__ __forceinline__ void lp_finish(const logprobs_args &p, int64_t row, c
     }
 }
 
-/* 8 waves of a SIMD hold 2047 rows at once (159 us; with 7, 164); of fp32 logits the registers do not suffice, and memory is the
+/* 8 waves of a SIMD hold 2047 rows at once (157 us; with 7, 164); of fp32 logits the registers do not suffice, and memory is the
  * bound. */
 template <typename T>
 __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 7 : 8) void sera_logprobs_kernel(logprobs_args p) {
@@ -352,8 +361,8 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 7 : 8) void sera_logp
         if (__ballot(top > least) || (least == -INFINITY && list.n < p.top)) look(step, top);
     }
     lp_join_group(a, list, keys, sums, counts, lane, wave);
+    if (p.splits == 1) return lp_finish<T>(p, row, a, list, lane, wave);
     if (wave) return;
-    if (p.splits == 1) return lp_finish<T>(p, row, a, list, lane);
     const size_t part = (size_t)row * p.splits + split;
     float *const ws = p.workspace;
     if (lane == 0) {
@@ -370,6 +379,7 @@ __global__ __launch_bounds__(64 * kWaves) void sera_logprobs_join_kernel(logprob
     __shared__ lp_key keys[kWaves][kRoom];
     __shared__ float sums[kWaves][3];
     __shared__ int counts[kWaves];
+    __shared__ uint32_t most[64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t row = blockIdx.x;
     const float *const ws = p.workspace + 3 * (size_t)row * p.splits;
@@ -380,25 +390,39 @@ __global__ __launch_bounds__(64 * kWaves) void sera_logprobs_join_kernel(logprob
     list.top = p.top;
     list.least = 0;
     lp_sum a = {kLowest, 0.0f, 0.0f};
-    for (int i = 64 * wave + lane; i < p.splits; i += 64 * kWaves) {
-        const lp_sum b = {ws[3 * i], ws[3 * i + 1], ws[3 * i + 2]};
-        lp_join(a, b);
+    lp_key key[kMostSplits * SERA_LOGPROBS_MAX_TOP / (64 * kWaves)];
+    const int n = p.splits * p.top;
+    uint32_t largest = 0;
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(key) / sizeof(key[0])); i++) {
+        const int at = 64 * kWaves * i + (int)threadIdx.x;
+        key[i] = at < n ? parts[at] : 0;
     }
+    if ((int)threadIdx.x < p.splits) a = {ws[3 * threadIdx.x], ws[3 * threadIdx.x + 1], ws[3 * threadIdx.x + 2]};
+    if (threadIdx.x < 64) most[lane] = 0;
+    __syncthreads();
     if (p.top) {
-        const int n = p.splits * p.top;
-        lp_key most = 0;
-#pragma unroll 4
-        for (int i = 64 * wave + lane; i < n; i += 64 * kWaves) most = parts[i] > most ? parts[i] : most;
-        const lp_key mine[1] = {most};
-        list.least = lp_nth_key(mine, p.top);
-        for (int i = 64 * wave; i < n; i += 64 * kWaves) {
-            if (list.n + 64 > kRoom) list.cut(lane);
-            const lp_key key = i + lane < n ? parts[i + lane] : 0;
-            list.put(key, key != 0 && key >= list.least, lane);
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(key) / sizeof(key[0])); i++) {
+            const uint32_t high = (uint32_t)(key[i] >> 32);
+            largest = high > largest ? high : largest;
+        }
+        atomicMax(&most[lane], largest);
+        __syncthreads();
+        const uint32_t mine[1] = {most[lane]};
+        bool exact;
+        int larger;
+        const lp_key least = (lp_key)lp_nth(mine, p.top, &exact, &larger) << 32;
+#pragma unroll 1
+        for (int i = 0; i < n; i += 64 * kWaves) {
+            if (list.n > kRoom - 64) list.cut(lane);
+            list.put(key[0], key[0] != 0 && key[0] >= least, lane);
+#pragma unroll
+            for (int j = 1; j < (int)(sizeof(key) / sizeof(key[0])); j++) key[j - 1] = key[j];
         }
     }
     lp_join_group(a, list, keys, sums, counts, lane, wave);
-    if (wave == 0) lp_finish<T>(p, row, a, list, lane);
+    lp_finish<T>(p, row, a, list, lane, wave);
 }
 
 namespace {
@@ -420,7 +444,7 @@ hipError_t lp_go(const logprobs_args &p, hipStream_t s) {
 int sera_logprobs_splits(int rows, int vocab, int cus) {
     const int64_t most = vocab / 4 / kLeastUnits, want = 2ll * cus / rows;
     const int64_t n = most < want ? most : want;
-    return n < 1 ? 1 : n > 64 ? 64 : (int)n;
+    return n < 1 ? 1 : n > kMostSplits ? kMostSplits : (int)n;
 }
 
 /* Floats of the partial sums (the lists lie behind them, 16-byte aligned). */
