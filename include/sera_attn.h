@@ -170,7 +170,8 @@ typedef struct {
  * for its place in the sequence. They differ where a cache was thinned
  * (sera_kv_evict) and its tokens have other places than they had in the text.
  * Rows of a sequence outside the bounds come out of q as NaN, those in front of
- * a sequence's start as zeros; rows of no sequence are left as they are. One launch. */
+ * a sequence's start as zeros; rows of no sequence are left as they are. One
+ * launch. */
 int sera_kv_write_rope(const sera_kv_cache *cache, const sera_kv_batch *batch, const sera_qk_rope *rope, uint32_t type,
                        const void *q, int64_t q_stride, void *q_out, int64_t q_out_stride, int heads, const void *k,
                        int64_t k_stride, const void *v, int64_t v_stride, const int32_t *positions, void *stream);
@@ -183,14 +184,15 @@ int sera_kv_write_rope(const sera_kv_cache *cache, const sera_kv_batch *batch, c
  *                      the sequence's new rows and h's query heads,
  * where `before` counts for positions in front of the new rows only: the new
  * ones start at zero, whatever their places held. Both are device float arrays
- * [sequences][kv_heads][weights_stride] (weights_stride >= max_kv); `before` may be `weights`
- * (the sums go on in place) or NULL (they start with this call), and must not
- * overlap it otherwise. Places from kv_len on are left as they are, and so is all of a
- * sequence outside the bounds. Rows that come out as NaN (a lost page, keys that are
- * not finite) give NaN to the positions that they see. A batch without rows does nothing.
- * Results repeat bit for bit. The workspace is its own size, which grows with
- * rows * heads * max_kv where few rows go to long contexts
- * (their scores are kept for the sums, 4 bytes each). */
+ * [sequences][kv_heads][weights_stride] (weights_stride >= max_kv); `before`
+ * may be `weights` (the sums go on in place) or NULL (they start with this
+ * call), and must not overlap it otherwise. Places from kv_len on are left as
+ * they are, and so is all of a sequence outside the bounds. Rows that come out
+ * as NaN (a lost page, keys that are not finite) give NaN to the positions that
+ * they see. A batch without rows does nothing. Results repeat bit for bit. The
+ * workspace is its own size, which grows with rows * heads * max_kv where few
+ * rows go to long contexts (their scores are kept for the sums, 4 bytes each).
+ */
 size_t sera_attention_weights_workspace_bytes(const sera_kv_cache *cache, const sera_kv_batch *batch, int heads);
 int sera_attention_weights(const sera_kv_cache *cache, const sera_kv_batch *batch, uint32_t type, const void *q,
                            int64_t q_stride, void *out, int64_t out_stride, int heads, float scale, int window,
@@ -199,22 +201,24 @@ int sera_attention_weights(const sera_kv_cache *cache, const sera_kv_batch *batc
 
 /* Shortens every sequence of more than `keep` positions to `keep`: of each kv
  * head the first `sinks` positions stay, the last `recent` ones, and of those
- * between the ones with the largest weights (of equal ones the first; NaN counts as less
- * than anything), keep - sinks - recent of them. What stays keeps its order and moves,
- * with its bytes, to the places 0, 1, .. of the pages in new_table
- * [sequences][new_stride] (new_stride * page_tokens >= min(keep, max_kv)); its weights move to the
- * same places of new_weights (both [sequences][kv_heads][weights_stride], not
- * overlapping; places behind are left as they are). A sequence of up to `keep` positions moves as it is. new_len[b] is
- * the new length, kept [sequences][kv_heads][keep] the old positions in order,
- * -1 behind the last. Of the batch only sequences, max_kv, table_stride, kv_len
- * and page_table are used.
+ * between the ones with the largest weights (of equal ones the first; NaN
+ * counts as less than anything), keep - sinks - recent of them. What stays
+ * keeps its order and moves, with its bytes, to the places 0, 1, .. of the
+ * pages in new_table [sequences][new_stride] (new_stride * page_tokens >=
+ * min(keep, max_kv)); its weights move to the same places of new_weights (both
+ * [sequences][kv_heads][weights_stride], not overlapping; places behind are
+ * left as they are). A sequence of up to `keep` positions moves as it is.
+ * new_len[b] is the new length, kept [sequences][kv_heads][keep] the old
+ * positions in order, -1 behind the last. Of the batch only sequences, max_kv,
+ * table_stride, kv_len and page_table are used.
  *
- * The new pages belong to one sequence each and are not among the old ones of any
- * (they take the bytes while others still read theirs), so old pages may go on
- * being shared; but a sequence of up to `keep` positions may name its
- * own old pages again, in the same order. new_len must not be kv_len. A sequence whose length is outside 0..max_kv
- * moves nothing, has new_len -1 and only -1 in kept; tokens of a page that is
- * not in the pool arrive as NaN, and to a new page that is not none are written. Two launches. */
+ * The new pages belong to one sequence each and are not among the old ones of
+ * any (they take the bytes while others still read theirs), so old pages may go
+ * on being shared; but a sequence of up to `keep` positions may name its own
+ * old pages again, in the same order. new_len must not overlap kv_len. A
+ * sequence whose length is outside 0..max_kv moves nothing, has new_len -1 and
+ * only -1 in kept; tokens of a page that is not in the pool arrive as NaN, and
+ * to a new page that is not none are written. Two launches. */
 int sera_kv_evict(const sera_kv_cache *cache, const sera_kv_batch *batch, int keep, int recent, int sinks,
                   const float *weights, float *new_weights, int64_t weights_stride, const int32_t *new_table,
                   int64_t new_stride, int32_t *new_len, int32_t *kept, void *stream);

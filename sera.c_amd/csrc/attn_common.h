@@ -19,7 +19,7 @@ struct attn_args {
     int few_rows;                   /* rows of one of its partial results */
     float *workspace;
     int cus;                        /* compute units of the device */
-    float *lse;                     /* log2 of each row's sum of 2^s', [rows][heads], for the weights; NULL: not wanted */
+    float *lse;                     /* log2 of each row's sum of 2^s', [rows][heads], for the weights, or NULL */
     float *scores;                  /* s' of the few-row kernel, [sequences][kv_heads][few_rows][pitch], or NULL */
     size_t pitch;
     const float *before;            /* sums so far, or NULL */
@@ -31,9 +31,9 @@ struct attn_args {
 struct attn_sums {
     int few_rows;                   /* columns of a sequence in the few-row kernel, at most; 0: it has no part */
     size_t pitch;                   /* floats from one row of scores (or sums) to the next */
-    int groups, share;              /* of all other sequences: workgroups of a sequence and head at most, units (blocks of 32
-                                     * columns over 256 positions) of one */
-    size_t slots;                   /* places of 256 sums for a sequence and head */
+    int groups, share;              /* of all other sequences: workgroups of a sequence and head at most, units
+                                     * (blocks of 32 columns over 512 positions) of one */
+    size_t slots;                   /* places of 512 sums for a sequence and head */
     size_t scores_bytes;            /* of the workspace; the ranges' sums lie behind */
     float *scores, *partial;
 };

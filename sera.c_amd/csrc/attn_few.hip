@@ -156,7 +156,9 @@ __global__ __launch_bounds__(64 * NW, OCC) void sera_attn_few_kernel(kv_args a, 
     /* Tokens of this lane: A row `col` of operand u is token QT * (col / 4) + 4 u + col % 4; its scores are
      * the tokens QT * quarter + 4 u + i. V pieces are those same tokens of one channel. */
     const int k_token = QT * (col >> 2) + (col & 3), v_token = QT * quarter;
-    float *keep[CT];        /* rows of scores, as q's: columns past the last have its q and write its scores once more */
+    /* Rows of scores, as q's: columns past the last have its q and write its scores once more, so that every lane stores
+     * and no wait for a load becomes one for a store as well (64 sequences of 8192 positions: 461 us instead of 471). */
+    float *keep[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ct++)
         keep[ct] = KEEP ? t.scores + ((size_t)(b * a.kv_heads + head) * t.few_rows +
@@ -270,7 +272,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void sera_attn_few_kernel(kv_args a, 
                             x[4 * u + i] = attn_sees(t, pos[ct], j0 + 4 * u + i) ? x[4 * u + i] : -INFINITY;
                 if (KEEP) {
                     float *to = keep[ct] + j0;
-    #pragma unroll
+#pragma unroll
                     for (int u = 0; u < NS; u++)
                         *(attn_f4 *)(to + 4 * u) = attn_f4{x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]};
                 }

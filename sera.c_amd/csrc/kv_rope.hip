@@ -1,19 +1,18 @@
 /*
- * kv_rope.hip - rows into the paged cache with q's and k's heads normed and
- * rotated on the way.
+ * kv_rope.hip - rows into the paged cache with q's and k's heads normed and rotated on the way.
  *
  *   x' = (x * (1 / sqrt(mean(x^2) + eps))) * gamma          over a head's channels
  *   (a, b) -> (a cos t - b sin t, a sin t + b cos t)        t = position * inv_freq[i]
  *
- * A workgroup has a 16-token block of a sequence and some of its heads. The
- * block's sines and cosines are made once, in LDS, for all of them: position *
- * inv_freq / 2 pi in 64 bits, less the whole turns, then fp32. A head's channels lie in the
- * 16-byte accesses of one row's lanes, so the mean and the partner of a
- * channel come from other lanes of the row. q goes back to rows, k and v to the cache as
- * kv_write puts them there. The workgroups of a block lie beside each other, as its rows do in memory.
+ * A workgroup has a 16-token block of a sequence and some of its heads. The block's sines and cosines are made once,
+ * in LDS, for all of them: position * inv_freq / 2 pi in 64 bits, less the whole turns, then fp32. A head's channels
+ * lie in the 16-byte accesses of one row's lanes, so the mean and the partner of a channel come from other lanes of
+ * the row. q goes back to rows, k and v to the cache as kv_write puts them there. The workgroups of a block lie
+ * beside each other, as its rows do in memory.
  *
- * Bound by memory: each row is read and written once. A prompt of 2048 fp32 rows (64 heads of q, 8 of k and v, 128 channels,
- * fp16 cache): 39 us for 160 MB, 4.1 TB/s of the 5.2 that a copy reaches. 16 single tokens: 6.4 us, which is latency.
+ * Bound by memory: each row is read and written once. A prompt of 2048 fp32 rows (64 heads of q, 8 of k and v, 128
+ * channels, fp16 cache): 39 us for 160 MB, 4.1 TB/s of the 5.2 that a copy reaches. 16 single tokens: 6.4 us, which
+ * is latency.
  */
 #include "attn_common.h"
 #include "kv_device.h"
@@ -106,8 +105,8 @@ struct kv_same {
 
 }  // namespace
 
-/* Item i of a block: q's head i, or behind those of a kv head the halves of its K and of its V. A workgroup has
- * `per` of them. */
+/* Item i of a block: q's head i, or behind those of a kv head the halves of its K and of its V. A workgroup has `per`
+ * of them. */
 template <int TYPE, typename T, int D>
 __global__ __launch_bounds__(256) void sera_kv_rope_kernel(kv_args a, rope_args r, const T *q, int64_t q_stride,
                                                            T *q_out, int64_t q_out_stride, const T *__restrict__ k,
@@ -223,9 +222,10 @@ namespace {
 template <int TYPE, typename T, int D>
 void rope_go(const kv_args &a, const rope_args &r, const void *q, int64_t qs, void *q_out, int64_t qos, const void *k,
              int64_t ks, const void *v, int64_t vs, hipStream_t s) {
-    /* Items of a workgroup: one for each wave, and more of them only where that leaves 4 workgroups for every compute unit,
-     * as each makes its block's angles and finds its sequence anew. A prompt of 2048 rows of 64 heads (fp32): 4 items 45 us, 16 39 us;
-     * 9 chunks of 701 rows of 20 heads of 64 (bf16): 4 items 12.9 us, 12 9.5 us; single tokens of 16: 4 items 6.4 us, 8 7.6 us. */
+    /* Items of a workgroup: one for each wave, and more of them only where that leaves 4 workgroups for every compute
+     * unit, as each makes its block's angles and finds its sequence anew. A prompt of 2048 rows of 64 heads (fp32): 4
+     * items 45 us, 16 39 us; 9 chunks of up to 701 rows of 20 heads of 64 (bf16): 4 items 12.9 us, 12 9.5 us; single
+     * tokens of 16: 4 items 6.4 us, 8 7.6 us. */
     const int64_t slots = kv_slots(a.rows, a.sequences, kBlock, 2), blocks = slots < a.rows ? slots : a.rows;
     const int64_t items = r.heads + 4 * a.kv_heads, want = 4 * ((blocks * items + 16 * r.cus - 1) / (16 * r.cus));
     const int per = (int)(want < items ? want : items);

@@ -1,6 +1,5 @@
 /*
- * logprobs.h - what the kernels of sera_logprobs take, and their launcher
- * (internal).
+ * logprobs.h - what the kernels of sera_logprobs take, and their launcher (internal).
  */
 #ifndef LOGPROBS_H
 #define LOGPROBS_H

@@ -1,29 +1,27 @@
 /*
- * logprobs.hip - log probabilities, entropy and the most likely tokens of
- * rows of logits, in one pass over them.
+ * logprobs.hip - log probabilities, entropy and the most likely tokens of rows of logits, in one pass over them.
  *
  * With m the running maximum, s = sum e^(x - m) and t = sum e^(x - m) (x - m):
  *
  *   log p(x) = (x - m) - log s       H = log s - t / s
  *
- * (x log2(e) - m log2(e) in one instruction instead of a difference and a product would leave an
- * error of m's size: exponents of 2^20 and more come out wrong.)
+ * (x log2(e) - m log2(e) in one instruction instead of a difference and a product would leave an error of m's size:
+ * exponents of 2^20 and more come out wrong.)
  *
- * A wave takes a piece of a row, 16 elements of a lane at a time. The top: a
- * wave holds candidates in LDS as 64-bit keys, the logit as a whole number of the same order
- * above the inverted id, so no two are alike and equal logits are in the order of
- * their ids. The workgroup keeps the maximum of each lane number over its waves: the top-th largest of these 64
- * bounds the top from below, and what is not below it has to be looked at. For almost
- * all elements that is one comparison of the largest of 16. A step that has such elements
- * reads them once more, out of the cache, so that the many others keep no registers for it. A
- * full list is cut to its top, and so are at the end the four lists of a workgroup
- * to one; a row that is split over workgroups leaves (m, s, t) and a
- * list of each, which a second launch joins in the same way.
+ * A wave takes a piece of a row, 16 elements of a lane at a time. The top: a wave holds candidates in LDS as 64-bit
+ * keys, the logit as a whole number of the same order above the inverted id, so no two are alike and equal logits are
+ * in the order of their ids. The workgroup keeps the maximum of each lane number over its waves: the top-th largest
+ * of these 64 bounds the top from below, and what is not below it has to be looked at. For almost all elements that
+ * is one comparison of the largest of 16. A step that has such elements reads them once more, out of the cache, so
+ * that the many others keep no registers for it. A full list is cut to its top, and so are at the end the four lists
+ * of a workgroup to one; a row that is split over workgroups leaves (m, s, t) and a list of each, which a second
+ * launch joins in the same way.
  *
- * Bound by reading the logits, and of 16-bit ones by the vector instructions (8 an element and an
- * exponential). 2047 rows of 151937 bf16 logits: 119 us without a top (5.2 TB/s, what a copy reaches), 157 us with the top 8;
- * 1008 rows of 151936 fp32 logits with the top 8: 112 us (5.5 TB/s). 16 rows: 11 + 4 us, 1 row: 8.5 + 6.5 us, which is latency. A
- * threshold of each wave by itself, its list's top-th, made the first 250 us: four times as many steps had something to look at.
+ * Bound by reading the logits, and of 16-bit ones by the vector instructions (8 an element and an exponential). 2047
+ * rows of 151937 bf16 logits: 119 us without a top (5.2 TB/s, what a copy reaches), 157 us with the top 8; 1008 rows
+ * of 151936 fp32 logits with the top 8: 112 us (5.5 TB/s). 16 rows: 11 + 4 us, 1 row: 8.5 + 6.5 us, which is latency.
+ * A threshold of each wave by itself, its list's top-th, made the first 250 us: four times as many steps had
+ * something to look at.
  */
 #include "logprobs.h"
 #include "../../include/sera_logprobs.h"
@@ -67,7 +65,7 @@ struct lp_sum {
 
 /* The sums around a maximum m that is as large or larger. */
 __device__ __forceinline__ void lp_raise(lp_sum &a, float m) {
-    const float d = fmaxf(a.m - m, -200.0f);      /* no weight is left beyond; held there, no product with 0 is undefined */
+    const float d = fmaxf(a.m - m, -200.0f);  /* beyond, no weight is left; held, no product with 0 is undefined */
     const float f = __builtin_amdgcn_exp2f(d * kLog2E);
     a.t = f * fmaf(d, a.s, a.t);
     a.s *= f;
@@ -98,9 +96,9 @@ __device__ __forceinline__ void lp_join_wave(lp_sum &a) {
     lp_join_lane<32>(a);
 }
 
-/* The n-th largest of a wave's numbers, or one between it and the next smaller (so as many are as large); 0 if there are
- * fewer than n above 0. Two bits at a time, as a bit's latency is a comparison, a count and a branch. *larger: how many are over it, if it
- * is the number itself. */
+/* The n-th largest of a wave's numbers, or one between it and the next smaller (so as many are as large); 0 if there
+ * are fewer than n above 0. Two bits at a time, as a bit's latency is a comparison, a count and a branch. *larger:
+ * how many are over it, if it is the number itself. */
 template <int N>
 __device__ __forceinline__ uint32_t lp_nth(const uint32_t (&k)[N], int n, bool *exact, int *larger) {
     uint32_t at = 0;
@@ -252,8 +250,8 @@ __device__ __forceinline__ void lp_finish(const logprobs_args &p, int64_t row, c
     }
 }
 
-/* 8 waves of a SIMD hold 2047 rows at once (157 us; with 7, 164); of fp32 logits the registers do not suffice, and memory is the
- * bound. */
+/* 8 waves of a SIMD hold 2047 rows at once (157 us; with 7, 164); of fp32 logits the registers do not suffice, and
+ * memory is the bound. */
 template <typename T>
 __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 7 : 8) void sera_logprobs_kernel(logprobs_args p) {
     constexpr int VEC = 16 / (int)sizeof(T), UNROLL = 16 / VEC;
@@ -265,8 +263,8 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 7 : 8) void sera_logp
     const int64_t row = blockIdx.x;
     const int split = blockIdx.y, piece = split * kWaves + wave, pieces = p.splits * kWaves;
     const T *x = (const T *)p.logits + row * p.stride;
-    /* The row's whole 16-byte units, in equal shares; the elements in front of them are a step of the first wave, those
-     * behind them one of the last. */
+    /* The row's whole 16-byte units, in equal shares; the elements in front of them are a step of the first wave,
+     * those behind them one of the last. */
     const int front = min((int)(-(uintptr_t)x & 15u) / (int)sizeof(T), p.vocab);
     const int units = (p.vocab - front) / VEC, back = p.vocab - front - units * VEC;
     const int per = (units + pieces - 1) / pieces, u0 = min(piece * per, units), u1 = min(u0 + per, units);
@@ -291,7 +289,8 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 7 : 8) void sera_logp
         *id = (step < 0 ? 0 : p.vocab - back) + min(lane, n - 1);
         return i == 0 && lane < n ? 1 : 0;
     };
-    /* Always and in one way, so that nothing waits for a load before the next step; what a step has not got is taken out of it there. */
+    /* Always and in one way, so that nothing waits for a load before the next step; what a step has not got is taken
+     * out of it there. */
     const lp_global first = (lp_global)(units ? (const lp_words *)(x + front) : &lp_no_unit);
     const auto load = [&](int step, lp_unit *w) {
 #pragma unroll

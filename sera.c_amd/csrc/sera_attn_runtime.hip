@@ -318,7 +318,8 @@ int sera_kv_evict(const sera_kv_cache *cache, const sera_kv_batch *batch, int ke
     if (!new_table || !new_len || !kept || ((uintptr_t)new_table & 3u) || ((uintptr_t)new_len & 3u) ||
         ((uintptr_t)kept & 3u))
         return fail(-1, "%s: new_table, new_len and kept must be 4-byte aligned device pointers", tag);
-    if (new_len == batch->kv_len) return fail(-1, "%s: new_len must not be kv_len", tag);
+    if (overlap(new_len, batch->kv_len, (int64_t)batch->sequences * 4))
+        return fail(-1, "%s: new_len must not overlap kv_len", tag);
     const int64_t sums = (int64_t)batch->sequences * cache->kv_heads;
     if (check_weights(tag, weights, new_weights, sums, weights_stride, batch->max_kv)) return -1;
     if (overlap(weights, new_weights, sums * weights_stride * 4))

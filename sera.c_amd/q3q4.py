@@ -731,8 +731,10 @@ def _flat(name, t, dtype, shape, device):
 
 
 class Rope:
-    """What q's and k's heads go through (sera_qk_rope): RMSNorm with a gamma (float32 [head_dim], None: no norm), then a turn of the first 2 *
-    len(inv_freq) channels, pair i by position * inv_freq[i] (float32, None: no turn)."""
+    """What q's and k's heads go through (sera_qk_rope): RMSNorm with a gamma
+    (float32 [head_dim], None: no norm), then a turn of the first
+    2 * len(inv_freq) channels, pair i by position * inv_freq[i] (float32, None:
+    no turn). The tensors are kept."""
 
     def __init__(self, inv_freq=None, q_gamma=None, k_gamma=None, eps=1e-6, pairing=ROPE_HALVES):
         import torch
@@ -749,8 +751,10 @@ class Rope:
 
 
 def kv_write_rope(cache, batch, rope, q, q_out, k, v, positions=None, stream=None):
-    """kv_write of k normed and rotated, and q into q_out the same way (q_out may be q); k, v [rows, kv_heads * head_dim],
-    q, q_out [rows, heads * head_dim] of one type. positions: int32 [rows], by default each row's place in its sequence."""
+    """kv_write of k normed and rotated, and q into q_out the same way (q_out
+    may be q); k, v [rows, kv_heads * head_dim], q, q_out [rows, heads *
+    head_dim] of one type. positions: int32 [rows], by default each row's place
+    in its sequence."""
     import torch
     ty, kp, ks, vp, vs = _pair(cache, batch, cache.width, k, v)
     width = q.shape[-1] if len(q.shape) else 0
@@ -776,6 +780,8 @@ def kv_write_rope(cache, batch, rope, q, q_out, k, v, positions=None, stream=Non
 def attention_weights_workspace(cache, batch, heads):
     """Scratch for attention_weights() with this batch's bounds."""
     import torch
+    if cache.device < 0:
+        raise Q3Q4Error(f"the cache's data must be a device tensor, got {cache.data.device}")
     with torch.cuda.device(cache.data.device):
         n = load().sera_attention_weights_workspace_bytes(cache.ref, batch.ref, heads)
     return torch.empty(n, dtype=torch.uint8, device=cache.data.device) if n else None
@@ -790,9 +796,12 @@ def _sums(name, t, cache, batch):
     return p, t.shape[2]
 
 
-def attention_weights(cache, batch, q, out, scale, weights, before=None, window=0, sinks=0, workspace=None, stream=None):
-    """attention(), and weights [sequences, kv_heads, max_kv or more] (float32) = before + what each position got from the
-    new rows, summed over them and the query heads of its kv head. before: the same shape, may be weights; None: zero."""
+def attention_weights(cache, batch, q, out, scale, weights, before=None, window=0, sinks=0, workspace=None,
+                      stream=None):
+    """attention(), and weights [sequences, kv_heads, max_kv or more] (float32)
+    = before + what each position got from the new rows, summed over them and
+    the query heads of its kv head. before: the same shape, may be weights;
+    None: zero."""
     width = q.shape[-1] if len(q.shape) else 0
     ty, qp, qs, op, os_ = _pair(cache, batch, width, q, out)
     if width % cache.head_dim:
@@ -809,9 +818,11 @@ def attention_weights(cache, batch, q, out, scale, weights, before=None, window=
 
 
 def kv_evict(cache, batch, keep, weights, new_table, new_len, new_weights, kept, recent=0, sinks=0, stream=None):
-    """Shortens each sequence to `keep` positions: the first `sinks`, the last `recent` and those of the largest weights, for every kv
-    head by itself; they move to the pages of new_table [sequences, entries] (int32). new_len [sequences] and kept
-    [sequences, kv_heads, keep] (int32) tell what stayed, new_weights (as weights) has their sums."""
+    """Shortens each sequence to `keep` positions: the first `sinks`, the last
+    `recent` and those of the largest weights, for every kv head by itself; they
+    move to the pages of new_table [sequences, entries] (int32), which are none
+    of the old ones. new_len [sequences] and kept [sequences, kv_heads, keep]
+    (int32) tell what stayed, new_weights (as weights) has their sums."""
     import torch
     n = batch.kv_len.numel()
     if cache.device < 0 or batch.device != cache.device:
@@ -834,9 +845,17 @@ def kv_evict(cache, batch, keep, weights, new_table, new_len, new_weights, kept,
 # Log probabilities (include/sera_logprobs.h)
 # ---------------------------------------------------------------------------
 
+def _check_logits(logits):
+    if len(logits.shape) != 2:
+        raise Q3Q4Error(f"logits must be [rows, vocab], got {tuple(logits.shape)}")
+    if logits.get_device() < 0:
+        raise Q3Q4Error(f"logits must be a device tensor, got {logits.device}")
+
+
 def logprobs_workspace(logits, top=0):
     """Scratch for logprobs() of logits [rows, vocab] (None: none needed)."""
     import torch
+    _check_logits(logits)
     with torch.cuda.device(logits.device):
         n = load().sera_logprobs_workspace_bytes(logits.shape[0], logits.shape[1], top)
     return torch.empty(n, dtype=torch.uint8, device=logits.device) if n else None
@@ -844,16 +863,14 @@ def logprobs_workspace(logits, top=0):
 
 def logprobs(logits, tokens=None, token_logprobs=None, entropy=None, top_ids=None, top_logprobs=None, workspace=None,
              stream=None):
-    """Of logits [rows, vocab] (float32, float16 or bfloat16): the log probabilities of tokens [rows, n] (int32) into
-    token_logprobs [rows, n], the entropy into entropy [rows], the most likely tokens into top_ids (int32) and top_logprobs
-    [rows, top]; float32 results. What is None is not computed."""
+    """Of logits [rows, vocab] (float32, float16 or bfloat16): the log
+    probabilities of tokens [rows, n] (int32) into token_logprobs [rows, n], the
+    entropy into entropy [rows], the most likely tokens into top_ids (int32) and
+    top_logprobs [rows, top]; float32 results. What is None is not computed."""
     import torch
-    if len(logits.shape) != 2:
-        raise Q3Q4Error(f"logits must be [rows, vocab], got {tuple(logits.shape)}")
+    _check_logits(logits)
     rows, vocab = logits.shape
     device = logits.get_device()
-    if device < 0:
-        raise Q3Q4Error(f"logits must be a device tensor, got {logits.device}")
     if rows and vocab == 0:
         raise Q3Q4Error("logits of no tokens")
     ty, xp, stride = _rows(logits, rows, vocab, device) if vocab else (0, 0, 0)

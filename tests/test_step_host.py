@@ -126,6 +126,7 @@ def test_weights_refusals(L, bad, msg):
     (dict(new_stride=0), "new positions"), (dict(keep=65, new_stride=1), "new positions"), (dict(new_table=None), "new_table"),
     (dict(new_len=None), "new_len"), (dict(kept=None), "kept"), (dict(kept=66), "aligned"), (dict(new_len=128), "kv_len"),
     (dict(weights=None), "weights"), (dict(new_weights=None), "weights"), (dict(new_weights=1 << 20), "overlap"),
+    (dict(new_len=132), "kv_len"), (dict(new_len=124), "kv_len"),
     (dict(new_weights=(1 << 20) + 4 * 1599), "overlap"), (dict(stride=99), "apart"),
 ])
 def test_evict_refusals(L, bad, msg):
@@ -235,6 +236,8 @@ def test_python_weights_and_evict_refusals():
     c, b = cache_and_batch()
     with pytest.raises(q3q4.Q3Q4Error, match="one device"):
         q3q4.attention_weights(c, b, r, r, 0.1, torch.zeros(2, 1, 16))
+    with pytest.raises(q3q4.Q3Q4Error, match="device tensor"):
+        q3q4.attention_weights_workspace(c, b, 1)
     new = (ints(2, 1), ints(2), torch.zeros(2, 1, 16), ints(2, 1, 8))
     with pytest.raises(q3q4.Q3Q4Error, match="one device"):
         q3q4.kv_evict(c, b, 8, torch.zeros(2, 1, 16), *new)
@@ -248,6 +251,10 @@ def test_python_logprobs_refusals():
         q3q4.logprobs(torch.zeros(5))
     with pytest.raises(q3q4.Q3Q4Error, match="device tensor"):
         q3q4.logprobs(torch.zeros(2, 5))
+    with pytest.raises(q3q4.Q3Q4Error, match="rows, vocab"):
+        q3q4.logprobs_workspace(torch.zeros(5))
+    with pytest.raises(q3q4.Q3Q4Error, match="device tensor"):
+        q3q4.logprobs_workspace(torch.zeros(2, 5))
 
 
 # ---- the oracle ---------------------------------------------------------------
