@@ -2,17 +2,19 @@
  * kv_evict.hip - shortening of cached sequences: which positions of a kv head stay, and their move to new pages.
  *
  * Choice: a workgroup for each sequence and kv head. Weights become whole numbers of the same order; the smallest one
- * that stays is built bit by bit, each bit by counting how many are as large. Then each wave walks a run of positions
- * of its own, held in registers up to 16384 positions, and writes what stays behind what the runs before it keep,
- * which a count of each run says.
+ * that stays is built of four digits of 8 bits, each from counts in LDS of how many have which. Then each wave walks
+ * a run of positions of its own, held in registers up to 24576 positions, and writes what stays behind what the runs
+ * before it keep, which a count of each run says.
  *
  * Move: a wave for K or V of 16 new places of a head. A K row is a run of bytes. A V token is an element of each
  * channel's 16, so whole blocks of 16 old tokens come as they lie, go through LDS, and the tokens that stay are
  * picked from there.
  *
  * The move is bound by memory, the choice by the latency of its steps. 64 sequences of 8192 positions to half (8 kv
- * heads, 128 channels, fp16 cache): 32 us and 533 us, for 2.7 GB the rate of a copy; of V's blocks of 16 tokens hardly
- * one is without any that stays, so V is read whole. 24 sequences of up to 3001 (8-bit cache): 16 us and 27 us.
+ * heads, 128 channels, fp16 cache): 22 us and 533 us, for 2.7 GB the rate of a copy; of V's blocks of 16 tokens
+ * hardly one is without any that stays, so V is read whole. 24 sequences of up to 3001 (8-bit cache): 9 us and 27 us.
+ * The choice alone, of one sequence: 3001 positions 8 us, 16000 23 us, 200000 265 us; with the cut built two bits at
+ * a time by counts over all waves 13, 25 and 496 us.
  */
 #include "attn_common.h"
 #include "sera_dpp.h"
@@ -20,7 +22,7 @@
 
 namespace {
 
-constexpr int kKeepWaves = 4;
+constexpr uint32_t kProtected = 0xffffffffu;            /* more than any weight's number */
 
 /* A weight as a whole number of the same order, from 2 on; NaN is 1. */
 __device__ __forceinline__ uint32_t keep_key(float w) {
@@ -43,12 +45,14 @@ typedef uint32_t move_u4 __attribute__((ext_vector_type(4)));
 
 }  // namespace
 
-/* R: 64-position rows of a wave's run that are held in registers (the run fits); 0: they are read again each time. */
-template <int R>
-__global__ __launch_bounds__(64 * kKeepWaves) void sera_kv_keep_kernel(kv_args a, evict_args t) {
-    __shared__ int part[2][kKeepWaves][4], part_eq[kKeepWaves];
+/* W waves. R: 64-position rows of a wave's run that are held in registers (the run fits); 0: they are read again each
+ * time. */
+template <int W, int R>
+__global__ __launch_bounds__(64 * W) void sera_kv_keep_kernel(kv_args a, evict_args t) {
+    __shared__ int counts[4][256], part[W], part_eq[W];
     const int b = (int)(blockIdx.z * gridDim.y + blockIdx.y), head = (int)blockIdx.x;
     if (b >= a.sequences) return;
+    constexpr int BATCH = R == 0 || R > 8 ? 8 : R;      /* loads on their way */
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int len = a.kv_len[b];
     const bool bad = len < 0 || len > a.max_kv, all = !bad && len <= t.keep;
@@ -58,23 +62,25 @@ __global__ __launch_bounds__(64 * kKeepWaves) void sera_kv_keep_kernel(kv_args a
     float *__restrict__ to = t.new_weights + place * t.weights_stride;
     const int count = bad ? 0 : min(len, t.keep);
     if (head == 0 && tid == 0) t.new_len[b] = bad ? -1 : count;
-    for (int x = count + tid; x < t.keep; x += 64 * kKeepWaves) kept[x] = -1;
+    for (int x = count + tid; x < t.keep; x += 64 * W) kept[x] = -1;
     if (bad) return;
     if (all) {
-        for (int x = tid; x < len; x += 64 * kKeepWaves) {
+        for (int x = tid; x < len; x += 64 * W) {
             kept[x] = x;
             to[x] = w[x];
         }
         return;
     }
     const int lo = t.sinks, hi = len - t.recent;
+    for (int x = tid; x < 4 * 256; x += 64 * W) counts[x >> 8][x & 255] = 0;
+    __syncthreads();
 
     /* A wave's run of positions. Those outside the middle count as the largest there are, places behind the run as
      * none. */
-    const int run = ((len + kKeepWaves - 1) / kKeepWaves + 63) & ~63;
+    const int run = ((len + W - 1) / W + 63) & ~63;
     const int from = min(wave * run, len), end = min(from + run, len);
     uint32_t key[R ? R : 1];
-    const auto key_of = [&](float v, int j) { return j >= end ? 0u : j < lo || j >= hi ? 0xffffffffu : keep_key(v); };
+    const auto key_of = [&](float v, int j) { return j >= end ? 0u : j < lo || j >= hi ? kProtected : keep_key(v); };
     if (R) {
         float v[R ? R : 1];
 #pragma unroll
@@ -88,47 +94,61 @@ __global__ __launch_bounds__(64 * kKeepWaves) void sera_kv_keep_kernel(kv_args a
 #pragma unroll
             for (int r = 0; r < R; r++) each(from + 64 * r, key[r]);
         } else {
-            for (int x = from; x < end; x += 64) each(x, key_of(w[min(x + lane, len - 1)], x + lane));
+            for (int x = from; x < end; x += 64 * BATCH) {
+                float v[BATCH];
+#pragma unroll
+                for (int i = 0; i < BATCH; i++) v[i] = w[min(x + 64 * i + lane, len - 1)];
+#pragma unroll
+                for (int i = 0; i < BATCH; i++) each(x + 64 * i, key_of(v[i], x + 64 * i + lane));
+            }
         }
     };
 
-    /* Of all, those outside the middle among them, t.keep stay: those above `cut`, and the first `ties` of those
-     * equal to it. The cut is the t.keep-th largest, built bit by bit; as soon as exactly that many reach it, it is
-     * the number below. */
-    uint32_t cut = 0u;
-    int larger = 0, turn = 0;
-    bool exact = false;
-    for (int bit = 30; bit >= 0 && !exact; bit -= 2) {          /* two bits: three counts */
-        int n[3] = {0, 0, 0};
+    /* Of the middle `ties` stay: those above `cut`, and the first of those equal to it. The cut is the ties-th
+     * largest, built of four digits: how many have each digit behind those found so far, and which one the ties-th
+     * has. As soon as all of a digit stay, the cut is the number below. */
+    int ties = t.keep - t.sinks - t.recent;
+    uint32_t cut = ties ? 0u : kProtected - 1u;
+    for (int place = 3; place >= 0 && ties; place--) {
+        int *const count = counts[place];
         rows([&](int, uint32_t k) {
-#pragma unroll
-            for (int i = 0; i < 3; i++) n[i] += k >= (cut | (uint32_t)(i + 1) << bit);
+            const bool in = k != 0u && k != kProtected && (place == 3 || (k ^ cut) >> (8 * place + 8) == 0u);
+            const uint64_t all = __ballot(in);
+            if (!all) return;
+            const uint32_t digit = k >> (8 * place) & 255u;
+            const uint32_t one = __builtin_amdgcn_readlane(digit, __builtin_ctzll(all));
+            if (__ballot(in && digit != one) == 0) {            /* equal weights would queue for one counter */
+                if (lane == 0) atomicAdd(&count[one], __popcll(all));
+            } else if (in) {
+                atomicAdd(&count[digit], 1);
+            }
         });
-        turn ^= 1;
-#pragma unroll
-        for (int i = 0; i < 3; i++) {
-            n[i] = keep_wave_sum(n[i]);
-            if (lane == 0) part[turn][wave][i] = n[i];
-        }
         __syncthreads();
-        const uint32_t base = cut;
+        /* A lane has four digits, the highest lane the highest. */
+        int n[4], above = 0;
 #pragma unroll
-        for (int i = 0; i < 3; i++) {
-            int all = 0;
+        for (int i = 0; i < 4; i++) above += n[i] = count[4 * lane + i];
+        int upto = above;                                       /* of this lane and those over it */
 #pragma unroll
-            for (int x = 0; x < kKeepWaves; x++) all += part[turn][x][i];
-            /* the highest that as many reach; the one above it has fewer */
-            if (all >= t.keep) cut = base | (uint32_t)(i + 1) << bit;
-            else if (cut == (i ? base | (uint32_t)i << bit : base)) larger = all;
-            exact |= all == t.keep;
-            if (all <= t.keep) break;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int x = __shfl_down(upto, o, 64);
+            upto += lane + o < 64 ? x : 0;
+        }
+        above = upto - above;
+        int digit = -1, over = 0, same = 0;
+#pragma unroll
+        for (int i = 3; i >= 0; i--) {
+            if (above < ties && ties <= above + n[i]) digit = 4 * lane + i, over = above, same = n[i];
+            above += n[i];
+        }
+        const int has = __builtin_ctzll(__ballot(digit >= 0));  /* one lane has: more than `ties` are in the middle */
+        cut |= (uint32_t)__builtin_amdgcn_readlane(digit, has) << (8 * place);
+        ties -= __builtin_amdgcn_readlane(over, has);
+        if (ties == __builtin_amdgcn_readlane(same, has)) {
+            cut--;
+            ties = 0;
         }
     }
-    if (exact) {
-        cut--;
-        larger = t.keep;
-    }
-    const int ties = t.keep - larger;
 
     int sure = 0, equal = 0;
     rows([&](int, uint32_t k) {
@@ -137,17 +157,16 @@ __global__ __launch_bounds__(64 * kKeepWaves) void sera_kv_keep_kernel(kv_args a
     });
     sure = keep_wave_sum(sure);
     equal = keep_wave_sum(equal);
-    __syncthreads();
     if (lane == 0) {
-        part[0][wave][0] = sure;
+        part[wave] = sure;
         part_eq[wave] = equal;
     }
     __syncthreads();
     int at = 0, seen = 0;
 #pragma unroll
-    for (int x = 0; x < kKeepWaves; x++)
+    for (int x = 0; x < W; x++)
         if (x < wave) {
-            at += part[0][x][0] + max(min(ties - seen, part_eq[x]), 0);
+            at += part[x] + max(min(ties - seen, part_eq[x]), 0);
             seen += part_eq[x];
         }
     const unsigned long long below = (1ull << lane) - 1ull;
@@ -165,7 +184,6 @@ __global__ __launch_bounds__(64 * kKeepWaves) void sera_kv_keep_kernel(kv_args a
         seen += __popcll(tied);
     };
     if constexpr (R > 0) {
-        constexpr int BATCH = 8;        /* loads on their way */
 #pragma unroll
         for (int r = 0; r < R; r += BATCH) {
             float v[BATCH];
@@ -175,9 +193,12 @@ __global__ __launch_bounds__(64 * kKeepWaves) void sera_kv_keep_kernel(kv_args a
             for (int i = 0; i < BATCH; i++) put(from + 64 * (r + i), key[r + i], v[i]);
         }
     } else {
-        for (int x = from; x < end; x += 64) {
-            const float v = w[min(x + lane, len - 1)];
-            put(x, key_of(v, x + lane), v);
+        for (int x = from; x < end; x += 64 * BATCH) {
+            float v[BATCH];
+#pragma unroll
+            for (int i = 0; i < BATCH; i++) v[i] = w[min(x + 64 * i + lane, len - 1)];
+#pragma unroll
+            for (int i = 0; i < BATCH; i++) put(x + 64 * i, key_of(v[i], x + 64 * i + lane), v[i]);
         }
     }
 }
@@ -290,11 +311,17 @@ __global__ __launch_bounds__(256) void sera_kv_move_kernel(kv_args a, evict_args
 hipError_t sera_launch_kv_evict(uint32_t cache_type, int dim, const kv_args &a, const evict_args &t, hipStream_t s) {
     const int y = a.sequences < 32768 ? a.sequences : 32768;
     const unsigned z = (unsigned)((a.sequences + y - 1) / y);
-    const dim3 heads((unsigned)a.kv_heads, (unsigned)y, z), threads(64 * kKeepWaves);
-    if (a.max_kv <= 16 * 64 * kKeepWaves) hipLaunchKernelGGL(sera_kv_keep_kernel<16>, heads, threads, 0, s, a, t);
-    else if (a.max_kv <= 32 * 64 * kKeepWaves) hipLaunchKernelGGL(sera_kv_keep_kernel<32>, heads, threads, 0, s, a, t);
-    else if (a.max_kv <= 64 * 64 * kKeepWaves) hipLaunchKernelGGL(sera_kv_keep_kernel<64>, heads, threads, 0, s, a, t);
-    else hipLaunchKernelGGL(sera_kv_keep_kernel<0>, heads, threads, 0, s, a, t);
+    const dim3 heads((unsigned)a.kv_heads, (unsigned)y, z);
+    /* Eight waves as long as their registers hold a sequence (built two bits at a time, 3001 positions took 13 us, 15
+     * with four waves and 17 with sixteen; 16000 took 25, 28 with sixteen). Then sixteen, and beyond what those hold
+     * as well, where the weights are read five times: 200000 positions took 490 us, 710 with eight. */
+#define SERA_KEEP(W, R) hipLaunchKernelGGL((sera_kv_keep_kernel<W, R>), heads, dim3(64 * W), 0, s, a, t)
+    if (a.max_kv <= 8 * 64 * 8) SERA_KEEP(8, 8);
+    else if (a.max_kv <= 16 * 64 * 8) SERA_KEEP(8, 16);
+    else if (a.max_kv <= 32 * 64 * 8) SERA_KEEP(8, 32);
+    else if (a.max_kv <= 24 * 64 * 16) SERA_KEEP(16, 24);
+    else SERA_KEEP(16, 0);
+#undef SERA_KEEP
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const int most = t.keep < a.max_kv ? t.keep : a.max_kv, blocks = (most + 15) / 16;
