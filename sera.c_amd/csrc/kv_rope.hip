@@ -81,8 +81,8 @@ struct rope_turn {
             for (int e = 0; e < VEC; e += 2) {
                 const float c = cosine[t][i + e / 2], s = sine[t][i + e / 2];
                 const float a = x[e], b = x[e + 1];
-                x[e] = turns ? a * c - b * s : a;
-                x[e + 1] = turns ? a * s + b * c : b;
+                x[e] = turns ? fmaf(a, c, -(b * s)) : a;
+                x[e + 1] = turns ? fmaf(a, s, b * c) : b;
             }
         } else {
             const int i = d0 & (half - 1);
@@ -92,7 +92,7 @@ struct rope_turn {
 #pragma unroll
             for (int e = 0; e < VEC; e++) {
                 const float c = cosine[t][i + e], s = sine[t][i + e] * sign;
-                x[e] = turns ? x[e] * c + y[e] * s : x[e];
+                x[e] = turns ? fmaf(x[e], c, y[e] * s) : x[e];
             }
         }
     }
@@ -159,7 +159,11 @@ __global__ __launch_bounds__(256) void sera_kv_rope_kernel(kv_args a, rope_args 
             const int at = r.positions ? r.positions[row + t] : u.pos0 + t;
             double turns = (double)at * (double)r.inv_freq[i] * 0.15915494309189535;   /* 1 / (2 pi) */
             turns -= rint(turns);
-            sincospif((float)(2.0 * turns), &sine[t][i], &cosine[t][i]);
+            const float h = (float)(2.0 * turns), rest = (float)((2.0 * turns - h) * M_PI);   /* what h rounds off */
+            float s, c;
+            sincospif(h, &s, &c);
+            sine[t][i] = fmaf(rest, c, s);
+            cosine[t][i] = fmaf(-rest, s, c);
         }
     }
     __syncthreads();
