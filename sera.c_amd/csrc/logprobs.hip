@@ -18,7 +18,7 @@
  * launch joins in the same way.
  *
  * Bound by reading the logits, and of 16-bit ones by the vector instructions (8 an element and an exponential). 2047
- * rows of 151937 bf16 logits: 119 us without a top (5.2 TB/s, what a copy reaches), 157 us with the top 8; 1008 rows
+ * rows of 151937 bf16 logits: 120 us without a top (5.2 TB/s, what a copy reaches), 160 us with the top 8; 1008 rows
  * of 151936 fp32 logits with the top 8: 112 us (5.5 TB/s). 16 rows: 11 + 4 us, 1 row: 8.5 + 6.5 us, which is latency.
  * A threshold of each wave by itself, its list's top-th, made the first 250 us: four times as many steps had
  * something to look at.
@@ -58,16 +58,18 @@ __device__ __forceinline__ float lp_below(uint32_t o) {
     return o < 0x00800001u ? -INFINITY : lp_value(o - (o == 0x80000000u ? 2 : 1));
 }
 
-/* Running sums of a lane. m is not -inf. */
+/* Running sums of a lane, in 64 bits (which take 16 elements' at a time): a token that stands out has nearly all of s, and
+ * the entropy is what the others add to it. m is not -inf. */
 struct lp_sum {
-    float m, s, t;
+    float m;
+    double s, t;
 };
 
 /* The sums around a maximum m that is as large or larger. */
 __device__ __forceinline__ void lp_raise(lp_sum &a, float m) {
     const float d = fmaxf(a.m - m, -200.0f);  /* beyond, no weight is left; held, no product with 0 is undefined */
-    const float f = __builtin_amdgcn_exp2f(d * kLog2E);
-    a.t = f * fmaf(d, a.s, a.t);
+    const double f = __builtin_amdgcn_exp2f(d * kLog2E);
+    a.t = f * fma((double)d, a.s, a.t);
     a.s *= f;
     a.m = m;
 }
@@ -80,11 +82,16 @@ __device__ __forceinline__ void lp_join(lp_sum &a, lp_sum b) {
 }
 
 template <int OFF>
+__device__ __forceinline__ double lp_partner(double x) {
+    return __hiloint2double(__float_as_int(xor_partner<OFF>(__int_as_float(__double2hiint(x)))),
+                            __float_as_int(xor_partner<OFF>(__int_as_float(__double2loint(x)))));
+}
+template <int OFF>
 __device__ __forceinline__ void lp_join_lane(lp_sum &a) {
     lp_sum b;
     b.m = xor_partner<OFF>(a.m);
-    b.s = xor_partner<OFF>(a.s);
-    b.t = xor_partner<OFF>(a.t);
+    b.s = lp_partner<OFF>(a.s);
+    b.t = lp_partner<OFF>(a.t);
     lp_join(a, b);
 }
 __device__ __forceinline__ void lp_join_wave(lp_sum &a) {
@@ -201,13 +208,11 @@ __device__ const lp_words lp_no_unit = {0u, 0u, 0u, 0u};
 }  // namespace
 
 /* Joins the waves of a workgroup: the sums for all of them, the lists into that of wave 0. */
-__device__ __forceinline__ void lp_join_group(lp_sum &a, lp_list &list, lp_key (*keys)[kRoom], float (*sums)[3],
+__device__ __forceinline__ void lp_join_group(lp_sum &a, lp_list &list, lp_key (*keys)[kRoom], lp_sum *sums,
                                               int *counts, int lane, int wave) {
     lp_join_wave(a);
     if (lane == 0) {
-        sums[wave][0] = a.m;
-        sums[wave][1] = a.s;
-        sums[wave][2] = a.t;
+        sums[wave] = a;
         counts[wave] = list.n;
     }
     __syncthreads();
@@ -219,8 +224,8 @@ __device__ __forceinline__ void lp_join_group(lp_sum &a, lp_list &list, lp_key (
         if (lane == 0) counts[wave] = list.n;
         __syncthreads();
     }
-    a = {sums[0][0], sums[0][1], sums[0][2]};
-    for (int w = 1; w < kWaves; w++) lp_join(a, {sums[w][0], sums[w][1], sums[w][2]});
+    a = sums[0];
+    for (int w = 1; w < kWaves; w++) lp_join(a, sums[w]);
     if (wave) return;
     for (int w = 1; w < kWaves; w++)
         for (int i = lane, n = counts[w]; i - lane < n; i += 64) list.put(keys[w][min(i, n - 1)], i < n, lane);
@@ -232,31 +237,32 @@ template <typename T>
 __device__ __forceinline__ void lp_finish(const logprobs_args &p, int64_t row, const lp_sum &a, const lp_list &list,
                                           int lane, int wave) {
     const T *x = (const T *)p.logits + row * p.stride;
-    const bool fine = a.s > 0.0f && a.s < INFINITY;
-    const float nan = __builtin_nanf(""), log_s = logf(a.s);
+    const bool fine = a.s > 0.0 && a.s < INFINITY;
+    const float nan = __builtin_nanf("");
+    const double log_s = log(a.s);
     if (wave) {
         for (int i = 64 * (wave - 1) + lane; i < p.per_row; i += 64 * (kWaves - 1)) {
             const int token = p.tokens[row * p.per_row + i];
             float y = nan;
-            if (fine && token >= 0 && token < p.vocab) y = (lp_f32(x[token]) - a.m) - log_s;
+            if (fine && token >= 0 && token < p.vocab) y = (float)((double)(lp_f32(x[token]) - a.m) - log_s);
             p.token_logprobs[row * p.per_row + i] = y;
         }
-        if (p.entropy && threadIdx.x == 64) p.entropy[row] = fine ? log_s - a.t / a.s : nan;
+        if (p.entropy && threadIdx.x == 64) p.entropy[row] = fine ? (float)(log_s - a.t / a.s) : nan;
     } else if (lane < p.top) {
         const lp_key mine = lane < list.n ? list.keys[lane] : 0;
         const int at = fine && lane < list.n ? list.place(mine) : lane;
         p.top_ids[row * p.top + at] = fine ? (int)~(uint32_t)mine : -1;
-        p.top_logprobs[row * p.top + at] = fine ? (lp_value((uint32_t)(mine >> 32)) - a.m) - log_s : nan;
+        p.top_logprobs[row * p.top + at] = fine ? (float)((double)(lp_value((uint32_t)(mine >> 32)) - a.m) - log_s) : nan;
     }
 }
 
-/* 8 waves of a SIMD hold 2047 rows at once (157 us; with 7, 164); of fp32 logits the registers do not suffice, and
+/* 8 waves of a SIMD hold 2047 rows at once (157 us instead of 164 with 7); of fp32 logits the registers do not suffice, and
  * memory is the bound. */
 template <typename T>
 __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 7 : 8) void sera_logprobs_kernel(logprobs_args p) {
     constexpr int VEC = 16 / (int)sizeof(T), UNROLL = 16 / VEC;
     __shared__ lp_key keys[kWaves][kRoom];
-    __shared__ float sums[kWaves][3];
+    __shared__ lp_sum sums[kWaves];
     __shared__ int counts[kWaves];
     __shared__ uint32_t most[64], bound;            /* of the lanes' largest, and what follows from them */
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -276,7 +282,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 7 : 8) void sera_logp
     list.n = 0;
     list.top = p.top;
     list.least = 0;
-    lp_sum a = {kLowest, 0.0f, 0.0f};
+    lp_sum a = {kLowest, 0.0, 0.0};
 
     /* Unit i of a step for a lane: the id of its first element, and how many of its elements there are. */
     const auto unit = [&](int step, int i, int lane, int *id) {
@@ -345,50 +351,48 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 7 : 8) void sera_logp
                 int id;
                 const int n = unit(step, k / VEC, lane, &id);
                 if (k % VEC >= n) y[k] = -INFINITY;
-                else if (n < VEC) y[k] = lp_f32(x[id]);
+                else if (k == 0 && n < VEC) y[k] = lp_f32(x[id]);
             }
         }
 #pragma unroll
         for (int k = 0; k < 16; k++) top = fmaxf(top, y[k]);
         if (__ballot(top > a.m)) lp_raise(a, fmaxf(a.m, top));
+        float s = 0.0f, t = 0.0f;       /* of this step: small weights one by one would be lost beside a large sum */
 #pragma unroll
         for (int k = 0; k < 16; k++) {
             const float d = y[k] - a.m, w = __builtin_amdgcn_exp2f(d * kLog2E);
-            a.s += w;
-            a.t = fmaf(w, fmaxf(d, -200.0f), a.t);
+            s += w;
+            t = fmaf(w, fmaxf(d, -200.0f), t);
         }
+        a.s += s;
+        a.t += t;
         if (__ballot(top > least) || (least == -INFINITY && list.n < p.top)) look(step, top);
     }
     lp_join_group(a, list, keys, sums, counts, lane, wave);
     if (p.splits == 1) return lp_finish<T>(p, row, a, list, lane, wave);
     if (wave) return;
     const size_t part = (size_t)row * p.splits + split;
-    float *const ws = p.workspace;
-    if (lane == 0) {
-        ws[3 * part] = a.m;
-        ws[3 * part + 1] = a.s;
-        ws[3 * part + 2] = a.t;
-    }
+    if (lane == 0) ((lp_sum *)p.workspace)[part] = a;
     if (lane < p.top)
-        ((lp_key *)(ws + p.sums))[part * p.top + lane] = lane < list.n ? list.keys[lane] : 0;
+        ((lp_key *)(p.workspace + p.sums))[part * p.top + lane] = lane < list.n ? list.keys[lane] : 0;
 }
 
 template <typename T>
 __global__ __launch_bounds__(64 * kWaves) void sera_logprobs_join_kernel(logprobs_args p) {
     __shared__ lp_key keys[kWaves][kRoom];
-    __shared__ float sums[kWaves][3];
+    __shared__ lp_sum sums[kWaves];
     __shared__ int counts[kWaves];
     __shared__ uint32_t most[64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t row = blockIdx.x;
-    const float *const ws = p.workspace + 3 * (size_t)row * p.splits;
+    const lp_sum *const ws = (const lp_sum *)p.workspace + (size_t)row * p.splits;
     const lp_key *const parts = (const lp_key *)(p.workspace + p.sums) + (size_t)row * p.splits * p.top;
     lp_list list;
     list.keys = keys[wave];
     list.n = 0;
     list.top = p.top;
     list.least = 0;
-    lp_sum a = {kLowest, 0.0f, 0.0f};
+    lp_sum a = {kLowest, 0.0, 0.0};
     lp_key key[kMostSplits * SERA_LOGPROBS_MAX_TOP / (64 * kWaves)];
     const int n = p.splits * p.top;
     uint32_t largest = 0;
@@ -397,7 +401,7 @@ __global__ __launch_bounds__(64 * kWaves) void sera_logprobs_join_kernel(logprob
         const int at = 64 * kWaves * i + (int)threadIdx.x;
         key[i] = at < n ? parts[at] : 0;
     }
-    if ((int)threadIdx.x < p.splits) a = {ws[3 * threadIdx.x], ws[3 * threadIdx.x + 1], ws[3 * threadIdx.x + 2]};
+    if ((int)threadIdx.x < p.splits) a = ws[threadIdx.x];
     if (threadIdx.x < 64) most[lane] = 0;
     __syncthreads();
     if (p.top) {
@@ -447,7 +451,9 @@ int sera_logprobs_splits(int rows, int vocab, int cus) {
 }
 
 /* Floats of the partial sums (the lists lie behind them, 16-byte aligned). */
-size_t sera_logprobs_sums(int rows, int splits) { return ((size_t)rows * splits * 3 + 3) & ~(size_t)3; }
+size_t sera_logprobs_sums(int rows, int splits) {
+    return ((size_t)rows * splits * sizeof(lp_sum) / sizeof(float) + 3) & ~(size_t)3;
+}
 
 hipError_t sera_launch_logprobs(uint32_t type, const logprobs_args &p, hipStream_t s) {
     if (type == 0u) return lp_go<float>(p, s);
