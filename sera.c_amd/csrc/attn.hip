@@ -160,7 +160,7 @@ __global__ __launch_bounds__(256) void sera_attn_join_kernel(kv_args a, attn_arg
 #pragma unroll
         for (int e = 0; e < E; e++) o.v[e] = kv_from_f32<T>(first + i < 0 ? 0.0f : y[e] / l);
         *(attn_vec<T, E> *)((T *)t.out + (s.row0 + i) * t.out_stride + (int64_t)h * D + E * lane) = o;
-        if (t.lse && lane == 0) t.lse[(size_t)(s.row0 + i) * t.heads + h] = attn_lse(top, l);
+        if (t.norms && lane == 0) t.norms[(size_t)(s.row0 + i) * t.heads + h] = attn_norm(top, l);
     }
 }
 
@@ -187,10 +187,10 @@ void shorten(attn_plan &p, const kv_args &a, const attn_args &t) {
 
 }  // namespace
 
-/* The workspace of a call that wants the weights' sums: partial results, each row's z, then what the sums need. */
-static size_t lse_at(const attn_plans &p) { return (p.bytes + 15) & ~(size_t)15; }
+/* The workspace of a call that wants the weights' sums: partial results, each row's norm, then what the sums need. */
+static size_t norms_at(const attn_plans &p) { return (p.bytes + 15) & ~(size_t)15; }
 static size_t sums_at(const attn_plans &p, const kv_args &a, int heads) {
-    return (lse_at(p) + (size_t)a.rows * heads * sizeof(float) + 15) & ~(size_t)15;
+    return (norms_at(p) + (size_t)a.rows * heads * sizeof(float2) + 15) & ~(size_t)15;
 }
 static attn_sums sums_of(const attn_plans &p, const kv_args &a, int heads, int cus, size_t *bytes) {
     return sera_attn_sums_plan(a, p.few.columns ? p.few_rows : 0,
@@ -219,7 +219,7 @@ hipError_t sera_launch_attn(uint32_t cache_type, uint32_t type, int dim, const k
         sums = sums_of(p, a, t.heads, t.cus, &n);
         sums.scores = (float *)(ws + sums_at(p, a, t.heads));
         sums.partial = (float *)((uint8_t *)sums.scores + sums.scores_bytes);
-        t.lse = (float *)(ws + lse_at(p));
+        t.norms = (float2 *)(ws + norms_at(p));
         t.scores = sums.scores;
         t.pitch = sums.pitch;
     }

@@ -19,7 +19,7 @@ struct attn_args {
     int few_rows;                   /* rows of one of its partial results */
     float *workspace;
     int cus;                        /* compute units of the device */
-    float *lse;                     /* log2 of each row's sum of 2^s', [rows][heads], for the weights, or NULL */
+    float2 *norms;                  /* attn_norm of each row, [rows][heads], for the weights, or NULL */
     float *scores;                  /* s' of the few-row kernel, [sequences][kv_heads][few_rows][pitch], or NULL */
     size_t pitch;
     const float *before;            /* sums so far, or NULL */

@@ -78,8 +78,14 @@ __device__ __forceinline__ int attn_page(const kv_args &a, int b, int pos, int l
 
 __device__ __forceinline__ float attn_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-/* log2 of a row's sum of 2^s' from its maximum and its sum of weights. */
-__device__ __forceinline__ float attn_lse(float m, float l) { return m - kAttnBias + __builtin_amdgcn_logf(l); }
+/* What a score becomes a weight by, 2^(s' - z) * r, from a row's maximum and its sum of weights. z is log2 of the sum but
+ * for a factor of 2; what that addition rounds off goes into r with the rest, so that scores keep all of their bits. A
+ * row without weights has an r of 0. */
+__device__ __forceinline__ float2 attn_norm(float m, float l) {
+    const float shift = m - kAttnBias, e = (float)__builtin_amdgcn_frexp_expf(l), z = shift + e, y = z - shift;
+    const float off = (shift - (z - y)) + (e - y);
+    return make_float2(z, l == 0.0f ? 0.0f : attn_exp2(-off) / __builtin_amdgcn_frexp_mantf(l));
+}
 
 /* The power of two that brings the largest |q| of a row near 2^10 (products
  * and sums then stay clear of fp16's and fp32's borders whatever the rows' size),

@@ -405,8 +405,8 @@ __global__ __launch_bounds__(64 * NW, OCC) void sera_attn_few_kernel(kv_args a, 
 #pragma unroll
                 for (int x = 0; x < 4; x++) y[x] = s.len - s.n + i < 0 ? 0.0f : sum[x] / lt;
                 attn_store4((T *)t.out + (s.row0 + i) * t.out_stride + q0 + (rr - i * t.group) * D + d, y);
-                if (t.lse && d == 0)
-                    t.lse[(size_t)(s.row0 + i) * t.heads + head * t.group + rr - i * t.group] = attn_lse(mt, lt);
+                if (t.norms && d == 0)
+                    t.norms[(size_t)(s.row0 + i) * t.heads + head * t.group + rr - i * t.group] = attn_norm(mt, lt);
             }
         }
     }

@@ -648,7 +648,7 @@ void sera_attn_tile_kernel(kv_args a, attn_args t, int slots, int splits, int ch
         ml[2 * k] = m;
         ml[2 * k + 1] = l;
     }
-    if (splits == 1 && t.lse && half == 0 && w0 + col < rows) t.lse[partial(32 * rg + col)] = attn_lse(m, l);
+    if (splits == 1 && t.norms && half == 0 && w0 + col < rows) t.norms[partial(32 * rg + col)] = attn_norm(m, l);
     constexpr int ROWS = 64 / (D / 4);
 #pragma unroll 4
     for (int i = 0; i < 32 / ROWS; i++) {

@@ -1,9 +1,9 @@
 /*
  * attn_weights.hip - the weight that every cached position gets from the rows of a call, after its attention:
  *
- *   w_j = sum over rows i, query heads of 2^(s'_ij - z_i),   z_i = log2(sum_j 2^(s'_ij))
+ *   w_j = sum over rows i, query heads of 2^(s'_ij - z_i) r_i,   2^z_i / r_i = sum_j 2^(s'_ij)
  *
- * with s' = scale * q . k * log2(e), as attention has them, and z left by its kernels (t.lse).
+ * with s' = scale * q . k * log2(e), as attention has them, and z and r left by its kernels (t.norms).
  *
  * Few rows: the kernel that streams the cache has the scores; it leaves them (4 bytes for each position and column),
  * and what is left to do is one pass over those.
@@ -17,12 +17,13 @@
  * sums in their order.
  *
  * Many rows are bound by the matrix instructions, and beside them by the exponentials and the columns' way through LDS:
- * the weights of one half of a wave's positions are made under the products of the other, and of the two waves of a
- * SIMD one converts columns while the other multiplies. 1024 rows of 64 heads at the end of 16384 positions (8 kv
- * heads, 128 channels, fp16 cache): 385 us with 16-bit rows and 565 us with fp32 ones, whose products are two, 0.8 of
- * the rate of a large library product; a prompt of 2048 fp32 rows: 110 us behind the attention's 160 us. Few rows are
- * bound by memory: 64 sequences of 8192 positions (8 kv heads, groups of 8, bf16 rows) leave 134 MB of scores in the
- * 461 us in which the attention streams 2.1 GB of cache, and one pass over them takes 33 us (4.1 TB/s).
+ * the weights of one half of a wave's positions are made under the products of the other, and of the two waves of a SIMD
+ * one converts columns while the other multiplies. r goes into z there, rounded to fp32 (2^-24 |z| of a weight, less than
+ * its score's own error); as a factor of every weight it cost 5%. 1024 rows of 64 heads at the end of 16384 positions (8
+ * kv heads, 128 channels, fp16 cache): 435 us with 16-bit rows, 600 us with fp32 ones, whose products are two (0.8 of the
+ * rate of a large library product); a prompt of 2048 fp32 rows: 110 us behind the attention's 160 us. Few rows are bound
+ * by memory: 64 sequences of 8192 positions (8 kv heads, groups of 8, bf16 rows) leave 134 MB of scores in the 461 us in
+ * which the attention streams 2.1 GB of cache, and one pass over them takes 33 us (4.1 TB/s).
  */
 #include "attn_device.h"
 #include "sera_launch.h"
@@ -141,7 +142,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void sera_attn_columns_kernel(kv_ar
          * there are). */
         int at_r = 32 * c0 + my_col, at_i = at_r / t.group, at_g = at_r - at_i * t.group;
         attn_vec<T, VEC> in[2][LOADS];
-        float z[2];
+        float2 z[2];
         bool there[2];                    /* not past the last column, which have no weight */
         const bool loads = 32 * TPC == 64 * kWaves || my_col < 32;
         const auto load = [&](int place) {
@@ -151,7 +152,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void sera_attn_columns_kernel(kv_ar
             const T *q = (const T *)t.q + (s.row0 + i) * t.q_stride + (int64_t)h * D + VEC * sub;
 #pragma unroll
             for (int k = 0; k < LOADS; k++) in[place][k] = *(const attn_vec<T, VEC> *)(q + TPC * VEC * k);
-            z[place] = t.lse[(size_t)(s.row0 + i) * t.heads + h];
+            z[place] = t.norms[(size_t)(s.row0 + i) * t.heads + h];
             at_r += 32;
             at_i += step_i;
             at_g += step_g;
@@ -178,7 +179,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void sera_attn_columns_kernel(kv_ar
             const float up = ldexpf(sign, e2);
             if (sub == 0) {
                 cz[buf][0][my_col] = ldexpf(fabsf(t.scale_log2), -e2);
-                cz[buf][1][my_col] = there[place] ? z[place] : INFINITY;
+                cz[buf][1][my_col] = there[place] ? z[place].x - __builtin_amdgcn_logf(z[place].y) : INFINITY;
             }
 #pragma unroll
             for (int k = 0; k < LOADS; k++) {
@@ -406,11 +407,11 @@ __global__ __launch_bounds__(256) void sera_attn_sums_kernel(kv_args a, attn_arg
     attn_f4 w = {0.0f, 0.0f, 0.0f, 0.0f};
     if (rows <= t.few_columns) {
         const float *x = p.scores + place * p.few_rows * p.pitch + j;
-        const float *z = t.lse + (size_t)s.row0 * t.heads + head * t.group;
+        const float2 *z = t.norms + (size_t)s.row0 * t.heads + head * t.group;
         if (j < s.len)
             for (int r = 0, i = 0, g = 0; r < rows; r += BATCH) {
                 attn_f4 y[BATCH];
-                float l[BATCH];
+                float2 l[BATCH];
                 int pos[BATCH];
 #pragma unroll
                 for (int k = 0; k < BATCH; k++) {
@@ -426,7 +427,8 @@ __global__ __launch_bounds__(256) void sera_attn_sums_kernel(kv_args a, attn_arg
                 for (int k = 0; k < BATCH; k++)
 #pragma unroll
                     for (int e = 0; e < 4; e++)
-                        w[e] += pos[k] >= 0 && attn_sees(t, pos[k], j + e) ? attn_exp2(y[k][e] - l[k]) : 0.0f;
+                        if (pos[k] >= 0 && attn_sees(t, pos[k], j + e))
+                            w[e] = fmaf(attn_exp2(y[k][e] - l[k].x), l[k].y, w[e]);
             }
     } else {
         /* units in front of the tile's */
@@ -505,8 +507,8 @@ attn_sums sera_attn_sums_plan(const kv_args &a, int few_rows, int group, int cus
         const int64_t n = ((int64_t)a.max_kv - x * kTokens) * group / 32 + 2;
         units += n < blocks ? n : blocks;
     }
-    /* A workgroup runs on a CU; each has an equal share of all units, of 8 at least: the start of one costs
-     * some 5. */
+    /* A workgroup runs on a CU; each has an equal share of all units, of 8 at least: the start of one costs some 5.
+     */
     const int64_t sequences = (a.rows + a.max_new - 1) / a.max_new;
     int64_t share = (units * sequences * a.kv_heads + cus - 1) / cus;
     if (share < 8) share = 8;

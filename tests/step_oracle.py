@@ -33,8 +33,7 @@ def weights_of(K, q, length, scale, window, sinks):
     """(sums, tolerance) [kv heads, length] of one sequence's new rows q [n, heads, dim], keys K [kv heads, length, dim].
 
     Tolerance. As for attention a weight is off by 2 * 2^-19 (sum|q k| scale + 1) of itself (its score, and the scores of
-    the sum that it is divided by); the logarithm of that sum is held in fp32, |score| 2^-23 again, inside the same.
-    Sums of m weights in fp32: m 2^-24 of them."""
+    the sum that it is divided by). Sums of m weights in fp32: m 2^-24 of them."""
     n, heads, _ = q.shape
     g = heads // K.shape[0]
     w, tol = np.zeros((K.shape[0], length)), np.zeros((K.shape[0], length))
