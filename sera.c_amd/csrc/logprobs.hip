@@ -18,10 +18,11 @@
  * launch joins in the same way.
  *
  * Bound by reading the logits, and of 16-bit ones by the vector instructions (8 an element and an exponential). 2047
- * rows of 151937 bf16 logits: 120 us without a top (5.2 TB/s, what a copy reaches), 160 us with the top 8; 1008 rows
- * of 151936 fp32 logits with the top 8: 112 us (5.5 TB/s). 16 rows: 11 + 4 us, 1 row: 8.5 + 6.5 us, which is latency.
- * A threshold of each wave by itself, its list's top-th, made the first 250 us: four times as many steps had
- * something to look at.
+ * rows of 151937 bf16 logits: 120 us without a top (5.2 TB/s, what a copy reaches), 139 us with the top 8; 1008 rows
+ * of 151936 fp32 logits with the top 8: 115 us (5.3 TB/s). 16 rows: 11 + 4 us, 1 row: 8.5 + 6 us, which is latency. A
+ * long top of short rows costs more than the rows, as nearly every step has some of it: the top 64 of 538 rows of
+ * 19950 54 us, the top 5 20 us, none 11 us. A threshold of each wave by itself, its list's top-th, made the first 250
+ * us: four times as many steps had something to look at.
  */
 #include "logprobs.h"
 #include "../../include/sera_logprobs.h"
@@ -58,8 +59,8 @@ __device__ __forceinline__ float lp_below(uint32_t o) {
     return o < 0x00800001u ? -INFINITY : lp_value(o - (o == 0x80000000u ? 2 : 1));
 }
 
-/* Running sums of a lane, in 64 bits (which take 16 elements' at a time): a token that stands out has nearly all of s, and
- * the entropy is what the others add to it. m is not -inf. */
+/* Running sums of a lane, in 64 bits (which take 16 elements' at a time): a token that stands out has nearly all of
+ * s, and the entropy is what the others add to it. m is not -inf. */
 struct lp_sum {
     float m;
     double s, t;
@@ -103,14 +104,38 @@ __device__ __forceinline__ void lp_join_wave(lp_sum &a) {
     lp_join_lane<32>(a);
 }
 
-/* The n-th largest of a wave's numbers, or one between it and the next smaller (so as many are as large); 0 if there
- * are fewer than n above 0. Two bits at a time, as a bit's latency is a comparison, a count and a branch. *larger:
- * how many are over it, if it is the number itself. */
+/* The bits that any lane has, wave-uniform. */
+__device__ __forceinline__ uint32_t lp_any(uint32_t x) {
+    int y = (int)x;
+    y |= xor_partner<1>(y);
+    y |= xor_partner<2>(y);
+    y |= xor_partner<4>(y);
+    y |= xor_partner<8>(y);
+    y |= xor_partner<16>(y);
+    y |= xor_partner<32>(y);
+    return (uint32_t)__builtin_amdgcn_readfirstlane(y);
+}
+
+/* The n-th largest of a wave's numbers, or one between it and the next smaller (so as many are as large); if there
+ * are fewer than n above 0, one that those are not below. Two bits at a time, as a bit's latency is a comparison, a
+ * count and a branch, and only from the first to the last bit in which those above 0 differ (of the logits that may
+ * be in a top few do, and the low ones of bf16 never). *larger: how many are over it, if it is the number itself. */
 template <int N>
 __device__ __forceinline__ uint32_t lp_nth(const uint32_t (&k)[N], int n, bool *exact, int *larger) {
-    uint32_t at = 0;
+    uint32_t any = 0, lacks = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        any |= k[i];
+        lacks |= k[i] ? ~k[i] : 0u;
+    }
+    any = lp_any(any);
+    const uint32_t differ = any & lp_any(lacks), common = any & ~differ;
     *larger = 0;
-    for (int bit = 30; bit >= 0; bit -= 2) {
+    *exact = false;
+    if (!differ) return common;
+    int bit = (31 - __builtin_clz(differ)) & ~1;
+    uint32_t at = common & ~((4u << bit) - 1u);
+    for (;; bit -= 2) {
         int count[3] = {0, 0, 0};
 #pragma unroll
         for (int j = 0; j < 3; j++)
@@ -123,9 +148,9 @@ __device__ __forceinline__ uint32_t lp_nth(const uint32_t (&k)[N], int n, bool *
             *exact = true;
             return at;
         }
+        const uint32_t rest = (1u << bit) - 1u;
+        if (!(differ & rest)) return at | (common & rest);
     }
-    *exact = false;
-    return at;
 }
 
 /* The same of 64-bit numbers. */
@@ -256,10 +281,10 @@ __device__ __forceinline__ void lp_finish(const logprobs_args &p, int64_t row, c
     }
 }
 
-/* 8 waves of a SIMD hold 2047 rows at once (157 us instead of 164 with 7); of fp32 logits the registers do not suffice, and
- * memory is the bound. */
+/* 8 waves of a SIMD hold 2047 rows at once (157 us when it was 164 with 7). fp32 logits need more registers, and
+ * memory is the bound there. */
 template <typename T>
-__global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 7 : 8) void sera_logprobs_kernel(logprobs_args p) {
+__global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 6 : 8) void sera_logprobs_kernel(logprobs_args p) {
     constexpr int VEC = 16 / (int)sizeof(T), UNROLL = 16 / VEC;
     __shared__ lp_key keys[kWaves][kRoom];
     __shared__ lp_sum sums[kWaves];
