@@ -83,8 +83,8 @@ attn_plans plan_of(const kv_args &a, int dim, int heads, int cus) {
  * splits have any goes by unit: a sequence's rows in the few-row kernel, `columns`
  * of them in the tile kernel. Latency, mostly: sequence, then maxima and sums together
  * (one context of 513 tokens in 5 splits: 4 us; 32768 rows in two: 22 us for
- * 50 MB, 28 when the sums of a row tile lay together and not those of a row). */
-template <typename T, int D>
+ * 50 MB, 28 when the sums of a row tile lay together and not those of a row). KEEP: the rows' norms are left. */
+template <typename T, int D, bool KEEP>
 __global__ __launch_bounds__(256) void sera_attn_join_kernel(kv_args a, attn_args t, attn_plan few, attn_plan tile,
                                                              size_t tile_sums) {
     constexpr int E = D / 64;
@@ -160,20 +160,26 @@ __global__ __launch_bounds__(256) void sera_attn_join_kernel(kv_args a, attn_arg
 #pragma unroll
         for (int e = 0; e < E; e++) o.v[e] = kv_from_f32<T>(first + i < 0 ? 0.0f : y[e] / l);
         *(attn_vec<T, E> *)((T *)t.out + (s.row0 + i) * t.out_stride + (int64_t)h * D + E * lane) = o;
-        if (t.norms && lane == 0) t.norms[(size_t)(s.row0 + i) * t.heads + h] = attn_norm(top, l);
+        if (KEEP && lane == 0) t.norms[(size_t)(s.row0 + i) * t.heads + h] = attn_norm(top, l);
     }
 }
 
 namespace {
 
-template <typename T>
-void join_t(int dim, const kv_args &a, const attn_args &t, const attn_plans &p, hipStream_t s) {
+template <typename T, bool KEEP>
+void join_d(int dim, const kv_args &a, const attn_args &t, const attn_plans &p, hipStream_t s) {
     const dim3 grid((unsigned)a.rows, (unsigned)((t.heads + 3) / 4));
     const size_t at = p.few_bytes / sizeof(float);
     if (dim == 64)
-        hipLaunchKernelGGL((sera_attn_join_kernel<T, 64>), grid, dim3(256), 0, s, a, t, p.few, p.tile, at);
+        hipLaunchKernelGGL((sera_attn_join_kernel<T, 64, KEEP>), grid, dim3(256), 0, s, a, t, p.few, p.tile, at);
     else
-        hipLaunchKernelGGL((sera_attn_join_kernel<T, 128>), grid, dim3(256), 0, s, a, t, p.few, p.tile, at);
+        hipLaunchKernelGGL((sera_attn_join_kernel<T, 128, KEEP>), grid, dim3(256), 0, s, a, t, p.few, p.tile, at);
+}
+
+template <typename T>
+void join_t(int dim, const kv_args &a, const attn_args &t, const attn_plans &p, hipStream_t s) {
+    if (t.norms) join_d<T, true>(dim, a, t, p, s);
+    else join_d<T, false>(dim, a, t, p, s);
 }
 
 /* A window's rows see fewer tiles than a whole context has. */

@@ -57,7 +57,7 @@ struct few_piece<(int)SERA_KV_Q8> { typedef attn_u2 v; };
 
 }  // namespace
 
-/* KEEP: the scores are left for the weights' sums. */
+/* KEEP: the scores and the rows' norms are left for the weights' sums. */
 template <int TYPE, typename T, int D, int CT, int NW, int OCC, bool PAIR, bool KEEP>
 __global__ __launch_bounds__(64 * NW, OCC) void sera_attn_few_kernel(kv_args a, attn_args t, int splits, int chunk) {
     using F = few_shape<TYPE, D>;
@@ -405,7 +405,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void sera_attn_few_kernel(kv_args a, 
 #pragma unroll
                 for (int x = 0; x < 4; x++) y[x] = s.len - s.n + i < 0 ? 0.0f : sum[x] / lt;
                 attn_store4((T *)t.out + (s.row0 + i) * t.out_stride + q0 + (rr - i * t.group) * D + d, y);
-                if (t.norms && d == 0)
+                if (KEEP && d == 0)
                     t.norms[(size_t)(s.row0 + i) * t.heads + head * t.group + rr - i * t.group] = attn_norm(mt, lt);
             }
         }

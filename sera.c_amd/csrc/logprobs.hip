@@ -277,7 +277,8 @@ __device__ __forceinline__ void lp_finish(const logprobs_args &p, int64_t row, c
         const lp_key mine = lane < list.n ? list.keys[lane] : 0;
         const int at = fine && lane < list.n ? list.place(mine) : lane;
         p.top_ids[row * p.top + at] = fine ? (int)~(uint32_t)mine : -1;
-        p.top_logprobs[row * p.top + at] = fine ? (float)((double)(lp_value((uint32_t)(mine >> 32)) - a.m) - log_s) : nan;
+        const float y = lp_value((uint32_t)(mine >> 32));
+        p.top_logprobs[row * p.top + at] = fine ? (float)((double)(y - a.m) - log_s) : nan;
     }
 }
 
