@@ -1,6 +1,6 @@
 /*
  * attn.hip - attention of packed rows over the paged cache: which kernel takes
- * a call and how it is cut up, and the kernel that joins contexts split over
+ * a call and how it is cut up, and the kernels that join contexts split over
  * workgroups.
  *
  *   s_j = scale * q . k_j,  o = sum_j 2^(s_j' - m) v_j / sum_j 2^(s_j' - m)
@@ -8,7 +8,7 @@
  * with s' = s * log2(e) and m a running maximum, in one pass over the
  * visible positions j.
  */
-#include "attn_device.h"
+#include "attn_sums.h"
 #include "sera_launch.h"
 
 namespace {
@@ -77,16 +77,14 @@ attn_plans plan_of(const kv_args &a, int dim, int heads, int cus) {
     return p;
 }
 
-}  // namespace
-
 /* Joins the partial sums of a row: a wave for each (row, query head). How many
  * splits have any goes by unit: a sequence's rows in the few-row kernel, `columns`
  * of them in the tile kernel. Latency, mostly: sequence, then maxima and sums together
  * (one context of 513 tokens in 5 splits: 4 us; 32768 rows in two: 22 us for
  * 50 MB, 28 when the sums of a row tile lay together and not those of a row). KEEP: the rows' norms are left. */
 template <typename T, int D, bool KEEP>
-__global__ __launch_bounds__(256) void sera_attn_join_kernel(kv_args a, attn_args t, attn_plan few, attn_plan tile,
-                                                             size_t tile_sums) {
+__device__ __forceinline__ void join_row(const kv_args &a, const attn_args &t, const attn_plan &few,
+                                         const attn_plan &tile, size_t tile_sums) {
     constexpr int E = D / 64;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int i;
@@ -164,6 +162,36 @@ __global__ __launch_bounds__(256) void sera_attn_join_kernel(kv_args a, attn_arg
     }
 }
 
+}  // namespace
+
+template <typename T, int D, bool KEEP>
+__global__ __launch_bounds__(256) void sera_attn_join_kernel(kv_args a, attn_args t, attn_plan few, attn_plan tile,
+                                                             size_t tile_sums) {
+    join_row<T, D, KEEP>(a, t, few, tile, tile_sums);
+}
+
+/* The join, and beside it in the same launch the weights' sums of few rows, which need the norms and not the result (one
+ * token over 1025 positions: 6 us, 4 and 5.5 one after the other). Blocks behind the rows' have `blocks` of 1024
+ * positions for every sequence and kv head. */
+template <typename T, int D>
+__global__ __launch_bounds__(256) void sera_attn_join_sums_kernel(kv_args a, attn_args t, attn_plan few, attn_sums p,
+                                                                  int blocks) {
+    if ((int)blockIdx.x < a.rows) {
+        join_row<T, D, false>(a, t, few, attn_plan(), 0);
+        return;
+    }
+    __shared__ float2 norms[kFewNorms];
+    const int64_t at = (int64_t)((int)blockIdx.x - a.rows) * gridDim.y + blockIdx.y, array = at / blocks;
+    if (array >= (int64_t)a.sequences * a.kv_heads) return;
+    const int head = (int)(array % a.kv_heads), b = (int)(array / a.kv_heads), block0 = (int)(at % blocks) * 1024;
+    const kv_seq s = kv_sequence(a, b);
+    if (s.bad || block0 >= s.len) return;
+    attn_few_norms(a, t, p, s, head, norms);
+    __syncthreads();
+    const int j = block0 + 4 * (int)threadIdx.x;
+    if (j < s.len) attn_put_sums(t, s, (size_t)array, j, attn_few_sums(t, p, s, (size_t)array, j, norms));
+}
+
 namespace {
 
 template <typename T, bool KEEP>
@@ -180,6 +208,17 @@ template <typename T>
 void join_t(int dim, const kv_args &a, const attn_args &t, const attn_plans &p, hipStream_t s) {
     if (t.norms) join_d<T, true>(dim, a, t, p, s);
     else join_d<T, false>(dim, a, t, p, s);
+}
+
+template <typename T>
+void join_sums(int dim, const kv_args &a, const attn_args &t, const attn_plans &p, const attn_sums &sums, hipStream_t s) {
+    const int blocks = (a.max_kv + 1023) / 1024, y = (t.heads + 3) / 4;
+    const int64_t all = (int64_t)a.sequences * a.kv_heads * blocks;
+    const dim3 grid((unsigned)(a.rows + (all + y - 1) / y), (unsigned)y);
+    if (dim == 64)
+        hipLaunchKernelGGL((sera_attn_join_sums_kernel<T, 64>), grid, dim3(256), 0, s, a, t, p.few, sums, blocks);
+    else
+        hipLaunchKernelGGL((sera_attn_join_sums_kernel<T, 128>), grid, dim3(256), 0, s, a, t, p.few, sums, blocks);
 }
 
 /* A window's rows see fewer tiles than a whole context has. */
@@ -236,6 +275,9 @@ hipError_t sera_launch_attn(uint32_t cache_type, uint32_t type, int dim, const k
      * have few tiles for more (one of 513 tokens: 11 us with four, 14 with eight). */
     p.few.waves = cache_type == SERA_KV_Q8 && p.few.columns <= 16 && p.few.splits == 1 &&
                   (int64_t)a.sequences * a.kv_heads <= args.cus ? 8 : 4;
+    sums.splits = p.few.splits;
+    sums.chunk = p.few.chunk;
+    sums.dim = dim;
     hipError_t e = hipSuccess;
     if (p.tile.columns) {
         attn_args u = t;
@@ -243,6 +285,12 @@ hipError_t sera_launch_attn(uint32_t cache_type, uint32_t type, int dim, const k
         e = sera_launch_attn_tile(cache_type, type, dim, a, u, p.tile, s);
     }
     if (e == hipSuccess && p.few.columns) e = sera_launch_attn_few(cache_type, type, dim, a, t, p.few, s);
+    if (e == hipSuccess && t.weights && p.bytes && !p.tile.columns) {
+        if (type == SERA_TYPE_F32) join_sums<float>(dim, a, t, p, sums, s);
+        else if (type == SERA_TYPE_F16) join_sums<_Float16>(dim, a, t, p, sums, s);
+        else join_sums<__bf16>(dim, a, t, p, sums, s);
+        return hipGetLastError();
+    }
     if (e == hipSuccess && p.bytes) {
         if (type == SERA_TYPE_F32) join_t<float>(dim, a, t, p, s);
         else if (type == SERA_TYPE_F16) join_t<_Float16>(dim, a, t, p, s);

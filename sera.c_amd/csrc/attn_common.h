@@ -30,6 +30,7 @@ struct attn_args {
 /* How the weights' sums are made. */
 struct attn_sums {
     int few_rows;                   /* columns of a sequence in the few-row kernel, at most; 0: it has no part */
+    int splits, chunk, dim;         /* of its partial results */
     size_t pitch;                   /* floats from one row of scores (or sums) to the next */
     int groups, share;              /* of all other sequences: workgroups of a sequence and head at most, units
                                      * (blocks of 32 columns over 512 positions) of one */

@@ -26,7 +26,7 @@
  * rows) leave 134 MB of scores in the 461 us in which the attention streams 2.1 GB of cache, and one pass over them
  * takes 33 us (4.1 TB/s).
  */
-#include "attn_device.h"
+#include "attn_sums.h"
 #include "sera_launch.h"
 
 namespace {
@@ -395,43 +395,26 @@ __global__ __launch_bounds__(64 * kWaves, 2) void sera_attn_columns_kernel(kv_ar
 
 /* The sums of few rows from their scores, and of many from the workgroups' parts: four positions a thread. */
 __global__ __launch_bounds__(256) void sera_attn_sums_kernel(kv_args a, attn_args t, attn_sums p) {
+    __shared__ float2 norms[kFewNorms];
     const int b = (int)(blockIdx.z * gridDim.y + blockIdx.y);
     if (b >= a.sequences) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int head = (int)blockIdx.x % a.kv_heads, w0 = ((int)blockIdx.x / a.kv_heads * 4 + wave) * 256;
+    const int head = (int)blockIdx.x % a.kv_heads, block0 = (int)blockIdx.x / a.kv_heads * 1024, w0 = block0 + 256 * wave;
     const int j = w0 + 4 * lane, tile = w0 / kTokens;
     const kv_seq s = kv_sequence(a, b);
-    if (s.bad || w0 >= s.len) return;
-    const int first = s.len - s.n, rows = s.n * t.group;
+    if (s.bad || block0 >= s.len) return;
+    const bool few = s.n * t.group <= t.few_columns;
+    if (few) {
+        attn_few_norms(a, t, p, s, head, norms);
+        __syncthreads();
+    }
+    if (w0 >= s.len) return;
     const size_t place = (size_t)b * a.kv_heads + head;
-    constexpr int BATCH = 8;        /* loads on their way */
     attn_f4 w = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (rows <= t.few_columns) {
-        const float *x = p.scores + place * p.few_rows * p.pitch + j;
-        const float2 *z = t.norms + (size_t)s.row0 * t.heads + head * t.group;
-        if (j < s.len)
-            for (int r = 0, i = 0, g = 0; r < rows; r += BATCH) {
-                attn_f4 y[BATCH];
-                float2 l[BATCH];
-                int pos[BATCH];
-#pragma unroll
-                for (int k = 0; k < BATCH; k++) {
-                    y[k] = *(const attn_f4 *)(x + (size_t)min(r + k, rows - 1) * p.pitch);
-                    l[k] = z[(size_t)min(i, s.n - 1) * t.heads + g];
-                    pos[k] = r + k < rows ? first + i : -1;
-                    if (++g == t.group) {
-                        g = 0;
-                        i++;
-                    }
-                }
-#pragma unroll
-                for (int k = 0; k < BATCH; k++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (pos[k] >= 0 && attn_sees(t, pos[k], j + e))
-                            w[e] = fmaf(attn_exp2(y[k][e] - l[k].x), l[k].y, w[e]);
-            }
+    if (few) {
+        if (j < s.len) w = attn_few_sums(t, p, s, place, j, norms);
     } else {
+        constexpr int BATCH = 8;        /* loads on their way */
         /* units in front of the tile's */
         int64_t u0 = 0;
         for (int x = lane; x < tile; x += 64) {
@@ -455,10 +438,7 @@ __global__ __launch_bounds__(256) void sera_attn_sums_kernel(kv_args a, attn_arg
             }
         }
     }
-    const size_t at = place * (size_t)t.weights_stride + j;
-#pragma unroll
-    for (int e = 0; e < 4; e++)
-        if (j + e < s.len) t.weights[at + e] = (t.before && j + e < first ? t.before[at + e] : 0.0f) + w[e];
+    attn_put_sums(t, s, place, j, w);
 }
 
 namespace {
