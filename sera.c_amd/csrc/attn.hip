@@ -170,8 +170,8 @@ __global__ __launch_bounds__(256) void sera_attn_join_kernel(kv_args a, attn_arg
     join_row<T, D, KEEP>(a, t, few, tile, tile_sums);
 }
 
-/* The join, and beside it in the same launch the weights' sums of few rows, which need the norms and not the result (one
- * token over 1025 positions: 6 us, 4 and 5.5 one after the other). Blocks behind the rows' have `blocks` of 1024
+/* The join, and beside it in the same launch the weights' sums of few rows, which need the norms and not the result
+ * (one token over 1025 positions: 6 us, 4 and 5.5 one after the other). Blocks behind the rows' have `blocks` of 1024
  * positions for every sequence and kv head. */
 template <typename T, int D>
 __global__ __launch_bounds__(256) void sera_attn_join_sums_kernel(kv_args a, attn_args t, attn_plan few, attn_sums p,
@@ -211,7 +211,8 @@ void join_t(int dim, const kv_args &a, const attn_args &t, const attn_plans &p, 
 }
 
 template <typename T>
-void join_sums(int dim, const kv_args &a, const attn_args &t, const attn_plans &p, const attn_sums &sums, hipStream_t s) {
+void join_sums(int dim, const kv_args &a, const attn_args &t, const attn_plans &p, const attn_sums &sums,
+               hipStream_t s) {
     const int blocks = (a.max_kv + 1023) / 1024, y = (t.heads + 3) / 4;
     const int64_t all = (int64_t)a.sequences * a.kv_heads * blocks;
     const dim3 grid((unsigned)(a.rows + (all + y - 1) / y), (unsigned)y);

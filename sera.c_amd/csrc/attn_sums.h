@@ -9,10 +9,10 @@
 
 constexpr int kFewNorms = 32;       /* columns of the few-row kernel */
 
-/* The norms of a sequence's and kv head's columns, by four waves: as the few-row kernel left them, or of a context split
- * over workgroups from what each of those left (as the join has them, which may run at the same time). */
-__device__ __forceinline__ void attn_few_norms(const kv_args &a, const attn_args &t, const attn_sums &p, const kv_seq &s,
-                                               int head, float2 *norms) {
+/* The norms of a sequence's and kv head's columns, by four waves: as the few-row kernel left them, or of a context
+ * split over workgroups from what each of those left (as the join has them, which may run at the same time). */
+__device__ __forceinline__ void attn_few_norms(const kv_args &a, const attn_args &t, const attn_sums &p,
+                                               const kv_seq &s, int head, float2 *norms) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), rows = s.n * t.group;
     if (p.splits < 2) {
         if (tid < rows) {

@@ -399,8 +399,8 @@ __global__ __launch_bounds__(256) void sera_attn_sums_kernel(kv_args a, attn_arg
     const int b = (int)(blockIdx.z * gridDim.y + blockIdx.y);
     if (b >= a.sequences) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int head = (int)blockIdx.x % a.kv_heads, block0 = (int)blockIdx.x / a.kv_heads * 1024, w0 = block0 + 256 * wave;
-    const int j = w0 + 4 * lane, tile = w0 / kTokens;
+    const int head = (int)blockIdx.x % a.kv_heads, block0 = (int)blockIdx.x / a.kv_heads * 1024;
+    const int w0 = block0 + 256 * wave, j = w0 + 4 * lane, tile = w0 / kTokens;
     const kv_seq s = kv_sequence(a, b);
     if (s.bad || block0 >= s.len) return;
     const bool few = s.n * t.group <= t.few_columns;
