@@ -44,9 +44,9 @@ size_t sera_logprobs_workspace_bytes(int rows, int vocab, int top);
  * outside 0..vocab-1 has log probability NaN. A row that holds a NaN or +inf,
  * or nothing but -inf, has no distribution: NaN everywhere, and top ids of -1.
  *
- * Sums are in fp32 around a maximum. One or two launches; results repeat bit
- * for bit. workspace: 16-byte aligned, sera_logprobs_workspace_bytes(), used by
- * one call at a time. */
+ * Sums are around a maximum, in fp32 of 16 elements and in 64 bits of those.
+ * One or two launches; results repeat bit for bit. workspace: 16-byte aligned,
+ * sera_logprobs_workspace_bytes(), used by one call at a time. */
 int sera_logprobs(uint32_t type, const void *logits, int64_t stride, int rows, int vocab, const int32_t *tokens,
                   int per_row, float *token_logprobs, float *entropy, int top, int32_t *top_ids, float *top_logprobs,
                   void *workspace, size_t workspace_bytes, void *stream);

@@ -104,6 +104,14 @@ def test_long_contexts(torch, length, keep):  # noqa: F811
     check(torch, s, weights_of(s, s.rng, "ties"), keep, keep // 4, 4)
 
 
+@pytest.mark.parametrize("length", [4096, 4097, 8192, 8193, 16384, 16385, 24576, 24577])
+@pytest.mark.parametrize("spread", ["spread", "equal", "signs"])
+def test_lengths_around_what_registers_hold(torch, length, spread):  # noqa: F811
+    print(f"case {length} {spread}", flush=True)
+    s = Setup(torch, ao.Q8, F32, [0, 0], [length, length // 3], kv_heads=1, dim=64, page=128)
+    check(torch, s, weights_of(s, s.rng, spread), length // 2, 100, 3)
+
+
 def test_shared_pages_stay(torch):  # noqa: F811
     """Branches that share a prefix are thinned each to pages of its own; the shared ones stay as they were."""
     s = Setup(torch, ao.F16, F32, [0] * 5, [300] * 5, kv_heads=2, page=16, shared=15)

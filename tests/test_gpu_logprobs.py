@@ -1,7 +1,8 @@
 """sera_logprobs on the GPU against the 64-bit oracle.
 
-Tolerances. A lane sums at most m = vocab / 256 + 64 exponentials in fp32 (a wave has a quarter of a row or less), and
-joins some ten times: the sum is off by (m + 20) 2^-24 of itself, and each exponential by (2 |x - max| + 2) 2^-24, which for
+Tolerances. A lane sums at most m = vocab / 256 + 64 exponentials (a wave has a quarter of a row or less), and
+joins some ten times: in fp32 throughout the sum would be off by (m + 20) 2^-24 of itself (16 elements' are, and those are
+added up in 64 bits), and each exponential by (2 |x - max| + 2) 2^-24, which for
 the weights that count is below 2^-19. Their logarithm is as far off absolutely; a log probability adds the rounding of x - max and of
 the result. The entropy is the difference of such a logarithm and a mean of x - max, whose terms are off as the weights are.
 The top's ids are exact.
@@ -108,6 +109,17 @@ def test_equal_logits_come_in_the_order_of_their_ids(torch):  # noqa: F811
         got = check(torch, x, some(2, 30000, 2), 64, f"{io} equal")
         assert (got[2] == np.arange(64)).all()
         check(torch, logits(torch, 3, 30000, io).round(), some(3, 30000, 2), 50, f"{io} few values")
+
+
+@pytest.mark.parametrize("io", [F32, BF16])
+@pytest.mark.parametrize("rows", [1, 600])
+def test_a_token_that_stands_out(torch, io, rows):  # noqa: F811
+    """Nearly all of a row's sum in one token: the entropy is what the many small weights beside it add up to."""
+    x = logits(torch, rows, 20000, io, rows, 1.0)
+    at = torch.arange(rows, device="cuda") * 31 % 20000
+    for height in (14.0, 20.0, 30.0):
+        x[torch.arange(rows, device="cuda"), at] = height
+        check(torch, x, at[:, None].int().cpu().numpy(), 3, f"{io} {rows} rows, {height}")
 
 
 @pytest.mark.parametrize("vocab", [9000, 151936])

@@ -171,6 +171,15 @@ def test_in_place_and_out_of_a_fused_buffer(torch):  # noqa: F811
         check(torch, s, spec, w[:, :384], buf[:, :384], w[:, 384:576], w[:, 576:768], before)
 
 
+@pytest.mark.parametrize("rows,heads,kv_heads", [(3000, 24, 8), (1777, 40, 10)])
+def test_several_heads_a_workgroup(torch, rows, heads, kv_heads):  # noqa: F811
+    """Enough rows that a wave turns several heads, the last workgroup of a block fewer, and some q's heads and k's."""
+    print(f"case {rows} rows {heads} over {kv_heads} heads", flush=True)
+    s = Setup(torch, ao.F16, BF16, [rows, 5], [rows + 30, 5], heads=heads, kv_heads=kv_heads, dim=64, page=64)
+    rope, spec = make(torch, s, 64, so.HALVES)
+    check(torch, s, spec, *run(torch, s, rope))
+
+
 def test_many_sequences(torch):  # noqa: F811
     rng = np.random.default_rng(1)
     news = [int(n) for n in rng.integers(0, 4, 300)]
