@@ -20,7 +20,8 @@ struct attn_args {
     float *workspace;
     int cus;                        /* compute units of the device */
     float2 *norms;                  /* attn_norm of each row, [rows][heads], for the weights, or NULL */
-    float *scores;                  /* s' of the few-row kernel, [sequences][kv_heads][few_rows][pitch], or NULL */
+    float *scores;                  /* s' of the few-row kernel, [sequences][kv_heads][pitch / 32][few_rows][32], or
+                                     * NULL */
     size_t pitch;
     const float *before;            /* sums so far, or NULL */
     float *weights;                 /* [sequences][kv_heads][weights_stride] */
@@ -31,7 +32,7 @@ struct attn_args {
 struct attn_sums {
     int few_rows;                   /* columns of a sequence in the few-row kernel, at most; 0: it has no part */
     int splits, chunk, dim;         /* of its partial results */
-    size_t pitch;                   /* floats from one row of scores (or sums) to the next */
+    size_t pitch;                   /* positions that scores have a place for, of each sequence */
     int groups, share;              /* of all other sequences: workgroups of a sequence and head at most, units
                                      * (blocks of 32 columns over 512 positions) of one */
     size_t slots;                   /* places of 512 sums for a sequence and head */

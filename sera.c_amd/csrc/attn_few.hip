@@ -157,12 +157,13 @@ __global__ __launch_bounds__(64 * NW, OCC) void sera_attn_few_kernel(kv_args a, 
      * the tokens QT * quarter + 4 u + i. V pieces are those same tokens of one channel. */
     const int k_token = QT * (col >> 2) + (col & 3), v_token = QT * quarter;
     /* Rows of scores, as q's: columns past the last have its q and write its scores once more, so that every lane stores
-     * and no wait for a load becomes one for a store as well (64 sequences of 8192 positions: 461 us instead of 471). */
+     * and no wait for a load becomes one for a store as well (64 sequences of 8192 positions: 461 us instead of 471;
+     * 457 since the scores of a tile lie together). */
     float *keep[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ct++)
-        keep[ct] = KEEP ? t.scores + ((size_t)(b * a.kv_heads + head) * t.few_rows +
-                                      min(ct * 16 + (PAIR ? col & 7 : col), rows - 1)) * t.pitch : nullptr;
+        keep[ct] = KEEP ? t.scores + (size_t)(b * a.kv_heads + head) * t.few_rows * t.pitch +
+                              min(ct * 16 + (PAIR ? col & 7 : col), rows - 1) * TT + v_token : nullptr;
     attn_u4 kr[NS][KP];
     typename few_piece<TYPE>::v vr[NC];
     attn_f4 ks[Q8 ? NS : 1], vs[Q8 ? NS : 1];
@@ -271,7 +272,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void sera_attn_few_kernel(kv_args a, 
                         for (int i = 0; i < 4; i++)
                             x[4 * u + i] = attn_sees(t, pos[ct], j0 + 4 * u + i) ? x[4 * u + i] : -INFINITY;
                 if (KEEP) {
-                    float *to = keep[ct] + j0;
+                    float *to = keep[ct] + (size_t)(j0 - v_token) * t.few_rows;
 #pragma unroll
                     for (int u = 0; u < NS; u++)
                         *(attn_f4 *)(to + 4 * u) = attn_f4{x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]};

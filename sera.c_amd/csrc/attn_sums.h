@@ -60,7 +60,8 @@ __device__ __forceinline__ attn_f4 attn_few_sums(const attn_args &t, const attn_
                                                  int j, const float2 *norms) {
     constexpr int BATCH = 8;        /* loads on their way */
     const int first = s.len - s.n, rows = s.n * t.group;
-    const float *const x = p.scores + place * p.few_rows * p.pitch + j;
+    constexpr int TILE = 1 << kAttnShift;
+    const float *const x = p.scores + (place * p.pitch + (j & -TILE)) * p.few_rows + j % TILE;
     attn_f4 w = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int r = 0, i = 0, g = 0; r < rows; r += BATCH) {
         attn_f4 y[BATCH];
@@ -68,7 +69,7 @@ __device__ __forceinline__ attn_f4 attn_few_sums(const attn_args &t, const attn_
         int pos[BATCH];
 #pragma unroll
         for (int k = 0; k < BATCH; k++) {
-            y[k] = *(const attn_f4 *)(x + (size_t)min(r + k, rows - 1) * p.pitch);
+            y[k] = *(const attn_f4 *)(x + min(r + k, rows - 1) * TILE);
             l[k] = norms[min(r + k, rows - 1)];
             pos[k] = r + k < rows ? first + i : -1;
             if (++g == t.group) {

@@ -23,7 +23,7 @@
  * of 16384 positions (8 kv heads, 128 channels, fp16 cache): 435 us with 16-bit rows, 600 us with fp32 ones, whose
  * products are two (0.8 of the rate of a large library product); a prompt of 2048 fp32 rows: 110 us behind the
  * attention's 160 us. Few rows are bound by memory: 64 sequences of 8192 positions (8 kv heads, groups of 8, bf16
- * rows) leave 134 MB of scores in the 461 us in which the attention streams 2.1 GB of cache, and one pass over them
+ * rows) leave 134 MB of scores in the 457 us in which the attention streams 2.1 GB of cache, and one pass over them
  * takes 33 us (4.1 TB/s).
  */
 #include "attn_sums.h"
