@@ -18,10 +18,10 @@
  * launch joins in the same way.
  *
  * Bound by reading the logits, and of 16-bit ones by the vector instructions (8 an element and an exponential). 2047
- * rows of 151937 bf16 logits: 120 us without a top (5.2 TB/s, what a copy reaches), 139 us with the top 8; 1008 rows
+ * rows of 151937 bf16 logits: 120 us without a top (5.2 TB/s, what a copy reaches), 130 us with the top 8; 1008 rows
  * of 151936 fp32 logits with the top 8: 115 us (5.3 TB/s). 16 rows: 11 + 4 us, 1 row: 8.5 + 6 us, which is latency. A
  * long top of short rows costs more than the rows, as nearly every step has some of it: the top 64 of 538 rows of
- * 19950 54 us, the top 5 20 us, none 11 us. A threshold of each wave by itself, its list's top-th, made the first 250
+ * 19950 54 us, the top 5 18 us, none 11 us. A threshold of each wave by itself, its list's top-th, made the first 250
  * us: four times as many steps had something to look at.
  */
 #include "logprobs.h"
@@ -332,13 +332,17 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 6 : 8) void sera_logp
 
     /* What is not over `least` has no place in the top; but -inf has one until the list is as long. */
     float least = p.top ? -INFINITY : INFINITY;
+    int known = 0;                                  /* candidates when the bound was found */
     const auto look = [&](int step, float top) {
         const uint32_t now = lp_order(top), had = atomicMax(&most[lane], now), mine[1] = {had > now ? had : now};
-        bool exact;
-        int larger;
-        const uint32_t nth = lp_nth(mine, p.top, &exact, &larger);
-        if (lane == 0) atomicMax(&bound, nth);
-        least = fmaxf(least, lp_below(nth));
+        if (list.n - known >= p.top || least == -INFINITY) {       /* else the bound has not gone far */
+            bool exact;
+            int larger;
+            const uint32_t nth = lp_nth(mine, p.top, &exact, &larger);
+            if (lane == 0) atomicMax(&bound, nth);
+            least = fmaxf(least, lp_below(nth));
+            known = list.n;
+        }
         const bool all = least == -INFINITY && list.n < p.top;
         uint64_t lanes = __ballot(top > least || all);
         while (lanes) {                             /* 4 lanes' elements at a time */
@@ -353,7 +357,10 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 6 : 8) void sera_logp
             float y = -INFINITY;
             if (of < 64 && e < n) y = lp_f32(x[id += e]);
             const bool is = of < 64 && e < n && (y > least || all);
-            if (list.n > kRoom - 64) list.cut(lane);
+            if (list.n > kRoom - 64) {
+                list.cut(lane);
+                known = -kRoom;
+            }
             list.put((lp_key)lp_order(y) << 32 | (uint32_t)~id, is && y == y, lane);
         }
         /* The ids that follow are higher: equal logits come behind the list's. */
