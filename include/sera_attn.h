@@ -187,9 +187,10 @@ int sera_kv_write_rope(const sera_kv_cache *cache, const sera_kv_batch *batch, c
  * [sequences][kv_heads][weights_stride] (weights_stride >= max_kv); `before`
  * may be `weights` (the sums go on in place) or NULL (they start with this
  * call), and must not overlap it otherwise. Places from kv_len on are left as
- * they are, and so is all of a sequence outside the bounds. Rows that come out
- * as NaN (a lost page, keys that are not finite) give NaN to the positions that
- * they see. A batch without rows does nothing. Results repeat bit for bit. The
+ * they are, and so is all of a sequence outside the bounds. Rows whose scores
+ * have no softmax (one that is NaN or +inf, or all of them -inf: a lost page,
+ * keys that are not finite) give NaN to the positions that they see. A batch
+ * without rows does nothing. Results repeat bit for bit. The
  * workspace is its own size, which grows with rows * heads * max_kv where few
  * rows go to long contexts (their scores are kept for the sums, 4 bytes each).
  */

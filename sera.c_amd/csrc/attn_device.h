@@ -84,7 +84,7 @@ __device__ __forceinline__ float attn_exp2(float x) { return __builtin_amdgcn_ex
 __device__ __forceinline__ float2 attn_norm(float m, float l) {
     const float shift = m - kAttnBias, e = (float)__builtin_amdgcn_frexp_expf(l), z = shift + e, y = z - shift;
     const float off = (shift - (z - y)) + (e - y);
-    return make_float2(z, l == 0.0f ? 0.0f : attn_exp2(-off) / __builtin_amdgcn_frexp_mantf(l));
+    return make_float2(z, l == 0.0f ? __builtin_nanf("") : attn_exp2(-off) / __builtin_amdgcn_frexp_mantf(l));
 }
 
 /* The power of two that brings the largest |q| of a row near 2^10 (products
