@@ -219,7 +219,8 @@ int sera_attention_weights(const sera_kv_cache *cache, const sera_kv_batch *batc
  * old pages again, in the same order. new_len must not overlap kv_len. A
  * sequence whose length is outside 0..max_kv moves nothing, has new_len -1 and
  * only -1 in kept; tokens of a page that is not in the pool arrive as NaN, and
- * to a new page that is not none are written. Two launches. */
+ * to a new page that is not none are written. kv_heads * min(keep, max_kv) is
+ * to stay below 2^29 (one launch moves it). Two launches. */
 int sera_kv_evict(const sera_kv_cache *cache, const sera_kv_batch *batch, int keep, int recent, int sinks,
                   const float *weights, float *new_weights, int64_t weights_stride, const int32_t *new_table,
                   int64_t new_stride, int32_t *new_len, int32_t *kept, void *stream);

@@ -31,6 +31,8 @@ constexpr int64_t kMaxPages = 0x7fffffff;
 /* Positions, rows and grid units are 32-bit in the kernels, with tile ends
  * and rows * group past them: both stay far below 2^31. */
 constexpr int kMaxPositions = 1 << 28, kMaxRows = 1 << 22, kMaxSequences = 1 << 20;
+/* Workgroups of 256 threads in x: a launch has less than 2^32 threads there. */
+constexpr int64_t kMaxGrid = ((int64_t)1 << 24) - 1;
 
 bool geometry_ok(uint32_t type, int page_tokens, int kv_heads, int head_dim) {
     return (type == SERA_KV_F16 || type == SERA_KV_Q8) && page_tokens >= 16 && page_tokens <= kMaxPageTokens &&
@@ -315,6 +317,9 @@ int sera_kv_evict(const sera_kv_cache *cache, const sera_kv_batch *batch, int ke
     if (new_stride < (most + cache->page_tokens - 1) / cache->page_tokens)
         return fail(-1, "%s: %lld new positions in %lld pages of %d tokens", tag, (long long)most,
                     (long long)new_stride, cache->page_tokens);
+    if (cache->kv_heads * ((most + 31) / 32) > kMaxGrid)
+        return fail(-1, "%s: %lld positions that stay, of %d kv heads, are more than one launch moves", tag,
+                    (long long)most, cache->kv_heads);
     if (!new_table || !new_len || !kept || ((uintptr_t)new_table & 3u) || ((uintptr_t)new_len & 3u) ||
         ((uintptr_t)kept & 3u))
         return fail(-1, "%s: new_table, new_len and kept must be 4-byte aligned device pointers", tag);
