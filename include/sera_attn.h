@@ -190,7 +190,8 @@ int sera_kv_write_rope(const sera_kv_cache *cache, const sera_kv_batch *batch, c
  * they are, and so is all of a sequence outside the bounds. Rows whose scores
  * have no softmax (one that is NaN or +inf, or all of them -inf: a lost page,
  * keys that are not finite) give NaN to the positions that they see. A batch
- * without rows does nothing. Results repeat bit for bit. The
+ * without rows does nothing. kv_heads * max_kv is to stay below 2^34 (one
+ * launch makes the sums). Results repeat bit for bit. The
  * workspace is its own size, which grows with rows * heads * max_kv where few
  * rows go to long contexts (their scores are kept for the sums, 4 bytes each).
  */

@@ -213,8 +213,10 @@ void join_t(int dim, const kv_args &a, const attn_args &t, const attn_plans &p, 
 template <typename T>
 void join_sums(int dim, const kv_args &a, const attn_args &t, const attn_plans &p, const attn_sums &sums,
                hipStream_t s) {
-    const int blocks = (a.max_kv + 1023) / 1024, y = (t.heads + 3) / 4;
-    const int64_t all = (int64_t)a.sequences * a.kv_heads * blocks;
+    const int blocks = (a.max_kv + 1023) / 1024;
+    const int64_t all = (int64_t)a.sequences * a.kv_heads * blocks;     /* 2^25 at most: split contexts are few */
+    int y = (t.heads + 3) / 4;
+    while (a.rows + (all + y - 1) / y > kAttnMaxGrid) y *= 2;
     const dim3 grid((unsigned)(a.rows + (all + y - 1) / y), (unsigned)y);
     if (dim == 64)
         hipLaunchKernelGGL((sera_attn_join_sums_kernel<T, 64>), grid, dim3(256), 0, s, a, t, p.few, sums, blocks);

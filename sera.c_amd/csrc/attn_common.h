@@ -69,6 +69,8 @@ struct attn_plan {
     int slots;           /* tile kernel: row tiles, of `columns` rows each, at most */
     int splits, chunk;   /* workgroups over a context, tiles of each */
 };
+/* Workgroups of 256 threads in x: a launch has less than 2^32 threads there. */
+constexpr int64_t kAttnMaxGrid = ((int64_t)1 << 24) - 1;
 constexpr int kAttnShift = 5;       /* log2 of a tile's tokens */
 
 hipError_t sera_launch_kv_move(bool write, uint32_t cache_type, uint32_t type, int dim, const kv_args &a, void *k,

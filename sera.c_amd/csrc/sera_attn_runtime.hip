@@ -31,8 +31,6 @@ constexpr int64_t kMaxPages = 0x7fffffff;
 /* Positions, rows and grid units are 32-bit in the kernels, with tile ends
  * and rows * group past them: both stay far below 2^31. */
 constexpr int kMaxPositions = 1 << 28, kMaxRows = 1 << 22, kMaxSequences = 1 << 20;
-/* Workgroups of 256 threads in x: a launch has less than 2^32 threads there. */
-constexpr int64_t kMaxGrid = ((int64_t)1 << 24) - 1;
 
 bool geometry_ok(uint32_t type, int page_tokens, int kv_heads, int head_dim) {
     return (type == SERA_KV_F16 || type == SERA_KV_Q8) && page_tokens >= 16 && page_tokens <= kMaxPageTokens &&
@@ -183,6 +181,9 @@ int attend(const char *tag, const sera_kv_cache *cache, const sera_kv_batch *bat
         return -1;
     if (weigh) {
         const int64_t sums = (int64_t)batch->sequences * cache->kv_heads;
+        if (cache->kv_heads * (((int64_t)batch->max_kv + 1023) / 1024) > kAttnMaxGrid)
+            return fail(-1, "%s: %d positions of %d kv heads are more than one launch sums", tag, batch->max_kv,
+                        cache->kv_heads);
         if (check_weights(tag, before ? before : weights, weights, sums, weights_stride, batch->max_kv)) return -1;
         if (before && before != weights && overlap(before, weights, sums * weights_stride * 4))
             return fail(-1, "%s: before and weights overlap and are not the same", tag);
@@ -317,7 +318,7 @@ int sera_kv_evict(const sera_kv_cache *cache, const sera_kv_batch *batch, int ke
     if (new_stride < (most + cache->page_tokens - 1) / cache->page_tokens)
         return fail(-1, "%s: %lld new positions in %lld pages of %d tokens", tag, (long long)most,
                     (long long)new_stride, cache->page_tokens);
-    if (cache->kv_heads * ((most + 31) / 32) > kMaxGrid)
+    if (cache->kv_heads * ((most + 31) / 32) > kAttnMaxGrid)
         return fail(-1, "%s: %lld positions that stay, of %d kv heads, are more than one launch moves", tag,
                     (long long)most, cache->kv_heads);
     if (!new_table || !new_len || !kept || ((uintptr_t)new_table & 3u) || ((uintptr_t)new_len & 3u) ||

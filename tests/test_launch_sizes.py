@@ -13,3 +13,12 @@ def test_evictions_of_more_positions_than_a_launch_moves(L, kv_heads, keep, fits
     """A workgroup of 256 threads for 32 positions of a kv head. What fits is refused for what is missing besides."""
     rc, err = call(L, "evict", kv_heads=kv_heads, keep=keep, kept=None, **FAR)
     assert rc == -1 and ("kept must be" if fits else "one launch") in err, (rc, err)
+
+
+@pytest.mark.parametrize("kv_heads,max_kv,fits", [(64, 1 << 28, False), (1024, 1 << 24, False), (1024, (1 << 24) - 1024, True),
+                                                  (63, 1 << 28, True)])
+def test_sums_of_more_positions_than_a_launch_has(L, kv_heads, max_kv, fits):  # noqa: F811
+    """A workgroup of 256 threads for 1024 positions of a kv head."""
+    rc, err = call(L, "weights", kv_heads=kv_heads, heads=kv_heads, max_kv=max_kv, table_stride=1 << 30, qs=1 << 20, os=1 << 20,
+                   stride=max_kv, before=1 << 50, ws=None)
+    assert rc == -1 and ("workspace must be" if fits else "one launch") in err, (rc, err)
