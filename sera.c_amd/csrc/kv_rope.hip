@@ -232,7 +232,11 @@ void rope_go(const kv_args &a, const rope_args &r, const void *q, int64_t qs, vo
      * tokens of 16: 4 items 6.4 us, 8 7.6 us. */
     const int64_t slots = kv_slots(a.rows, a.sequences, kBlock, 2), blocks = slots < a.rows ? slots : a.rows;
     const int64_t items = r.heads + 4 * a.kv_heads, want = 4 * ((blocks * items + 16 * r.cus - 1) / (16 * r.cus));
-    const int per = (int)(want < items ? want : items);
+    /* and as many as a launch's limit takes, where nearly all slots of very many sequences are empty (2^20 of them have
+     * 2^21 slots, for up to 7 workgroups each) */
+    const int64_t groups = kAttnMaxGrid / slots, least = (items + groups - 1) / groups;
+    const int64_t wanted = want > least ? want : least;
+    const int per = (int)(wanted < items ? wanted : items);
     hipLaunchKernelGGL((sera_kv_rope_kernel<TYPE, T, D>), dim3((unsigned)(slots * ((items + per - 1) / per))),
                        dim3(256), 0, s, a, r, (const T *)q, qs, (T *)q_out, qos, (const T *)k, ks, (const T *)v, vs,
                        per);
