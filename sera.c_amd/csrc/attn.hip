@@ -265,6 +265,7 @@ hipError_t sera_launch_attn(uint32_t cache_type, uint32_t type, int dim, const k
         uint8_t *const ws = (uint8_t *)t.workspace;
         size_t n;
         sums = sums_of(p, a, t.heads, t.cus, &n);
+        sera_attn_sums_shorten(sums, a, t, t.group);
         sums.scores = (float *)(ws + sums_at(p, a, t.heads));
         sums.partial = (float *)((uint8_t *)sums.scores + sums.scores_bytes);
         t.norms = (float2 *)(ws + norms_at(p));

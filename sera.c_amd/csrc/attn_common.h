@@ -35,6 +35,7 @@ struct attn_sums {
     size_t pitch;                   /* positions that scores have a place for, of each sequence */
     int groups, share;              /* of all other sequences: workgroups of a sequence and head at most, units
                                      * (blocks of 32 columns over 512 positions) of one */
+    int64_t units;                  /* of a sequence and head, at most */
     size_t slots;                   /* places of 512 sums for a sequence and head */
     size_t scores_bytes;            /* of the workspace; the ranges' sums lie behind */
     float *scores, *partial;
@@ -83,6 +84,7 @@ hipError_t sera_launch_attn(uint32_t cache_type, uint32_t type, int dim, const k
 hipError_t sera_launch_attn_tile(uint32_t cache_type, uint32_t type, int dim, const kv_args &a, const attn_args &t,
                                  const attn_plan &p, hipStream_t s);
 attn_sums sera_attn_sums_plan(const kv_args &a, int few_rows, int group, int cus, size_t *bytes);
+void sera_attn_sums_shorten(attn_sums &p, const kv_args &a, const attn_args &t, int group);
 hipError_t sera_launch_attn_sums(uint32_t cache_type, uint32_t type, int dim, const kv_args &a, const attn_args &t,
                                  const attn_sums &p, bool many, hipStream_t s);
 hipError_t sera_launch_kv_rope(uint32_t cache_type, uint32_t type, int dim, const kv_args &a, const rope_args &r,

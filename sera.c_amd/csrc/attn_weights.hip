@@ -13,8 +13,8 @@
  * rows, scaled, split into fp16 terms and laid into LDS in the order of B fragments by all waves, a block ahead of
  * the products. A lane has one column of a block, so z is one number a lane, and its sums stay in the lane until the
  * end. Blocks of columns that see any of 512 positions are the units of work (positions alone are few: 32 workgroups
- * for a prompt of 2048 and 8 kv heads); every workgroup has an equal run of them, and the last kernel adds the runs'
- * sums in their order.
+ * for a prompt of 2048 and 8 kv heads); every workgroup has an equal run of them, of fewer where a window hides
+ * most, and the last kernel adds the runs' sums in their order.
  *
  * Many rows are bound by the matrix instructions, and beside them by the exponentials and the columns' way through
  * LDS: the weights of one half of a wave's positions are made under the products of the other, and of the two waves
@@ -465,6 +465,34 @@ void columns_t(uint32_t type, int dim, const kv_args &a, const attn_args &t, con
 
 }  // namespace
 
+/* A workgroup runs on a CU; each has an equal share of all units, of 8 at least: the start of one costs some 5. */
+static void share_units(attn_sums &p, const kv_args &a, int cus) {
+    const int64_t sequences = (a.rows + a.max_new - 1) / a.max_new;
+    int64_t share = (p.units * sequences * a.kv_heads + cus - 1) / cus;
+    if (share < 8) share = 8;
+    if (share > 0x3fffffff) share = 0x3fffffff;
+    if (p.groups && share * p.groups < p.units) share = (p.units + p.groups - 1) / p.groups;
+    p.share = (int)share;
+    p.groups = (int)((p.units + share - 1) / share);
+}
+
+/* With a window a sequence has fewer units, and they are shared anew; the workspace, whose size knows no window, has room
+ * for as many workgroups as before and no more. A row sees as many tiles as its window touches, and those of sinks; each
+ * tile that rows see any of has two blocks begun. 1024 rows of 64 heads at the end of 16384 positions with a window of
+ * 512 and 4 sinks (8 kv heads, fp32 rows, fp16 cache): the sums take 110 us, in shares of the whole context 870, as few
+ * workgroups had any. */
+void sera_attn_sums_shorten(attn_sums &p, const kv_args &a, const attn_args &t, int group) {
+    if (!t.window || !p.groups) return;
+    const int64_t rows = a.max_new, blocks = (rows * group + 31) / 32;
+    const int64_t touched = ((int64_t)t.window + kTokens - 2) / kTokens + 1;
+    const int64_t sinks = ((int64_t)(t.sinks < a.max_kv ? t.sinks : a.max_kv) + kTokens - 1) / kTokens;
+    const int64_t units = sinks * blocks + (rows * touched * group + 31) / 32 +
+                          2 * ((rows + t.window + kTokens - 2) / kTokens + 1);
+    if (units >= p.units) return;
+    p.units = units;
+    share_units(p, a, t.cus);
+}
+
 /* How the sums are made, with few_rows columns of each sequence at most in the kernel of few rows (0: none goes
  * there) and groups of `group` columns for each of max_new rows at most elsewhere (0: none). Bytes of workspace in
  * *bytes. */
@@ -488,14 +516,8 @@ attn_sums sera_attn_sums_plan(const kv_args &a, int few_rows, int group, int cus
         const int64_t n = ((int64_t)a.max_kv - x * kTokens) * group / 32 + 2;
         units += n < blocks ? n : blocks;
     }
-    /* A workgroup runs on a CU; each has an equal share of all units, of 8 at least: the start of one costs some 5.
-     */
-    const int64_t sequences = (a.rows + a.max_new - 1) / a.max_new;
-    int64_t share = (units * sequences * a.kv_heads + cus - 1) / cus;
-    if (share < 8) share = 8;
-    if (share > 0x3fffffff) share = 0x3fffffff;
-    p.share = (int)share;
-    p.groups = (int)((units + share - 1) / share);
+    p.units = units;
+    share_units(p, a, cus);
     p.slots = (size_t)(p.groups + tiles);
     *bytes += arrays * p.slots * kTokens * sizeof(float);
     return p;
