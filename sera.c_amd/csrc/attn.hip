@@ -186,8 +186,10 @@ __global__ __launch_bounds__(256) void sera_attn_join_sums_kernel(kv_args a, att
     const int head = (int)(array % a.kv_heads), b = (int)(array / a.kv_heads), block0 = (int)(at % blocks) * 1024;
     const kv_seq s = kv_sequence(a, b);
     if (s.bad || block0 >= s.len) return;
-    attn_few_norms(a, t, p, s, head, norms);
-    __syncthreads();
+    if (attn_few_seen(t, s, block0, 1024)) {
+        attn_few_norms(a, t, p, s, head, norms);
+        __syncthreads();
+    }
     const int j = block0 + 4 * (int)threadIdx.x;
     if (j < s.len) attn_put_sums(t, s, (size_t)array, j, attn_few_sums(t, p, s, (size_t)array, j, norms));
 }

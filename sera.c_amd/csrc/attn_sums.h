@@ -55,6 +55,12 @@ __device__ __forceinline__ void attn_few_norms(const kv_args &a, const attn_args
     }
 }
 
+/* Whether a row of the sequence may see any of positions j .. j+n-1. What none sees, in front of the first row's window and
+ * behind the sinks, has no scores: the attention kernel goes by the same range, and leaves their places as they are. */
+__device__ __forceinline__ bool attn_few_seen(const attn_args &t, const kv_seq &s, int j, int n) {
+    return t.window == 0 || j < t.sinks || j + n - 1 > max(s.len - s.n, 0) - t.window;
+}
+
 /* The sums of positions j .. j+3. */
 __device__ __forceinline__ attn_f4 attn_few_sums(const attn_args &t, const attn_sums &p, const kv_seq &s, size_t place,
                                                  int j, const float2 *norms) {
@@ -63,6 +69,7 @@ __device__ __forceinline__ attn_f4 attn_few_sums(const attn_args &t, const attn_
     constexpr int TILE = 1 << kAttnShift;
     const float *const x = p.scores + (place * p.pitch + (j & -TILE)) * p.few_rows + j % TILE;
     attn_f4 w = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (!attn_few_seen(t, s, j, 4)) return w;
     for (int r = 0, i = 0, g = 0; r < rows; r += BATCH) {
         attn_f4 y[BATCH];
         float2 l[BATCH];

@@ -404,7 +404,7 @@ __global__ __launch_bounds__(256) void sera_attn_sums_kernel(kv_args a, attn_arg
     const kv_seq s = kv_sequence(a, b);
     if (s.bad || block0 >= s.len) return;
     const bool few = s.n * t.group <= t.few_columns;
-    if (few) {
+    if (few && attn_few_seen(t, s, block0, 1024)) {
         attn_few_norms(a, t, p, s, head, norms);
         __syncthreads();
     }

@@ -52,3 +52,34 @@ def test_the_work_of_a_window_is_shared_by_all(torch, news, lens, window, sinks)
     for b, n in enumerate(each):
         print(f"  sequence {b}: {n} units, {written[b * kv_heads]} places of sums", flush=True)
         assert min(written[b * kv_heads:(b + 1) * kv_heads]) >= n / (2 * share)
+
+
+def test_steps_with_a_window_do_not_read_the_scores_of_the_whole_context(torch):  # noqa: F811
+    """64 single tokens over 8192 positions of which 16 are seen: the sums may take some times the attention itself, but not
+    the time of the whole context's scores (268 MB, some 50 us; the attention some 10)."""
+    cache, batch, q = setup(torch, [1] * 64, [8192] * 64, 128, 8)
+    out, weights = torch.empty_like(q), torch.zeros(64, 8, 8192, device="cuda")
+    ws, ws2 = q3q4.attention_weights_workspace(cache, batch, 128), q3q4.attention_workspace(cache, batch, 128)
+
+    def time_of(step):
+        step()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            for _ in range(20):
+                step()
+        best = 1e9
+        for _ in range(7):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            g.replay()
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b) * 50)
+        return best
+
+    whole = time_of(lambda: q3q4.attention_weights(cache, batch, q, out, 0.1, weights, None, workspace=ws))
+    both = time_of(lambda: q3q4.attention_weights(cache, batch, q, out, 0.1, weights, None, 16, workspace=ws))
+    alone = time_of(lambda: q3q4.attention(cache, batch, q, out, 0.1, 16, workspace=ws2))
+    print(f"  whole {whole:.1f} us, with a window {both:.1f}, its attention alone {alone:.1f}", flush=True)
+    assert both < 4 * alone
