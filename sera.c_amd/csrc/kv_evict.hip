@@ -11,10 +11,9 @@
  * picked from there.
  *
  * The move is bound by memory, the choice by the latency of its steps. 64 sequences of 8192 positions to half (8 kv
- * heads, 128 channels, fp16 cache): 22 us and 533 us, for 2.7 GB the rate of a copy; of V's blocks of 16 tokens
- * hardly one is without any that stays, so V is read whole. 24 sequences of up to 3001 (8-bit cache): 9 us and 27 us.
- * The choice alone, of one sequence: 3001 positions 8 us, 16000 23 us, 200000 265 us; with the cut built two bits at
- * a time by counts over all waves 13, 25 and 496 us.
+ * heads, 128 channels, fp16 cache): 21 us and 533 us, for 2.7 GB the rate of a copy; of V's blocks of 16 tokens
+ * hardly one is without any that stays, so V is read whole. 24 sequences of up to 3001 (8-bit cache): 8.3 us and 27
+ * us. The choice alone, of one sequence: 3001 positions 7.6 us, 16000 19 us, 200000 286 us.
  */
 #include "attn_common.h"
 #include "sera_dpp.h"
@@ -312,13 +311,15 @@ hipError_t sera_launch_kv_evict(uint32_t cache_type, int dim, const kv_args &a, 
     const int y = a.sequences < 32768 ? a.sequences : 32768;
     const unsigned z = (unsigned)((a.sequences + y - 1) / y);
     const dim3 heads((unsigned)a.kv_heads, (unsigned)y, z);
-    /* Eight waves as long as their registers hold a sequence (built two bits at a time, 3001 positions took 13 us, 15
-     * with four waves and 17 with sixteen; 16000 took 25, 28 with sixteen). Then sixteen, and beyond what those hold
-     * as well, where the weights are read five times: 200000 positions took 490 us, 710 with eight. */
+    /* Eight waves for short sequences, where more of them only wait for each other (24 of 3001 positions 8.3 us, 8.4 with
+     * sixteen, 10.6 with four), then sixteen (64 of 8192: 20.9 us, 22.1 with eight; one of 16000: 18.8 and 23.4), and
+     * beyond what those hold as well, where the weights are read up to six times, for four digits, the counts and the
+     * places (one of 65536: 83 us, 123 with eight; of 200000: 286 and 434). The form goes by the bound, as the lengths
+     * are the device's: 24 of 3001 take 13.5 us with a bound of 16000, 13.2 with one of 131072. */
 #define SERA_KEEP(W, R) hipLaunchKernelGGL((sera_kv_keep_kernel<W, R>), heads, dim3(64 * W), 0, s, a, t)
     if (a.max_kv <= 8 * 64 * 8) SERA_KEEP(8, 8);
-    else if (a.max_kv <= 16 * 64 * 8) SERA_KEEP(8, 16);
-    else if (a.max_kv <= 32 * 64 * 8) SERA_KEEP(8, 32);
+    else if (a.max_kv <= 8 * 64 * 16) SERA_KEEP(16, 8);
+    else if (a.max_kv <= 16 * 64 * 16) SERA_KEEP(16, 16);
     else if (a.max_kv <= 24 * 64 * 16) SERA_KEEP(16, 24);
     else SERA_KEEP(16, 0);
 #undef SERA_KEEP
