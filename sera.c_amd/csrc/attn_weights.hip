@@ -19,7 +19,8 @@
  * Many rows are bound by the matrix instructions, and beside them by the exponentials and the columns' way through
  * LDS: the weights of one half of a wave's positions are made under the products of the other, and of the two waves
  * of a SIMD one converts columns while the other multiplies. r goes into z there, rounded to fp32 (2^-24 |z| of a
- * weight, less than its score's own error); as a factor of every weight it cost 5%. 1024 rows of 64 heads at the end
+ * weight, less than its score's own error: z is log2 of the sum of 2^s' but for a factor of 2, whatever the scales of
+ * 8-bit values); as a factor of every weight it cost 5%. 1024 rows of 64 heads at the end
  * of 16384 positions (8 kv heads, 128 channels, fp16 cache): 435 us with 16-bit rows, 600 us with fp32 ones, whose
  * products are two (0.8 of the rate of a large library product); a prompt of 2048 fp32 rows: 110 us behind the
  * attention's 160 us. Few rows are bound by memory: 64 sequences of 8192 positions (8 kv heads, groups of 8, bf16
